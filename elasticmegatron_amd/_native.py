@@ -43,7 +43,8 @@ EXPORTS = (
     "emrs_plan_stats_get", "emrs_plan_execute", "emrs_plan_destroy", "emrs_get_tuning",
     "emrs_set_tuning", "emrs_synth_fill", "emrs_synth_verify", "emrs_plan_compare", "emrs_xor_checksum",
     "emrs_plan_compare_static", "emrs_plan_prepare", "emrs_ipc_export", "emrs_ipc_open", "emrs_ipc_close",
-    "emrs_ipc_open_count",
+    "emrs_ipc_open_count", "emrs_loss_workspace", "emrs_loss_forward", "emrs_loss_backward", "emrs_muon_workspace",
+    "emrs_muon_step", "emrs_adamw_step",
 )
 
 # struct emrs_compare_stats
@@ -73,6 +74,46 @@ class Tuning(ctypes.Structure):
                 ("lanes", ctypes.c_uint32), ("units", ctypes.c_uint32), ("buffer_ops", ctypes.c_uint32),
                 ("chunk_index", ctypes.c_uint32), ("warm_tables", ctypes.c_uint32)]
 
+
+class Loss(ctypes.Structure):
+    """struct emrs_loss"""
+
+    _fields_ = [("dtype", ctypes.c_uint32), ("n_shards", ctypes.c_uint32), ("tokens", ctypes.c_uint64),
+                ("hidden_size", ctypes.c_uint64), ("hidden", ctypes.c_void_p), ("hidden_stride", ctypes.c_uint64),
+                ("weights", ctypes.c_void_p), ("weight_strides", ctypes.c_void_p), ("shard_rows", ctypes.c_void_p),
+                ("vocab_start", ctypes.c_uint64), ("vocab_size", ctypes.c_uint64), ("target", ctypes.c_void_p),
+                ("ignore_index", ctypes.c_int64), ("lse", ctypes.c_void_p), ("target_logit", ctypes.c_void_p),
+                ("loss", ctypes.c_void_p), ("grad_loss", ctypes.c_void_p), ("grad_hidden", ctypes.c_void_p),
+                ("grad_weights", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class Muon(ctypes.Structure):
+    """struct emrs_muon"""
+
+    _fields_ = [("count", ctypes.c_uint32), ("grad_dtype", ctypes.c_uint32), ("rows", ctypes.c_uint64),
+                ("cols", ctypes.c_uint64), ("grad", ctypes.c_void_p), ("momentum", ctypes.c_void_p),
+                ("main", ctypes.c_void_p), ("image", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("grad_stride", ctypes.c_uint64), ("momentum_stride", ctypes.c_uint64),
+                ("main_stride", ctypes.c_uint64), ("image_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64),
+                ("steps", ctypes.c_uint32), ("nesterov", ctypes.c_uint32), ("coefficients", ctypes.c_void_p),
+                ("mu", ctypes.c_float), ("eps", ctypes.c_float), ("decay", ctypes.c_float), ("rate", ctypes.c_float),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class AdamW(ctypes.Structure):
+    """struct emrs_adamw"""
+
+    _fields_ = [("n", ctypes.c_uint64), ("main", ctypes.c_void_p), ("exp_avg", ctypes.c_void_p),
+                ("exp_avg_sq", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("grad_dtype", ctypes.c_uint32),
+                ("step", ctypes.c_uint32), ("image", ctypes.c_void_p), ("lr", ctypes.c_double),
+                ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+                ("weight_decay", ctypes.c_double)]
+
+
+EMRS_FP32, EMRS_BF16, EMRS_FP16 = 0, 1, 2
+EMRS_LOSS_MAX_SHARDS = 64
+EMRS_MUON_MAX_MATRICES = 32
+EMRS_MUON_MAX_STEPS = 16
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -124,6 +165,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.emrs_ipc_close.argtypes = [P]
     lib.emrs_ipc_open_count.restype = I
     lib.emrs_ipc_open_count.argtypes = []
+    lib.emrs_loss_workspace.restype = I
+    lib.emrs_loss_workspace.argtypes = [ctypes.POINTER(Loss), I, ctypes.POINTER(U64)]
+    lib.emrs_muon_workspace.restype = I
+    lib.emrs_muon_workspace.argtypes = [ctypes.POINTER(Muon), ctypes.POINTER(U64)]
+    for fn, record in ((lib.emrs_loss_forward, Loss), (lib.emrs_loss_backward, Loss), (lib.emrs_muon_step, Muon),
+                       (lib.emrs_adamw_step, AdamW)):
+        fn.restype = I
+        fn.argtypes = [ctypes.POINTER(record), P]
     if lib.emrs_abi_version() != 8:
         raise RuntimeError("libemrs ABI version mismatch")
     _lib = lib
@@ -322,3 +371,36 @@ def ipc_close(ptr: int) -> None:
 def ipc_open_count() -> int:
     """Allocations this process holds open through :func:`ipc_open`."""
     return int(load().emrs_ipc_open_count())
+
+
+# ----- operators of a training step -----
+
+
+def loss_workspace(a: Loss, backward: bool) -> int:
+    """emrs_loss_workspace: bytes of workspace that the call wants."""
+    n = ctypes.c_uint64()
+    _check(load().emrs_loss_workspace(ctypes.byref(a), 1 if backward else 0, ctypes.byref(n)), "emrs_loss_workspace")
+    return int(n.value)
+
+
+def loss_forward(a: Loss, stream: int = 0) -> None:
+    _check(load().emrs_loss_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_loss_forward")
+
+
+def loss_backward(a: Loss, stream: int = 0) -> None:
+    _check(load().emrs_loss_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_loss_backward")
+
+
+def muon_workspace(a: Muon) -> int:
+    """emrs_muon_workspace: bytes of workspace that the call wants."""
+    n = ctypes.c_uint64()
+    _check(load().emrs_muon_workspace(ctypes.byref(a), ctypes.byref(n)), "emrs_muon_workspace")
+    return int(n.value)
+
+
+def muon_step(a: Muon, stream: int = 0) -> None:
+    _check(load().emrs_muon_step(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_muon_step")
+
+
+def adamw_step(a: AdamW, stream: int = 0) -> None:
+    _check(load().emrs_adamw_step(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_adamw_step")

@@ -10,6 +10,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -32,16 +34,30 @@ def hipcc() -> str:
 
 
 def build_native(verbose: bool = False) -> str:
+    """Each source compiles in a process of its own, as many at once as there are CPUs (at most 8)."""
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-    tmp = LIB + ".tmp"
-    cmd = [hipcc(), *HIPCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC, *srcs, "-o", tmp]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("hipcc failed:\n" + res.stdout + res.stderr)
+    flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    logs = []
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o") for s in srcs]
+
+        def compile_one(src_obj):
+            src, obj = src_obj
+            return subprocess.run([hipcc(), *flags, "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", src, "-o", obj],
+                                  capture_output=True, text=True)
+
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            logs += pool.map(compile_one, zip(srcs, objs))
+        out = LIB + ".tmp"
+        if all(r.returncode == 0 for r in logs):
+            logs.append(subprocess.run([hipcc(), *HIPCC_FLAGS, *objs, "-o", out], capture_output=True, text=True))
+    failed = [r for r in logs if r.returncode != 0]
+    if failed:
+        raise RuntimeError("hipcc failed:\n" + "".join(r.stdout + r.stderr for r in failed))
     if verbose:
         noise = "is not a recognized feature for this target"
-        print("\n".join(l for l in (res.stdout + res.stderr).splitlines() if noise not in l))
-    os.replace(tmp, LIB)
+        print("\n".join(l for r in logs for l in (r.stdout + r.stderr).splitlines() if noise not in l))
+    os.replace(out, LIB)
     return LIB
 
 

@@ -52,6 +52,12 @@ int fail(int code, const std::string &msg) {
   return code;
 }
 void clear_error() { g_last_error.clear(); }
+int need_device() {
+  int n = 0;
+  if (hipGetDeviceCount(&n) == hipSuccess && n > 0) return EMRS_OK;
+  (void)hipGetLastError();
+  return fail(EMRS_ERR_NO_DEVICE, "no HIP device is visible");
+}
 }  // namespace emrs_internal
 
 namespace {

@@ -1,0 +1,528 @@
+// Newton-Schulz orthogonalisation, and the Muon update around it.
+//
+// X_0 = U / (|U|_F + eps) has singular values in [0, 1]; a step X <- a X + (b A + c A^2) X, A = X X^T, maps
+// each of them by s -> a s + b s^3 + c s^5 and keeps the singular vectors.  With S the shorter side and L the
+// longer, A is S x S, and a step costs three products:
+//   A = X X^T          S S L multiply-adds by half: symmetric, tiles on and below the diagonal are computed
+//   B = b A + c A A    S S S by half, b A in the epilogue
+//   X = a X + B X      S S L, a X in the epilogue
+// Each product wants its summed index contiguous: X [S][L] for the first, X^T [L][S] for the last, so the
+// epilogue of the last writes both.  All live in the workspace, with rows and columns padded to 64 by zeros,
+// which the products keep zero.
+//
+// Operands are fp16: X, A and B are bounded (singular values stay under 1.3 with the usual coefficients), so
+// powers of two keep their entries near 1, and fp16's 11 bits then round 8 times finer than bf16's 8 at the
+// same rate.  A rounding of X is noise over all directions, and directions of small singular values grow by
+// a in each step that follows, noise and all: so X is held as the sum of two fp16 parts (22 bits) in every
+// step but the last two, where the noise has two steps at most to grow.  There a X goes into the polynomial,
+// P = a I + b A + c A^2: near the end P is close to 0.7 I where b A + c A^2 is close to -2.7 I, and has a
+// quarter of its rounding; before, P's rounding on the diagonal would be such noise itself.  An error of A
+// enters by the polynomial's slope, b + 2 c A, of size 0.7 at the end.  Against 64 bits the result is then
+// below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 (4e-2 with one part throughout, 3e-1 with
+// bf16), which is the rounding of the bf16 that it is written in.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "emrs.h"
+#include "gemm.h"
+#include "internal.h"
+
+namespace {
+
+using emrs_gemm::f32x4;
+using emrs_gemm::Product;
+using emrs_gemm::Where;
+using emrs_internal::fail;
+using half = _Float16;
+using half4 = emrs_gemm::Vec<_Float16>::x4;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+
+constexpr float kGramScale = 64.f;  // of A and B: entries of a Gram matrix with spectrum in [0, 1.7]
+constexpr int kSide = 64;
+constexpr int kMaxMatrices = EMRS_MUON_MAX_MATRICES;
+constexpr int kMaxNormBlocks = 512;
+
+template <class P>
+struct Table {
+  P p[kMaxMatrices];
+};
+
+struct Update {  // where the matrix that is orthogonalised comes from
+  Table<const void *> grad;
+  Table<float *> momentum;
+  int64_t grad_stride, momentum_stride;
+  int32_t rows, cols;
+  uint32_t grad_dtype;
+  int32_t has_momentum, nesterov;
+  float mu;
+};
+
+__device__ inline float grad_at(const void *p, uint32_t dtype, int64_t i) {
+  return dtype == EMRS_FP32 ? static_cast<const float *>(p)[i]
+                            : dtype == EMRS_BF16 ? (float)static_cast<const __bf16 *>(p)[i] : (float)static_cast<const half *>(p)[i];
+}
+
+__device__ inline f32x4 grad4_at(const void *p, uint32_t dtype, int64_t i) {
+  if (dtype == EMRS_FP32) return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+  f32x4 v;
+  if (dtype == EMRS_BF16) {
+    const bf16x4 g = *reinterpret_cast<const bf16x4 *>(static_cast<const __bf16 *>(p) + i);
+    for (int r = 0; r < 4; ++r) v[r] = (float)g[r];
+  } else {
+    const half4 g = *reinterpret_cast<const half4 *>(static_cast<const half *>(p) + i);
+    for (int r = 0; r < 4; ++r) v[r] = (float)g[r];
+  }
+  return v;
+}
+
+__device__ inline float block_sum(float v) {
+  __shared__ float part[4];
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return part[0] + part[1] + part[2] + part[3];
+}
+
+// momentum = mu momentum + grad, and each workgroup's share of |update|^2.  Rows go to the workgroups in
+// turn.  No atomics: the sums are the same on every run.
+template <bool kWide>
+__global__ __launch_bounds__(256) void momentum_kernel(Update u, float *norms) {
+  const int b = blockIdx.y;
+  const void *grad = u.grad.p[b];
+  float *buf = u.has_momentum ? u.momentum.p[b] : nullptr;
+  float sum = 0.f;
+  for (int64_t r = blockIdx.x; r < u.rows; r += gridDim.x) {
+    const int64_t g0 = r * u.grad_stride, m0 = r * u.momentum_stride;
+    if (kWide) {
+      for (int c = threadIdx.x * 4; c < u.cols; c += 1024) {
+        f32x4 g = grad4_at(grad, u.grad_dtype, g0 + c);
+        if (buf) {
+          f32x4 m = *reinterpret_cast<const f32x4 *>(buf + m0 + c);
+          m = u.mu * m + g;
+          *reinterpret_cast<f32x4 *>(buf + m0 + c) = m;
+          g = u.nesterov ? g + u.mu * m : m;
+        }
+        for (int i = 0; i < 4; ++i) sum += g[i] * g[i];
+      }
+    } else {
+      for (int c = threadIdx.x; c < u.cols; c += 256) {
+        float g = grad_at(grad, u.grad_dtype, g0 + c);
+        if (buf) {
+          const float m = u.mu * buf[m0 + c] + g;
+          buf[m0 + c] = m;
+          g = u.nesterov ? g + u.mu * m : m;
+        }
+        sum += g * g;
+      }
+    }
+  }
+  sum = block_sum(sum);
+  if (threadIdx.x == 0) norms[b * gridDim.x + blockIdx.x] = sum;
+}
+
+// One orientation of X in the workspace: [rows][stride] fp16, the second part (if any) `low` elements on.
+struct Image {
+  half *p;
+  int64_t stride, batch, low;
+};
+
+// X_0 in both orientations, its two parts, and the padding's zeros.
+__global__ __launch_bounds__(256) void pack_kernel(Update u, const float *norms, int blocks, float eps, float scale, Image straight,
+                                                   Image across, int parts) {
+  __shared__ float tile[kSide][kSide + 1];
+  const int b = blockIdx.z, r0 = blockIdx.y * kSide, c0 = blockIdx.x * kSide;
+  float norm = 0.f;
+  for (int i = threadIdx.x; i < blocks; i += 256) norm += norms[b * blocks + i];
+  norm = sqrtf(block_sum(norm));
+  const float by = scale / (norm + eps);
+  const int x = threadIdx.x % kSide;
+  const void *grad = u.grad.p[b];
+  const float *buf = u.has_momentum ? u.momentum.p[b] : nullptr;
+  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
+    const int r = r0 + y, c = c0 + x;
+    float v = 0.f;
+    if (r < u.rows && c < u.cols) {
+      if (buf) {
+        v = buf[r * u.momentum_stride + c];
+        if (u.nesterov) v = grad_at(grad, u.grad_dtype, r * u.grad_stride + c) + u.mu * v;
+      } else {
+        v = grad_at(grad, u.grad_dtype, r * u.grad_stride + c);
+      }
+      v *= by;
+    }
+    tile[y][x] = v;
+    half *o = straight.p + b * straight.batch + r * straight.stride + c;
+    const half hi = (half)v;
+    o[0] = hi;
+    if (parts > 1) o[straight.low] = (half)(v - (float)hi);
+  }
+  __syncthreads();
+  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
+    const float v = tile[x][y];
+    half *o = across.p + b * across.batch + (c0 + y) * across.stride + r0 + x;
+    const half hi = (half)v;
+    o[0] = hi;
+    if (parts > 1) o[across.low] = (half)(v - (float)hi);
+  }
+}
+
+// The same element on both sides of the diagonal.  A tile on the diagonal computes both itself: with two
+// parts they differ in their sums' order, so each is stored where it belongs and nowhere twice.
+__device__ inline void store_symmetric(half *out, int64_t stride, int m, int n, half4 v, bool mirror) {
+  *reinterpret_cast<half4 *>(out + n * stride + m) = v;
+  if (mirror)
+    for (int r = 0; r < 4; ++r) out[(m + r) * stride + n] = v[r];
+}
+
+struct StoreGram {
+  half *out;
+  int64_t stride, batch;
+  float by;
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+    half *o = out + w.batch * batch;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
+        if (m >= p.m || n >= p.n) continue;
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)(acc[i][j][r] * by);
+        store_symmetric(o, stride, m, n, v, w.m0 != w.n0);
+      }
+  }
+};
+
+// a I + b A + c A A, the polynomial of the steps with one part; without a I (a = 0) of the others.
+struct StorePolynomial {
+  half *out;
+  const half *gram;
+  int64_t stride, batch;
+  float a, b, c;  // a times the scale of A, c over it
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+    half *o = out + w.batch * batch;
+    const half *in = gram + w.batch * batch;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
+        if (m >= p.m || n >= p.n) continue;
+        const half4 x = *reinterpret_cast<const half4 *>(in + n * stride + m);
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)((m + r == n ? a : 0.f) + b * (float)x[r] + c * acc[i][j][r]);
+        store_symmetric(o, stride, m, n, v, w.m0 != w.n0);
+      }
+  }
+};
+
+// The product, plus a X from both its parts where the polynomial is without it.
+__device__ inline f32x4 applied(const half *x, int64_t low, int parts, float a, f32x4 acc) {
+  if (parts == 1) return acc * (1.f / kGramScale);
+  const half4 hi = *reinterpret_cast<const half4 *>(x);
+  const half4 lo = *reinterpret_cast<const half4 *>(x + low);
+  f32x4 v;
+  for (int r = 0; r < 4; ++r) v[r] = a * ((float)hi[r] + (float)lo[r]) + acc[r] * (1.f / kGramScale);
+  return v;
+}
+
+// The next X (m: the longer side), in both orientations.
+struct StoreIterate {
+  Image in, out, across;
+  int32_t in_parts, out_parts;
+  float a;
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+    const half *x = in.p + w.batch * in.batch;
+    half *o = out.p + w.batch * out.batch, *t = across.p + w.batch * across.batch;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
+        if (m >= p.m || n >= p.n) continue;
+        const f32x4 v = applied(x + n * in.stride + m, in.low, in_parts, a, acc[i][j]);
+        half4 hi, lo;
+        for (int r = 0; r < 4; ++r) {
+          hi[r] = (half)v[r];
+          lo[r] = (half)(v[r] - (float)hi[r]);
+        }
+        *reinterpret_cast<half4 *>(o + n * out.stride + m) = hi;
+        for (int r = 0; r < 4; ++r) t[(m + r) * across.stride + n] = hi[r];
+        if (out_parts > 1) {
+          *reinterpret_cast<half4 *>(o + out.low + n * out.stride + m) = lo;
+          for (int r = 0; r < 4; ++r) t[across.low + (m + r) * across.stride + n] = lo[r];
+        }
+      }
+  }
+};
+
+// The last X: the result, or the update of the weights and their bf16 image.  m runs along the caller's rows.
+struct StoreResult {
+  Image in;
+  int32_t in_parts;
+  float a, by;  // by: over the scale of X
+  int32_t rows, cols;
+  Table<void *> out, image;
+  Table<float *> main;
+  int64_t out_stride, image_stride, main_stride;
+  int32_t has_out, has_image, has_main;
+  int32_t wide;
+  float keep, rate;
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &) const {
+    const half *x = in.p + w.batch * in.batch;
+    __bf16 *o = has_out ? static_cast<__bf16 *>(out.p[w.batch]) : nullptr;
+    __bf16 *img = has_image ? static_cast<__bf16 *>(image.p[w.batch]) : nullptr;
+    float *mn = has_main ? main.p[w.batch] : nullptr;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int c = m0 + i * 16 + (lane >> 4) * 4;
+        const int64_t r = n0 + j * 16 + (lane & 15);
+        if (c >= cols || r >= rows) continue;
+        f32x4 v = applied(x + r * in.stride + c, in.low, in_parts, a, acc[i][j]) * by;
+        if (wide) {
+          if (mn) {
+            f32x4 *at = reinterpret_cast<f32x4 *>(mn + r * main_stride + c);
+            v = *at * keep - rate * v;
+            *at = v;
+          }
+          bf16x4 h;
+          for (int k = 0; k < 4; ++k) h[k] = (__bf16)v[k];
+          if (o) *reinterpret_cast<bf16x4 *>(o + r * out_stride + c) = h;
+          if (img) *reinterpret_cast<bf16x4 *>(img + r * image_stride + c) = h;
+          continue;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (c + k >= cols) continue;
+          float u = v[k];
+          if (mn) {
+            float *at = mn + r * main_stride + c + k;
+            u = *at * keep - rate * u;
+            *at = u;
+          }
+          if (o) o[r * out_stride + c + k] = (__bf16)u;
+          if (img) img[r * image_stride + c + k] = (__bf16)u;
+        }
+      }
+  }
+};
+
+struct Sizes {
+  uint64_t s, l;                             // padded sides
+  uint64_t x[2], xt[2], gram, poly, norms, total;  // offsets; x and xt hold both parts of every matrix
+  uint32_t blocks;                           // workgroups of the norm, a matrix
+};
+
+uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+Sizes sizes_of(const emrs_muon *a) {
+  Sizes z{};
+  z.s = round_up(std::min(a->rows, a->cols), kSide);
+  z.l = round_up(std::max(a->rows, a->cols), kSide);
+  z.blocks = (uint32_t)std::min<uint64_t>(a->rows, kMaxNormBlocks);
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  for (int i = 0; i < 2; ++i) z.x[i] = take(2 * a->count * z.s * z.l * 2);
+  for (int i = 0; i < 2; ++i) z.xt[i] = take(2 * a->count * z.s * z.l * 2);
+  z.gram = take(a->count * z.s * z.s * 2);
+  z.poly = take(a->count * z.s * z.s * 2);
+  z.norms = take((uint64_t)a->count * z.blocks * 4);
+  z.total = at;
+  return z;
+}
+
+int check(const emrs_muon *a) {
+  if (!a) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: NULL argument");
+  if (a->count == 0 || a->count > kMaxMatrices) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: 1 to 32 matrices wanted");
+  if (a->grad_dtype > EMRS_FP16) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: gradients are fp32, bf16 or fp16");
+  // Rows of a tile lie within 32-bit byte offsets of each other.
+  if (a->rows == 0 || a->cols == 0 || a->rows > (1u << 20) || a->cols > (1u << 20))
+    return fail(EMRS_ERR_TOO_LARGE, "muon: sides of 1 to 2^20 wanted");
+  if (std::min(a->rows, a->cols) > 32768) return fail(EMRS_ERR_TOO_LARGE, "muon: the shorter side is at most 32768");
+  if (a->steps == 0 || a->steps > EMRS_MUON_MAX_STEPS) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: 1 to 16 steps wanted");
+  return EMRS_OK;
+}
+
+int check_matrices(const emrs_muon *a) {
+  if (!a->coefficients || !a->grad) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: NULL coefficients or gradients");
+  if (!a->out && !a->main) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: neither out nor main is given");
+  if (a->out && a->main) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: out and main exclude each other");
+  if (a->image && !a->main) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: an image needs main");
+  const uint64_t grad_bytes = a->grad_dtype == EMRS_FP32 ? 4 : 2;
+  auto each = [&](const void *const *p, uint64_t stride, uint64_t bytes, const char *what) {
+    if (!p) return (int)EMRS_OK;
+    if (a->rows > 1 && (stride < a->cols || stride > (1ull << 40)))
+      return fail(EMRS_ERR_INVALID_ARGUMENT, std::string("muon: rows of ") + what + " overlap or lie too far apart");
+    for (uint32_t i = 0; i < a->count; ++i) {
+      if (!p[i]) return fail(EMRS_ERR_INVALID_ARGUMENT, std::string("muon: a NULL matrix in ") + what);
+      if (reinterpret_cast<uintptr_t>(p[i]) % bytes)
+        return fail(EMRS_ERR_MISALIGNED, std::string("muon: ") + what + " is off its type's alignment");
+    }
+    return (int)EMRS_OK;
+  };
+  int rc = each(a->grad, a->grad_stride, grad_bytes, "grad");
+  if (!rc) rc = each(reinterpret_cast<const void *const *>(a->momentum), a->momentum_stride, 4, "momentum");
+  if (!rc) rc = each(reinterpret_cast<const void *const *>(a->main), a->main_stride, 4, "main");
+  if (!rc) rc = each(reinterpret_cast<const void *const *>(a->image), a->image_stride, 2, "image");
+  if (!rc) rc = each(reinterpret_cast<const void *const *>(a->out), a->out_stride, 2, "out");
+  return rc;
+}
+
+// Whether groups of four elements of every row lie on their own size.
+bool fours(const emrs_muon *a, const void *const *p, uint64_t stride, uint64_t bytes) {
+  if (!p) return true;
+  if (a->cols % 4 || (a->rows > 1 && stride % 4)) return false;
+  for (uint32_t i = 0; i < a->count; ++i)
+    if (reinterpret_cast<uintptr_t>(p[i]) % (4 * bytes)) return false;
+  return true;
+}
+
+#define TRY(expr)                                                                                   \
+  do {                                                                                              \
+    const hipError_t e_ = (expr);                                                                   \
+    if (e_ != hipSuccess) return fail(EMRS_ERR_HIP, std::string("muon: ") + hipGetErrorString(e_)); \
+  } while (0)
+
+int step(const emrs_muon *a, hipStream_t st) {
+  const Sizes z = sizes_of(a);
+  char *ws = static_cast<char *>(a->workspace);
+  const bool tall = a->rows > a->cols;
+  const uint64_t grad_bytes = a->grad_dtype == EMRS_FP32 ? 4 : 2;
+
+  Update u{};
+  for (uint32_t i = 0; i < a->count; ++i) {
+    u.grad.p[i] = a->grad[i];
+    if (a->momentum) u.momentum.p[i] = a->momentum[i];
+  }
+  u.grad_stride = a->grad_stride, u.momentum_stride = a->momentum_stride;
+  u.rows = (int)a->rows, u.cols = (int)a->cols;
+  u.grad_dtype = a->grad_dtype;
+  u.has_momentum = a->momentum != nullptr, u.nesterov = a->nesterov != 0;
+  u.mu = a->mu;
+  float *norms = reinterpret_cast<float *>(ws + z.norms);
+  const bool wide = fours(a, a->grad, a->grad_stride, grad_bytes) &&
+                    fours(a, reinterpret_cast<const void *const *>(a->momentum), a->momentum_stride, 4);
+  const dim3 grid(z.blocks, a->count);
+  if (wide)
+    momentum_kernel<true><<<grid, 256, 0, st>>>(u, norms);
+  else
+    momentum_kernel<false><<<grid, 256, 0, st>>>(u, norms);
+  TRY(hipGetLastError());
+
+  // Entries of an orthogonal S x L matrix are 1 / sqrt(L): the scale of X brings them to 1.
+  const float scale = std::ldexp(1.f, (int)std::lround(0.5 * std::log2((double)z.l)));
+  auto parts_of = [&](uint32_t k) { return a->steps - k > 2 ? 2 : 1; };
+  const int64_t area = (int64_t)(z.s * z.l), low = (int64_t)a->count * area;
+  auto x = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.x[i]), (int64_t)z.l, area, low}; };
+  auto xt = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.xt[i]), (int64_t)z.s, area, low}; };
+  half *gram = reinterpret_cast<half *>(ws + z.gram), *poly = reinterpret_cast<half *>(ws + z.poly);
+  const int64_t square = (int64_t)(z.s * z.s);
+
+  const dim3 tiles(round_up(a->cols, kSide) / kSide, round_up(a->rows, kSide) / kSide, a->count);
+  pack_kernel<<<tiles, 256, 0, st>>>(u, norms, (int)z.blocks, a->eps, scale, tall ? xt(0) : x(0), tall ? x(0) : xt(0), parts_of(0));
+  TRY(hipGetLastError());
+
+  for (uint32_t k = 0; k < a->steps; ++k) {
+    const float *f = a->coefficients + 3 * k;
+    const int now = k & 1, parts = parts_of(k);
+    const Image in = x(now), in_t = xt(now);
+    Product g{};
+    g.a[0] = g.b[0] = g.a[1] = g.b[2] = in.p;
+    g.b[1] = g.a[2] = in.p + low;
+    g.a_stride = g.b_stride = in.stride, g.a_batch = g.b_batch = area;
+    g.m = g.n = (int)z.s, g.k = (int)z.l;
+    g.parts = parts == 2 ? 3 : 1;
+    g.batch = (int)a->count, g.symmetric = 1;
+    TRY((emrs_gemm::launch<half>(g, StoreGram{gram, (int64_t)z.s, square, kGramScale / (scale * scale)}, st)));
+
+    Product q{};
+    q.a[0] = q.b[0] = gram;
+    q.a_stride = q.b_stride = (int64_t)z.s, q.a_batch = q.b_batch = square;
+    q.m = q.n = q.k = (int)z.s;
+    q.parts = 1, q.batch = (int)a->count, q.symmetric = 1;
+    TRY((emrs_gemm::launch<half>(q, StorePolynomial{poly, gram, (int64_t)z.s, square, parts == 1 ? f[0] * kGramScale : 0.f, f[1], f[2] / kGramScale}, st)));
+
+    Product r{};
+    const bool last = k + 1 == a->steps, turned = last && tall;
+    const half *x_parts[2] = {in_t.p, in_t.p + low};
+    for (int i = 0; i < parts; ++i) {
+      (turned ? r.b : r.a)[i] = x_parts[i];
+      (turned ? r.a : r.b)[i] = poly;
+    }
+    r.a_stride = r.b_stride = (int64_t)z.s;
+    r.a_batch = turned ? square : area, r.b_batch = turned ? area : square;
+    r.m = (int)(turned ? z.s : z.l), r.n = (int)(turned ? z.l : z.s), r.k = (int)z.s;
+    r.parts = parts, r.batch = (int)a->count;
+    if (!last) {
+      TRY((emrs_gemm::launch<half>(r, StoreIterate{in, x(now ^ 1), xt(now ^ 1), parts, parts_of(k + 1), f[0]}, st)));
+      continue;
+    }
+    StoreResult e{};
+    e.in = turned ? in_t : in;
+    e.in_parts = parts, e.a = f[0], e.by = 1.f / scale;
+    e.rows = (int)a->rows, e.cols = (int)a->cols;
+    e.wide = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
+             fours(a, reinterpret_cast<const void *const *>(a->image), a->image_stride, 2) &&
+             fours(a, reinterpret_cast<const void *const *>(a->out), a->out_stride, 2);
+    for (uint32_t i = 0; i < a->count; ++i) {
+      if (a->out) e.out.p[i] = a->out[i];
+      if (a->image) e.image.p[i] = a->image[i];
+      if (a->main) e.main.p[i] = a->main[i];
+    }
+    e.out_stride = a->out_stride, e.image_stride = a->image_stride, e.main_stride = a->main_stride;
+    e.has_out = a->out != nullptr, e.has_image = a->image != nullptr, e.has_main = a->main != nullptr;
+    e.keep = 1.f - a->decay, e.rate = a->rate;
+    TRY((emrs_gemm::launch<half>(r, e, st)));
+  }
+  return EMRS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int emrs_muon_workspace(const emrs_muon *a, uint64_t *bytes) {
+  emrs_internal::clear_error();
+  const int rc = check(a);
+  if (rc) return rc;
+  if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: NULL argument");
+  *bytes = sizes_of(a).total;
+  return EMRS_OK;
+}
+
+int emrs_muon_step(const emrs_muon *a, void *stream) {
+  emrs_internal::clear_error();
+  int rc = check(a);
+  if (!rc) rc = check_matrices(a);
+  if (rc) return rc;
+  const uint64_t want = sizes_of(a).total;
+  if (!a->workspace || a->workspace_bytes < want)
+    return fail(EMRS_ERR_INVALID_ARGUMENT,
+                "muon: the workspace holds " + std::to_string(a->workspace_bytes) + " bytes of " + std::to_string(want));
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(EMRS_ERR_MISALIGNED, "muon: the workspace is off 256 bytes");
+  rc = emrs_internal::need_device();
+  if (rc) return rc;
+  return step(a, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

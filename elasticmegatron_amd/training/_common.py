@@ -1,0 +1,34 @@
+"""What the operators share: types, devices and workspaces."""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _native
+
+DTYPE_CODES = {torch.float32: _native.EMRS_FP32, torch.bfloat16: _native.EMRS_BF16, torch.float16: _native.EMRS_FP16}
+
+
+def dtype_code(t: torch.Tensor, what: str, allowed=tuple(DTYPE_CODES)) -> int:
+    if t.dtype not in allowed:
+        raise TypeError(f"{what} is {t.dtype}: one of {', '.join(str(d) for d in allowed)} is wanted")
+    return DTYPE_CODES[t.dtype]
+
+
+def on_device(what: str, t: torch.Tensor, device: torch.device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} is no tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{what} is on {t.device}: a GPU is wanted")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the others on {device}")
+
+
+def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Scratch of one call.  The caching allocator's blocks lie on 512 bytes, and one that is freed after the
+    call is reused by later work of the same stream only."""
+    return torch.empty(max(1, nbytes), dtype=torch.uint8, device=device)
+
+
+def stream_of(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream

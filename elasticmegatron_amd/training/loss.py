@@ -1,0 +1,184 @@
+"""Cross entropy over a large vocabulary, from hidden states and the output layer's weight.
+
+    x_tv = hidden_t . weight_v,  lse_t = log sum_v exp(x_tv),  loss_t = lse_t - x_t,target_t
+
+over the vocabulary rows v < ``vocab_size``.  The logits are never kept: the forward pass reduces them as
+they are computed, and the backward pass computes them again in pieces of the vocabulary.  The weight is
+one tensor or the consecutive vocabulary shards of tensor parallelism, as a state's bf16 arena holds them;
+rows at and past ``vocab_size`` are the padding of the vocabulary and count nowhere.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from .. import _native
+from ._common import dtype_code, on_device, stream_of, workspace
+
+Weight = Union[torch.Tensor, Sequence[torch.Tensor]]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [n, h] with unit column stride and rows that do not overlap."""
+    n, h = t.shape
+    if (h > 1 and t.stride(1) != 1) or (n > 1 and not h <= t.stride(0) <= 1 << 21):
+        return t.contiguous()
+    return t
+
+
+class _Call:
+    """The checked arguments of one loss, and the record that the native calls take."""
+
+    def __init__(self, hidden, weight, target, vocab_start, vocab_size, ignore_index):
+        shards = [weight] if isinstance(weight, torch.Tensor) else list(weight)
+        if not 1 <= len(shards) <= _native.EMRS_LOSS_MAX_SHARDS:
+            raise ValueError(f"{len(shards)} vocabulary shards: 1 to {_native.EMRS_LOSS_MAX_SHARDS} are wanted")
+        if not isinstance(hidden, torch.Tensor):
+            raise TypeError("hidden is no tensor")
+        self.device = hidden.device
+        on_device("hidden", hidden, self.device)
+        on_device("target", target, self.device)
+        code = dtype_code(hidden, "hidden", (torch.bfloat16, torch.float16))
+        if target.dtype != torch.int64:
+            raise TypeError(f"target is {target.dtype}: torch.int64 is wanted")
+        if hidden.dim() < 1 or target.shape != hidden.shape[:-1]:
+            raise ValueError(f"target {tuple(target.shape)} does not fit hidden {tuple(hidden.shape)}")
+        h = hidden.shape[-1]
+        for i, w in enumerate(shards):
+            on_device(f"weight shard {i}", w, self.device)
+            if w.dtype != hidden.dtype:
+                raise TypeError(f"weight shard {i} is {w.dtype}, hidden {hidden.dtype}")
+            if w.dim() != 2 or w.shape[1] != h:
+                raise ValueError(f"weight shard {i} is {tuple(w.shape)}: [rows, {h}] is wanted")
+        rows = [w.shape[0] for w in shards]
+        if vocab_start < 0:
+            raise ValueError("vocab_start is negative")
+        if vocab_size is None:
+            vocab_size = vocab_start + sum(rows)
+        if vocab_size < 0:
+            raise ValueError("vocab_size is negative")
+        self.hidden = _rows(hidden.detach().reshape(-1, h))
+        self.shards = [_rows(w.detach()) for w in shards]
+        self.target = target.reshape(-1).contiguous()
+        n = len(shards)
+        pointers, strides, counts = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
+        for i, w in enumerate(self.shards):
+            pointers[i], strides[i], counts[i] = w.data_ptr(), w.stride(0), rows[i]
+        self._tables = (pointers, strides, counts)
+        a = self.record = _native.Loss()
+        a.dtype, a.n_shards, a.tokens, a.hidden_size = code, n, self.target.numel(), h
+        a.hidden, a.hidden_stride = self.hidden.data_ptr(), self.hidden.stride(0)
+        a.weights, a.weight_strides, a.shard_rows = (ctypes.addressof(x) for x in self._tables)
+        a.vocab_start, a.vocab_size = vocab_start, vocab_size
+        a.target, a.ignore_index = self.target.data_ptr(), ignore_index
+
+    def forward(self, with_loss: bool) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+        a, t = self.record, self.target.numel()
+        out = torch.empty(3 if with_loss else 2, t, dtype=torch.float32, device=self.device)
+        lse, logit, loss = out[0], out[1], out[2] if with_loss else None
+        if t:
+            a.lse, a.target_logit, a.loss = lse.data_ptr(), logit.data_ptr(), loss.data_ptr() if with_loss else None
+            scratch = workspace(_native.loss_workspace(a, False), self.device)
+            a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
+            with torch.cuda.device(self.device):
+                _native.loss_forward(a, stream_of(self.device))
+        return lse, logit, loss
+
+    def backward(self, lse, grad_loss, want_hidden: bool, want_weights: Sequence[bool]):
+        a = self.record
+        gh = torch.empty(self.hidden.shape, dtype=self.hidden.dtype, device=self.device) if want_hidden else None
+        gw = [torch.empty(w.shape, dtype=w.dtype, device=self.device) if want else None
+              for w, want in zip(self.shards, want_weights)]
+        if not self.target.numel() or not any(w.shape[0] for w in self.shards):  # sums over nothing
+            for g in (gh, *gw):
+                if g is not None:
+                    g.zero_()
+            return gh, gw
+        table = (ctypes.c_uint64 * len(gw))(*(0 if g is None else g.data_ptr() for g in gw))
+        a.lse, a.grad_loss = lse.data_ptr(), grad_loss.data_ptr()
+        a.grad_hidden = None if gh is None else gh.data_ptr()
+        a.grad_weights = ctypes.addressof(table) if any(want_weights) else None
+        scratch = workspace(_native.loss_workspace(a, True), self.device)
+        a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
+        with torch.cuda.device(self.device):
+            _native.loss_backward(a, stream_of(self.device))
+        return gh, gw
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, target, vocab_size, ignore_index, *shards):
+        call = _Call(hidden, shards, target, 0, vocab_size, ignore_index)
+        lse, _, loss = call.forward(True)
+        ctx.save_for_backward(hidden, target, lse, *shards)
+        ctx.rest = (vocab_size, ignore_index)
+        return loss.view(target.shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        hidden, target, lse, *shards = ctx.saved_tensors
+        vocab_size, ignore_index = ctx.rest
+        call = _Call(hidden, shards, target, 0, vocab_size, ignore_index)
+        grad_loss = grad_loss.reshape(-1).to(torch.float32).contiguous()
+        gh, gw = call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
+        return (None if gh is None else gh.view(hidden.shape), None, None, None, *gw)
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, *, vocab_size: Optional[int] = None,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """The loss of every token of ``hidden`` [..., h] (bf16 or fp16) against ``weight`` (one tensor [V, h]
+    or its consecutive vocabulary shards, of the same type) at ``target`` [...] (int64).
+
+    ``vocab_size``: rows of the vocabulary that count; the rows from there on are padding, which may hold
+    anything and gets zero gradients.  ``ignore_index``: tokens of this target have loss 0 and add nothing
+    to any gradient, whatever their hidden state holds.  A target outside the vocabulary has loss inf.
+    ``reduction``: ``"none"`` (fp32, the shape of ``target``), ``"sum"``, or ``"mean"`` over the tokens that
+    count (NaN where none does).  Differentiable once, to ``hidden`` and to every shard.
+    """
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"reduction {reduction!r}: 'none', 'sum' or 'mean' is wanted")
+    shards = [weight] if isinstance(weight, torch.Tensor) else list(weight)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (hidden, *shards)):
+        loss = _LinearCrossEntropy.apply(hidden, target, vocab_size, ignore_index, *shards)
+    else:
+        loss = _Call(hidden, shards, target, 0, vocab_size, ignore_index).forward(True)[2].view(target.shape)
+    if reduction == "none":
+        return loss
+    total = loss.sum()
+    return total if reduction == "sum" else total / (target != ignore_index).sum()
+
+
+def vocab_statistics(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, *, vocab_start: int = 0,
+                     vocab_size: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(lse, target_logit)`` over the vocabulary rows that this process holds, the first of them row
+    ``vocab_start`` of the vocabulary: fp32, the shape of ``target``.  Where the target's row is elsewhere,
+    ``target_logit`` is -inf; where no row counts, so is ``lse``."""
+    lse, logit, _ = _Call(hidden, weight, target, vocab_start, vocab_size, -100).forward(False)
+    return lse.view(target.shape), logit.view(target.shape)
+
+
+def merge_vocab_statistics(lse: torch.Tensor, target_logit: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(lse, target_logit)`` of the whole vocabulary from those of every process, stacked along dim 0.
+    The loss is their difference; the merged ``lse`` is what :func:`vocab_gradients` takes."""
+    return torch.logsumexp(lse, 0), target_logit.amax(0)
+
+
+def vocab_gradients(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor, *,
+                    vocab_start: int = 0, vocab_size: Optional[int] = None,
+                    ignore_index: int = -100) -> Tuple[torch.Tensor, List[torch.Tensor]]:
+    """``(grad_hidden, grad_weights)`` from the rows that this process holds: its share of the gradient to
+    ``hidden`` (the whole is the sum over the processes) and the gradients of its own shards.
+
+    ``lse`` is of the whole vocabulary; ``grad_loss`` is the loss's gradient for each token."""
+    call = _Call(hidden, weight, target, vocab_start, vocab_size, ignore_index)
+    for what, t in (("lse", lse), ("grad_loss", grad_loss)):
+        on_device(what, t, call.device)
+        if t.shape != target.shape:
+            raise ValueError(f"{what} {tuple(t.shape)} does not fit target {tuple(target.shape)}")
+    lse, grad_loss = (t.detach().reshape(-1).to(torch.float32).contiguous() for t in (lse, grad_loss))
+    gh, gw = call.backward(lse, grad_loss, True, [True] * len(call.shards))
+    return gh.view(hidden.shape), gw

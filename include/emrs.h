@@ -447,6 +447,101 @@ int emrs_ipc_close(void *ptr);
 /* Number of allocations this process holds open through emrs_ipc_open. */
 int emrs_ipc_open_count(void);
 
+/* ---- Operators of a training step on resident state ----
+ *
+ * 16-bit operands, sums, softmax statistics and norms in 32 bits.  All memory is the caller's: each
+ * operator says how large a workspace it wants, and overwrites it.  Nothing waits for the device. */
+
+/* element types */
+#define EMRS_FP32 0u
+#define EMRS_BF16 1u
+#define EMRS_FP16 2u
+
+/* Loss of every token from the output layer's weight, without keeping the logits.  With x = hidden[t] . w[v]
+ * over the vocabulary rows v < vocab_size of all shards:
+ *   lse[t] = log sum_v exp(x), target_logit[t] = x at v = target[t], loss[t] = lse[t] - target_logit[t],
+ * 0 where target[t] == ignore_index.  A target in none of these rows has target_logit -inf and loss +inf.
+ * Backward: d = grad_loss[t] (exp(x - lse[t]) - [v == target[t]]), 0 for ignored tokens;
+ *   grad_hidden[t] = sum_v d w[v], grad_weights[v] = sum_t d hidden[t]; rows >= vocab_size get zeros.
+ * The hidden states of ignored tokens and the rows >= vocab_size may hold anything, NaN included. */
+typedef struct emrs_loss {
+  uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16: hidden, weights and their gradients */
+  uint32_t n_shards;              /* consecutive vocabulary shards, 1 to EMRS_LOSS_MAX_SHARDS */
+  uint64_t tokens;                /* may be 0 */
+  uint64_t hidden_size;           /* >= 1 */
+  const void *hidden;             /* [tokens][hidden_size], rows hidden_stride elements apart */
+  uint64_t hidden_stride;
+  const void *const *weights;     /* per shard [shard_rows][hidden_size] */
+  const uint64_t *weight_strides;
+  const uint64_t *shard_rows;
+  uint64_t vocab_start;           /* vocabulary index of the first shard's first row */
+  uint64_t vocab_size;
+  const int64_t *target;          /* [tokens] */
+  int64_t ignore_index;
+  float *lse;                     /* [tokens]: written by forward, read by backward */
+  float *target_logit;            /* [tokens]: forward */
+  float *loss;                    /* [tokens]: forward; may be NULL */
+  const float *grad_loss;         /* [tokens]: backward */
+  void *grad_hidden;              /* [tokens][hidden_size], contiguous; may be NULL */
+  void *const *grad_weights;      /* per shard, contiguous; NULL or entries NULL: not wanted */
+  void *workspace;                /* 256-byte aligned */
+  uint64_t workspace_bytes;
+} emrs_loss;
+
+#define EMRS_LOSS_MAX_SHARDS 64u
+
+/* Bytes of workspace that emrs_loss_forward (backward = 0) or emrs_loss_backward (1) wants. */
+int emrs_loss_workspace(const emrs_loss *loss, int backward, uint64_t *bytes);
+int emrs_loss_forward(const emrs_loss *loss, void *stream);
+int emrs_loss_backward(const emrs_loss *loss, void *stream);
+
+/* Newton-Schulz orthogonalisation of `count` matrices of one shape, alone or as the Muon update.
+ *   update = grad                                             (momentum == NULL)
+ *   momentum = mu momentum + grad, update = grad + mu momentum (nesterov) or momentum
+ *   X = update / (|update|_F + eps); per step with its (a, b, c): A = X X^T, X = a X + (b A + c A A) X
+ *   out = X                                                   (out != NULL, bf16)
+ *   main = main (1 - decay) - rate X, image = main as bf16    (main != NULL)
+ * Matrices are row-major with unit column stride; *_stride: elements between rows. */
+typedef struct emrs_muon {
+  uint32_t count;                 /* 1 to EMRS_MUON_MAX_MATRICES */
+  uint32_t grad_dtype;            /* EMRS_FP32, EMRS_BF16 or EMRS_FP16 */
+  uint64_t rows, cols;            /* >= 1 */
+  const void *const *grad;
+  float *const *momentum;
+  float *const *main;
+  void *const *image;             /* bf16; NULL: none */
+  void *const *out;               /* bf16 */
+  uint64_t grad_stride, momentum_stride, main_stride, image_stride, out_stride;
+  uint32_t steps;                 /* 1 to EMRS_MUON_MAX_STEPS */
+  uint32_t nesterov;
+  const float *coefficients;      /* steps x (a, b, c) */
+  float mu, eps, decay, rate;
+  void *workspace;                /* 256-byte aligned */
+  uint64_t workspace_bytes;
+} emrs_muon;
+
+#define EMRS_MUON_MAX_MATRICES 32u
+#define EMRS_MUON_MAX_STEPS 16u
+
+int emrs_muon_workspace(const emrs_muon *muon, uint64_t *bytes);
+int emrs_muon_step(const emrs_muon *muon, void *stream);
+
+/* AdamW on n elements, in place:
+ *   exp_avg = beta1 exp_avg + (1 - beta1) g, exp_avg_sq = beta2 exp_avg_sq + (1 - beta2) g g
+ *   main = main (1 - lr weight_decay) - lr (exp_avg / (1 - beta1^step)) / (sqrt(exp_avg_sq / (1 - beta2^step)) + eps)
+ *   image = main as bf16 (image != NULL) */
+typedef struct emrs_adamw {
+  uint64_t n;
+  float *main, *exp_avg, *exp_avg_sq;
+  const void *grad;
+  uint32_t grad_dtype;            /* EMRS_FP32, EMRS_BF16 or EMRS_FP16 */
+  uint32_t step;                  /* >= 1 */
+  void *image;
+  double lr, beta1, beta2, eps, weight_decay;
+} emrs_adamw;
+
+int emrs_adamw_step(const emrs_adamw *adamw, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
