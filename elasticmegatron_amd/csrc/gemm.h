@@ -48,18 +48,19 @@ constexpr int kStage = 64;  // k of one LDS stage: rows of 128 bytes
 constexpr int kXcds = 8;
 constexpr int kGroup = 8;   // tiles of m that are walked before the next n: what one XCD's CUs share
 
-// Up to three products that are summed into one C: operands that are held as a sum of two 16-bit parts
-// multiply as hi*hi + hi*lo + lo*hi, which is only more k.
+// An operand that is held as a sum of two 16-bit parts has them side by side in its rows, hi | lo, and
+// multiplies as hi hi + hi lo + lo hi, which is only more k: the operand's own k starts again where k
+// reaches its wrap.
 struct Product {
-  const void *a[3];
-  const void *b[3];
+  const void *a, *b;
   int64_t a_stride, b_stride;      // elements between rows, multiples of 8
   int64_t a_batch, b_batch;        // elements between the matrices of a batch
-  int32_t m, n, k;                 // k a multiple of 8
-  int32_t parts;                   // 1 to 3
+  int32_t m, n, k;                 // k a multiple of 8, and of 64 where an operand wraps
+  int32_t a_wrap, b_wrap;          // multiples of 64; kNoWrap
   int32_t batch;
   int32_t symmetric;               // only tiles on and below the diagonal (m >= n) are computed
 };
+constexpr int32_t kNoWrap = 0x7fffffff;
 
 template <int BM_, int BN_, int WM_, int WN_>
 struct Tile {
@@ -122,39 +123,66 @@ __device__ inline Where tile_of(const Product &p) {
 // Of the row's place among 16 alone, so that a wave reads its fragments at constant offsets of one address.
 __device__ inline int swizzle(int row) { return (row ^ ((row >> 3) & 1)) & 7; }
 
-template <class T, int LOADS, int WAVES>
+// What a lane loads of an operand's stage: the same 16 bytes of row `lane / 8` of each of its wave's groups
+// of eight rows, which lie a constant apart.
+template <int WAVES>
 struct Loader {
-  int voffset[LOADS];
-  int unit;  // the 16-byte unit of a row that this lane loads, per load: alternates with the row group
-  __device__ void init(int64_t stride, int wave, int lane) {
-    for (int j = 0; j < LOADS; ++j) {
-      const int row = (wave + j * WAVES) * 8 + (lane >> 3);
-      voffset[j] = (int)(row * stride * 2) + (((lane & 7) ^ swizzle(row)) << 4);
-    }
+  int voffset;
+  int unit;  // first k, within a stage, of the 16 bytes
+  int apart; // bytes from a wave's group of rows to its next
+  __device__ __forceinline__ void init(int64_t stride, int wave, int lane) {
+    static_assert(WAVES % 2 == 0, "a wave's groups of eight rows are all even or all odd");
+    const int row = wave * 8 + (lane >> 3), c = (lane & 7) ^ swizzle(row);
+    unit = c * 8;
+    voffset = (int)(row * stride * 2) + (c << 4);
+    apart = (int)(WAVES * 8 * stride * 2);
   }
-  // k0: first k of the stage; tail: k that are left from there, when fewer than a stage.
-  __device__ void load(__amdgpu_buffer_rsrc_t r, char *lds, int k0, int k, int wave, int lane) const {
-    for (int j = 0; j < LOADS; ++j) {
-      const int group = wave + j * WAVES;
-      int v = voffset[j];
-      if (k - k0 < kStage) {
-        const int c = (lane & 7) ^ swizzle(group * 8 + (lane >> 3));
-        v = c * 8 < k - k0 ? v : (int)0x80000000;  // past the buffer's end: reads zeros
-      }
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + group * 1024), 16, v,
-                                               k0 * 2, 0, 0);
-    }
+  // Fewer than a stage's k are left: lanes whose 16 bytes are past them go past the buffer's end instead.
+  __device__ __forceinline__ void cut(int left) { voffset = unit < left ? voffset : (int)0x80000000; }
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char *lds, int j, int k0, int wave) const {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * WAVES) * 1024), 16,
+                                             voffset, j * apart + k0 * 2, 0, 0);
   }
 };
 
 // The buffer that holds a tile's rows of one operand: nothing past its last row's last k is read.
 template <class T>
-__device__ inline __amdgpu_buffer_rsrc_t rows_buffer(const void *base, int64_t batch, int64_t first, int rows, int64_t stride,
-                                                     int k) {
-  const T *p = static_cast<const T *>(base) + batch + first * stride;
-  const int64_t bytes = ((int64_t)(rows - 1) * stride + k) * 2;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, (int)bytes, 0x00020000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const T *base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, 0x00020000);
 }
+
+// This wave's loads into LDS have landed and its LDS reads are in registers, and so are every other wave's:
+// a barrier alone waits for neither.
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The loads of one stage, to be started one by one.
+template <class Cfg>
+struct Loads {
+  static constexpr int kCount = Cfg::A_LOADS + Cfg::B_LOADS;
+  const Loader<Cfg::WAVES> &loader_a;
+  const Loader<Cfg::WAVES> &loader_b;
+  __amdgpu_buffer_rsrc_t a_rows, b_rows;
+  char *a, *b;
+  int a_k, b_k, wave;
+  __device__ __forceinline__ void operator()(int q) const {
+    if (q < Cfg::A_LOADS)
+      loader_a.load(a_rows, a, q, a_k, wave);
+    else
+      loader_b.load(b_rows, b, q - Cfg::A_LOADS, b_k, wave);
+  }
+};
+
+struct NoLoads {
+  static constexpr int kCount = 0;
+  __device__ void operator()(int) const {}
+};
 
 template <class T, class Cfg, class Epilogue>
 __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilogue epilogue) {
@@ -167,21 +195,33 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
 
-  Loader<T, Cfg::A_LOADS, Cfg::WAVES> la;
-  Loader<T, Cfg::B_LOADS, Cfg::WAVES> lb;
+  Loader<Cfg::WAVES> la, lb;
   la.init(p.a_stride, wave, lane);
   lb.init(p.b_stride, wave, lane);
-  const int a_rows = min(Cfg::BM, p.m - w.m0), b_rows = min(Cfg::BN, p.n - w.n0);
-  const int stages = (p.k + kStage - 1) / kStage, total = stages * p.parts;
-  int part = 0, stage = 0;
-  auto load = [&](char *a, char *b) {
-    const int k0 = stage * kStage;
-    la.load(rows_buffer<T>(p.a[part], w.batch * p.a_batch, w.m0, a_rows, p.a_stride, p.k), a, k0, p.k, wave, lane);
-    lb.load(rows_buffer<T>(p.b[part], w.batch * p.b_batch, w.n0, b_rows, p.b_stride, p.k), b, k0, p.k, wave, lane);
-    if (++stage == stages) {
-      stage = 0;
-      ++part;
-    }
+  auto bytes = [&](int rows, int64_t stride, int wrap) {
+    const int columns = p.k <= wrap ? p.k : max(wrap, p.k - wrap);
+    return (int)(((rows - 1) * stride + columns) * 2);
+  };
+  const int a_bytes = bytes(min(Cfg::BM, p.m - w.m0), p.a_stride, p.a_wrap);
+  const int b_bytes = bytes(min(Cfg::BN, p.n - w.n0), p.b_stride, p.b_wrap);
+  const T *const a_base = static_cast<const T *>(p.a) + w.batch * p.a_batch + w.m0 * p.a_stride;
+  const T *const b_base = static_cast<const T *>(p.b) + w.batch * p.b_batch + w.n0 * p.b_stride;
+  const int total = (p.k + kStage - 1) / kStage;
+  int k0 = 0;
+  // The next stage's loads; past the last stage they read zeros.
+  auto next_stage = [&](char *a, char *b) __attribute__((always_inline)) {
+    const int left = p.k - k0;
+    const bool any = left > 0;
+    const Loads<Cfg> n{la, lb, rows_buffer<T>(a_base, any ? a_bytes : 0), rows_buffer<T>(b_base, any ? b_bytes : 0), a, b,
+                       k0 >= p.a_wrap ? k0 - p.a_wrap : k0, k0 >= p.b_wrap ? k0 - p.b_wrap : k0, wave};
+    k0 += kStage;
+    if (any && left < kStage) la.cut(left), lb.cut(left);
+    return n;
+  };
+  auto load = [&](char *a, char *b) __attribute__((always_inline)) {
+    const Loads<Cfg> n = next_stage(a, b);
+#pragma unroll
+    for (int q = 0; q < Loads<Cfg>::kCount; ++q) n(q);
   };
 
   f32x4 acc[Cfg::MI][Cfg::NI];
@@ -193,36 +233,53 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   const int row = lane & 15, c = lane >> 4;
   const int unit[2] = {(c ^ swizzle(row)) << 4, ((4 + c) ^ swizzle(row)) << 4};
   const int a_at = (wm * Cfg::WM + row) * 128, b_at = (wn * Cfg::WN + row) * 128;
-  auto compute = [&](const char *a, const char *b) {
+  struct Fragments {
+    x8 a[Cfg::MI], b[Cfg::NI];
+  } even, odd;  // of the first and the second 32 k of a stage
+  auto read_one = [&](Fragments &f, const char *a, const char *b, int kk, int r) __attribute__((always_inline)) {
+    if (r < Cfg::NI)
+      f.b[r] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + r * 2048);
+    else
+      f.a[r - Cfg::NI] = *reinterpret_cast<const x8 *>(a + a_at + unit[kk] + (r - Cfg::NI) * 2048);
+  };
+  // 32 k of a stage: multiplies `now` while it reads `next`, and starts the loads of another stage.  Pinned in
+  // this order: LDS reads in the shadow of every second or third matrix instruction, done well before the
+  // end, and the loads spread over all of them, at the rate at which the CU can take them.
+  auto half = [&](const Fragments &now, Fragments &next, const char *a, const char *b, int kk, auto start) __attribute__((always_inline)) {
+    constexpr int products = Cfg::MI * Cfg::NI, reads = Cfg::MI + Cfg::NI, loads = decltype(start)::kCount;
+    constexpr int per = products * 3 / 4 / reads > 0 ? products * 3 / 4 / reads : 1;
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      x8 fa[Cfg::MI], fb[Cfg::NI];
+    for (int q = 0; q < products; ++q) {
+      acc[q / Cfg::NI][q % Cfg::NI] = mfma(now.a[q / Cfg::NI], now.b[q % Cfg::NI], acc[q / Cfg::NI][q % Cfg::NI]);
+      if (q % per == 0 && q / per < reads) read_one(next, a, b, kk, q / per);
 #pragma unroll
-      for (int j = 0; j < Cfg::NI; ++j) fb[j] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + j * 2048);
-#pragma unroll
-      for (int i = 0; i < Cfg::MI; ++i) fa[i] = *reinterpret_cast<const x8 *>(a + a_at + unit[kk] + i * 2048);
-#pragma unroll
-      for (int i = 0; i < Cfg::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < Cfg::NI; ++j) acc[i][j] = mfma(fa[i], fb[j], acc[i][j]);
+      for (int l = (q * loads + products - 1) / products; l < ((q + 1) * loads + products - 1) / products; ++l) start(l);
       __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int r = (products + per - 1) / per; r < reads; ++r) read_one(next, a, b, kk, r);
+  };
+  // A stage.  Its first fragments are in registers: the second ones are read while the first multiply.  Then
+  // every wave has read all of it, and the next stage has arrived: the loads of the one after that go into
+  // its place, and the next stage's first fragments are read while the second ones multiply.
+  auto stage = [&](char *a, char *b, const char *a_next, const char *b_next) __attribute__((always_inline)) {
+    half(even, odd, a, b, 1, NoLoads{});
+    arrive();
+    half(odd, even, a_next, b_next, 0, next_stage(a, b));
   };
 
   load(a_even, b_even);
+  load(a_odd, b_odd);
+  arrive();
+#pragma unroll
+  for (int r = 0; r < Cfg::MI + Cfg::NI; ++r) read_one(even, a_even, b_even, 0, r);
   int it = 0;
   for (; it + 1 < total; it += 2) {
-    __syncthreads();  // the even stage is filled, and every wave is done with the odd one
-    load(a_odd, b_odd);
-    compute(a_even, b_even);
-    __syncthreads();
-    if (it + 2 < total) load(a_even, b_even);
-    compute(a_odd, b_odd);
+    stage(a_even, b_even, a_odd, b_odd);
+    stage(a_odd, b_odd, a_even, b_even);
   }
-  if (it < total) {
-    __syncthreads();
-    compute(a_even, b_even);
-  }
+  if (it < total) stage(a_even, b_even, a_odd, b_odd);
+  arrive();  // no load may still be on its way into LDS that another workgroup gets
   epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p);
 }
 
@@ -233,17 +290,17 @@ inline Shape shape_of(const Product &p) {
   return tile_count<Large>(p) >= 192 ? kLarge : tile_count<Medium>(p) >= 128 ? kMedium : kSmall;
 }
 
+template <class T, class Cfg, class Epilogue>
+void launch_as(const Product &p, const Epilogue &e, hipStream_t stream) {
+  product_kernel<T, Cfg><<<(uint32_t)tile_count<Cfg>(p), Cfg::THREADS, 0, stream>>>(p, e);
+}
+
 template <class T, class Epilogue>
 hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
   switch (shape_of(p)) {
-    case kLarge:
-      product_kernel<T, Large, Epilogue><<<(uint32_t)tile_count<Large>(p), Large::THREADS, 0, stream>>>(p, e);
-      break;
-    case kMedium:
-      product_kernel<T, Medium, Epilogue><<<(uint32_t)tile_count<Medium>(p), Medium::THREADS, 0, stream>>>(p, e);
-      break;
-    case kSmall:
-      product_kernel<T, Small, Epilogue><<<(uint32_t)tile_count<Small>(p), Small::THREADS, 0, stream>>>(p, e);
+    case kLarge: launch_as<T, Large>(p, e, stream); break;
+    case kMedium: launch_as<T, Medium>(p, e, stream); break;
+    case kSmall: launch_as<T, Small>(p, e, stream); break;
   }
   return hipGetLastError();
 }

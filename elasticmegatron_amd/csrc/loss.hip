@@ -50,30 +50,41 @@ struct TileStatistics {
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int wm, int lane, const Product &p) const {
     const int64_t slot = (int64_t)(w.m0 / Cfg::BM) * Cfg::WAVES_M + wm;
     const int m = m0 + (lane >> 4) * 4;
+    if (m0 + Cfg::WM > valid) {
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m + i * 16 + r >= valid)
+#pragma unroll
+            for (int j = 0; j < Cfg::NI; ++j) acc[i][j][r] = -INFINITY;
+    }
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int t = n0 + j * 16 + (lane & 15);
       const bool in = t < p.n;
-      const int64_t at = in ? target[t] - first : -1;
-      float top = -INFINITY;
+      const int64_t at = (in ? target[t] : -1) - first - m;  // among this lane's rows: 16 i + r
+      if (__any(at >= 0 && at < Cfg::WM && at % 16 < 4)) {
+#pragma unroll
+        for (int i = 0; i < Cfg::MI; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (in && at == i * 16 + r && m + i * 16 + r < valid) target_logit[t] = acc[i][j][r];
+      }
+      float top = acc[0][j][0];
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int v = m + i * 16 + r;
-          if (v >= valid) acc[i][j][r] = -INFINITY;
-          top = fmaxf(top, acc[i][j][r]);
-          if (v < valid && v == at) target_logit[t] = acc[i][j][r];
-        }
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
       // No row that counts: the exponentials below are then of -inf, 0.  fmaxf drops NaN; the sum has it.
-      const float shift = top == -INFINITY ? 0.f : top;
+      const float shift = top == -INFINITY ? 0.f : top * kLog2e;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum += exp_of(acc[i][j][r] - shift);
+        for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -shift));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (in && lane < 16) pairs[slot * p.n + t] = float2{top, sum};
@@ -349,21 +360,22 @@ int piece_operands(const emrs_loss *a, const Sizes &s, uint32_t shard, uint64_t 
   char *ws = static_cast<char *>(a->workspace);
   const T *w = static_cast<const T *>(a->weights[shard]) + lo * a->weight_strides[shard];
   *p = Product{};
-  p->b[0] = s.pad_hidden ? ws + s.hidden : a->hidden;
+  p->b = s.pad_hidden ? ws + s.hidden : a->hidden;
   p->b_stride = s.pad_hidden ? s.k : a->tokens > 1 ? a->hidden_stride : s.k;
-  p->a[0] = w;
+  p->a = w;
   p->a_stride = a->shard_rows[shard] > 1 ? a->weight_strides[shard] : s.k;
   if (s.pad_weight) {
     pad_kernel<T><<<dim3(rows, (s.k + 255) / 256), 256, 0, st>>>(w, a->weight_strides[shard], a->hidden_size,
                                                                  reinterpret_cast<T *>(ws + s.weight), s.k);
     TRY(hipGetLastError());
-    p->a[0] = ws + s.weight;
+    p->a = ws + s.weight;
     p->a_stride = s.k;
   }
   p->m = rows;
   p->n = a->tokens;
   p->k = s.k;
-  p->parts = p->batch = 1;
+  p->batch = 1;
+  p->a_wrap = p->b_wrap = emrs_gemm::kNoWrap;
   return EMRS_OK;
 }
 
@@ -457,10 +469,11 @@ int backward(const emrs_loss *a, hipStream_t st) {
                           a->hidden_size, wt, padded, nullptr, 0, st);
         if (rc) return rc;
         Product q{};
-        q.a[0] = wt, q.b[0] = d;
+        q.a = wt, q.b = d;
         q.a_stride = q.b_stride = padded;
         q.m = a->hidden_size, q.n = a->tokens, q.k = padded;
-        q.parts = q.batch = 1;
+        q.batch = 1;
+        q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
         const StoreRows<T> out{left ? nullptr : static_cast<T *>(a->grad_hidden), left || begun ? sum : nullptr, begun,
                                (int64_t)a->hidden_size, wide && reinterpret_cast<uintptr_t>(a->grad_hidden) % 8 == 0, scale};
         TRY((emrs_gemm::launch<T>(q, out, st)));
@@ -468,10 +481,11 @@ int backward(const emrs_loss *a, hipStream_t st) {
       }
       if (gw) {
         Product q{};
-        q.a[0] = ht, q.b[0] = dt;
+        q.a = ht, q.b = dt;
         q.a_stride = q.b_stride = s.tokens_padded;
         q.m = a->hidden_size, q.n = rows, q.k = s.tokens_padded;
-        q.parts = q.batch = 1;
+        q.batch = 1;
+        q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
         const StoreRows<T> out{gw + lo * a->hidden_size, nullptr, 0, (int64_t)a->hidden_size,
                                wide && reinterpret_cast<uintptr_t>(gw) % 8 == 0, scale};
         TRY((emrs_gemm::launch<T>(q, out, st)));

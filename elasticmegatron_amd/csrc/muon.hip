@@ -126,7 +126,8 @@ __global__ __launch_bounds__(256) void momentum_kernel(Update u, float *norms) {
   if (threadIdx.x == 0) norms[b * gridDim.x + blockIdx.x] = sum;
 }
 
-// One orientation of X in the workspace: [rows][stride] fp16, the second part (if any) `low` elements on.
+// One orientation of X in the workspace: [rows][stride] fp16, the second part (if any) `low` elements on in
+// the same row.
 struct Image {
   half *p;
   int64_t stride, batch, low;
@@ -268,7 +269,9 @@ struct StoreIterate {
   }
 };
 
-// The last X: the result, or the update of the weights and their bf16 image.  m runs along the caller's rows.
+// The last X: the result, or the update of the weights and their bf16 image.  m runs along the caller's rows,
+// which are written four elements at a time where they lie so (kWide).
+template <bool kWide>
 struct StoreResult {
   Image in;
   int32_t in_parts;
@@ -278,7 +281,6 @@ struct StoreResult {
   Table<float *> main;
   int64_t out_stride, image_stride, main_stride;
   int32_t has_out, has_image, has_main;
-  int32_t wide;
   float keep, rate;
 
   template <class Cfg>
@@ -288,14 +290,15 @@ struct StoreResult {
     __bf16 *img = has_image ? static_cast<__bf16 *>(image.p[w.batch]) : nullptr;
     float *mn = has_main ? main.p[w.batch] : nullptr;
 #pragma unroll
-    for (int j = 0; j < Cfg::NI; ++j)
+    for (int j = 0; j < Cfg::NI; ++j) {
+      __builtin_amdgcn_sched_barrier(0);  // the loads of one column at a time: registers
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int c = m0 + i * 16 + (lane >> 4) * 4;
         const int64_t r = n0 + j * 16 + (lane & 15);
         if (c >= cols || r >= rows) continue;
         f32x4 v = applied(x + r * in.stride + c, in.low, in_parts, a, acc[i][j]) * by;
-        if (wide) {
+        if (kWide) {
           if (mn) {
             f32x4 *at = reinterpret_cast<f32x4 *>(mn + r * main_stride + c);
             v = *at * keep - rate * v;
@@ -320,6 +323,7 @@ struct StoreResult {
           if (img) img[r * image_stride + c + k] = (__bf16)u;
         }
       }
+    }
   }
 };
 
@@ -403,6 +407,23 @@ bool fours(const emrs_muon *a, const void *const *p, uint64_t stride, uint64_t b
     if (e_ != hipSuccess) return fail(EMRS_ERR_HIP, std::string("muon: ") + hipGetErrorString(e_)); \
   } while (0)
 
+template <bool kWide>
+StoreResult<kWide> result(const emrs_muon *a, const Image &in, int parts, float factor, float scale) {
+  StoreResult<kWide> e{};
+  e.in = in, e.in_parts = parts;
+  e.a = factor, e.by = 1.f / scale;
+  e.rows = (int)a->rows, e.cols = (int)a->cols;
+  for (uint32_t i = 0; i < a->count; ++i) {
+    if (a->out) e.out.p[i] = a->out[i];
+    if (a->image) e.image.p[i] = a->image[i];
+    if (a->main) e.main.p[i] = a->main[i];
+  }
+  e.out_stride = a->out_stride, e.image_stride = a->image_stride, e.main_stride = a->main_stride;
+  e.has_out = a->out != nullptr, e.has_image = a->image != nullptr, e.has_main = a->main != nullptr;
+  e.keep = 1.f - a->decay, e.rate = a->rate;
+  return e;
+}
+
 int step(const emrs_muon *a, hipStream_t st) {
   const Sizes z = sizes_of(a);
   char *ws = static_cast<char *>(a->workspace);
@@ -432,9 +453,9 @@ int step(const emrs_muon *a, hipStream_t st) {
   // Entries of an orthogonal S x L matrix are 1 / sqrt(L): the scale of X brings them to 1.
   const float scale = std::ldexp(1.f, (int)std::lround(0.5 * std::log2((double)z.l)));
   auto parts_of = [&](uint32_t k) { return a->steps - k > 2 ? 2 : 1; };
-  const int64_t area = (int64_t)(z.s * z.l), low = (int64_t)a->count * area;
-  auto x = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.x[i]), (int64_t)z.l, area, low}; };
-  auto xt = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.xt[i]), (int64_t)z.s, area, low}; };
+  const int64_t area = 2 * (int64_t)(z.s * z.l);
+  auto x = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.x[i]), 2 * (int64_t)z.l, area, (int64_t)z.l}; };
+  auto xt = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.xt[i]), 2 * (int64_t)z.s, area, (int64_t)z.s}; };
   half *gram = reinterpret_cast<half *>(ws + z.gram), *poly = reinterpret_cast<half *>(ws + z.poly);
   const int64_t square = (int64_t)(z.s * z.s);
 
@@ -447,52 +468,43 @@ int step(const emrs_muon *a, hipStream_t st) {
     const int now = k & 1, parts = parts_of(k);
     const Image in = x(now), in_t = xt(now);
     Product g{};
-    g.a[0] = g.b[0] = g.a[1] = g.b[2] = in.p;
-    g.b[1] = g.a[2] = in.p + low;
+    g.a = g.b = in.p;
     g.a_stride = g.b_stride = in.stride, g.a_batch = g.b_batch = area;
-    g.m = g.n = (int)z.s, g.k = (int)z.l;
-    g.parts = parts == 2 ? 3 : 1;
+    g.m = g.n = (int)z.s, g.k = (int)z.l * (parts == 2 ? 3 : 1);
+    // hi hi + hi lo + lo hi
+    g.a_wrap = parts == 2 ? (int)z.l : emrs_gemm::kNoWrap, g.b_wrap = parts == 2 ? 2 * (int)z.l : emrs_gemm::kNoWrap;
     g.batch = (int)a->count, g.symmetric = 1;
     TRY((emrs_gemm::launch<half>(g, StoreGram{gram, (int64_t)z.s, square, kGramScale / (scale * scale)}, st)));
 
     Product q{};
-    q.a[0] = q.b[0] = gram;
+    q.a = q.b = gram;
     q.a_stride = q.b_stride = (int64_t)z.s, q.a_batch = q.b_batch = square;
     q.m = q.n = q.k = (int)z.s;
-    q.parts = 1, q.batch = (int)a->count, q.symmetric = 1;
+    q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
+    q.batch = (int)a->count, q.symmetric = 1;
     TRY((emrs_gemm::launch<half>(q, StorePolynomial{poly, gram, (int64_t)z.s, square, parts == 1 ? f[0] * kGramScale : 0.f, f[1], f[2] / kGramScale}, st)));
 
     Product r{};
     const bool last = k + 1 == a->steps, turned = last && tall;
-    const half *x_parts[2] = {in_t.p, in_t.p + low};
-    for (int i = 0; i < parts; ++i) {
-      (turned ? r.b : r.a)[i] = x_parts[i];
-      (turned ? r.a : r.b)[i] = poly;
-    }
-    r.a_stride = r.b_stride = (int64_t)z.s;
+    // P hi + P lo
+    const int32_t wrap = parts == 2 ? (int)z.s : emrs_gemm::kNoWrap;
+    r.a = turned ? poly : in_t.p, r.b = turned ? in_t.p : poly;
+    r.a_stride = turned ? (int64_t)z.s : in_t.stride, r.b_stride = turned ? in_t.stride : (int64_t)z.s;
     r.a_batch = turned ? square : area, r.b_batch = turned ? area : square;
-    r.m = (int)(turned ? z.s : z.l), r.n = (int)(turned ? z.l : z.s), r.k = (int)z.s;
-    r.parts = parts, r.batch = (int)a->count;
+    r.a_wrap = turned ? wrap : emrs_gemm::kNoWrap, r.b_wrap = turned ? emrs_gemm::kNoWrap : wrap;
+    r.m = (int)(turned ? z.s : z.l), r.n = (int)(turned ? z.l : z.s), r.k = (int)z.s * parts;
+    r.batch = (int)a->count;
     if (!last) {
       TRY((emrs_gemm::launch<half>(r, StoreIterate{in, x(now ^ 1), xt(now ^ 1), parts, parts_of(k + 1), f[0]}, st)));
       continue;
     }
-    StoreResult e{};
-    e.in = turned ? in_t : in;
-    e.in_parts = parts, e.a = f[0], e.by = 1.f / scale;
-    e.rows = (int)a->rows, e.cols = (int)a->cols;
-    e.wide = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
-             fours(a, reinterpret_cast<const void *const *>(a->image), a->image_stride, 2) &&
-             fours(a, reinterpret_cast<const void *const *>(a->out), a->out_stride, 2);
-    for (uint32_t i = 0; i < a->count; ++i) {
-      if (a->out) e.out.p[i] = a->out[i];
-      if (a->image) e.image.p[i] = a->image[i];
-      if (a->main) e.main.p[i] = a->main[i];
-    }
-    e.out_stride = a->out_stride, e.image_stride = a->image_stride, e.main_stride = a->main_stride;
-    e.has_out = a->out != nullptr, e.has_image = a->image != nullptr, e.has_main = a->main != nullptr;
-    e.keep = 1.f - a->decay, e.rate = a->rate;
-    TRY((emrs_gemm::launch<half>(r, e, st)));
+    const bool wide_rows = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
+                           fours(a, reinterpret_cast<const void *const *>(a->image), a->image_stride, 2) &&
+                           fours(a, reinterpret_cast<const void *const *>(a->out), a->out_stride, 2);
+    const Image &from = turned ? in_t : in;
+    const hipError_t e = wide_rows ? emrs_gemm::launch<half>(r, result<true>(a, from, parts, f[0], scale), st)
+                                   : emrs_gemm::launch<half>(r, result<false>(a, from, parts, f[0], scale), st);
+    TRY(e);
   }
   return EMRS_OK;
 }
