@@ -57,18 +57,20 @@ struct Product {
   int64_t a_batch, b_batch;        // elements between the matrices of a batch
   int32_t m, n, k;                 // k a multiple of 8, and of 64 where an operand wraps
   int32_t a_wrap, b_wrap;          // multiples of 64; kNoWrap
+  int32_t k_end;                   // 0, or where batches are runs of k: all of k, which the last run may pass
   int32_t batch;
   int32_t symmetric;               // only tiles on and below the diagonal (m >= n) are computed
 };
 constexpr int32_t kNoWrap = 0x7fffffff;
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int GROUPS_ = 1>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_;
   static constexpr int WAVES_M = BM / WM_, WAVES_N = BN / WN_, WAVES = WAVES_M * WAVES_N;
   static constexpr int WM = WM_, WN = WN_;
   static constexpr int MI = WM / 16, NI = WN / 16;
-  static constexpr int THREADS = WAVES * 64;
+  static constexpr int GROUPS = GROUPS_;  // of waves that share a tile, each over its own run of k
+  static constexpr int THREADS = WAVES * GROUPS * 64;
   static constexpr int A_LOADS = BM / 8 / WAVES, B_LOADS = BN / 8 / WAVES;
   static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole 1 KB loads per wave");
 };
@@ -78,7 +80,7 @@ struct Tile {
 // give every CU a large one.
 using Large = Tile<256, 256, 128, 64>;
 using Medium = Tile<128, 128, 64, 64>;
-using Small = Tile<64, 64, 32, 32>;
+using Small = Tile<64, 64, 32, 32, 4>;
 
 __host__ __device__ inline int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
 template <class Cfg>
@@ -89,6 +91,13 @@ __host__ inline int64_t tile_count(const Product &p) {
 
 struct Where {
   int m0, n0, batch;
+};
+
+// What an epilogue is beside its run(): where operand a of a matrix of the batch begins.
+struct Operand {
+  __device__ __forceinline__ const void *operand(const Product &p, int batch) const {
+    return static_cast<const char *>(p.a) + batch * p.a_batch * 2;
+  }
 };
 
 // The tile of a workgroup.  Workgroups go to the XCDs in turn; each XCD gets a run of consecutive tiles,
@@ -184,33 +193,47 @@ struct NoLoads {
   __device__ void operator()(int) const {}
 };
 
+// Where a group after the first leaves sum q of its lanes: the second in the first array, and so on.
+template <class Cfg>
+__device__ __forceinline__ f32x4 &spill(char (*first)[Cfg::BM * 128], char (*second)[Cfg::BN * 128], char (*third)[Cfg::BM * 128], int group,
+                                        int q, int wave, int lane) {
+  static_assert(Cfg::GROUPS <= 4 && Cfg::BM * Cfg::BN * 4 <= Cfg::GROUPS * 128 * (Cfg::BM < Cfg::BN ? Cfg::BM : Cfg::BN), "they fit");
+  char *base = group == 1 ? first[0] : group == 2 ? second[0] : third[0];
+  return reinterpret_cast<f32x4 *>(base)[(q * Cfg::WAVES + wave) * 64 + lane];
+}
+
 template <class T, class Cfg, class Epilogue>
 __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilogue epilogue) {
   using x8 = typename Vec<T>::x8;
-  __shared__ __attribute__((aligned(1024))) char a_even[Cfg::BM * 128];
-  __shared__ __attribute__((aligned(1024))) char a_odd[Cfg::BM * 128];
-  __shared__ __attribute__((aligned(1024))) char b_even[Cfg::BN * 128];
-  __shared__ __attribute__((aligned(1024))) char b_odd[Cfg::BN * 128];
+  // One array for each stage: the compiler then knows which of them a load into LDS and a read have in common.
+  __shared__ __attribute__((aligned(1024))) char a_evens[Cfg::GROUPS][Cfg::BM * 128];
+  __shared__ __attribute__((aligned(1024))) char a_odds[Cfg::GROUPS][Cfg::BM * 128];
+  __shared__ __attribute__((aligned(1024))) char b_evens[Cfg::GROUPS][Cfg::BN * 128];
+  __shared__ __attribute__((aligned(1024))) char b_odds[Cfg::GROUPS][Cfg::BN * 128];
   const Where w = tile_of<Cfg>(p);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = Cfg::GROUPS > 1 ? all / Cfg::WAVES : 0, wave = Cfg::GROUPS > 1 ? all % Cfg::WAVES : all;
+  char *const a_even = a_evens[group], *const a_odd = a_odds[group], *const b_even = b_evens[group], *const b_odd = b_odds[group];
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
 
   Loader<Cfg::WAVES> la, lb;
   la.init(p.a_stride, wave, lane);
   lb.init(p.b_stride, wave, lane);
+  const int k = p.k_end ? min(p.k, max(0, p.k_end - w.batch * p.k)) : p.k;
   auto bytes = [&](int rows, int64_t stride, int wrap) {
-    const int columns = p.k <= wrap ? p.k : max(wrap, p.k - wrap);
+    const int columns = k <= wrap ? k : max(wrap, k - wrap);
     return (int)(((rows - 1) * stride + columns) * 2);
   };
   const int a_bytes = bytes(min(Cfg::BM, p.m - w.m0), p.a_stride, p.a_wrap);
   const int b_bytes = bytes(min(Cfg::BN, p.n - w.n0), p.b_stride, p.b_wrap);
-  const T *const a_base = static_cast<const T *>(p.a) + w.batch * p.a_batch + w.m0 * p.a_stride;
+  const T *const a_base = static_cast<const T *>(epilogue.operand(p, w.batch)) + w.m0 * p.a_stride;
   const T *const b_base = static_cast<const T *>(p.b) + w.batch * p.b_batch + w.n0 * p.b_stride;
-  const int total = (p.k + kStage - 1) / kStage;
-  int k0 = 0;
+  // Stages of a group; those past the last k are zeros.
+  const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
+  int k0 = group * total * kStage;
   // The next stage's loads; past the last stage they read zeros.
   auto next_stage = [&](char *a, char *b) __attribute__((always_inline)) {
-    const int left = p.k - k0;
+    const int left = k - k0;
     const bool any = left > 0;
     const Loads<Cfg> n{la, lb, rows_buffer<T>(a_base, any ? a_bytes : 0), rows_buffer<T>(b_base, any ? b_bytes : 0), a, b,
                        k0 >= p.a_wrap ? k0 - p.a_wrap : k0, k0 >= p.b_wrap ? k0 - p.b_wrap : k0, wave};
@@ -280,6 +303,19 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   }
   if (it < total) stage(a_even, b_even, a_odd, b_odd);
   arrive();  // no load may still be on its way into LDS that another workgroup gets
+  if constexpr (Cfg::GROUPS > 1) {
+    // The groups' sums pass through their own stages' LDS to the first group, in the order of k.
+    if (group > 0) {
+#pragma unroll
+      for (int q = 0; q < Cfg::MI * Cfg::NI; ++q) spill<Cfg>(a_evens, b_evens, a_odds, group, q, wave, lane) = acc[q / Cfg::NI][q % Cfg::NI];
+    }
+    arrive();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < Cfg::GROUPS; ++g)
+#pragma unroll
+      for (int q = 0; q < Cfg::MI * Cfg::NI; ++q) acc[q / Cfg::NI][q % Cfg::NI] += spill<Cfg>(a_evens, b_evens, a_odds, g, q, wave, lane);
+  }
   epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p);
 }
 

@@ -5,11 +5,15 @@
 // maximum and a sum of exponentials for each token (and picks out the target's x); a second kernel joins
 // the tiles' pairs.  Nothing of size tokens x vocabulary is written.
 // Backward: x is computed again, a piece of the vocabulary at a time.  The product's epilogue turns it into
-// d_tv = g_t (exp(x_tv - lse_t) - [v = target_t]) in the operands' type, in both orientations, and two
-// products read that: grad_h = d w (summed over the pieces in 32 bits) and grad_w = d^T h.
+// d_tv = g_t (exp(x_tv - lse_t) - [v = target_t]), in both orientations, and two products read that:
+// grad_h = d w (summed over the pieces in 32 bits) and grad_w = d^T h.
 //
-// d is rounded to 16 bits because it is an operand of the matrix instructions, as the gradients that it
-// makes are; in fp16 it is scaled first, so that the gradient weight of a long batch does not underflow.
+// d is an operand of the matrix instructions, and so rounded to 16 bits: to fp16, whose 11 bits leave the
+// gradients with the rounding of their own type alone (in bf16, d's rounding would be as large as theirs).
+// fp16's range is met by powers of two: d is scaled by the largest |g|, and copies of w and h, which the
+// products want transposed anyway, by their largest entry; bf16's 8 bits lose nothing in them.
+//
+// Equal vocabulary shards (those of tensor parallelism are) go through every kernel together, as a batch.
 
 #include <hip/hip_runtime.h>
 
@@ -17,6 +21,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "emrs.h"
 #include "gemm.h"
@@ -30,25 +35,45 @@ using emrs_gemm::Where;
 using emrs_internal::fail;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint64_t kPieceBytes = 64ull << 20;  // of d in one orientation: both, and what reads them, stay near the caches
+constexpr uint64_t kPieceBytes = 128ull << 20;  // of d in one orientation
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
+using half = _Float16;
+using half4 = emrs_gemm::Vec<_Float16>::x4;
+
+struct Table {
+  const void *p[EMRS_LOSS_MAX_SHARDS];
+};
+
+// A piece of the vocabulary: the same `rows` rows of every shard of a group.
+struct Piece {
+  Table weights;          // first row of the piece in each shard
+  int64_t first, shard;   // vocabulary index of the first shard's first row here; rows from a shard to the next
+  int64_t vocab;          // rows from this vocabulary index on do not count
+
+  __device__ __forceinline__ const void *operand(const Product &, int batch) const { return weights.p[batch]; }
+  __host__ __device__ int64_t first_of(int batch) const { return first + batch * shard; }
+  __device__ __forceinline__ int valid(int batch, int rows) const {
+    return (int)min((int64_t)rows, max((int64_t)0, vocab - first_of(batch)));
+  }
+};
+
 // ---- forward ----
 
 // Reduces a tile of x (m: vocabulary rows, n: tokens) to one (maximum, sum) pair per token and wave row.
-struct TileStatistics {
-  float2 *pairs;          // [slots][tokens]
+struct TileStatistics : Piece {
+  float2 *pairs;          // [batch x slots][tokens]
   float *target_logit;    // [tokens]
   const int64_t *target;
-  int64_t first;          // vocabulary index of m = 0
-  int32_t valid;          // rows m < valid count
+  int64_t slots;          // of one shard
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int wm, int lane, const Product &p) const {
-    const int64_t slot = (int64_t)(w.m0 / Cfg::BM) * Cfg::WAVES_M + wm;
+    const int64_t slot = w.batch * slots + (int64_t)(w.m0 / Cfg::BM) * Cfg::WAVES_M + wm, first = first_of(w.batch);
+    const int valid = this->valid(w.batch, p.m);
     const int m = m0 + (lane >> 4) * 4;
     if (m0 + Cfg::WM > valid) {
 #pragma unroll
@@ -129,22 +154,22 @@ __global__ __launch_bounds__(kMergeThreads) void merge_statistics_kernel(const f
 // ---- backward ----
 
 // d of a piece, in both orientations, with zeros up to the padded sizes (the next products sum over them).
-template <class T>
-struct LogitGradients {
-  T *d;                   // [tokens][d_stride]: m contiguous
-  T *dt;                  // [rows][dt_stride]: n contiguous
-  int32_t d_stride, dt_stride;
+struct LogitGradients : Piece {
+  half *d;                // [tokens][shards x padded rows]: m contiguous; NULL: not wanted
+  half *dt;               // [shards x padded rows][padded tokens]: n contiguous; NULL: not wanted
+  int32_t d_stride, dt_stride, padded;
   const float *lse, *grad_loss;
   const int64_t *target;
-  int64_t ignore, first;
-  int32_t valid;
-  const float *scale;     // fp16: what d is multiplied by; NULL: 1
+  int64_t ignore;
+  const float *scale;     // of d
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &, int m0, int n0, int, int lane, const Product &p) const {
-    using x4 = typename emrs_gemm::Vec<T>::x4;
-    const int m = m0 + (lane >> 4) * 4;
-    const float by = scale ? scale[0] : 1.f;
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+    const int m = m0 + (lane >> 4) * 4, valid = this->valid(w.batch, p.m);
+    const int64_t first = first_of(w.batch);
+    const float by = scale[0];
+    half *const out_d = d ? d + w.batch * padded : nullptr;
+    half *const out_dt = dt ? dt + (int64_t)w.batch * padded * dt_stride : nullptr;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int t = n0 + j * 16 + (lane & 15);
@@ -156,34 +181,32 @@ struct LogitGradients {
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int v = m + i * 16;
-        x4 out;
+        half4 out;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float e = exp_of(acc[i][j][r] - l) - (v + r == at ? 1.f : 0.f);
-          out[r] = (T)(counts && v + r < valid ? e * g : 0.f);
-          if (dt && v + r < p.m && t < dt_stride) dt[(int64_t)(v + r) * dt_stride + t] = out[r];
+          out[r] = (half)(counts && v + r < valid ? e * g : 0.f);
+          if (out_dt && v + r < padded && t < dt_stride) out_dt[(int64_t)(v + r) * dt_stride + t] = out[r];
         }
-        if (d && in && v < d_stride) *reinterpret_cast<x4 *>(d + (int64_t)t * d_stride + v) = out;
+        if (out_d && in && v < padded) *reinterpret_cast<half4 *>(out_d + (int64_t)t * d_stride + v) = out;
       }
     }
   }
 };
 
-// C as 16-bit rows out[n][m], scaled; `sum` (32 bits, same layout) carries a sum over several products.
-template <class T>
-struct StoreRows {
-  T *out;                 // NULL: only the running sum is kept
-  float *sum;             // NULL: C alone
-  int32_t add;            // the sum holds a value already
-  int64_t stride;         // elements between rows of out and of sum
-  int32_t wide;           // four elements can be stored at once
-  const float *scale;     // what C is divided by; NULL: 1
+// A run of k of each product for itself: C of run b goes to sum[b], in 32 bits and unscaled, on top of what
+// an earlier piece left there.
+struct StoreSums : emrs_gemm::Operand {
+  float *sum;             // [batch][n][stride]
+  int64_t stride, batch;
+  int32_t add;
+  int32_t wide;
+  const float *scale_a, *scale_b;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &, int m0, int n0, int, int lane, const Product &p) const {
-    using x4 = typename emrs_gemm::Vec<T>::x4;
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
     const int m = m0 + (lane >> 4) * 4;
-    const float by = scale ? 1.f / scale[0] : 1.f;  // a power of two
+    const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int n = n0 + j * 16 + (lane & 15);
@@ -192,75 +215,166 @@ struct StoreRows {
       for (int i = 0; i < Cfg::MI; ++i) {
         const int at = m + i * 16;
         if (at >= p.m) continue;
-        const int64_t o = (int64_t)n * stride + at;
-        f32x4 c = acc[i][j];
+        float *const o = sum + w.batch * batch + n * stride + at;
+        f32x4 c = acc[i][j] * by;
         if (wide) {
-          if (sum) {
-            if (add) c += *reinterpret_cast<const f32x4 *>(sum + o);
-            if (!out) *reinterpret_cast<f32x4 *>(sum + o) = c;
-          }
-          if (out) {
-            x4 v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = (T)(c[r] * by);
-            *reinterpret_cast<x4 *>(out + o) = v;
-          }
+          if (add) c += *reinterpret_cast<const f32x4 *>(o);
+          *reinterpret_cast<f32x4 *>(o) = c;
           continue;
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (at + r >= p.m) continue;
-          float v = c[r];
-          if (sum) {
-            if (add) v += sum[o + r];
-            if (!out) sum[o + r] = v;
-          }
-          if (out) out[o + r] = (T)(v * by);
-        }
+        for (int r = 0; r < 4; ++r)
+          if (at + r < p.m) o[r] = c[r] + (add ? o[r] : 0.f);
       }
     }
   }
 };
 
-// A power of two that brings the largest |grad_loss| to 2^15: fp16 then keeps d of probabilities down to
-// 2^-29 of it out of the subnormals.  1 where there is nothing to scale.
-__global__ __launch_bounds__(1024) void gradient_scale_kernel(const float *grad_loss, const int64_t *target, int64_t ignore,
-                                                             int tokens, float *scale) {
-  __shared__ float part[16];
-  float top = 0.f;
-  for (int t = threadIdx.x; t < tokens; t += 1024)
-    if (target[t] != ignore) top = fmaxf(top, fabsf(grad_loss[t]));
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+// C as 16-bit rows out[n][m], on top of a sum of earlier pieces if there is one.
+template <class T>
+struct StoreRows : emrs_gemm::Operand {
+  Table out;              // of each matrix of the batch
+  const float *sum;       // NULL: C alone (a batch of one)
+  int64_t stride;         // elements between rows of out and of sum
+  int32_t wide;           // four elements can be stored at once
+  const float *scale_a, *scale_b;
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+    using x4 = typename emrs_gemm::Vec<T>::x4;
+    const int m = m0 + (lane >> 4) * 4;
+    const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
+    T *const to = static_cast<T *>(const_cast<void *>(out.p[w.batch]));
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j) {
+      const int n = n0 + j * 16 + (lane & 15);
+      if (n >= p.n) continue;
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int at = m + i * 16;
+        if (at >= p.m) continue;
+        const int64_t o = n * stride + at;
+        f32x4 c = acc[i][j] * by;
+        if (wide) {
+          if (sum) c += *reinterpret_cast<const f32x4 *>(sum + o);
+          x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = (T)c[r];
+          *reinterpret_cast<x4 *>(to + o) = v;
+          continue;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (at + r < p.m) to[o + r] = (T)(c[r] + (sum ? sum[o + r] : 0.f));
+      }
+    }
+  }
+};
+
+// The sum of several sums, as 16 bits.
+template <class T>
+__global__ __launch_bounds__(256) void join_sums_kernel(const float *sum, int sums, int64_t each, T *out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= each) return;
+  float v = sum[i];
+  for (int s = 1; s < sums; ++s) v += sum[s * each + i];
+  out[i] = (T)v;
+}
+
+// ---- scales: powers of two that bring the largest finite entry to [2^13, 2^14), and |grad_loss| likewise ----
+
+constexpr int kScaleBlocks = 256;
+
+__device__ inline float block_max(float v) {
+  __shared__ float part[4];
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
   __syncthreads();
-  if (threadIdx.x) return;
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, part[i]);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+__device__ inline float scale_of(float top) {
   int e = 0;
-  if (top > 0.f && top < INFINITY) frexpf(top, &e);  // top <= 2^e
-  scale[0] = ldexpf(1.f, min(max(15 - e, -100), 100));
+  if (top > 0.f && top < INFINITY) frexpf(top, &e);
+  return ldexpf(1.f, min(max(14 - e, -100), 100));
+}
+
+// Largest finite |entry| of the rows of each matrix, without those of ignored tokens: one value a workgroup.
+template <class T>
+__global__ __launch_bounds__(256) void largest_kernel(Piece piece, int64_t stride, int rows, int cols, const int64_t *target, int64_t ignore,
+                                                      float *largest) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  const T *in = static_cast<const T *>(piece.weights.p[blockIdx.y]);
+  const int valid = piece.valid(blockIdx.y, rows);
+  const bool wide = cols % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+  float top = 0.f;
+  for (int r = blockIdx.x; r < valid; r += gridDim.x) {
+    if (target && target[r] == ignore) continue;
+    const T *row = in + r * stride;
+    if (wide) {
+      for (int c = threadIdx.x * 8; c < cols; c += 2048) {
+        const x8 v = *reinterpret_cast<const x8 *>(row + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = fabsf((float)v[i]);
+          top = a < INFINITY ? fmaxf(top, a) : top;
+        }
+      }
+    } else {
+      for (int c = threadIdx.x; c < cols; c += 256) {
+        const float a = fabsf((float)row[c]);
+        top = a < INFINITY ? fmaxf(top, a) : top;
+      }
+    }
+  }
+  top = block_max(top);
+  if (threadIdx.x == 0) largest[blockIdx.y * gridDim.x + blockIdx.x] = top;
+}
+
+// The scale of what `largest` was taken of; with `count` 0 that of grad_loss, whose largest is looked for here.
+__global__ __launch_bounds__(256) void scale_kernel(const float *largest, int count, const float *grad_loss, const int64_t *target,
+                                                    int64_t ignore, int tokens, float *scale) {
+  float top = 0.f;
+  for (int i = threadIdx.x; i < count; i += 256) top = fmaxf(top, largest[i]);
+  if (count == 0)
+    for (int t = threadIdx.x; t < tokens; t += 256) {
+      const float a = fabsf(grad_loss[t]);
+      if (target[t] != ignore && a < INFINITY) top = fmaxf(top, a);
+    }
+  top = block_max(top);
+  if (threadIdx.x == 0) scale[0] = scale_of(top);
 }
 
 // ---- operands in the layout that the products read ----
 
 constexpr int kSide = 64;
 
-// out[c][r] = in[r][c] for r < rows and c < cols, with zeros up to `padded` r and where keep says so.
+// out[c][r] = scale in[r][c] for the rows that count and every c, with zeros in the others, up to `padded` r
+// for each matrix of the group, one beside the other.
 template <class T>
-__global__ __launch_bounds__(256) void transpose_kernel(const T *in, int64_t in_stride, int rows, int cols, T *out,
-                                                        int64_t out_stride, int padded, const int64_t *target, int64_t ignore) {
-  __shared__ T tile[kSide][kSide + 2];
+__global__ __launch_bounds__(256) void transpose_kernel(Piece piece, int64_t in_stride, int rows, int cols, half *out, int64_t out_stride,
+                                                        int padded, const int64_t *target, int64_t ignore, const float *scale) {
+  __shared__ half tile[kSide][kSide + 2];
   const int r0 = blockIdx.x * kSide, c0 = blockIdx.y * kSide;
+  const T *in = static_cast<const T *>(piece.weights.p[blockIdx.z]);
+  const int valid = piece.valid(blockIdx.z, rows);
+  const float by = scale[0];
   const int x = threadIdx.x % kSide;
   for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
     const int r = r0 + y, c = c0 + x;
-    const bool keep = r < rows && c < cols && !(target && target[r] == ignore);
-    tile[y][x] = keep ? in[(int64_t)r * in_stride + c] : (T)0.f;
+    const bool keep = r < valid && c < cols && !(target && target[r] == ignore);
+    tile[y][x] = keep ? (half)((float)in[r * in_stride + c] * by) : (half)0.f;
   }
   __syncthreads();
   for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
     const int c = c0 + y, r = r0 + x;
-    if (c < cols && r < padded) out[(int64_t)c * out_stride + r] = tile[x][y];
+    if (c < cols && r < padded) out[c * out_stride + (int64_t)blockIdx.z * padded + r] = tile[x][y];
   }
+}
+
+__global__ void ones_kernel(float *p, int n) {
+  if ((int)threadIdx.x < n) p[threadIdx.x] = 1.f;
 }
 
 // out[r][c] = in[r][c], with zeros from `cols` up to the padded row: operands whose rows do not lie on 16 bytes.
@@ -275,13 +389,21 @@ bool on_16(const void *p, uint64_t stride, uint64_t k) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && k % 8 == 0;
 }
 
+// Shards that go through every kernel together: equal ones, or one.
+struct Group {
+  uint32_t first, count;
+};
+
 // Where the workspace's parts lie, and how the vocabulary is cut.
 struct Sizes {
   uint64_t k;              // the hidden size, padded where an operand is copied
   bool pad_hidden, pad_weight;
-  uint64_t piece;          // vocabulary rows that are worked on at once
+  Group groups[EMRS_LOSS_MAX_SHARDS];
+  uint32_t n_groups;
+  uint64_t piece;          // rows of each shard of a group that are worked on at once
   uint64_t tokens_padded;
-  uint64_t pairs, hidden, weight, sum, d, dt, ht, wt, scale, total;  // offsets
+  uint64_t splits;         // runs of k that grad_hidden's products are cut into
+  uint64_t pairs, hidden, weight, sum, d, dt, ht, wt, scales, largest, total;  // offsets
 };
 
 int check(const emrs_loss *a) {
@@ -310,25 +432,43 @@ int check(const emrs_loss *a) {
   return EMRS_OK;
 }
 
+Product logits_of(const emrs_loss *a, const Sizes &s, const Group &g, uint64_t rows) {
+  Product p{};
+  p.b_stride = s.pad_hidden ? s.k : a->tokens > 1 ? a->hidden_stride : s.k;
+  p.a_stride = s.pad_weight || a->shard_rows[g.first] == 1 ? s.k : a->weight_strides[g.first];
+  p.m = rows, p.n = a->tokens, p.k = s.k;
+  p.a_wrap = p.b_wrap = emrs_gemm::kNoWrap;
+  p.batch = g.count;
+  return p;
+}
+
 Sizes sizes_of(const emrs_loss *a, bool backward) {
   Sizes s{};
-  uint64_t most = 0, slots = 0;
+  uint64_t most = 1, shards = 1;
   s.pad_hidden = !on_16(a->hidden, a->tokens > 1 ? a->hidden_stride : 8, a->hidden_size);
+  bool equal = true;
   for (uint32_t i = 0; i < a->n_shards; ++i) {
     most = std::max(most, a->shard_rows[i]);
     s.pad_weight |= !on_16(a->weights[i], a->shard_rows[i] > 1 ? a->weight_strides[i] : 8, a->hidden_size);
+    equal &= a->shard_rows[i] == a->shard_rows[0] && a->weight_strides[i] == a->weight_strides[0];
   }
+  s.n_groups = equal ? 1 : a->n_shards;
+  for (uint32_t i = 0; i < s.n_groups; ++i) s.groups[i] = equal ? Group{0, a->n_shards} : Group{i, 1};
+  if (equal) shards = a->n_shards;
   s.k = a->hidden_size % 8 ? round_up(a->hidden_size, 64) : a->hidden_size;
   s.tokens_padded = round_up(std::max<uint64_t>(a->tokens, 1), 64);
-  s.piece = round_up(std::max<uint64_t>(most, 1), 256);
+  s.piece = round_up(most, 256);
   if (backward || s.pad_weight)
-    s.piece = std::min(s.piece, std::max<uint64_t>(kPieceBytes / 2 / s.tokens_padded / 256, 4) * 256);
-  for (uint32_t i = 0; i < a->n_shards; ++i)
-    for (uint64_t lo = 0; lo < a->shard_rows[i]; lo += s.piece) {
-      Product p{};
-      p.m = std::min(s.piece, a->shard_rows[i] - lo), p.n = a->tokens, p.batch = 1;
-      slots += emrs_gemm::wave_rows(p);
-    }
+    s.piece = std::min(s.piece, std::max<uint64_t>(kPieceBytes / 2 / s.tokens_padded / shards / 256, 1) * 256);
+  uint64_t slots = 0;
+  for (uint32_t i = 0; i < s.n_groups; ++i)
+    for (uint64_t lo = 0; lo < a->shard_rows[s.groups[i].first]; lo += s.piece)
+      slots += emrs_gemm::wave_rows(logits_of(a, s, s.groups[i], std::min(s.piece, a->shard_rows[s.groups[i].first] - lo))) * s.groups[i].count;
+  // grad_hidden's product has few tiles where there are few tokens: its sum over the vocabulary is cut into
+  // runs of at least 1024 rows, as many as give every CU a tile.
+  const uint64_t k = round_up(std::min(s.piece, most), 64) * shards;
+  const uint64_t tiles = ((a->hidden_size + 127) / 128) * ((a->tokens + 127) / 128);
+  s.splits = std::max<uint64_t>(1, std::min(256 / std::max<uint64_t>(tiles, 1), k / 1024));
   uint64_t at = 0;
   auto take = [&](bool wanted, uint64_t bytes) {
     const uint64_t here = at;
@@ -337,13 +477,14 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   };
   s.pairs = take(!backward, slots * a->tokens * sizeof(float2));
   s.hidden = take(s.pad_hidden, a->tokens * s.k * 2);
-  s.weight = take(s.pad_weight, s.piece * s.k * 2);
-  s.sum = take(backward && a->grad_hidden, a->tokens * a->hidden_size * 4);
-  s.d = take(backward && a->grad_hidden, a->tokens * s.piece * 2);
-  s.wt = take(backward && a->grad_hidden, a->hidden_size * s.piece * 2);
-  s.dt = take(backward && a->grad_weights, s.piece * s.tokens_padded * 2);
+  s.weight = take(s.pad_weight, shards * s.piece * s.k * 2);
+  s.sum = take(backward && a->grad_hidden, s.splits * a->tokens * a->hidden_size * 4);
+  s.d = take(backward && a->grad_hidden, a->tokens * shards * s.piece * 2);
+  s.wt = take(backward && a->grad_hidden, a->hidden_size * shards * s.piece * 2);
+  s.dt = take(backward && a->grad_weights, shards * s.piece * s.tokens_padded * 2);
   s.ht = take(backward && a->grad_weights, a->hidden_size * s.tokens_padded * 2);
-  s.scale = take(backward, 256);
+  s.scales = take(backward, 256);
+  s.largest = take(backward, kScaleBlocks * EMRS_LOSS_MAX_SHARDS * 4);
   s.total = at;
   return s;
 }
@@ -354,64 +495,65 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
     if (e_ != hipSuccess) return fail(EMRS_ERR_HIP, std::string("loss: ") + hipGetErrorString(e_));     \
   } while (0)
 
-// The operands of one piece: its weight rows, copied into padded rows where they do not lie on 16 bytes.
+Piece piece_of(const emrs_loss *a, const Group &g, uint64_t first, uint64_t lo) {
+  Piece c{};
+  for (uint32_t i = 0; i < g.count; ++i)
+    c.weights.p[i] = static_cast<const char *>(a->weights[g.first + i]) + lo * a->weight_strides[g.first + i] * 2;
+  c.first = (int64_t)(first + lo), c.shard = (int64_t)a->shard_rows[g.first], c.vocab = (int64_t)a->vocab_size;
+  return c;
+}
+
+// The same piece as an operand of the logits' product: copied into padded rows where its own do not lie on 16 bytes.
 template <class T>
-int piece_operands(const emrs_loss *a, const Sizes &s, uint32_t shard, uint64_t lo, uint64_t rows, hipStream_t st, Product *p) {
-  char *ws = static_cast<char *>(a->workspace);
-  const T *w = static_cast<const T *>(a->weights[shard]) + lo * a->weight_strides[shard];
-  *p = Product{};
-  p->b = s.pad_hidden ? ws + s.hidden : a->hidden;
-  p->b_stride = s.pad_hidden ? s.k : a->tokens > 1 ? a->hidden_stride : s.k;
-  p->a = w;
-  p->a_stride = a->shard_rows[shard] > 1 ? a->weight_strides[shard] : s.k;
-  if (s.pad_weight) {
-    pad_kernel<T><<<dim3(rows, (s.k + 255) / 256), 256, 0, st>>>(w, a->weight_strides[shard], a->hidden_size,
-                                                                 reinterpret_cast<T *>(ws + s.weight), s.k);
+int aligned_piece(const emrs_loss *a, const Sizes &s, const Group &g, uint64_t rows, Piece *c, hipStream_t st) {
+  if (!s.pad_weight) return EMRS_OK;
+  T *out = reinterpret_cast<T *>(static_cast<char *>(a->workspace) + s.weight);
+  for (uint32_t i = 0; i < g.count; ++i, out += rows * s.k) {
+    pad_kernel<T><<<dim3(rows, (s.k + 255) / 256), 256, 0, st>>>(static_cast<const T *>(c->weights.p[i]), a->weight_strides[g.first + i],
+                                                                 (int)a->hidden_size, out, s.k);
     TRY(hipGetLastError());
-    p->a = ws + s.weight;
-    p->a_stride = s.k;
+    c->weights.p[i] = out;
   }
-  p->m = rows;
-  p->n = a->tokens;
-  p->k = s.k;
-  p->batch = 1;
-  p->a_wrap = p->b_wrap = emrs_gemm::kNoWrap;
   return EMRS_OK;
 }
 
 template <class T>
-int pad_hidden(const emrs_loss *a, const Sizes &s, hipStream_t st) {
+int aligned_hidden(const emrs_loss *a, const Sizes &s, const void **hidden, hipStream_t st) {
+  *hidden = a->hidden;
   if (!s.pad_hidden) return EMRS_OK;
-  pad_kernel<T><<<dim3(a->tokens, (s.k + 255) / 256), 256, 0, st>>>(static_cast<const T *>(a->hidden), a->hidden_stride, a->hidden_size,
-                                                                    reinterpret_cast<T *>(static_cast<char *>(a->workspace) + s.hidden), s.k);
+  T *out = reinterpret_cast<T *>(static_cast<char *>(a->workspace) + s.hidden);
+  pad_kernel<T><<<dim3(a->tokens, (s.k + 255) / 256), 256, 0, st>>>(static_cast<const T *>(a->hidden), a->hidden_stride, (int)a->hidden_size,
+                                                                    out, s.k);
   TRY(hipGetLastError());
+  *hidden = out;
   return EMRS_OK;
-}
-
-int32_t valid_rows(const emrs_loss *a, uint64_t first, uint64_t rows) {
-  return (int32_t)(a->vocab_size <= first ? 0 : std::min(rows, a->vocab_size - first));
 }
 
 template <class T>
 int forward(const emrs_loss *a, hipStream_t st) {
   const Sizes s = sizes_of(a, false);
-  char *ws = static_cast<char *>(a->workspace);
-  float2 *pairs = reinterpret_cast<float2 *>(ws + s.pairs);
-  int rc = pad_hidden<T>(a, s, st);
+  float2 *pairs = reinterpret_cast<float2 *>(static_cast<char *>(a->workspace) + s.pairs);
+  const void *hidden;
+  int rc = aligned_hidden<T>(a, s, &hidden, st);
   if (rc) return rc;
   uint64_t first = a->vocab_start;
   int64_t slots = 0;
-  for (uint32_t i = 0; i < a->n_shards; first += a->shard_rows[i], ++i)
-    for (uint64_t lo = 0; lo < a->shard_rows[i]; lo += s.piece) {
-      const uint64_t rows = std::min(s.piece, a->shard_rows[i] - lo);
-      Product p;
-      rc = piece_operands<T>(a, s, i, lo, rows, st, &p);
+  for (uint32_t i = 0; i < s.n_groups; ++i) {
+    const Group &g = s.groups[i];
+    const uint64_t all = a->shard_rows[g.first];
+    for (uint64_t lo = 0; lo < all; lo += s.piece) {
+      const uint64_t rows = std::min(s.piece, all - lo);
+      Piece c = piece_of(a, g, first, lo);
+      rc = aligned_piece<T>(a, s, g, rows, &c, st);
       if (rc) return rc;
-      const TileStatistics e{pairs + slots * (int64_t)a->tokens, a->target_logit, a->target, (int64_t)(first + lo),
-                             valid_rows(a, first + lo, rows)};
-      TRY((emrs_gemm::launch<T>(p, e, st)));
-      slots += emrs_gemm::wave_rows(p);
+      Product p = logits_of(a, s, g, rows);
+      p.b = hidden;
+      const int64_t each = emrs_gemm::wave_rows(p);
+      TRY((emrs_gemm::launch<T>(p, TileStatistics{c, pairs + slots * (int64_t)a->tokens, a->target_logit, a->target, each}, st)));
+      slots += each * g.count;
     }
+    first += all * g.count;
+  }
   const int64_t last = (int64_t)std::max(a->vocab_start, std::min(first, a->vocab_size));
   merge_statistics_kernel<<<(a->tokens + kMergeTokens - 1) / kMergeTokens, kMergeThreads, 0, st>>>(
       pairs, slots, (int)a->tokens, a->target, a->ignore_index, (int64_t)a->vocab_start, last, a->lse, a->target_logit, a->loss);
@@ -419,11 +561,19 @@ int forward(const emrs_loss *a, hipStream_t st) {
   return EMRS_OK;
 }
 
+// scale * transpose of a group's piece (or of the hidden states); fp16 is copied as it is.
 template <class T>
-int transpose(const T *in, int64_t in_stride, int64_t rows, int64_t cols, T *out, int64_t out_stride, const int64_t *target,
-              int64_t ignore, hipStream_t st) {
-  const dim3 grid((out_stride + kSide - 1) / kSide, (cols + kSide - 1) / kSide);
-  transpose_kernel<T><<<grid, 256, 0, st>>>(in, in_stride, (int)rows, (int)cols, out, out_stride, (int)out_stride, target, ignore);
+int transposed(const Piece &c, uint32_t count, int64_t stride, int64_t rows, int64_t cols, half *out, int64_t out_stride, int64_t padded,
+               const int64_t *target, int64_t ignore, float *largest, float *scale, hipStream_t st) {
+  const int blocks = std::is_same<T, half>::value ? 0 : (int)std::min<int64_t>(rows, kScaleBlocks);
+  if (blocks) {
+    largest_kernel<T><<<dim3(blocks, count), 256, 0, st>>>(c, stride, (int)rows, (int)cols, target, ignore, largest);
+    TRY(hipGetLastError());
+    scale_kernel<<<1, 256, 0, st>>>(largest, blocks * (int)count, nullptr, nullptr, 0, 0, scale);
+    TRY(hipGetLastError());
+  }
+  const dim3 grid((padded + kSide - 1) / kSide, (cols + kSide - 1) / kSide, count);
+  transpose_kernel<T><<<grid, 256, 0, st>>>(c, stride, (int)rows, (int)cols, out, out_stride, (int)padded, target, ignore, scale);
   TRY(hipGetLastError());
   return EMRS_OK;
 }
@@ -432,65 +582,103 @@ template <class T>
 int backward(const emrs_loss *a, hipStream_t st) {
   const Sizes s = sizes_of(a, true);
   char *ws = static_cast<char *>(a->workspace);
-  T *d = reinterpret_cast<T *>(ws + s.d), *wt = reinterpret_cast<T *>(ws + s.wt);
-  T *dt = reinterpret_cast<T *>(ws + s.dt), *ht = reinterpret_cast<T *>(ws + s.ht);
-  float *sum = reinterpret_cast<float *>(ws + s.sum), *scale = nullptr;
-  int rc = pad_hidden<T>(a, s, st);
+  half *d = reinterpret_cast<half *>(ws + s.d), *wt = reinterpret_cast<half *>(ws + s.wt);
+  half *dt = reinterpret_cast<half *>(ws + s.dt), *ht = reinterpret_cast<half *>(ws + s.ht);
+  float *sum = reinterpret_cast<float *>(ws + s.sum), *largest = reinterpret_cast<float *>(ws + s.largest);
+  float *d_scale = reinterpret_cast<float *>(ws + s.scales), *h_scale = d_scale + 1, *w_scale = d_scale + 2;
+  const int64_t h = (int64_t)a->hidden_size, tokens = (int64_t)a->tokens;
+  const void *hidden;
+  int rc = aligned_hidden<T>(a, s, &hidden, st);
   if (rc) return rc;
-  if (a->dtype == EMRS_FP16) {
-    scale = reinterpret_cast<float *>(ws + s.scale);
-    gradient_scale_kernel<<<1, 1024, 0, st>>>(a->grad_loss, a->target, a->ignore_index, (int)a->tokens, scale);
+  scale_kernel<<<1, 256, 0, st>>>(nullptr, 0, a->grad_loss, a->target, a->ignore_index, (int)tokens, d_scale);
+  TRY(hipGetLastError());
+  if (std::is_same<T, half>::value) {
+    ones_kernel<<<1, 64, 0, st>>>(h_scale, 2);
     TRY(hipGetLastError());
   }
   if (a->grad_weights) {
-    rc = transpose<T>(static_cast<const T *>(a->hidden), a->hidden_stride, a->tokens, a->hidden_size, ht, s.tokens_padded, a->target,
-                      a->ignore_index, st);
+    Piece all{};
+    all.weights.p[0] = a->hidden, all.vocab = tokens;
+    rc = transposed<T>(all, 1, a->hidden_stride, tokens, h, ht, s.tokens_padded, s.tokens_padded, a->target, a->ignore_index, largest, h_scale, st);
     if (rc) return rc;
   }
+  const bool fours = h % 4 == 0;
   uint64_t first = a->vocab_start, left = 0;
-  for (uint32_t i = 0; i < a->n_shards; ++i) left += (a->shard_rows[i] + s.piece - 1) / s.piece;
+  for (uint32_t i = 0; i < s.n_groups; ++i) left += (a->shard_rows[s.groups[i].first] + s.piece - 1) / s.piece;
   bool begun = false;
-  for (uint32_t i = 0; i < a->n_shards; first += a->shard_rows[i], ++i)
-    for (uint64_t lo = 0; lo < a->shard_rows[i]; lo += s.piece) {
-      const uint64_t rows = std::min(s.piece, a->shard_rows[i] - lo), padded = round_up(rows, 64);
-      T *gw = a->grad_weights ? static_cast<T *>(a->grad_weights[i]) : nullptr;
-      const int32_t valid = valid_rows(a, first + lo, rows);
+  for (uint32_t i = 0; i < s.n_groups; ++i) {
+    const Group &g = s.groups[i];
+    const uint64_t all = a->shard_rows[g.first];
+    uint32_t wanted = 0;
+    for (uint32_t k = 0; a->grad_weights && k < g.count; ++k) wanted += a->grad_weights[g.first + k] != nullptr;
+    for (uint64_t lo = 0; lo < all; lo += s.piece) {
+      const uint64_t rows = std::min(s.piece, all - lo), padded = round_up(rows, 64);
       --left;
-      Product p;
-      rc = piece_operands<T>(a, s, i, lo, rows, st, &p);
+      if (!a->grad_hidden && !wanted) continue;
+      const Piece own = piece_of(a, g, first, lo);
+      Piece c = own;
+      rc = aligned_piece<T>(a, s, g, rows, &c, st);
       if (rc) return rc;
-      if (!a->grad_hidden && !gw) continue;
-      const LogitGradients<T> e{a->grad_hidden ? d : nullptr, gw ? dt : nullptr, (int32_t)padded, (int32_t)s.tokens_padded,
-                                a->lse, a->grad_loss, a->target, a->ignore_index, (int64_t)(first + lo), valid, scale};
-      TRY((emrs_gemm::launch<T>(p, e, st)));
-      const bool wide = a->hidden_size % 4 == 0;
+      Product p = logits_of(a, s, g, rows);
+      p.b = hidden;
+      TRY((emrs_gemm::launch<T>(p, LogitGradients{c, a->grad_hidden ? d : nullptr, wanted ? dt : nullptr, (int32_t)(g.count * padded),
+                                                  (int32_t)s.tokens_padded, (int32_t)padded, a->lse, a->grad_loss, a->target, a->ignore_index, d_scale}, st)));
       if (a->grad_hidden) {
-        rc = transpose<T>(static_cast<const T *>(a->weights[i]) + lo * a->weight_strides[i], a->weight_strides[i], valid,
-                          a->hidden_size, wt, padded, nullptr, 0, st);
+        rc = transposed<T>(own, g.count, a->weight_strides[g.first], rows, h, wt, g.count * padded, padded, nullptr, 0, largest, w_scale, st);
         if (rc) return rc;
         Product q{};
         q.a = wt, q.b = d;
-        q.a_stride = q.b_stride = padded;
-        q.m = a->hidden_size, q.n = a->tokens, q.k = padded;
-        q.batch = 1;
+        q.a_stride = q.b_stride = g.count * padded;
+        q.m = h, q.n = tokens;
         q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
-        const StoreRows<T> out{left ? nullptr : static_cast<T *>(a->grad_hidden), left || begun ? sum : nullptr, begun,
-                               (int64_t)a->hidden_size, wide && reinterpret_cast<uintptr_t>(a->grad_hidden) % 8 == 0, scale};
-        TRY((emrs_gemm::launch<T>(q, out, st)));
+        if (s.splits > 1) {
+          // Runs of k as a batch: multiples of 64, the last one shorter (its stages past the end are zeros).
+          q.batch = (int32_t)s.splits;
+          q.k = (int32_t)round_up((g.count * padded + s.splits - 1) / s.splits, 64);
+          q.a_batch = q.b_batch = q.k;
+          q.k_end = (int32_t)(g.count * padded);
+          TRY((emrs_gemm::launch<half>(q, StoreSums{{}, sum, h, tokens * h, begun, fours, d_scale, w_scale}, st)));
+        } else {
+          q.batch = 1, q.k = (int32_t)(g.count * padded);
+          const bool last = left == 0;
+          if (!last) {
+            TRY((emrs_gemm::launch<half>(q, StoreSums{{}, sum, h, tokens * h, begun, fours, d_scale, w_scale}, st)));
+          } else {
+            StoreRows<T> out{};
+            out.out.p[0] = a->grad_hidden, out.sum = begun ? sum : nullptr, out.stride = h;
+            out.wide = fours && reinterpret_cast<uintptr_t>(a->grad_hidden) % 8 == 0;
+            out.scale_a = d_scale, out.scale_b = w_scale;
+            TRY((emrs_gemm::launch<half>(q, out, st)));
+          }
+        }
         begun = true;
       }
-      if (gw) {
+      for (uint32_t k = 0; wanted && k < g.count; k += wanted == g.count ? g.count : 1) {
+        const uint32_t n = wanted == g.count ? g.count : 1;
+        if (!a->grad_weights[g.first + k]) continue;
         Product q{};
-        q.a = ht, q.b = dt;
-        q.a_stride = q.b_stride = s.tokens_padded;
-        q.m = a->hidden_size, q.n = rows, q.k = s.tokens_padded;
-        q.batch = 1;
+        q.a = ht, q.b = dt + (int64_t)k * padded * s.tokens_padded;
+        q.a_stride = q.b_stride = s.tokens_padded, q.b_batch = (int64_t)padded * s.tokens_padded;
+        q.m = h, q.n = rows, q.k = s.tokens_padded;
         q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
-        const StoreRows<T> out{gw + lo * a->hidden_size, nullptr, 0, (int64_t)a->hidden_size,
-                               wide && reinterpret_cast<uintptr_t>(gw) % 8 == 0, scale};
-        TRY((emrs_gemm::launch<T>(q, out, st)));
+        q.batch = n;
+        StoreRows<T> out{};
+        out.wide = fours;
+        for (uint32_t b = 0; b < n; ++b) {
+          T *gw = static_cast<T *>(a->grad_weights[g.first + k + b]) + lo * h;
+          out.out.p[b] = gw;
+          out.wide &= reinterpret_cast<uintptr_t>(gw) % 8 == 0;
+        }
+        out.stride = h, out.scale_a = d_scale, out.scale_b = h_scale;
+        TRY((emrs_gemm::launch<half>(q, out, st)));
       }
     }
+    first += all * g.count;
+  }
+  if (a->grad_hidden && s.splits > 1) {
+    join_sums_kernel<T><<<(uint32_t)((tokens * h + 255) / 256), 256, 0, st>>>(sum, (int)s.splits, tokens * h, static_cast<T *>(a->grad_hidden));
+    TRY(hipGetLastError());
+  }
   return EMRS_OK;
 }
 

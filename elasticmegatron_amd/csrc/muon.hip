@@ -181,7 +181,7 @@ __device__ inline void store_symmetric(half *out, int64_t stride, int m, int n, 
     for (int r = 0; r < 4; ++r) out[(m + r) * stride + n] = v[r];
 }
 
-struct StoreGram {
+struct StoreGram : emrs_gemm::Operand {
   half *out;
   int64_t stride, batch;
   float by;
@@ -203,7 +203,7 @@ struct StoreGram {
 };
 
 // a I + b A + c A A, the polynomial of the steps with one part; without a I (a = 0) of the others.
-struct StorePolynomial {
+struct StorePolynomial : emrs_gemm::Operand {
   half *out;
   const half *gram;
   int64_t stride, batch;
@@ -238,7 +238,7 @@ __device__ inline f32x4 applied(const half *x, int64_t low, int parts, float a, 
 }
 
 // The next X (m: the longer side), in both orientations.
-struct StoreIterate {
+struct StoreIterate : emrs_gemm::Operand {
   Image in, out, across;
   int32_t in_parts, out_parts;
   float a;
@@ -272,7 +272,7 @@ struct StoreIterate {
 // The last X: the result, or the update of the weights and their bf16 image.  m runs along the caller's rows,
 // which are written four elements at a time where they lie so (kWide).
 template <bool kWide>
-struct StoreResult {
+struct StoreResult : emrs_gemm::Operand {
   Image in;
   int32_t in_parts;
   float a, by;  // by: over the scale of X
@@ -474,7 +474,7 @@ int step(const emrs_muon *a, hipStream_t st) {
     // hi hi + hi lo + lo hi
     g.a_wrap = parts == 2 ? (int)z.l : emrs_gemm::kNoWrap, g.b_wrap = parts == 2 ? 2 * (int)z.l : emrs_gemm::kNoWrap;
     g.batch = (int)a->count, g.symmetric = 1;
-    TRY((emrs_gemm::launch<half>(g, StoreGram{gram, (int64_t)z.s, square, kGramScale / (scale * scale)}, st)));
+    TRY((emrs_gemm::launch<half>(g, StoreGram{{}, gram, (int64_t)z.s, square, kGramScale / (scale * scale)}, st)));
 
     Product q{};
     q.a = q.b = gram;
@@ -482,7 +482,7 @@ int step(const emrs_muon *a, hipStream_t st) {
     q.m = q.n = q.k = (int)z.s;
     q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
     q.batch = (int)a->count, q.symmetric = 1;
-    TRY((emrs_gemm::launch<half>(q, StorePolynomial{poly, gram, (int64_t)z.s, square, parts == 1 ? f[0] * kGramScale : 0.f, f[1], f[2] / kGramScale}, st)));
+    TRY((emrs_gemm::launch<half>(q, StorePolynomial{{}, poly, gram, (int64_t)z.s, square, parts == 1 ? f[0] * kGramScale : 0.f, f[1], f[2] / kGramScale}, st)));
 
     Product r{};
     const bool last = k + 1 == a->steps, turned = last && tall;
@@ -495,7 +495,7 @@ int step(const emrs_muon *a, hipStream_t st) {
     r.m = (int)(turned ? z.s : z.l), r.n = (int)(turned ? z.l : z.s), r.k = (int)z.s * parts;
     r.batch = (int)a->count;
     if (!last) {
-      TRY((emrs_gemm::launch<half>(r, StoreIterate{in, x(now ^ 1), xt(now ^ 1), parts, parts_of(k + 1), f[0]}, st)));
+      TRY((emrs_gemm::launch<half>(r, StoreIterate{{}, in, x(now ^ 1), xt(now ^ 1), parts, parts_of(k + 1), f[0]}, st)));
       continue;
     }
     const bool wide_rows = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
