@@ -79,7 +79,7 @@ struct Tile {
 // CU's matrix units against 96 KB of fragment reads.  The smaller tiles are for products that would not
 // give every CU a large one.
 using Large = Tile<256, 256, 128, 64>;
-using Medium = Tile<128, 128, 64, 64>;
+using Medium = Tile<128, 128, 64, 64, 2>;
 using Small = Tile<64, 64, 32, 32, 4>;
 
 __host__ __device__ inline int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
@@ -193,14 +193,57 @@ struct NoLoads {
   __device__ void operator()(int) const {}
 };
 
-// Where a group after the first leaves sum q of its lanes: the second in the first array, and so on.
+// Where a group after the first leaves sum q of its lanes: the stages' arrays, one after the other.
 template <class Cfg>
-__device__ __forceinline__ f32x4 &spill(char (*first)[Cfg::BM * 128], char (*second)[Cfg::BN * 128], char (*third)[Cfg::BM * 128], int group,
-                                        int q, int wave, int lane) {
-  static_assert(Cfg::GROUPS <= 4 && Cfg::BM * Cfg::BN * 4 <= Cfg::GROUPS * 128 * (Cfg::BM < Cfg::BN ? Cfg::BM : Cfg::BN), "they fit");
-  char *base = group == 1 ? first[0] : group == 2 ? second[0] : third[0];
-  return reinterpret_cast<f32x4 *>(base)[(q * Cfg::WAVES + wave) * 64 + lane];
+__device__ __forceinline__ f32x4 &left_sum(char *a, char *b, char *c, char *d, int group, int q, int wave, int lane) {
+  constexpr int block = Cfg::WAVES * 1024, each = Cfg::GROUPS * 128 * (Cfg::BM < Cfg::BN ? Cfg::BM : Cfg::BN) / block;
+  static_assert((Cfg::GROUPS - 1) * Cfg::MI * Cfg::NI <= 4 * each, "they fit");
+  const int at = (group - 1) * Cfg::MI * Cfg::NI + q;
+  char *const base = at < each ? a : at < 2 * each ? b : at < 3 * each ? c : d;
+  return reinterpret_cast<f32x4 *>(base + at % each * block + wave * 1024)[lane];
 }
+
+// A wave's tile in 16 bits, turned over in its part of LDS: accumulators go in, and 16-byte units of eight
+// consecutive m of an n, or of eight consecutive n of an m, come out.  Rows are of n; a row's units are
+// permuted by n, so that 16 lanes of different n meet different banks.  Nothing here waits for other waves.
+template <class Cfg>
+struct Turn {
+  static constexpr int kRow = Cfg::WM / 8, kMask = kRow - 1;  // units of a row
+  static constexpr int kPasses = Cfg::WM * Cfg::WN / 512;
+  static __device__ __forceinline__ int at(int n, int m) { return n * Cfg::WM * 2 + (((m >> 3) ^ n) & kMask) * 16 + (m & 7) * 2; }
+  template <class V>
+  static __device__ __forceinline__ void put(char *own, int i, int j, int lane, V v) {
+    static_assert(sizeof(V) == 8, "four values");
+    *reinterpret_cast<V *>(own + at(j * 16 + (lane & 15), i * 16 + (lane >> 4) * 4)) = v;
+  }
+  // store(m, n, unit): eight consecutive m.
+  template <class Store>
+  static __device__ __forceinline__ void along_m(const char *own, int lane, Store store) {
+#pragma unroll 4
+    for (int q = 0; q < kPasses; ++q) {
+      const int u = q * 64 + lane, n = u / kRow, m = u % kRow * 8;
+      store(m, n, *reinterpret_cast<const fp16x8 *>(own + at(n, m)));
+    }
+  }
+  // store(m, n, unit): eight consecutive n.  Sixteen lanes read a block of 4 n x 16 m as it lies, and each gets
+  // the four n of one m.
+  template <class Store>
+  static __device__ __forceinline__ void along_n(const char *own, int lane, Store store) {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    typedef __attribute__((address_space(3))) s16x4 *lds4;
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    const int t = lane & 15;
+#pragma unroll 4
+    for (int q = 0; q < kPasses; ++q) {
+      const int b = q * 4 + (lane >> 4), n = b % (Cfg::WN / 8) * 8, m = b / (Cfg::WN / 8) * 16;
+      char *const lo = const_cast<char *>(own) + at(n + (t >> 2), m + (t & 3) * 4);
+      char *const hi = const_cast<char *>(own) + at(n + 4 + (t >> 2), m + (t & 3) * 4);
+      const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)lo), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)hi);
+      const s16x8 v = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+      store(m + t, n, __builtin_bit_cast(fp16x8, v));
+    }
+  }
+};
 
 template <class T, class Cfg, class Epilogue>
 __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilogue epilogue) {
@@ -304,19 +347,28 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   if (it < total) stage(a_even, b_even, a_odd, b_odd);
   arrive();  // no load may still be on its way into LDS that another workgroup gets
   if constexpr (Cfg::GROUPS > 1) {
-    // The groups' sums pass through their own stages' LDS to the first group, in the order of k.
+    // The groups' sums pass through the stages' LDS to the first group, in the order of k.
     if (group > 0) {
 #pragma unroll
-      for (int q = 0; q < Cfg::MI * Cfg::NI; ++q) spill<Cfg>(a_evens, b_evens, a_odds, group, q, wave, lane) = acc[q / Cfg::NI][q % Cfg::NI];
+      for (int q = 0; q < Cfg::MI * Cfg::NI; ++q)
+        left_sum<Cfg>(a_evens[0], b_evens[0], a_odds[0], b_odds[0], group, q, wave, lane) = acc[q / Cfg::NI][q % Cfg::NI];
+    }
+    arrive();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 1; g < Cfg::GROUPS; ++g)
+#pragma unroll
+        for (int q = 0; q < Cfg::MI * Cfg::NI; ++q)
+          acc[q / Cfg::NI][q % Cfg::NI] += left_sum<Cfg>(a_evens[0], b_evens[0], a_odds[0], b_odds[0], g, q, wave, lane);
     }
     arrive();
     if (group > 0) return;
-#pragma unroll
-    for (int g = 1; g < Cfg::GROUPS; ++g)
-#pragma unroll
-      for (int q = 0; q < Cfg::MI * Cfg::NI; ++q) acc[q / Cfg::NI][q % Cfg::NI] += spill<Cfg>(a_evens, b_evens, a_odds, g, q, wave, lane);
   }
-  epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p);
+  // Each wave's own part of the stages' LDS, for its tile in 16 bits.
+  constexpr int part = Cfg::WM * Cfg::WN * 2, each = Cfg::GROUPS * 128 * (Cfg::BM < Cfg::BN ? Cfg::BM : Cfg::BN) / part;
+  static_assert(4 * each >= Cfg::WAVES, "they fit");
+  char *const own = (wave < each ? a_evens[0] : wave < 2 * each ? b_evens[0] : wave < 3 * each ? a_odds[0] : b_odds[0]) + wave % each * part;
+  epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p, own);
 }
 
 enum Shape { kLarge, kMedium, kSmall };

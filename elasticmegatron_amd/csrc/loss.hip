@@ -71,7 +71,7 @@ struct TileStatistics : Piece {
   int64_t slots;          // of one shard
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int wm, int lane, const Product &p) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int wm, int lane, const Product &p, char *) const {
     const int64_t slot = w.batch * slots + (int64_t)(w.m0 / Cfg::BM) * Cfg::WAVES_M + wm, first = first_of(w.batch);
     const int valid = this->valid(w.batch, p.m);
     const int m = m0 + (lane >> 4) * 4;
@@ -164,33 +164,40 @@ struct LogitGradients : Piece {
   const float *scale;     // of d
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4, valid = this->valid(w.batch, p.m);
     const int64_t first = first_of(w.batch);
     const float by = scale[0];
-    half *const out_d = d ? d + w.batch * padded : nullptr;
-    half *const out_dt = dt ? dt + (int64_t)w.batch * padded * dt_stride : nullptr;
+    using Turn = emrs_gemm::Turn<Cfg>;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int t = n0 + j * 16 + (lane & 15);
-      const bool in = t < p.n;
-      const int64_t label = in ? target[t] : ignore;
+      const int64_t label = t < p.n ? target[t] : ignore;
       const bool counts = label != ignore;
       const int64_t at = label - first;
-      const float g = counts ? grad_loss[t] * by : 0.f, l = counts ? lse[t] : 0.f;
+      const float g = counts ? grad_loss[t] * by : 0.f, l = counts ? lse[t] * kLog2e : 0.f;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int v = m + i * 16;
         half4 out;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp_of(acc[i][j][r] - l) - (v + r == at ? 1.f : 0.f);
+          const float e = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, -l)) - (v + r == at ? 1.f : 0.f);
           out[r] = (half)(counts && v + r < valid ? e * g : 0.f);
-          if (out_dt && v + r < padded && t < dt_stride) out_dt[(int64_t)(v + r) * dt_stride + t] = out[r];
         }
-        if (out_d && in && v < padded) *reinterpret_cast<half4 *>(out_d + (int64_t)t * d_stride + v) = out;
+        Turn::put(own, i, j, lane, out);
       }
     }
+    if (d)
+      Turn::along_m(own, lane, [&](int x, int t, emrs_gemm::fp16x8 v) __attribute__((always_inline)) {
+        if (m0 + x < padded && n0 + t < p.n)
+          *reinterpret_cast<emrs_gemm::fp16x8 *>(d + (int64_t)(n0 + t) * d_stride + w.batch * padded + m0 + x) = v;
+      });
+    if (dt)
+      Turn::along_n(own, lane, [&](int x, int t, emrs_gemm::fp16x8 v) __attribute__((always_inline)) {
+        if (m0 + x < padded && n0 + t < dt_stride)
+          *reinterpret_cast<emrs_gemm::fp16x8 *>(dt + (int64_t)(w.batch * padded + m0 + x) * dt_stride + n0 + t) = v;
+      });
   }
 };
 
@@ -204,7 +211,7 @@ struct StoreSums : emrs_gemm::Operand {
   const float *scale_a, *scale_b;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4;
     const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
 #pragma unroll
@@ -240,7 +247,7 @@ struct StoreRows : emrs_gemm::Operand {
   const float *scale_a, *scale_b;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     using x4 = typename emrs_gemm::Vec<T>::x4;
     const int m = m0 + (lane >> 4) * 4;
     const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
@@ -283,7 +290,7 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float *sum, int su
 
 // ---- scales: powers of two that bring the largest finite entry to [2^13, 2^14), and |grad_loss| likewise ----
 
-constexpr int kScaleBlocks = 256;
+constexpr int kScaleBlocks = 2048;
 
 __device__ inline float block_max(float v) {
   __shared__ float part[4];
@@ -355,21 +362,40 @@ constexpr int kSide = 64;
 template <class T>
 __global__ __launch_bounds__(256) void transpose_kernel(Piece piece, int64_t in_stride, int rows, int cols, half *out, int64_t out_stride,
                                                         int padded, const int64_t *target, int64_t ignore, const float *scale) {
-  __shared__ half tile[kSide][kSide + 2];
+  // Column c of the tile in row c of LDS; a row's 16-byte units of eight r are permuted by c, so that the
+  // eight columns that a lane reads in one row meet no other lane's bank.
+  __shared__ __attribute__((aligned(16))) half tile[kSide][kSide];
+  using x8 = typename emrs_gemm::Vec<T>::x8;
   const int r0 = blockIdx.x * kSide, c0 = blockIdx.y * kSide;
   const T *in = static_cast<const T *>(piece.weights.p[blockIdx.z]);
   const int valid = piece.valid(blockIdx.z, rows);
   const float by = scale[0];
-  const int x = threadIdx.x % kSide;
-  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
-    const int r = r0 + y, c = c0 + x;
-    const bool keep = r < valid && c < cols && !(target && target[r] == ignore);
-    tile[y][x] = keep ? (half)((float)in[r * in_stride + c] * by) : (half)0.f;
+  const bool wide = cols % 8 == 0 && in_stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = threadIdx.x + h * 256, r = at / 8, c = at % 8 * 8;
+    const bool keep = r0 + r < valid && !(target && target[r0 + r] == ignore);
+    const T *row = in + (r0 + r) * in_stride + c0 + c;
+    x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (T)0.f;
+    if (keep && wide && c0 + c < cols) {
+      v = *reinterpret_cast<const x8 *>(row);
+    } else if (keep) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + c + i < cols) v[i] = row[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tile[c + i][((r / 8 ^ (c / 8)) * 8) + r % 8] = (half)((float)v[i] * by);
   }
   __syncthreads();
-  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
-    const int c = c0 + y, r = r0 + x;
-    if (c < cols && r < padded) out[c * out_stride + (int64_t)blockIdx.z * padded + r] = tile[x][y];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = threadIdx.x + h * 256, c = at / 8, unit = at % 8, r = r0 + unit * 8;
+    if (c0 + c < cols && r < padded)
+      *reinterpret_cast<emrs_gemm::fp16x8 *>(out + (c0 + c) * out_stride + (int64_t)blockIdx.z * padded + r) =
+          *reinterpret_cast<const emrs_gemm::fp16x8 *>(&tile[c][(unit ^ (c / 8)) * 8]);
   }
 }
 

@@ -173,12 +173,20 @@ __global__ __launch_bounds__(256) void pack_kernel(Update u, const float *norms,
   }
 }
 
-// The same element on both sides of the diagonal.  A tile on the diagonal computes both itself: with two
-// parts they differ in their sums' order, so each is stored where it belongs and nowhere twice.
-__device__ inline void store_symmetric(half *out, int64_t stride, int m, int n, half4 v, bool mirror) {
-  *reinterpret_cast<half4 *>(out + n * stride + m) = v;
-  if (mirror)
-    for (int r = 0; r < 4; ++r) out[(m + r) * stride + n] = v[r];
+using half8 = emrs_gemm::fp16x8;
+
+// A wave's tile of a symmetric matrix, from LDS to its place and, off the diagonal, to the place across it.
+// (A tile on the diagonal holds both: with two parts they differ in their sums' order, and are stored once.)
+template <class Cfg>
+__device__ __forceinline__ void store_symmetric(half *out, int64_t stride, const Where &w, int m0, int n0, int lane, const Product &p,
+                                                const char *own) {
+  emrs_gemm::Turn<Cfg>::along_m(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
+    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(out + (n0 + y) * stride + m0 + x) = v;
+  });
+  if (w.m0 == w.n0) return;
+  emrs_gemm::Turn<Cfg>::along_n(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
+    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(out + (m0 + x) * stride + n0 + y) = v;
+  });
 }
 
 struct StoreGram : emrs_gemm::Operand {
@@ -187,18 +195,16 @@ struct StoreGram : emrs_gemm::Operand {
   float by;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
-    half *o = out + w.batch * batch;
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j)
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
-        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
-        if (m >= p.m || n >= p.n) continue;
         half4 v;
         for (int r = 0; r < 4; ++r) v[r] = (half)(acc[i][j][r] * by);
-        store_symmetric(o, stride, m, n, v, w.m0 != w.n0);
+        emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
       }
+    store_symmetric<Cfg>(out + w.batch * batch, stride, w, m0, n0, lane, p, own);
   }
 };
 
@@ -210,20 +216,21 @@ struct StorePolynomial : emrs_gemm::Operand {
   float a, b, c;  // a times the scale of A, c over it
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
-    half *o = out + w.batch * batch;
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const half *in = gram + w.batch * batch;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j)
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
-        if (m >= p.m || n >= p.n) continue;
-        const half4 x = *reinterpret_cast<const half4 *>(in + n * stride + m);
-        half4 v;
-        for (int r = 0; r < 4; ++r) v[r] = (half)((m + r == n ? a : 0.f) + b * (float)x[r] + c * acc[i][j][r]);
-        store_symmetric(o, stride, m, n, v, w.m0 != w.n0);
+        half4 v = half4{};
+        if (m < p.m && n < p.n) {
+          const half4 x = *reinterpret_cast<const half4 *>(in + n * stride + m);
+          for (int r = 0; r < 4; ++r) v[r] = (half)((m + r == n ? a : 0.f) + b * (float)x[r] + c * acc[i][j][r]);
+        }
+        emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
       }
+    store_symmetric<Cfg>(out + w.batch * batch, stride, w, m0, n0, lane, p, own);
   }
 };
 
@@ -237,35 +244,49 @@ __device__ inline f32x4 applied(const half *x, int64_t low, int parts, float a, 
   return v;
 }
 
-// The next X (m: the longer side), in both orientations.
+// The next X (m: the longer side), in both orientations: its first part, then, where it has one, its second.
 struct StoreIterate : emrs_gemm::Operand {
   Image in, out, across;
   int32_t in_parts, out_parts;
   float a;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
+    using Turn = emrs_gemm::Turn<Cfg>;
     const half *x = in.p + w.batch * in.batch;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j) {
+      __builtin_amdgcn_sched_barrier(0);  // the loads of one column at a time: registers
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
+        if (m < p.m && n < p.n) acc[i][j] = applied(x + n * in.stride + m, in.low, in_parts, a, acc[i][j]);
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)acc[i][j][r];
+        Turn::put(own, i, j, lane, v);
+      }
+    }
     half *o = out.p + w.batch * out.batch, *t = across.p + w.batch * across.batch;
+    store(o, t, m0, n0, lane, p, own, Turn{});
+    if (out_parts == 1) return;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j)
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
-        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
-        if (m >= p.m || n >= p.n) continue;
-        const f32x4 v = applied(x + n * in.stride + m, in.low, in_parts, a, acc[i][j]);
-        half4 hi, lo;
-        for (int r = 0; r < 4; ++r) {
-          hi[r] = (half)v[r];
-          lo[r] = (half)(v[r] - (float)hi[r]);
-        }
-        *reinterpret_cast<half4 *>(o + n * out.stride + m) = hi;
-        for (int r = 0; r < 4; ++r) t[(m + r) * across.stride + n] = hi[r];
-        if (out_parts > 1) {
-          *reinterpret_cast<half4 *>(o + out.low + n * out.stride + m) = lo;
-          for (int r = 0; r < 4; ++r) t[across.low + (m + r) * across.stride + n] = lo[r];
-        }
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)(acc[i][j][r] - (float)(half)acc[i][j][r]);
+        Turn::put(own, i, j, lane, v);
       }
+    store(o + out.low, t + across.low, m0, n0, lane, p, own, Turn{});
+  }
+  template <class Turn>
+  __device__ __forceinline__ void store(half *o, half *t, int m0, int n0, int lane, const Product &p, const char *own, Turn) const {
+    Turn::along_m(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
+      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(o + (n0 + y) * out.stride + m0 + x) = v;
+    });
+    Turn::along_n(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
+      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(t + (m0 + x) * across.stride + n0 + y) = v;
+    });
   }
 };
 
@@ -284,7 +305,7 @@ struct StoreResult : emrs_gemm::Operand {
   float keep, rate;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &) const {
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &, char *) const {
     const half *x = in.p + w.batch * in.batch;
     __bf16 *o = has_out ? static_cast<__bf16 *>(out.p[w.batch]) : nullptr;
     __bf16 *img = has_image ? static_cast<__bf16 *>(image.p[w.batch]) : nullptr;
@@ -326,6 +347,297 @@ struct StoreResult : emrs_gemm::Operand {
     }
   }
 };
+
+// ---- small matrices: the whole update of one in one workgroup ----
+//
+// A matrix whose X, in two parts, fits in a CU's LDS beside the polynomial stays there for all its steps: one
+// launch and no memory traffic in place of three launches a step, which cost 5 us each whatever their work.
+// X lies [s][l] (s: the shorter side, padded to 32; l to 64), units of 16 bytes permuted by s; the product
+// X <- P X takes the columns of X as rows through the transposing LDS read.  LDS reads bound it, so a
+// wave of the S x S products computes 32 x 32, on or below the diagonal; where that leaves waves over, KS of
+// them share one over k.  For P X a wave has all S of every 16th 16 of L.
+
+struct Small {
+  Update u;
+  Table<void *> out, image;
+  Table<float *> main;
+  int64_t out_stride, image_stride, main_stride;
+  int32_t has_out, has_image, has_main, tall, fours;
+  int32_t s, l, steps;
+  float eps, scale, keep, rate;
+  float coefficients[3 * EMRS_MUON_MAX_STEPS];
+};
+
+constexpr int kSmallLds = 160 * 1024, kSmallWaves = 16;
+
+constexpr int small_poly_stride(int s) { return s <= 64 ? 64 : 128; }
+constexpr int small_blocks(int s) { return (s / 32) * (s / 32 + 1) / 2; }         // of 32 x 32, with the diagonal's
+constexpr int small_shares(int s) { return s <= 32 ? 8 : s <= 64 ? 4 : 1; }       // waves of one over k
+constexpr int small_fixed(int s) { return 2 * s * small_poly_stride(s) + (small_shares(s) - 1) * small_blocks(s) * 4096; }
+constexpr int64_t small_bytes(int64_t s, int64_t l) { return 4 * s * l + small_fixed((int)s); }
+
+// Rows of tiles of P X that a wave may have, for S = 16 ST: as many as LDS can hold.
+template <int ST>
+constexpr int small_rounds() {
+  constexpr int s = 16 * ST, l = (kSmallLds - small_fixed(s)) / (4 * s) / 64 * 64;
+  return (l / 16 + kSmallWaves - 1) / kSmallWaves;
+}
+
+template <int ST>
+__global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(Small a) {
+  constexpr int S = 16 * ST, PS = small_poly_stride(S), R = small_rounds<ST>();
+  constexpr int KS = small_shares(S), BLOCKS = small_blocks(S);
+  static_assert(KS * BLOCKS <= kSmallWaves, "a wave each");
+  __shared__ __attribute__((aligned(1024))) char lds[kSmallLds];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lp = (a.l + 63) / 64 * 64;
+  half *const hi = reinterpret_cast<half *>(lds), *const lo = hi + S * lp, *const poly = lo + S * lp;
+  f32x4 *const shares = reinterpret_cast<f32x4 *>(poly + S * PS);
+  // Rows of a multiple of 256 bytes begin in the same bank: 16 units take part in the permutation, else 8.
+  const int x_mask = lp % 128 == 0 ? 15 : 7;
+  constexpr int p_mask = PS == 128 ? 15 : 7;
+  auto x_at = [&](int s, int l) { return s * lp + (((l >> 3) ^ (s & x_mask)) << 3) + (l & 7); };
+  auto p_at = [&](int s, int k) { return s * PS + (((k >> 3) ^ (s & p_mask)) << 3) + (k & 7); };
+
+  // The momentum, and the norm.  Eight elements a thread at once: their loads are on their way together.
+  constexpr int kThreads = kSmallWaves * 64, kBatch = 8;
+  const int rows = a.u.rows, cols = a.u.cols, n = rows * cols;
+  const void *const grad = a.u.grad.p[b];
+  float *const buf = a.u.has_momentum ? a.u.momentum.p[b] : nullptr;
+  const float over_cols = 1.f / (float)cols;  // n is below 2^16: the product's floor is the quotient
+  auto row_of = [&](int at, float over) { return (int)(((float)at + 0.5f) * over); };
+  float sum = 0.f;
+  for (int from = threadIdx.x; from < n; from += kThreads * kBatch) {
+    float g[kBatch], m[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = from + i * kThreads, r = row_of(at, over_cols), c = at - r * cols;
+      g[i] = at < n ? grad_at(grad, a.u.grad_dtype, r * a.u.grad_stride + c) : 0.f;
+      m[i] = buf && at < n ? buf[r * a.u.momentum_stride + c] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = from + i * kThreads, r = row_of(at, over_cols), c = at - r * cols;
+      float v = g[i];
+      if (buf) {
+        m[i] = a.u.mu * m[i] + g[i];
+        if (at < n) buf[r * a.u.momentum_stride + c] = m[i];
+        v = a.u.nesterov ? g[i] + a.u.mu * m[i] : m[i];
+      }
+      sum += v * v;
+    }
+  }
+  float *const part = reinterpret_cast<float *>(lds);
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) part[wave] = sum;
+  __syncthreads();
+  float norm = 0.f;
+  for (int i = 0; i < kSmallWaves; ++i) norm += part[i];
+  __syncthreads();
+  const float by = a.scale / (sqrtf(norm) + a.eps);
+  // X_0, with zeros in its padding.  Lanes run along the caller's rows.
+  const int all_cols = a.tall ? S : lp, all = S * lp;
+  const float over_all = 1.f / (float)all_cols;
+  for (int from = threadIdx.x; from < all; from += kThreads * kBatch) {
+    float g[kBatch], m[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = from + i * kThreads, r = row_of(at, over_all), c = at - r * all_cols;
+      const bool in = r < rows && c < cols;
+      g[i] = in ? grad_at(grad, a.u.grad_dtype, r * a.u.grad_stride + c) : 0.f;
+      m[i] = buf && in ? buf[r * a.u.momentum_stride + c] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int at = from + i * kThreads, r = row_of(at, over_all), c = at - r * all_cols;
+      if (at >= all) continue;
+      const float v = (buf ? a.u.nesterov ? g[i] + a.u.mu * m[i] : m[i] : g[i]) * by;
+      const half h = (half)v;
+      const int o = a.tall ? x_at(c, r) : x_at(r, c);
+      hi[o] = h;
+      lo[o] = (half)(v - (float)h);
+    }
+  }
+  __syncthreads();
+
+  typedef __attribute__((ext_vector_type(4))) short s16x4;
+  typedef __attribute__((ext_vector_type(8))) short s16x8;
+  typedef __attribute__((address_space(3))) s16x4 *lds4;
+  const int t = lane & 15, q = lane >> 4;
+  // This wave's block of the S x S products, rows from `bi` and columns from `bj` on, and its share of k.
+  const int share = wave / BLOCKS, block = wave % BLOCKS;
+  int bi = 0;
+  while ((bi + 1) * (bi + 2) / 2 <= block) ++bi;
+  const int bj = (block - bi * (bi + 1) / 2) * 32;
+  bi *= 32;
+  auto from_rows = [&](const half *x, int s, int k) { return *reinterpret_cast<const emrs_gemm::fp16x8 *>(x + x_at(s, k)); };
+  auto from_columns = [&](half *x, int l, int s) __attribute__((always_inline)) {  // eight s of column l + t
+    const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(x + x_at(s + (t >> 2), l + (t & 3) * 4)));
+    const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(x + x_at(s + 4 + (t >> 2), l + (t & 3) * 4)));
+    return __builtin_bit_cast(emrs_gemm::fp16x8, (s16x8)__builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  f32x4 acc[R][ST];
+#pragma unroll 1
+  for (int step = 0; step < a.steps; ++step) {
+    const float fa = a.coefficients[3 * step], fb = a.coefficients[3 * step + 1], fc = a.coefficients[3 * step + 2];
+    const bool split = a.steps - step > 2;
+    f32x4 gram[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) gram[i / 2][i % 2] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (share < KS) {
+#pragma unroll 1
+      for (int k = share * 32; k < lp; k += KS * 32) {
+        emrs_gemm::fp16x8 m[2], n[2], m_lo[2], n_lo[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          m[i] = from_rows(hi, bi + i * 16 + t, k + q * 8), n[i] = from_rows(hi, bj + i * 16 + t, k + q * 8);
+          if (split) m_lo[i] = from_rows(lo, bi + i * 16 + t, k + q * 8), n_lo[i] = from_rows(lo, bj + i * 16 + t, k + q * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f32x4 &c = gram[i / 2][i % 2];
+          c = emrs_gemm::mfma(m[i / 2], n[i % 2], c);
+          if (split) c = emrs_gemm::mfma(m_lo[i / 2], n[i % 2], emrs_gemm::mfma(m[i / 2], n_lo[i % 2], c));
+        }
+      }
+    }
+    if (KS > 1) {
+      if (share > 0 && share < KS)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) shares[(((share - 1) * BLOCKS + block) * 4 + i) * 64 + lane] = gram[i / 2][i % 2];
+      __syncthreads();
+      if (share == 0)
+#pragma unroll
+        for (int k = 1; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) gram[i / 2][i % 2] += shares[(((k - 1) * BLOCKS + block) * 4 + i) * 64 + lane];
+    }
+    // Entry (m, n) of a block goes to its place and, off the diagonal, across it.
+    auto put = [&](int i, half4 v) __attribute__((always_inline)) {
+      const int m = bi + i / 2 * 16 + q * 4, n = bj + i % 2 * 16 + t;
+      *reinterpret_cast<half4 *>(poly + p_at(n, m)) = v;
+      if (bi != bj)
+        for (int r = 0; r < 4; ++r) poly[p_at(m + r, n)] = v[r];
+    };
+    if (share == 0) {
+      const float g = kGramScale / (a.scale * a.scale);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        half4 v;  // rounded as the product that squares it sees it
+        for (int r = 0; r < 4; ++r) v[r] = (half)(gram[i / 2][i % 2][r] * g), gram[i / 2][i % 2][r] = (float)v[r];
+        put(i, v);
+      }
+    }
+    __syncthreads();
+    f32x4 square[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) square[i / 2][i % 2] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto from_poly = [&](int s, int k) { return *reinterpret_cast<const emrs_gemm::fp16x8 *>(poly + p_at(s, k)); };
+    if (share == 0) {
+#pragma unroll 2
+      for (int k = 0; k < S; k += 32) {
+        emrs_gemm::fp16x8 m[2], n[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[i] = from_poly(bi + i * 16 + t, k + q * 8), n[i] = from_poly(bj + i * 16 + t, k + q * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) square[i / 2][i % 2] = emrs_gemm::mfma(m[i / 2], n[i % 2], square[i / 2][i % 2]);
+      }
+    }
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = bi + i / 2 * 16 + q * 4, n = bj + i % 2 * 16 + t;
+        half4 v;
+        for (int r = 0; r < 4; ++r)
+          v[r] = (half)((!split && m + r == n ? fa * kGramScale : 0.f) + fb * gram[i / 2][i % 2][r] + fc / kGramScale * square[i / 2][i % 2][r]);
+        put(i, v);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int l = (wave + r * kSmallWaves) * 16;
+#pragma unroll
+      for (int j = 0; j < ST; ++j) acc[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (l < lp) {
+#pragma unroll 1
+        for (int k = 0; k < S; k += 32) {
+          const emrs_gemm::fp16x8 m = from_columns(hi, l, k + q * 8);
+          emrs_gemm::fp16x8 m_lo;
+          if (split) m_lo = from_columns(lo, l, k + q * 8);
+#pragma unroll
+          for (int j = 0; j < ST; ++j) {
+            const emrs_gemm::fp16x8 n = from_poly(j * 16 + t, k + q * 8);
+            acc[r][j] = emrs_gemm::mfma(m, n, acc[r][j]);
+            if (split) acc[r][j] = emrs_gemm::mfma(m_lo, n, acc[r][j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < ST; ++j) {
+          const int o = x_at(j * 16 + t, l + q * 4);
+          acc[r][j] *= 1.f / kGramScale;
+          if (split) {
+            const half4 x = *reinterpret_cast<const half4 *>(hi + o), y = *reinterpret_cast<const half4 *>(lo + o);
+            for (int i = 0; i < 4; ++i) acc[r][j][i] += fa * ((float)x[i] + (float)y[i]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (step + 1 == a.steps) break;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int l = (wave + r * kSmallWaves) * 16;
+      if (l >= lp) continue;
+#pragma unroll
+      for (int j = 0; j < ST; ++j) {
+        const int o = x_at(j * 16 + t, l + q * 4);
+        half4 x, y;
+        for (int i = 0; i < 4; ++i) x[i] = (half)acc[r][j][i], y[i] = (half)(acc[r][j][i] - (float)x[i]);
+        *reinterpret_cast<half4 *>(hi + o) = x;
+        *reinterpret_cast<half4 *>(lo + o) = y;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < ST; ++j) {
+      __builtin_amdgcn_sched_barrier(0);  // one tile's addresses at a time: registers
+      if (a.fours) {  // four of a row's elements, which lie so
+        const int l = (wave + r * kSmallWaves) * 16 + q * 4, s = j * 16 + t;
+        if (s >= a.s || l >= a.l) continue;
+        f32x4 v = acc[r][j] * (1.f / a.scale);
+        if (a.has_main) {
+          f32x4 *const w = reinterpret_cast<f32x4 *>(a.main.p[b] + s * a.main_stride + l);
+          v = *w * a.keep - a.rate * v;
+          *w = v;
+        }
+        bf16x4 h;
+        for (int i = 0; i < 4; ++i) h[i] = (__bf16)v[i];
+        if (a.has_out) *reinterpret_cast<bf16x4 *>(static_cast<__bf16 *>(a.out.p[b]) + s * a.out_stride + l) = h;
+        if (a.has_image) *reinterpret_cast<bf16x4 *>(static_cast<__bf16 *>(a.image.p[b]) + s * a.image_stride + l) = h;
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int l = (wave + r * kSmallWaves) * 16 + q * 4 + i, s = j * 16 + t;
+        if (s >= a.s || l >= a.l) continue;
+        const int64_t row = a.tall ? l : s, col = a.tall ? s : l;
+        float v = acc[r][j][i] * (1.f / a.scale);
+        if (a.has_main) {
+          float *const w = a.main.p[b] + row * a.main_stride + col;
+          v = *w * a.keep - a.rate * v;
+          *w = v;
+        }
+        if (a.has_out) static_cast<__bf16 *>(a.out.p[b])[row * a.out_stride + col] = (__bf16)v;
+        if (a.has_image) static_cast<__bf16 *>(a.image.p[b])[row * a.image_stride + col] = (__bf16)v;
+      }
+    }
+}
 
 struct Sizes {
   uint64_t s, l;                             // padded sides
@@ -407,6 +719,24 @@ bool fours(const emrs_muon *a, const void *const *p, uint64_t stride, uint64_t b
     if (e_ != hipSuccess) return fail(EMRS_ERR_HIP, std::string("muon: ") + hipGetErrorString(e_)); \
   } while (0)
 
+Small small_of(const emrs_muon *a, const Update &u, float scale, bool fours) {
+  Small k{};
+  k.u = u;
+  for (uint32_t i = 0; i < a->count; ++i) {
+    if (a->out) k.out.p[i] = a->out[i];
+    if (a->image) k.image.p[i] = a->image[i];
+    if (a->main) k.main.p[i] = a->main[i];
+  }
+  k.out_stride = a->out_stride, k.image_stride = a->image_stride, k.main_stride = a->main_stride;
+  k.has_out = a->out != nullptr, k.has_image = a->image != nullptr, k.has_main = a->main != nullptr;
+  k.tall = a->rows > a->cols, k.fours = fours && !k.tall;
+  k.s = (int)std::min(a->rows, a->cols), k.l = (int)std::max(a->rows, a->cols);
+  k.steps = (int)a->steps;
+  k.eps = a->eps, k.scale = scale, k.keep = 1.f - a->decay, k.rate = a->rate;
+  std::copy(a->coefficients, a->coefficients + 3 * a->steps, k.coefficients);
+  return k;
+}
+
 template <bool kWide>
 StoreResult<kWide> result(const emrs_muon *a, const Image &in, int parts, float factor, float scale) {
   StoreResult<kWide> e{};
@@ -441,6 +771,23 @@ int step(const emrs_muon *a, hipStream_t st) {
   u.has_momentum = a->momentum != nullptr, u.nesterov = a->nesterov != 0;
   u.mu = a->mu;
   float *norms = reinterpret_cast<float *>(ws + z.norms);
+  // Entries of an orthogonal S x L matrix are 1 / sqrt(L): the scale of X brings them to 1.
+  const float scale = std::ldexp(1.f, (int)std::lround(0.5 * std::log2((double)z.l)));
+  const bool wide_rows = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
+                         fours(a, reinterpret_cast<const void *const *>(a->image), a->image_stride, 2) &&
+                         fours(a, reinterpret_cast<const void *const *>(a->out), a->out_stride, 2);
+  const int small = (int)round_up(std::min(a->rows, a->cols), 32);
+  if (small <= 128 && small_bytes(small, (int64_t)z.l) <= kSmallLds) {
+    const Small k = small_of(a, u, scale, wide_rows);
+    switch (small) {
+      case 32: small_kernel<2><<<a->count, kSmallWaves * 64, 0, st>>>(k); break;
+      case 64: small_kernel<4><<<a->count, kSmallWaves * 64, 0, st>>>(k); break;
+      case 96: small_kernel<6><<<a->count, kSmallWaves * 64, 0, st>>>(k); break;
+      default: small_kernel<8><<<a->count, kSmallWaves * 64, 0, st>>>(k); break;
+    }
+    TRY(hipGetLastError());
+    return EMRS_OK;
+  }
   const bool wide = fours(a, a->grad, a->grad_stride, grad_bytes) &&
                     fours(a, reinterpret_cast<const void *const *>(a->momentum), a->momentum_stride, 4);
   const dim3 grid(z.blocks, a->count);
@@ -450,8 +797,6 @@ int step(const emrs_muon *a, hipStream_t st) {
     momentum_kernel<false><<<grid, 256, 0, st>>>(u, norms);
   TRY(hipGetLastError());
 
-  // Entries of an orthogonal S x L matrix are 1 / sqrt(L): the scale of X brings them to 1.
-  const float scale = std::ldexp(1.f, (int)std::lround(0.5 * std::log2((double)z.l)));
   auto parts_of = [&](uint32_t k) { return a->steps - k > 2 ? 2 : 1; };
   const int64_t area = 2 * (int64_t)(z.s * z.l);
   auto x = [&](int i) { return Image{reinterpret_cast<half *>(ws + z.x[i]), 2 * (int64_t)z.l, area, (int64_t)z.l}; };
@@ -498,9 +843,6 @@ int step(const emrs_muon *a, hipStream_t st) {
       TRY((emrs_gemm::launch<half>(r, StoreIterate{{}, in, x(now ^ 1), xt(now ^ 1), parts, parts_of(k + 1), f[0]}, st)));
       continue;
     }
-    const bool wide_rows = fours(a, reinterpret_cast<const void *const *>(a->main), a->main_stride, 4) &&
-                           fours(a, reinterpret_cast<const void *const *>(a->image), a->image_stride, 2) &&
-                           fours(a, reinterpret_cast<const void *const *>(a->out), a->out_stride, 2);
     const Image &from = turned ? in_t : in;
     const hipError_t e = wide_rows ? emrs_gemm::launch<half>(r, result<true>(a, from, parts, f[0], scale), st)
                                    : emrs_gemm::launch<half>(r, result<false>(a, from, parts, f[0], scale), st);

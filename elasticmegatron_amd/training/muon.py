@@ -27,30 +27,61 @@ MUON_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 WORKSPACE_BYTES = 8 << 30
 
 
-def _matrices(what: str, m: Matrices) -> List[torch.Tensor]:
-    if isinstance(m, torch.Tensor):
-        if m.dim() not in (2, 3):
-            raise ValueError(f"{what} has {m.dim()} dimensions: a matrix, or a stack of matrices, is wanted")
-        return [m] if m.dim() == 2 else list(m.unbind(0))
-    return list(m)
+class _Stack:
+    """Matrices of one kind and one shape: their addresses and the row stride that they share."""
 
+    def __init__(self, what: str, m: Matrices):
+        self.what = what
+        if isinstance(m, torch.Tensor):
+            if m.dim() not in (2, 3):
+                raise ValueError(f"{what} has {m.dim()} dimensions: a matrix, or a stack of matrices, is wanted")
+            self.tensors, self.count = [m], 1 if m.dim() == 2 else m.shape[0]
+        else:
+            self.tensors = list(m)
+            self.count = len(self.tensors)
+            for t in self.tensors:
+                if not isinstance(t, torch.Tensor):
+                    raise TypeError(f"{what} is no tensor")
+                if t.dim() != 2:
+                    raise ValueError(f"{what} has a member of {t.dim()} dimensions: matrices are wanted")
+        if self.count:
+            self.shape = self.tensors[0].shape[-2:]
+            self.dtype, self.device = self.tensors[0].dtype, self.tensors[0].device
 
-def _check(what: str, ms: List[torch.Tensor], count: int, shape, device, dtype=None) -> None:
-    if len(ms) != count:
-        raise ValueError(f"{what} holds {len(ms)} matrices, the others {count}")
-    for t in ms:
-        on_device(what, t, device)
-        if t.shape != shape or t.dim() != 2:
-            raise ValueError(f"{what} is {tuple(t.shape)}: {tuple(shape)} is wanted, for all matrices of a call")
-        if dtype is not None and t.dtype != dtype:
-            raise TypeError(f"{what} is {t.dtype}: {dtype} is wanted")
-        if t.dtype != ms[0].dtype:
-            raise TypeError(f"{what} holds matrices of several types")
+    def check(self, count: int, shape, device, dtype=None) -> None:
+        """Raises unless there are `count` matrices of that shape, on that device and of one type."""
+        if self.count != count:
+            raise ValueError(f"{self.what} holds {self.count} matrices, the others {count}")
+        for t in self.tensors:
+            on_device(self.what, t, device)
+            if t.shape[-2:] != shape:
+                raise ValueError(f"{self.what} is {tuple(t.shape[-2:])}: {tuple(shape)} is wanted, for all matrices of a call")
+            if dtype is not None and t.dtype != dtype:
+                raise TypeError(f"{self.what} is {t.dtype}: {dtype} is wanted")
+            if t.dtype != self.dtype:
+                raise TypeError(f"{self.what} holds matrices of several types")
 
+    def lay_out(self, copy: bool) -> None:
+        """Addresses and the row stride; matrices that lie otherwise are copied, or refused."""
+        rows, cols = self.shape
+        strides = {t.stride(-2) for t in self.tensors}
+        if any((cols > 1 and t.stride(-1) != 1) or (rows > 1 and t.stride(-2) < cols) for t in self.tensors) or (len(strides) > 1 and rows > 1):
+            if not copy:
+                raise ValueError(f"{self.what} is written in place: unit column stride and one row stride are wanted")
+            self.tensors = [t.contiguous() for t in self.tensors]
+        self.stride = self.tensors[0].stride(-2)
+        if len(self.tensors) == 1 and self.tensors[0].dim() == 3:
+            t = self.tensors[0]
+            step = t.stride(0) * t.element_size()
+            if not copy and self.count > 1 and step < ((rows - 1) * self.stride + cols) * t.element_size():
+                raise ValueError(f"{self.what} is written in place: its matrices overlap")
+            base = t.data_ptr()
+            self.addresses = [base + i * step for i in range(self.count)]
+        else:
+            self.addresses = [t.data_ptr() for t in self.tensors]
 
-def _in_rows(t: torch.Tensor) -> bool:
-    rows, cols = t.shape
-    return (cols == 1 or t.stride(1) == 1) and (rows == 1 or t.stride(0) >= cols)
+    def table(self, lo: int, hi: int):
+        return (ctypes.c_uint64 * (hi - lo))(*self.addresses[lo:hi])
 
 
 def _coefficients(c, steps: int):
@@ -62,62 +93,36 @@ def _coefficients(c, steps: int):
     return (ctypes.c_float * (3 * steps))(*(float(x) for r in rows for x in r))
 
 
-class _Stack:
-    """Matrices of one kind: their addresses and the row stride that they share."""
-
-    def __init__(self, what: str, ms: Optional[List[torch.Tensor]], copy: bool):
-        self.ms = ms
-        if ms is None:
-            return
-        strides = {t.stride(0) for t in ms}
-        if not all(map(_in_rows, ms)) or (len(strides) > 1 and ms[0].shape[0] > 1):
-            if not copy:
-                raise ValueError(f"{what} is written in place: unit column stride and one row stride are wanted")
-            self.ms = [t.contiguous() for t in ms]
-        self.stride = self.ms[0].stride(0)
-
-    def table(self, lo: int, hi: int):
-        return None if self.ms is None else (ctypes.c_uint64 * (hi - lo))(*(t.data_ptr() for t in self.ms[lo:hi]))
-
-
-def _run(grad, momentum, main, image, out, *, steps, coefficients, eps, mu, nesterov, decay, rate) -> None:
+def _run(kinds, *, steps, coefficients, eps, mu, nesterov, decay, rate) -> None:
     """One native call for as many matrices as its workspace allows, until all are done."""
-    device, (rows, cols) = grad.ms[0].device, grad.ms[0].shape
+    grad = kinds["grad"]
+    for name, k in kinds.items():
+        k.lay_out(copy=name == "grad")
     a = _native.Muon()
-    a.grad_dtype = dtype_code(grad.ms[0], "grad")
-    a.rows, a.cols, a.steps, a.nesterov = rows, cols, steps, int(nesterov)
+    a.grad_dtype = dtype_code(grad.tensors[0], "grad")
+    a.rows, a.cols, a.steps, a.nesterov = *grad.shape, steps, int(nesterov)
     a.coefficients = ctypes.addressof(coefficients)
     a.mu, a.eps, a.decay, a.rate = mu, eps, decay, rate
     a.count = 1
-    count = len(grad.ms)
-    at_once = min(count, _native.EMRS_MUON_MAX_MATRICES, max(1, WORKSPACE_BYTES // _native.muon_workspace(a)))
-    a.count = at_once
-    scratch = workspace(_native.muon_workspace(a), device)
+    at_once, size = grad.count, 0
+    if grad.count > 1:
+        at_once = min(grad.count, _native.EMRS_MUON_MAX_MATRICES, max(1, WORKSPACE_BYTES // _native.muon_workspace(a)))
+        a.count = at_once
+    size = _native.muon_workspace(a)
+    scratch = workspace(size, grad.device)
     a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
-    kinds = [("grad", grad), ("momentum", momentum), ("main", main), ("image", image), ("out", out)]
-    for lo in range(0, count, at_once):
-        hi = min(count, lo + at_once)
-        a.count = hi - lo
-        tables = [s.table(lo, hi) for _, s in kinds]
-        for (name, s), t in zip(kinds, tables):
-            setattr(a, name, None if t is None else ctypes.addressof(t))
-            if t is not None:
-                setattr(a, name + "_stride", s.stride)
-        with torch.cuda.device(device):
-            _native.muon_step(a, stream_of(device))
+    with torch.cuda.device(grad.device):
+        for lo in range(0, grad.count, at_once):
+            hi = min(grad.count, lo + at_once)
+            a.count = hi - lo
+            tables = {name: k.table(lo, hi) for name, k in kinds.items()}
+            for name, t in tables.items():
+                setattr(a, name, ctypes.addressof(t))
+                setattr(a, name + "_stride", kinds[name].stride)
+            _native.muon_step(a, stream_of(grad.device))
 
 
-def _head(grad: Matrices):
-    g = _matrices("grad", grad)
-    if not g:
-        return g, None, None
-    if not isinstance(g[0], torch.Tensor):
-        raise TypeError("grad is no tensor")
-    _check("grad", g, len(g), g[0].shape, g[0].device)
-    dtype_code(g[0], "grad")
-    return g, g[0].shape, g[0].device
-
-
+@torch.no_grad()
 def orthogonalise(matrices: Matrices, *, steps: int = 5, coefficients=MUON_COEFFICIENTS,
                   eps: float = 1e-7) -> Union[torch.Tensor, List[torch.Tensor]]:
     """``matrices`` (fp32, bf16 or fp16; one matrix, a stack [n, rows, cols], or a sequence of matrices of
@@ -126,16 +131,18 @@ def orthogonalise(matrices: Matrices, *, steps: int = 5, coefficients=MUON_COEFF
     ``coefficients``: (a, b, c), or one such triple for each step; they have to keep singular values in
     [0, 1] bounded.  A matrix of zeros stays zeros.
     """
-    g, shape, device = _head(matrices)
+    g = _Stack("matrices", matrices)
     coefficients = _coefficients(coefficients, steps)
-    stacked = torch.empty((len(g), *(shape or (0, 0))), dtype=torch.bfloat16, device=device)
-    if g and shape.numel():
-        _run(_Stack("matrices", [t.detach() for t in g], True), _Stack("", None, True), _Stack("", None, True),
-             _Stack("", None, True), _Stack("out", list(stacked.unbind(0)), False), steps=steps, coefficients=coefficients, eps=eps,
-             mu=0.0, nesterov=False, decay=0.0, rate=0.0)
-    if isinstance(matrices, torch.Tensor):
-        return stacked.view(matrices.shape)
-    return list(stacked.unbind(0))
+    single = isinstance(matrices, torch.Tensor)
+    if g.count:
+        g.check(g.count, g.shape, g.device)
+        dtype_code(g.tensors[0], "matrices")
+        out = torch.empty((g.count, *g.shape), dtype=torch.bfloat16, device=g.device)
+        if g.shape.numel():
+            _run({"grad": g, "out": _Stack("out", out)}, steps=steps, coefficients=coefficients, eps=eps, mu=0.0, nesterov=False,
+                 decay=0.0, rate=0.0)
+        return out.view(matrices.shape) if single else list(out.unbind(0))
+    return torch.empty(matrices.shape, dtype=torch.bfloat16, device=matrices.device) if single else []
 
 
 @torch.no_grad()
@@ -155,20 +162,21 @@ def muon_step(main: Matrices, momentum_buffer: Matrices, grad: Matrices, *, mode
     ``lr * rms_scale``, as AdamW's are with 0.2.  A matrix is taken as it is given: one that tensor
     parallelism or a distributed optimizer has cut is to be gathered first.
     """
-    g, shape, device = _head(grad)
-    w, b = _matrices("main", main), _matrices("momentum_buffer", momentum_buffer)
-    img = None if model is None else _matrices("model", model)
+    g, w, b = _Stack("grad", grad), _Stack("main", main), _Stack("momentum_buffer", momentum_buffer)
+    img = None if model is None else _Stack("model", model)
     coefficients = _coefficients(coefficients, steps)
-    if not g and not w and not b and not img:
+    if not g.count:
+        if w.count or b.count or (img is not None and img.count):
+            raise ValueError("grad holds no matrices")
         return
-    if not g:
-        raise ValueError("grad holds no matrices")
-    _check("main", w, len(g), shape, device, torch.float32)
-    _check("momentum_buffer", b, len(g), shape, device, torch.float32)
+    g.check(g.count, g.shape, g.device)
+    dtype_code(g.tensors[0], "grad")
+    w.check(g.count, g.shape, g.device, torch.float32)
+    b.check(g.count, g.shape, g.device, torch.float32)
+    kinds = {"grad": g, "momentum": b, "main": w}
     if img is not None:
-        _check("model", img, len(g), shape, device, torch.bfloat16)
-    if not shape.numel():
-        return
-    _run(_Stack("grad", g, True), _Stack("momentum_buffer", b, False), _Stack("main", w, False), _Stack("model", img, False),
-         _Stack("", None, False), steps=steps, coefficients=coefficients, eps=eps, mu=momentum, nesterov=nesterov,
-         decay=lr * weight_decay, rate=lr * rms_scale * math.sqrt(max(shape)))
+        img.check(g.count, g.shape, g.device, torch.bfloat16)
+        kinds["image"] = img
+    if g.shape.numel():
+        _run(kinds, steps=steps, coefficients=coefficients, eps=eps, mu=momentum, nesterov=nesterov, decay=lr * weight_decay,
+             rate=lr * rms_scale * math.sqrt(max(g.shape)))
