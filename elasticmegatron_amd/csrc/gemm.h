@@ -373,9 +373,19 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
 
 enum Shape { kLarge, kMedium, kSmall };
 
-// The largest tile that keeps most CUs busy: a larger one reads its operands fewer times from the caches.
+// What a launch of one tile size takes, in microseconds, by its rounds of 256 workgroups (each has a CU's LDS
+// for itself): measured are 1.25 for a large tile's stage, 1.05 for the stage that each of a medium tile's
+// two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside its stages.
+template <class Cfg>
+inline double cost_of(const Product &p, double stage, double fixed) {
+  const int64_t rounds = (tile_count<Cfg>(p) + 255) / 256, stages = (tiles_of(p.k, kStage) + Cfg::GROUPS - 1) / Cfg::GROUPS;
+  return (double)rounds * (fixed + stage * (double)stages);
+}
+
+// Large tiles read the operands fewer times; smaller ones give more CUs work, and their waves share a long k.
 inline Shape shape_of(const Product &p) {
-  return tile_count<Large>(p) >= 192 ? kLarge : tile_count<Medium>(p) >= 128 ? kMedium : kSmall;
+  const double large = cost_of<Large>(p, 1.25, 8), medium = cost_of<Medium>(p, 1.05, 4), small = cost_of<Small>(p, 0.95, 3);
+  return large <= medium && large <= small ? kLarge : medium <= small ? kMedium : kSmall;
 }
 
 template <class T, class Cfg, class Epilogue>

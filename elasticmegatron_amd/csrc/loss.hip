@@ -117,32 +117,102 @@ struct TileStatistics : Piece {
   }
 };
 
-constexpr int kMergeTokens = 16, kMergeThreads = 256;
+// ---- forward, one token ----
+//
+// The weight's bytes bound the call, and vector arithmetic keeps up with one token (with two it does not: 55 us
+// against the tiles' 51 on 32000 rows of 4096).  A workgroup reads 32 rows of a shard, eight at a time, each in
+// whole consecutive kilobytes, the order that memory serves fastest: 6.2 TB/s on 128256 rows of 4096 (tiles:
+// 4.6; a wave's 16 rows straight into fragments: 3.7).  Every thread multiplies 8 of each 2048 k for all eight
+// rows; the 256 partial sums of a row meet in LDS.
 
-// Joins the pairs of every tile: one workgroup for 16 tokens, 16 lanes apart over the slots.
+constexpr int kOneRows = 32, kOneAtOnce = 8, kOneThreads = 256;
+
+template <class T>
+__global__ __launch_bounds__(kOneThreads) void one_token_kernel(Piece piece, int64_t stride, int rows, const T *hidden, int k, float2 *pairs,
+                                                                float *target_logit, const int64_t *target) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  constexpr int lanes = kOneThreads / kOneAtOnce;  // threads that add one row's parts
+  __shared__ float part[kOneAtOnce][kOneThreads];
+  __shared__ float x[kOneRows];
+  const int m0 = blockIdx.x * kOneRows, batch = blockIdx.y, tid = threadIdx.x;
+  const T *const w = static_cast<const T *>(piece.weights.p[batch]);
+#pragma unroll 1
+  for (int pass = 0; pass < kOneRows; pass += kOneAtOnce) {
+    float acc[kOneAtOnce];
+#pragma unroll
+    for (int i = 0; i < kOneAtOnce; ++i) acc[i] = 0.f;
+#pragma unroll 2
+    for (int at = tid * 8; at < k; at += kOneThreads * 8) {
+      x8 a[kOneAtOnce];  // rows past the last one read it again, and are left out below
+#pragma unroll
+      for (int i = 0; i < kOneAtOnce; ++i)
+        a[i] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(w + min(m0 + pass + i, rows - 1) * stride + at));
+      const x8 b = *reinterpret_cast<const x8 *>(hidden + at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < kOneAtOnce; ++i) acc[i] = fmaf((float)a[i][e], (float)b[e], acc[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOneAtOnce; ++i) part[i][tid] = acc[i];
+    __syncthreads();
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < kOneThreads / lanes; ++i) v += part[tid / lanes][tid % lanes + i * lanes];
+#pragma unroll
+    for (int o = lanes / 2; o; o /= 2) v += __shfl_xor(v, o);
+    if (tid % lanes == 0) x[pass + tid / lanes] = v;
+  }
+  __syncthreads();
+  if (tid >= kOneRows) return;
+  const int valid = piece.valid(batch, rows);
+  const int64_t at = target[0] - piece.first_of(batch) - m0;
+  if (m0 + tid < valid && at == tid) target_logit[0] = x[tid];
+  const float own = m0 + tid < valid ? x[tid] : -INFINITY;
+  float top = own;
+  for (int o = kOneRows / 2; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+  float sum = exp_of(own - (top == -INFINITY ? 0.f : top));
+  for (int o = kOneRows / 2; o; o /= 2) sum += __shfl_xor(sum, o);
+  if (tid == 0) pairs[(int64_t)batch * gridDim.x + blockIdx.x] = float2{top, sum};
+}
+
+// Joins the pairs of every tile: a workgroup for kTokens tokens, the lanes of one token spread over the
+// slots, four of them at once.
+constexpr int kMergeThreads = 256;
+
+__device__ inline void join_pair(float &top, float &sum, float2 v) {
+  const float up = fmaxf(top, v.x), shift = up == -INFINITY ? 0.f : up;
+  sum = sum * exp_of(top - shift) + v.y * exp_of(v.x - shift);
+  top = up;
+}
+
+template <int kTokens>
 __global__ __launch_bounds__(kMergeThreads) void merge_statistics_kernel(const float2 *pairs, int64_t slots, int tokens,
                                                                          const int64_t *target, int64_t ignore, int64_t first,
                                                                          int64_t last, float *lse, float *target_logit,
                                                                          float *loss) {
+  constexpr int lanes = kMergeThreads / kTokens;
   __shared__ float2 part[kMergeThreads];
-  const int t = blockIdx.x * kMergeTokens + threadIdx.x % kMergeTokens;
+  const int t = blockIdx.x * kTokens + threadIdx.x % kTokens;
   float top = -INFINITY, sum = 0.f;
   if (t < tokens)
-    for (int64_t s = threadIdx.x / kMergeTokens; s < slots; s += kMergeThreads / kMergeTokens) {
-      const float2 v = pairs[s * tokens + t];
-      const float up = fmaxf(top, v.x), shift = up == -INFINITY ? 0.f : up;
-      sum = sum * exp_of(top - shift) + v.y * exp_of(v.x - shift);
-      top = up;
+    for (int64_t s = threadIdx.x / kTokens; s < slots; s += 4 * lanes) {
+      float2 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = s + i * lanes < slots ? pairs[(s + i * lanes) * tokens + t] : float2{-INFINITY, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) join_pair(top, sum, v[i]);
     }
   part[threadIdx.x] = float2{top, sum};
-  __syncthreads();
-  if (threadIdx.x >= kMergeTokens || t >= tokens) return;
-  for (int i = 1; i < kMergeThreads / kMergeTokens; ++i) {
-    const float2 v = part[i * kMergeTokens + threadIdx.x];
-    const float up = fmaxf(top, v.x), shift = up == -INFINITY ? 0.f : up;
-    sum = sum * exp_of(top - shift) + v.y * exp_of(v.x - shift);
-    top = up;
+  for (int half = lanes / 2; half; half /= 2) {
+    __syncthreads();
+    if ((int)threadIdx.x < half * kTokens) {
+      join_pair(top, sum, part[threadIdx.x + half * kTokens]);
+      part[threadIdx.x] = float2{top, sum};
+    }
   }
+  if (threadIdx.x >= kTokens || t >= tokens) return;
   const float l = (top == -INFINITY ? 0.f : top) + logf(sum);
   const int64_t at = target[t];
   const float x = at >= first && at < last ? target_logit[t] : -INFINITY;
@@ -468,6 +538,11 @@ Product logits_of(const emrs_loss *a, const Sizes &s, const Group &g, uint64_t r
   return p;
 }
 
+// Partial statistics that a shard's `rows` rows leave for each token.
+int64_t slots_of(const emrs_loss *a, const Product &p) {
+  return a->tokens == 1 ? emrs_gemm::tiles_of(p.m, kOneRows) : emrs_gemm::wave_rows(p);
+}
+
 Sizes sizes_of(const emrs_loss *a, bool backward) {
   Sizes s{};
   uint64_t most = 1, shards = 1;
@@ -489,7 +564,7 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   uint64_t slots = 0;
   for (uint32_t i = 0; i < s.n_groups; ++i)
     for (uint64_t lo = 0; lo < a->shard_rows[s.groups[i].first]; lo += s.piece)
-      slots += emrs_gemm::wave_rows(logits_of(a, s, s.groups[i], std::min(s.piece, a->shard_rows[s.groups[i].first] - lo))) * s.groups[i].count;
+      slots += slots_of(a, logits_of(a, s, s.groups[i], std::min(s.piece, a->shard_rows[s.groups[i].first] - lo))) * s.groups[i].count;
   // grad_hidden's product has few tiles where there are few tokens: its sum over the vocabulary is cut into
   // runs of at least 1024 rows, as many as give every CU a tile.
   const uint64_t k = round_up(std::min(s.piece, most), 64) * shards;
@@ -574,15 +649,25 @@ int forward(const emrs_loss *a, hipStream_t st) {
       if (rc) return rc;
       Product p = logits_of(a, s, g, rows);
       p.b = hidden;
-      const int64_t each = emrs_gemm::wave_rows(p);
-      TRY((emrs_gemm::launch<T>(p, TileStatistics{c, pairs + slots * (int64_t)a->tokens, a->target_logit, a->target, each}, st)));
+      const int64_t each = slots_of(a, p);
+      float2 *const out = pairs + slots * (int64_t)a->tokens;
+      if (a->tokens == 1) {
+        one_token_kernel<T><<<dim3((uint32_t)each, g.count), kOneThreads, 0, st>>>(c, p.a_stride, p.m, static_cast<const T *>(hidden), p.k, out,
+                                                                                a->target_logit, a->target);
+        TRY(hipGetLastError());
+      } else {
+        TRY((emrs_gemm::launch<T>(p, TileStatistics{c, out, a->target_logit, a->target, each}, st)));
+      }
       slots += each * g.count;
     }
     first += all * g.count;
   }
   const int64_t last = (int64_t)std::max(a->vocab_start, std::min(first, a->vocab_size));
-  merge_statistics_kernel<<<(a->tokens + kMergeTokens - 1) / kMergeTokens, kMergeThreads, 0, st>>>(
-      pairs, slots, (int)a->tokens, a->target, a->ignore_index, (int64_t)a->vocab_start, last, a->lse, a->target_logit, a->loss);
+  // Few tokens: all of a workgroup on one, so that its many slots are not read one after another.
+  const auto merge = a->tokens <= 256 ? merge_statistics_kernel<1> : merge_statistics_kernel<16>;
+  const uint64_t each = a->tokens <= 256 ? 1 : 16;
+  merge<<<(a->tokens + each - 1) / each, kMergeThreads, 0, st>>>(pairs, slots, (int)a->tokens, a->target, a->ignore_index, (int64_t)a->vocab_start,
+                                                              last, a->lse, a->target_logit, a->loss);
   TRY(hipGetLastError());
   return EMRS_OK;
 }

@@ -114,17 +114,15 @@ class _LinearCrossEntropy(torch.autograd.Function):
         call = _Call(hidden, shards, target, 0, vocab_size, ignore_index)
         lse, _, loss = call.forward(True)
         ctx.save_for_backward(hidden, target, lse, *shards)
-        ctx.rest = (vocab_size, ignore_index)
+        ctx.call = call  # views of the same inputs, checked already
         return loss.view(target.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        hidden, target, lse, *shards = ctx.saved_tensors
-        vocab_size, ignore_index = ctx.rest
-        call = _Call(hidden, shards, target, 0, vocab_size, ignore_index)
+        hidden, _, lse, *_ = ctx.saved_tensors  # raises where an input was changed in place
         grad_loss = grad_loss.reshape(-1).to(torch.float32).contiguous()
-        gh, gw = call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
+        gh, gw = ctx.call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
         return (None if gh is None else gh.view(hidden.shape), None, None, None, *gw)
 
 
