@@ -360,7 +360,7 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float *sum, int su
 
 // ---- scales: powers of two that bring the largest finite entry to [2^13, 2^14), and |grad_loss| likewise ----
 
-constexpr int kScaleBlocks = 2048;
+constexpr int kScaleBlocks = 1024;  // workgroups that look for the largest entries of one kind
 
 __device__ inline float block_max(float v) {
   __shared__ float part[4];
@@ -377,50 +377,72 @@ __device__ inline float scale_of(float top) {
   return ldexpf(1.f, min(max(14 - e, -100), 100));
 }
 
-// Largest finite |entry| of the rows of each matrix, without those of ignored tokens: one value a workgroup.
+// Rows of one kind that become a transposed operand: a group's weight rows, or the hidden states.
+struct Rows {
+  Piece piece;
+  int64_t stride;
+  int32_t rows, count;    // of each matrix; matrices
+  int32_t blocks;         // workgroups that look for a matrix's largest entry; 0: fp16, copied unscaled
+  const int64_t *target;  // NULL, or: rows whose target is `ignore` do not count
+  int64_t ignore;
+  float *largest;         // [count x blocks]
+  float *scale;           // written by the transposition
+};
+
 template <class T>
-__global__ __launch_bounds__(256) void largest_kernel(Piece piece, int64_t stride, int rows, int cols, const int64_t *target, int64_t ignore,
-                                                      float *largest) {
+__device__ float largest_of(const Rows &a, int matrix, int block, int cols) {
   using x8 = typename emrs_gemm::Vec<T>::x8;
-  const T *in = static_cast<const T *>(piece.weights.p[blockIdx.y]);
-  const int valid = piece.valid(blockIdx.y, rows);
-  const bool wide = cols % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+  const T *in = static_cast<const T *>(a.piece.weights.p[matrix]);
+  const int valid = a.piece.valid(matrix, a.rows);
+  const bool wide = cols % 8 == 0 && a.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
   float top = 0.f;
-  for (int r = blockIdx.x; r < valid; r += gridDim.x) {
-    if (target && target[r] == ignore) continue;
-    const T *row = in + r * stride;
+  for (int r = block; r < valid; r += a.blocks) {
+    if (a.target && a.target[r] == a.ignore) continue;
+    const T *row = in + r * a.stride;
     if (wide) {
       for (int c = threadIdx.x * 8; c < cols; c += 2048) {
         const x8 v = *reinterpret_cast<const x8 *>(row + c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float a = fabsf((float)v[i]);
-          top = a < INFINITY ? fmaxf(top, a) : top;
+          const float x = fabsf((float)v[i]);
+          top = x < INFINITY ? fmaxf(top, x) : top;
         }
       }
     } else {
       for (int c = threadIdx.x; c < cols; c += 256) {
-        const float a = fabsf((float)row[c]);
-        top = a < INFINITY ? fmaxf(top, a) : top;
+        const float x = fabsf((float)row[c]);
+        top = x < INFINITY ? fmaxf(top, x) : top;
       }
     }
   }
-  top = block_max(top);
-  if (threadIdx.x == 0) largest[blockIdx.y * gridDim.x + blockIdx.x] = top;
+  return block_max(top);
 }
 
-// The scale of what `largest` was taken of; with `count` 0 that of grad_loss, whose largest is looked for here.
-__global__ __launch_bounds__(256) void scale_kernel(const float *largest, int count, const float *grad_loss, const int64_t *target,
-                                                    int64_t ignore, int tokens, float *scale) {
+// Largest finite |entry| of what the next transpositions copy, one value a workgroup; and, by the last
+// workgroup, the scale of grad_loss (only with the first piece).
+template <class T>
+__global__ __launch_bounds__(256) void largest_kernel(Rows weights, Rows hidden, int cols, const float *grad_loss, const int64_t *target,
+                                                      int64_t ignore, int tokens, float *d_scale) {
+  int b = blockIdx.x;
+  const int w = weights.count * weights.blocks, h = hidden.count * hidden.blocks;
+  if (b < w) {
+    const float top = largest_of<T>(weights, b / weights.blocks, b % weights.blocks, cols);
+    if (threadIdx.x == 0) weights.largest[b] = top;
+    return;
+  }
+  b -= w;
+  if (b < h) {
+    const float top = largest_of<T>(hidden, 0, b, cols);
+    if (threadIdx.x == 0) hidden.largest[b] = top;
+    return;
+  }
   float top = 0.f;
-  for (int i = threadIdx.x; i < count; i += 256) top = fmaxf(top, largest[i]);
-  if (count == 0)
-    for (int t = threadIdx.x; t < tokens; t += 256) {
-      const float a = fabsf(grad_loss[t]);
-      if (target[t] != ignore && a < INFINITY) top = fmaxf(top, a);
-    }
+  for (int t = threadIdx.x; t < tokens; t += 256) {
+    const float a = fabsf(grad_loss[t]);
+    if (target[t] != ignore && a < INFINITY) top = fmaxf(top, a);
+  }
   top = block_max(top);
-  if (threadIdx.x == 0) scale[0] = scale_of(top);
+  if (threadIdx.x == 0) d_scale[0] = scale_of(top);
 }
 
 // ---- operands in the layout that the products read ----
@@ -428,24 +450,29 @@ __global__ __launch_bounds__(256) void scale_kernel(const float *largest, int co
 constexpr int kSide = 64;
 
 // out[c][r] = scale in[r][c] for the rows that count and every c, with zeros in the others, up to `padded` r
-// for each matrix of the group, one beside the other.
+// for each matrix, one beside the other.
 template <class T>
-__global__ __launch_bounds__(256) void transpose_kernel(Piece piece, int64_t in_stride, int rows, int cols, half *out, int64_t out_stride,
-                                                        int padded, const int64_t *target, int64_t ignore, const float *scale) {
+__global__ __launch_bounds__(256) void transpose_kernel(Rows a, int cols, half *out, int64_t out_stride, int padded) {
   // Column c of the tile in row c of LDS; a row's 16-byte units of eight r are permuted by c, so that the
   // eight columns that a lane reads in one row meet no other lane's bank.
   __shared__ __attribute__((aligned(16))) half tile[kSide][kSide];
   using x8 = typename emrs_gemm::Vec<T>::x8;
   const int r0 = blockIdx.x * kSide, c0 = blockIdx.y * kSide;
-  const T *in = static_cast<const T *>(piece.weights.p[blockIdx.z]);
-  const int valid = piece.valid(blockIdx.z, rows);
-  const float by = scale[0];
-  const bool wide = cols % 8 == 0 && in_stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
+  const T *in = static_cast<const T *>(a.piece.weights.p[blockIdx.z]);
+  const int valid = a.piece.valid(blockIdx.z, a.rows);
+  float by = 1.f;
+  if (a.blocks) {
+    float top = 0.f;
+    for (int i = threadIdx.x; i < a.count * a.blocks; i += 256) top = fmaxf(top, a.largest[i]);
+    by = scale_of(block_max(top));
+  }
+  if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) a.scale[0] = by;
+  const bool wide = cols % 8 == 0 && a.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int at = threadIdx.x + h * 256, r = at / 8, c = at % 8 * 8;
-    const bool keep = r0 + r < valid && !(target && target[r0 + r] == ignore);
-    const T *row = in + (r0 + r) * in_stride + c0 + c;
+    const bool keep = r0 + r < valid && !(a.target && a.target[r0 + r] == a.ignore);
+    const T *row = in + (r0 + r) * a.stride + c0 + c;
     x8 v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (T)0.f;
@@ -467,10 +494,6 @@ __global__ __launch_bounds__(256) void transpose_kernel(Piece piece, int64_t in_
       *reinterpret_cast<emrs_gemm::fp16x8 *>(out + (c0 + c) * out_stride + (int64_t)blockIdx.z * padded + r) =
           *reinterpret_cast<const emrs_gemm::fp16x8 *>(&tile[c][(unit ^ (c / 8)) * 8]);
   }
-}
-
-__global__ void ones_kernel(float *p, int n) {
-  if ((int)threadIdx.x < n) p[threadIdx.x] = 1.f;
 }
 
 // out[r][c] = in[r][c], with zeros from `cols` up to the padded row: operands whose rows do not lie on 16 bytes.
@@ -585,7 +608,7 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   s.dt = take(backward && a->grad_weights, shards * s.piece * s.tokens_padded * 2);
   s.ht = take(backward && a->grad_weights, a->hidden_size * s.tokens_padded * 2);
   s.scales = take(backward, 256);
-  s.largest = take(backward, kScaleBlocks * EMRS_LOSS_MAX_SHARDS * 4);
+  s.largest = take(backward, 2 * kScaleBlocks * 4);
   s.total = at;
   return s;
 }
@@ -672,19 +695,20 @@ int forward(const emrs_loss *a, hipStream_t st) {
   return EMRS_OK;
 }
 
-// scale * transpose of a group's piece (or of the hidden states); fp16 is copied as it is.
 template <class T>
-int transposed(const Piece &c, uint32_t count, int64_t stride, int64_t rows, int64_t cols, half *out, int64_t out_stride, int64_t padded,
-               const int64_t *target, int64_t ignore, float *largest, float *scale, hipStream_t st) {
-  const int blocks = std::is_same<T, half>::value ? 0 : (int)std::min<int64_t>(rows, kScaleBlocks);
-  if (blocks) {
-    largest_kernel<T><<<dim3(blocks, count), 256, 0, st>>>(c, stride, (int)rows, (int)cols, target, ignore, largest);
-    TRY(hipGetLastError());
-    scale_kernel<<<1, 256, 0, st>>>(largest, blocks * (int)count, nullptr, nullptr, 0, 0, scale);
-    TRY(hipGetLastError());
-  }
-  const dim3 grid((padded + kSide - 1) / kSide, (cols + kSide - 1) / kSide, count);
-  transpose_kernel<T><<<grid, 256, 0, st>>>(c, stride, (int)rows, (int)cols, out, out_stride, (int)padded, target, ignore, scale);
+Rows rows_of(const Piece &c, uint32_t count, int64_t stride, int64_t rows, const int64_t *target, int64_t ignore, float *largest, float *scale) {
+  Rows r{};
+  r.piece = c, r.stride = stride, r.rows = (int32_t)rows, r.count = (int32_t)count;
+  r.blocks = std::is_same<T, half>::value ? 0 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(rows, kScaleBlocks / count));
+  r.target = target, r.ignore = ignore;
+  r.largest = largest, r.scale = scale;
+  return r;
+}
+
+template <class T>
+int transpose(const Rows &r, int64_t cols, half *out, int64_t out_stride, int64_t padded, hipStream_t st) {
+  const dim3 grid((padded + kSide - 1) / kSide, (cols + kSide - 1) / kSide, r.count);
+  transpose_kernel<T><<<grid, 256, 0, st>>>(r, (int)cols, out, out_stride, (int)padded);
   TRY(hipGetLastError());
   return EMRS_OK;
 }
@@ -701,22 +725,13 @@ int backward(const emrs_loss *a, hipStream_t st) {
   const void *hidden;
   int rc = aligned_hidden<T>(a, s, &hidden, st);
   if (rc) return rc;
-  scale_kernel<<<1, 256, 0, st>>>(nullptr, 0, a->grad_loss, a->target, a->ignore_index, (int)tokens, d_scale);
-  TRY(hipGetLastError());
-  if (std::is_same<T, half>::value) {
-    ones_kernel<<<1, 64, 0, st>>>(h_scale, 2);
-    TRY(hipGetLastError());
-  }
-  if (a->grad_weights) {
-    Piece all{};
-    all.weights.p[0] = a->hidden, all.vocab = tokens;
-    rc = transposed<T>(all, 1, a->hidden_stride, tokens, h, ht, s.tokens_padded, s.tokens_padded, a->target, a->ignore_index, largest, h_scale, st);
-    if (rc) return rc;
-  }
+  Piece every{};
+  every.weights.p[0] = a->hidden, every.vocab = tokens;
+  const Rows h_rows = rows_of<T>(every, 1, (int64_t)a->hidden_stride, tokens, a->target, a->ignore_index, largest + kScaleBlocks, h_scale);
   const bool fours = h % 4 == 0;
   uint64_t first = a->vocab_start, left = 0;
   for (uint32_t i = 0; i < s.n_groups; ++i) left += (a->shard_rows[s.groups[i].first] + s.piece - 1) / s.piece;
-  bool begun = false;
+  bool begun = false, scaled = false;
   for (uint32_t i = 0; i < s.n_groups; ++i) {
     const Group &g = s.groups[i];
     const uint64_t all = a->shard_rows[g.first];
@@ -727,6 +742,20 @@ int backward(const emrs_loss *a, hipStream_t st) {
       --left;
       if (!a->grad_hidden && !wanted) continue;
       const Piece own = piece_of(a, g, first, lo);
+      const Rows w_rows = rows_of<T>(own, g.count, (int64_t)a->weight_strides[g.first], (int64_t)rows, nullptr, 0, largest, w_scale);
+      Rows none = h_rows;
+      none.count = 0;
+      const int blocks = (a->grad_hidden ? w_rows.count * w_rows.blocks : 0) + (scaled ? 0 : (a->grad_weights ? h_rows.blocks : 0) + 1);
+      if (blocks) {
+        largest_kernel<T><<<blocks, 256, 0, st>>>(a->grad_hidden ? w_rows : none, scaled || !a->grad_weights ? none : h_rows, (int)h, a->grad_loss,
+                                                  a->target, a->ignore_index, (int)tokens, d_scale);
+        TRY(hipGetLastError());
+      }
+      if (!scaled && a->grad_weights) {
+        rc = transpose<T>(h_rows, h, ht, (int64_t)s.tokens_padded, (int64_t)s.tokens_padded, st);
+        if (rc) return rc;
+      }
+      scaled = true;
       Piece c = own;
       rc = aligned_piece<T>(a, s, g, rows, &c, st);
       if (rc) return rc;
@@ -735,7 +764,7 @@ int backward(const emrs_loss *a, hipStream_t st) {
       TRY((emrs_gemm::launch<T>(p, LogitGradients{c, a->grad_hidden ? d : nullptr, wanted ? dt : nullptr, (int32_t)(g.count * padded),
                                                   (int32_t)s.tokens_padded, (int32_t)padded, a->lse, a->grad_loss, a->target, a->ignore_index, d_scale}, st)));
       if (a->grad_hidden) {
-        rc = transposed<T>(own, g.count, a->weight_strides[g.first], rows, h, wt, g.count * padded, padded, nullptr, 0, largest, w_scale, st);
+        rc = transpose<T>(w_rows, h, wt, (int64_t)(g.count * padded), (int64_t)padded, st);
         if (rc) return rc;
         Product q{};
         q.a = wt, q.b = d;

@@ -30,5 +30,10 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(1, nbytes), dtype=torch.uint8, device=device)
 
 
-def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+def run_on(device: torch.device, call, record) -> None:
+    """``call(record, stream)`` with ``device`` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        call(record, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(record, torch.cuda.current_stream(device).cuda_stream)

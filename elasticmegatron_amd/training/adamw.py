@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, stream_of
+from ._common import dtype_code, on_device, run_on
 
 
 @torch.no_grad()
@@ -46,5 +46,4 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
     a.main, a.exp_avg, a.exp_avg_sq, a.grad = (t.data_ptr() for t in (main, exp_avg, exp_avg_sq, grad))
     a.image = None if model is None else model.data_ptr()
     a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = lr, beta1, beta2, eps, weight_decay
-    with torch.cuda.device(device):
-        _native.adamw_step(a, stream_of(device))
+    run_on(device, _native.adamw_step, a)

@@ -16,7 +16,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, stream_of, workspace
+from ._common import dtype_code, on_device, run_on, workspace
 
 Weight = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -83,8 +83,7 @@ class _Call:
             a.lse, a.target_logit, a.loss = lse.data_ptr(), logit.data_ptr(), loss.data_ptr() if with_loss else None
             scratch = workspace(_native.loss_workspace(a, False), self.device)
             a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
-            with torch.cuda.device(self.device):
-                _native.loss_forward(a, stream_of(self.device))
+            run_on(self.device, _native.loss_forward, a)
         return lse, logit, loss
 
     def backward(self, lse, grad_loss, want_hidden: bool, want_weights: Sequence[bool]):
@@ -103,8 +102,7 @@ class _Call:
         a.grad_weights = ctypes.addressof(table) if any(want_weights) else None
         scratch = workspace(_native.loss_workspace(a, True), self.device)
         a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
-        with torch.cuda.device(self.device):
-            _native.loss_backward(a, stream_of(self.device))
+        run_on(self.device, _native.loss_backward, a)
         return gh, gw
 
 

@@ -15,7 +15,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, stream_of, workspace
+from ._common import dtype_code, on_device, run_on, workspace
 
 Matrices = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -111,15 +111,14 @@ def _run(kinds, *, steps, coefficients, eps, mu, nesterov, decay, rate) -> None:
     size = _native.muon_workspace(a)
     scratch = workspace(size, grad.device)
     a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
-    with torch.cuda.device(grad.device):
-        for lo in range(0, grad.count, at_once):
-            hi = min(grad.count, lo + at_once)
-            a.count = hi - lo
-            tables = {name: k.table(lo, hi) for name, k in kinds.items()}
-            for name, t in tables.items():
-                setattr(a, name, ctypes.addressof(t))
-                setattr(a, name + "_stride", kinds[name].stride)
-            _native.muon_step(a, stream_of(grad.device))
+    for lo in range(0, grad.count, at_once):
+        hi = min(grad.count, lo + at_once)
+        a.count = hi - lo
+        tables = {name: k.table(lo, hi) for name, k in kinds.items()}
+        for name, t in tables.items():
+            setattr(a, name, ctypes.addressof(t))
+            setattr(a, name + "_stride", kinds[name].stride)
+        run_on(grad.device, _native.muon_step, a)
 
 
 @torch.no_grad()
