@@ -396,19 +396,33 @@ __device__ float largest_of(const Rows &a, int matrix, int block, int cols) {
   const int valid = a.piece.valid(matrix, a.rows);
   const bool wide = cols % 8 == 0 && a.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
   float top = 0.f;
-  for (int r = block; r < valid; r += a.blocks) {
-    if (a.target && a.target[r] == a.ignore) continue;
-    const T *row = in + r * a.stride;
-    if (wide) {
-      for (int c = threadIdx.x * 8; c < cols; c += 2048) {
-        const x8 v = *reinterpret_cast<const x8 *>(row + c);
+  if (wide) {
+    // A run of consecutive rows a workgroup, four 16-byte units a thread on their way at a time.
+    const int units = cols / 8, each = (valid + a.blocks - 1) / a.blocks, r0 = block * each;
+    const int64_t n = (int64_t)max(0, min(each, valid - r0)) * units;
+    for (int64_t u = threadIdx.x; u < n; u += 4 * 256) {
+      x8 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t at = min(u + k * 256, n - 1);
+        const int r = r0 + (int)(at / units);
+        v[k] = *reinterpret_cast<const x8 *>(in + r * a.stride + at % units * 8);
+        if (a.target && a.target[r] == a.ignore)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[k][i] = (T)0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float x = fabsf((float)v[i]);
+          const float x = fabsf((float)v[k][i]);
           top = x < INFINITY ? fmaxf(top, x) : top;
         }
-      }
-    } else {
+    }
+  } else {
+    for (int r = block; r < valid; r += a.blocks) {
+      if (a.target && a.target[r] == a.ignore) continue;
+      const T *row = in + r * a.stride;
       for (int c = threadIdx.x; c < cols; c += 256) {
         const float x = fabsf((float)row[c]);
         top = x < INFINITY ? fmaxf(top, x) : top;
