@@ -258,16 +258,19 @@ struct LogitGradients : Piece {
         Turn::put(own, i, j, lane, out);
       }
     }
-    if (d)
+    // From a wave's corner on, offsets are 32 bits: 256 rows of 2^22 elements at most.
+    if (d) {
+      half *const to = d + (int64_t)n0 * d_stride + w.batch * padded + m0;
       Turn::along_m(own, lane, [&](int x, int t, emrs_gemm::fp16x8 v) __attribute__((always_inline)) {
-        if (m0 + x < padded && n0 + t < p.n)
-          *reinterpret_cast<emrs_gemm::fp16x8 *>(d + (int64_t)(n0 + t) * d_stride + w.batch * padded + m0 + x) = v;
+        if (m0 + x < padded && n0 + t < p.n) *reinterpret_cast<emrs_gemm::fp16x8 *>(to + (t * d_stride + x)) = v;
       });
-    if (dt)
+    }
+    if (dt) {
+      half *const to = dt + (int64_t)(w.batch * padded + m0) * dt_stride + n0;
       Turn::along_n(own, lane, [&](int x, int t, emrs_gemm::fp16x8 v) __attribute__((always_inline)) {
-        if (m0 + x < padded && n0 + t < dt_stride)
-          *reinterpret_cast<emrs_gemm::fp16x8 *>(dt + (int64_t)(w.batch * padded + m0 + x) * dt_stride + n0 + t) = v;
+        if (m0 + x < padded && n0 + t < dt_stride) *reinterpret_cast<emrs_gemm::fp16x8 *>(to + (x * dt_stride + t)) = v;
       });
+    }
   }
 };
 
@@ -284,18 +287,26 @@ struct StoreSums : emrs_gemm::Operand {
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4;
     const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
+    float *const to = sum + w.batch * batch;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int n = n0 + j * 16 + (lane & 15);
+      // What lies outside reads the last element inside: with no branch, these loads are on their way together.
+      f32x4 before[Cfg::MI];
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) before[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (wide && add)
+#pragma unroll
+        for (int i = 0; i < Cfg::MI; ++i)
+          before[i] = *reinterpret_cast<const f32x4 *>(to + min(n, p.n - 1) * stride + min(m + i * 16, p.m - 4));
       if (n >= p.n) continue;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int at = m + i * 16;
         if (at >= p.m) continue;
-        float *const o = sum + w.batch * batch + n * stride + at;
-        f32x4 c = acc[i][j] * by;
+        float *const o = to + n * stride + at;
+        const f32x4 c = acc[i][j] * by + before[i];
         if (wide) {
-          if (add) c += *reinterpret_cast<const f32x4 *>(o);
           *reinterpret_cast<f32x4 *>(o) = c;
           continue;
         }
@@ -325,15 +336,21 @@ struct StoreRows : emrs_gemm::Operand {
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       const int n = n0 + j * 16 + (lane & 15);
+      f32x4 before[Cfg::MI];
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) before[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (wide && sum)
+#pragma unroll
+        for (int i = 0; i < Cfg::MI; ++i)
+          before[i] = *reinterpret_cast<const f32x4 *>(sum + min(n, p.n - 1) * stride + min(m + i * 16, p.m - 4));
       if (n >= p.n) continue;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int at = m + i * 16;
         if (at >= p.m) continue;
         const int64_t o = n * stride + at;
-        f32x4 c = acc[i][j] * by;
+        const f32x4 c = acc[i][j] * by + before[i];
         if (wide) {
-          if (sum) c += *reinterpret_cast<const f32x4 *>(sum + o);
           x4 v;
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = (T)c[r];

@@ -175,17 +175,25 @@ __global__ __launch_bounds__(256) void pack_kernel(Update u, const float *norms,
 
 using half8 = emrs_gemm::fp16x8;
 
+// An offset from a wave's corner, held inside the matrix: what is read there is not stored, but is read with
+// no branch, so that many such loads are on their way together.  (A corner may lie outside: then it is negative.)
+__device__ __forceinline__ int inside(int at, int corner, int last) { return min(at, last - corner); }
+
 // A wave's tile of a symmetric matrix, from LDS to its place and, off the diagonal, to the place across it.
 // (A tile on the diagonal holds both: with two parts they differ in their sums' order, and are stored once.)
 template <class Cfg>
 __device__ __forceinline__ void store_symmetric(half *out, int64_t stride, const Where &w, int m0, int n0, int lane, const Product &p,
                                                 const char *own) {
+  // From a wave's corner on, offsets are 32 bits: 256 rows of 2^22 elements at most.
+  const int step = (int)stride;
+  half *const here = out + n0 * stride + m0;
   emrs_gemm::Turn<Cfg>::along_m(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
-    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(out + (n0 + y) * stride + m0 + x) = v;
+    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(here + (y * step + x)) = v;
   });
   if (w.m0 == w.n0) return;
+  half *const across = out + m0 * stride + n0;
   emrs_gemm::Turn<Cfg>::along_n(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
-    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(out + (m0 + x) * stride + n0 + y) = v;
+    if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(across + (x * step + y)) = v;
   });
 }
 
@@ -217,17 +225,16 @@ struct StorePolynomial : emrs_gemm::Operand {
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
-    const half *in = gram + w.batch * batch;
+    const half *const in = gram + w.batch * batch + n0 * stride + m0;
+    const int step = (int)stride;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j)
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
-        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
-        half4 v = half4{};
-        if (m < p.m && n < p.n) {
-          const half4 x = *reinterpret_cast<const half4 *>(in + n * stride + m);
-          for (int r = 0; r < 4; ++r) v[r] = (half)((m + r == n ? a : 0.f) + b * (float)x[r] + c * acc[i][j][r]);
-        }
+        const int m = i * 16 + (lane >> 4) * 4, n = j * 16 + (lane & 15);
+        const half4 x = *reinterpret_cast<const half4 *>(in + inside(m, m0, p.m - 4) + inside(n, n0, p.n - 1) * step);
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)((m0 + m + r == n0 + n ? a : 0.f) + b * (float)x[r] + c * acc[i][j][r]);
         emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
       }
     store_symmetric<Cfg>(out + w.batch * batch, stride, w, m0, n0, lane, p, own);
@@ -235,10 +242,10 @@ struct StorePolynomial : emrs_gemm::Operand {
 };
 
 // The product, plus a X from both its parts where the polynomial is without it.
-__device__ inline f32x4 applied(const half *x, int64_t low, int parts, float a, f32x4 acc) {
+__device__ __forceinline__ f32x4 applied(const half *x, int at, int low, int parts, float a, f32x4 acc) {
   if (parts == 1) return acc * (1.f / kGramScale);
-  const half4 hi = *reinterpret_cast<const half4 *>(x);
-  const half4 lo = *reinterpret_cast<const half4 *>(x + low);
+  const half4 hi = *reinterpret_cast<const half4 *>(x + at);
+  const half4 lo = *reinterpret_cast<const half4 *>(x + (at + low));
   f32x4 v;
   for (int r = 0; r < 4; ++r) v[r] = a * ((float)hi[r] + (float)lo[r]) + acc[r] * (1.f / kGramScale);
   return v;
@@ -253,20 +260,21 @@ struct StoreIterate : emrs_gemm::Operand {
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     using Turn = emrs_gemm::Turn<Cfg>;
-    const half *x = in.p + w.batch * in.batch;
+    const half *const x = in.p + w.batch * in.batch + n0 * in.stride + m0;
+    const int step = (int)in.stride, low = (int)in.low;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       __builtin_amdgcn_sched_barrier(0);  // the loads of one column at a time: registers
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
-        const int m = m0 + i * 16 + (lane >> 4) * 4, n = n0 + j * 16 + (lane & 15);
-        if (m < p.m && n < p.n) acc[i][j] = applied(x + n * in.stride + m, in.low, in_parts, a, acc[i][j]);
+        const int m = inside(i * 16 + (lane >> 4) * 4, m0, p.m - 4), n = inside(j * 16 + (lane & 15), n0, p.n - 1);
+        acc[i][j] = applied(x, n * step + m, low, in_parts, a, acc[i][j]);
         half4 v;
         for (int r = 0; r < 4; ++r) v[r] = (half)acc[i][j][r];
         Turn::put(own, i, j, lane, v);
       }
     }
-    half *o = out.p + w.batch * out.batch, *t = across.p + w.batch * across.batch;
+    half *const o = out.p + w.batch * out.batch + n0 * out.stride + m0, *const t = across.p + w.batch * across.batch + m0 * across.stride + n0;
     store(o, t, m0, n0, lane, p, own, Turn{});
     if (out_parts == 1) return;
 #pragma unroll
@@ -281,11 +289,12 @@ struct StoreIterate : emrs_gemm::Operand {
   }
   template <class Turn>
   __device__ __forceinline__ void store(half *o, half *t, int m0, int n0, int lane, const Product &p, const char *own, Turn) const {
+    const int o_step = (int)out.stride, t_step = (int)across.stride;
     Turn::along_m(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
-      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(o + (n0 + y) * out.stride + m0 + x) = v;
+      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(o + (y * o_step + x)) = v;
     });
     Turn::along_n(own, lane, [&](int x, int y, half8 v) __attribute__((always_inline)) {
-      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(t + (m0 + x) * across.stride + n0 + y) = v;
+      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<half8 *>(t + (x * t_step + y)) = v;
     });
   }
 };
@@ -305,25 +314,33 @@ struct StoreResult : emrs_gemm::Operand {
   float keep, rate;
 
   template <class Cfg>
-  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &, char *) const {
-    const half *x = in.p + w.batch * in.batch;
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *) const {
+    const half *const x = in.p + w.batch * in.batch + n0 * in.stride + m0;
     __bf16 *o = has_out ? static_cast<__bf16 *>(out.p[w.batch]) : nullptr;
     __bf16 *img = has_image ? static_cast<__bf16 *>(image.p[w.batch]) : nullptr;
     float *mn = has_main ? main.p[w.batch] : nullptr;
+    const int step = (int)in.stride, low = (int)in.low;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
       __builtin_amdgcn_sched_barrier(0);  // the loads of one column at a time: registers
+      f32x4 before[Cfg::MI];
+      if (kWide && mn)
+#pragma unroll
+        for (int i = 0; i < Cfg::MI; ++i)
+          before[i] = *reinterpret_cast<const f32x4 *>(mn + min(n0 + j * 16 + (lane & 15), rows - 1) * main_stride +
+                                                       min(m0 + i * 16 + (lane >> 4) * 4, cols - 4));
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int c = m0 + i * 16 + (lane >> 4) * 4;
         const int64_t r = n0 + j * 16 + (lane & 15);
+        // The workspace's rows and columns go on with zeros to multiples of 64, and past them this reads others.
+        f32x4 v = applied(x, inside(j * 16 + (lane & 15), n0, p.n - 1) * step + inside(i * 16 + (lane >> 4) * 4, m0, p.m - 4), low, in_parts, a,
+                          acc[i][j]) * by;
         if (c >= cols || r >= rows) continue;
-        f32x4 v = applied(x + r * in.stride + c, in.low, in_parts, a, acc[i][j]) * by;
         if (kWide) {
           if (mn) {
-            f32x4 *at = reinterpret_cast<f32x4 *>(mn + r * main_stride + c);
-            v = *at * keep - rate * v;
-            *at = v;
+            v = before[i] * keep - rate * v;
+            *reinterpret_cast<f32x4 *>(mn + r * main_stride + c) = v;
           }
           bf16x4 h;
           for (int k = 0; k < 4; ++k) h[k] = (__bf16)v[k];
