@@ -241,6 +241,49 @@ struct StorePolynomial : emrs_gemm::Operand {
   }
 };
 
+// A product of symmetric matrices that commute, in two parts like its operands (side by side in a row, the
+// second `stride` / 2 on): a I + b A + c A A for the polynomial, c alone for the others.
+struct StoreSquare : emrs_gemm::Operand {
+  half *out;
+  const half *in;         // A, or NULL
+  int64_t stride, batch;
+  float a, b, c;
+
+  template <class Cfg>
+  __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
+    const int step = (int)stride, low = step / 2;
+    const half *const from = in ? in + w.batch * batch + n0 * stride + m0 : nullptr;
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j) {
+      __builtin_amdgcn_sched_barrier(0);  // the loads of one column at a time: registers
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int m = i * 16 + (lane >> 4) * 4, n = j * 16 + (lane & 15);
+        acc[i][j] *= c;
+        if (from) {
+          const half *const x = from + inside(m, m0, p.m - 4) + inside(n, n0, p.n - 1) * step;
+          const half4 hi = *reinterpret_cast<const half4 *>(x), lo = *reinterpret_cast<const half4 *>(x + low);
+          for (int r = 0; r < 4; ++r) acc[i][j][r] += (m0 + m + r == n0 + n ? a : 0.f) + b * ((float)hi[r] + (float)lo[r]);
+        }
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)acc[i][j][r];
+        emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
+      }
+    }
+    half *const to = out + w.batch * batch;
+    store_symmetric<Cfg>(to, stride, w, m0, n0, lane, p, own);
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        half4 v;
+        for (int r = 0; r < 4; ++r) v[r] = (half)(acc[i][j][r] - (float)(half)acc[i][j][r]);
+        emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
+      }
+    store_symmetric<Cfg>(to + low, stride, w, m0, n0, lane, p, own);
+  }
+};
+
 // The product, plus a X from both its parts where the polynomial is without it.
 __device__ __forceinline__ f32x4 applied(const half *x, int at, int low, int parts, float a, f32x4 acc) {
   if (parts == 1) return acc * (1.f / kGramScale);
@@ -658,11 +701,22 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(Small a) {
 
 struct Sizes {
   uint64_t s, l;                             // padded sides
-  uint64_t x[2], xt[2], gram, poly, norms, total;  // offsets; x and xt hold both parts of every matrix
+  uint64_t x[2], xt[2], gram, poly, squares, norms, total;  // offsets; x and xt hold both parts of every matrix
   uint32_t blocks;                           // workgroups of the norm, a matrix
 };
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+// Whether the steps with two parts work on S x S matrices alone.  All of a step's polynomials commute:
+// A <- P A P and Q <- P Q take the place of X <- P X, and X <- Q X follows once.  With r = L / S that is
+// 4.5 r + 13.5 products of S S S for three steps in place of 10.5 r + 6, by the multiply-adds; where two more
+// launches and triangles that fill their last round badly count too, it pays from r = 2.5 on.  (Not for the
+// steps with one part: there the rounding of A, which grows by a^2 a step, would double the error.)
+constexpr int kSquares = 5;
+bool by_squares(const emrs_muon *a) {
+  const uint64_t s = std::min(a->rows, a->cols), l = std::max(a->rows, a->cols);
+  return a->steps > 3 && 2 * l >= 5 * s;
+}
 
 Sizes sizes_of(const emrs_muon *a) {
   Sizes z{};
@@ -679,6 +733,7 @@ Sizes sizes_of(const emrs_muon *a) {
   for (int i = 0; i < 2; ++i) z.xt[i] = take(2 * a->count * z.s * z.l * 2);
   z.gram = take(a->count * z.s * z.s * 2);
   z.poly = take(a->count * z.s * z.s * 2);
+  z.squares = take(by_squares(a) ? kSquares * a->count * z.s * 2 * z.s * 2 : 0);
   z.norms = take((uint64_t)a->count * z.blocks * 4);
   z.total = at;
   return z;
@@ -825,9 +880,57 @@ int step(const emrs_muon *a, hipStream_t st) {
   pack_kernel<<<tiles, 256, 0, st>>>(u, norms, (int)z.blocks, a->eps, scale, tall ? xt(0) : x(0), tall ? x(0) : xt(0), parts_of(0));
   TRY(hipGetLastError());
 
-  for (uint32_t k = 0; k < a->steps; ++k) {
+  int now = 0;
+  uint32_t done = 0;
+  if (by_squares(a)) {
+    const int64_t two = 2 * (int64_t)z.s, each = (int64_t)z.s * two;
+    half *const squares = reinterpret_cast<half *>(ws + z.squares);
+    auto matrix = [&](int i) { return squares + i * (int64_t)a->count * each; };
+    half *gram_of = matrix(0), *const p_of = matrix(1), *spare = matrix(2), *q_of = matrix(3), *q_next = matrix(4);
+    // hi hi + hi lo + lo hi
+    auto square = [&](const half *m, const half *n, half *out, const half *poly_of, float fa, float fb, float fc) {
+      Product g{};
+      g.a = m, g.b = n;
+      g.a_stride = g.b_stride = two, g.a_batch = g.b_batch = each;
+      g.m = g.n = (int)z.s, g.k = 3 * (int)z.s;
+      g.a_wrap = (int)z.s, g.b_wrap = 2 * (int)z.s;
+      g.batch = (int)a->count, g.symmetric = 1;
+      return emrs_gemm::launch<half>(g, StoreSquare{{}, out, poly_of, two, each, fa, fb, fc}, st);
+    };
+    const Image in = x(0), in_t = xt(0);
+    Product g{};
+    g.a = g.b = in.p;
+    g.a_stride = g.b_stride = in.stride, g.a_batch = g.b_batch = in.batch;
+    g.m = g.n = (int)z.s, g.k = 3 * (int)z.l;
+    g.a_wrap = (int)z.l, g.b_wrap = 2 * (int)z.l;
+    g.batch = (int)a->count, g.symmetric = 1;
+    TRY((emrs_gemm::launch<half>(g, StoreSquare{{}, gram_of, nullptr, two, each, 0.f, 0.f, kGramScale / (scale * scale)}, st)));
+    constexpr float one = 1.f / kGramScale;
+    for (; parts_of(done) == 2; ++done) {
+      const float *f = a->coefficients + 3 * done;
+      half *const p = done == 0 ? q_of : p_of;
+      TRY(square(gram_of, gram_of, p, gram_of, f[0] * kGramScale, f[1], f[2] * one));
+      if (parts_of(done + 1) == 2) {
+        TRY(square(p, gram_of, spare, nullptr, 0.f, 0.f, one));
+        TRY(square(spare, p, gram_of, nullptr, 0.f, 0.f, one));
+      }
+      if (done == 0) continue;
+      TRY(square(p, q_of, q_next, nullptr, 0.f, 0.f, one));
+      std::swap(q_of, q_next);
+    }
+    Product r{};
+    r.a = in_t.p, r.b = q_of;
+    r.a_stride = in_t.stride, r.b_stride = two;
+    r.a_batch = in_t.batch, r.b_batch = each;
+    r.m = (int)z.l, r.n = (int)z.s, r.k = 3 * (int)z.s;
+    r.a_wrap = (int)z.s, r.b_wrap = 2 * (int)z.s;
+    r.batch = (int)a->count;
+    TRY((emrs_gemm::launch<half>(r, StoreIterate{{}, in, x(1), xt(1), 1, 1, 0.f}, st)));
+    now = 1;
+  }
+  for (uint32_t k = done; k < a->steps; ++k, now ^= 1) {
     const float *f = a->coefficients + 3 * k;
-    const int now = k & 1, parts = parts_of(k);
+    const int parts = parts_of(k);
     const Image in = x(now), in_t = xt(now);
     Product g{};
     g.a = g.b = in.p;
