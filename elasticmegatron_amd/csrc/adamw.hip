@@ -34,35 +34,41 @@ __device__ inline void update(float &w, float &m, float &v, float g, const Facto
   w = w * f.keep - f.rate * m / (sqrtf(v * f.over2) + f.eps);
 }
 
-template <class G, bool kImage>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(uint64_t fours, float *w, float *m, float *v, const G *g, __bf16 *image,
-                                                         Factors f) {
-  const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= fours) return;
-  f32x4 a = reinterpret_cast<f32x4 *>(w)[i], b = reinterpret_cast<f32x4 *>(m)[i], c = reinterpret_cast<f32x4 *>(v)[i];
-  const typename Four<G>::type d = reinterpret_cast<const typename Four<G>::type *>(g)[i];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    float x = a[k], y = b[k], z = c[k];
-    update(x, y, z, (float)d[k], f);
-    a[k] = x, b[k] = y, c[k] = z;
-  }
-  reinterpret_cast<f32x4 *>(w)[i] = a;
-  reinterpret_cast<f32x4 *>(m)[i] = b;
-  reinterpret_cast<f32x4 *>(v)[i] = c;
-  if (kImage) {
-    typename Four<__bf16>::type h;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = (__bf16)a[k];
-    reinterpret_cast<typename Four<__bf16>::type *>(image)[i] = h;
-  }
+template <class V>
+__device__ inline V stream_in(const V *p) {
+  return __builtin_nontemporal_load(p);
 }
 
-// Element by element: the last three, and buffers that are off their vectors' alignment.
-template <class G, bool kImage>
-__global__ __launch_bounds__(kThreads) void adamw_scalar_kernel(uint64_t first, uint64_t n, float *w, float *m, float *v, const G *g,
-                                                                __bf16 *image, Factors f) {
-  const uint64_t i = first + (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+// Four elements a lane where they lie on their vectors, and the last three by a lane each.  Nothing is read
+// twice: the accesses bypass the caches' retention.
+template <class G, bool kImage, bool kWide>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(uint64_t fours, uint64_t n, float *w, float *m, float *v, const G *g, __bf16 *image,
+                                                         Factors f) {
+  using g4 = typename Four<G>::type;
+  using h4 = typename Four<__bf16>::type;
+  uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (kWide && i < fours) {
+    f32x4 a = stream_in(reinterpret_cast<const f32x4 *>(w) + i), b = stream_in(reinterpret_cast<const f32x4 *>(m) + i);
+    f32x4 c = stream_in(reinterpret_cast<const f32x4 *>(v) + i);
+    const g4 d = stream_in(reinterpret_cast<const g4 *>(g) + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x = a[k], y = b[k], z = c[k];
+      update(x, y, z, (float)d[k], f);
+      a[k] = x, b[k] = y, c[k] = z;
+    }
+    __builtin_nontemporal_store(a, reinterpret_cast<f32x4 *>(w) + i);
+    __builtin_nontemporal_store(b, reinterpret_cast<f32x4 *>(m) + i);
+    __builtin_nontemporal_store(c, reinterpret_cast<f32x4 *>(v) + i);
+    if (kImage) {
+      h4 h;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) h[k] = (__bf16)a[k];
+      __builtin_nontemporal_store(h, reinterpret_cast<h4 *>(image) + i);
+    }
+    return;
+  }
+  if (kWide) i += fours * 3;  // element 4 fours + (i - fours)
   if (i >= n) return;
   float x = w[i], y = m[i], z = v[i];
   update(x, y, z, (float)g[i], f);
@@ -77,13 +83,12 @@ int launch(const emrs_adamw *a, const Factors &f, hipStream_t st) {
   const G *g = static_cast<const G *>(a->grad);
   __bf16 *image = static_cast<__bf16 *>(a->image);
   const bool wide = on(a->main, 16) && on(a->exp_avg, 16) && on(a->exp_avg_sq, 16) && on(g, 4 * sizeof(G)) && on(image, 8);
-  const uint64_t fours = wide ? a->n / 4 : 0, rest = a->n - fours * 4;
-  if (fours)
-    adamw_kernel<G, kImage><<<(uint32_t)((fours + kThreads - 1) / kThreads), kThreads, 0, st>>>(fours, a->main, a->exp_avg,
-                                                                                              a->exp_avg_sq, g, image, f);
-  if (rest)
-    adamw_scalar_kernel<G, kImage><<<(uint32_t)((rest + kThreads - 1) / kThreads), kThreads, 0, st>>>(
-        fours * 4, a->n, a->main, a->exp_avg, a->exp_avg_sq, g, image, f);
+  const uint64_t fours = wide ? a->n / 4 : 0, lanes = fours + (a->n - fours * 4);
+  const uint32_t blocks = (uint32_t)((lanes + kThreads - 1) / kThreads);
+  if (wide)
+    adamw_kernel<G, kImage, true><<<blocks, kThreads, 0, st>>>(fours, a->n, a->main, a->exp_avg, a->exp_avg_sq, g, image, f);
+  else
+    adamw_kernel<G, kImage, false><<<blocks, kThreads, 0, st>>>(0, a->n, a->main, a->exp_avg, a->exp_avg_sq, g, image, f);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? EMRS_OK : fail(EMRS_ERR_HIP, std::string("adamw: ") + hipGetErrorString(e));
 }

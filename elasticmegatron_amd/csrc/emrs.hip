@@ -53,8 +53,14 @@ int fail(int code, const std::string &msg) {
 }
 void clear_error() { g_last_error.clear(); }
 int need_device() {
+  // A device that was there stays: asked once, not with every call.
+  static std::atomic<bool> seen{false};
+  if (seen.load(std::memory_order_relaxed)) return EMRS_OK;
   int n = 0;
-  if (hipGetDeviceCount(&n) == hipSuccess && n > 0) return EMRS_OK;
+  if (hipGetDeviceCount(&n) == hipSuccess && n > 0) {
+    seen.store(true, std::memory_order_relaxed);
+    return EMRS_OK;
+  }
   (void)hipGetLastError();
   return fail(EMRS_ERR_NO_DEVICE, "no HIP device is visible");
 }

@@ -18,8 +18,8 @@
 // P = a I + b A + c A^2: near the end P is close to 0.7 I where b A + c A^2 is close to -2.7 I, and has a
 // quarter of its rounding; before, P's rounding on the diagonal would be such noise itself.  An error of A
 // enters by the polynomial's slope, b + 2 c A, of size 0.7 at the end.  Against 64 bits the result is then
-// below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 (4e-2 with one part throughout, 3e-1 with
-// bf16), which is the rounding of the bf16 that it is written in.
+// below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 and 3e-3 for a matrix of rank one (4e-2 with one
+// part throughout, 3e-1 with bf16), about the rounding of the bf16 that it is written in.
 
 #include <hip/hip_runtime.h>
 
