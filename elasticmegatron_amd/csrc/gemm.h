@@ -133,32 +133,37 @@ __device__ inline Where tile_of(const Product &p) {
 __device__ inline int swizzle(int row) { return (row ^ ((row >> 3) & 1)) & 7; }
 
 // What a lane loads of an operand's stage: the same 16 bytes of row `lane / 8` of each of its wave's groups
-// of eight rows, which lie a constant apart.
-template <int WAVES>
+// of eight rows, which lie a constant apart.  Every group has a buffer of its own, from its first row to the
+// operand's last k: the hardware checks a lane's offset against a buffer's size, but not the scalar offset
+// (where k goes), so what places a row must not be scalar.
+template <class T, int LOADS, int WAVES>
 struct Loader {
   int voffset;
   int unit;  // first k, within a stage, of the 16 bytes
-  int apart; // bytes from a wave's group of rows to its next
-  __device__ __forceinline__ void init(int64_t stride, int wave, int lane) {
+  const T *base[LOADS];
+  int bytes[LOADS];  // 0: no row of the group is the operand's
+  // first: the tile's first row; rows: how many of its rows there are; columns: what a row holds.
+  __device__ __forceinline__ void init(const T *first, int64_t stride, int rows, int columns, int wave, int lane) {
     static_assert(WAVES % 2 == 0, "a wave's groups of eight rows are all even or all odd");
-    const int row = wave * 8 + (lane >> 3), c = (lane & 7) ^ swizzle(row);
+    const int row = lane >> 3, c = (lane & 7) ^ swizzle(wave * 8 + row);
     unit = c * 8;
     voffset = (int)(row * stride * 2) + (c << 4);
-    apart = (int)(WAVES * 8 * stride * 2);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int at = (wave + j * WAVES) * 8, here = rows - at;
+      base[j] = first + at * stride;
+      bytes[j] = here > 0 ? (int)(((here - 1) * stride + columns) * 2) : 0;
+    }
   }
   // Fewer than a stage's k are left: lanes whose 16 bytes are past them go past the buffer's end instead.
   __device__ __forceinline__ void cut(int left) { voffset = unit < left ? voffset : (int)0x80000000; }
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char *lds, int j, int k0, int wave) const {
+  // Load j of the stage from k0 on; none: zeros.
+  __device__ __forceinline__ void load(char *lds, int j, int k0, bool none, int wave) const {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base[j]), 0, none ? 0 : bytes[j], 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * WAVES) * 1024), 16,
-                                             voffset, j * apart + k0 * 2, 0, 0);
+                                             voffset, k0 * 2, 0, 0);
   }
 };
-
-// The buffer that holds a tile's rows of one operand: nothing past its last row's last k is read.
-template <class T>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const T *base, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base), 0, bytes, 0x00020000);
-}
 
 // This wave's loads into LDS have landed and its LDS reads are in registers, and so are every other wave's:
 // a barrier alone waits for neither.
@@ -172,19 +177,20 @@ __device__ __forceinline__ void arrive() {
 }
 
 // The loads of one stage, to be started one by one.
-template <class Cfg>
+template <class T, class Cfg>
 struct Loads {
   static constexpr int kCount = Cfg::A_LOADS + Cfg::B_LOADS;
-  const Loader<Cfg::WAVES> &loader_a;
-  const Loader<Cfg::WAVES> &loader_b;
-  __amdgpu_buffer_rsrc_t a_rows, b_rows;
+  const Loader<T, Cfg::A_LOADS, Cfg::WAVES> &loader_a;
+  const Loader<T, Cfg::B_LOADS, Cfg::WAVES> &loader_b;
   char *a, *b;
-  int a_k, b_k, wave;
+  int a_k, b_k;
+  bool none;
+  int wave;
   __device__ __forceinline__ void operator()(int q) const {
     if (q < Cfg::A_LOADS)
-      loader_a.load(a_rows, a, q, a_k, wave);
+      loader_a.load(a, q, a_k, none, wave);
     else
-      loader_b.load(b_rows, b, q - Cfg::A_LOADS, b_k, wave);
+      loader_b.load(b, q - Cfg::A_LOADS, b_k, none, wave);
   }
 };
 
@@ -259,35 +265,29 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   char *const a_even = a_evens[group], *const a_odd = a_odds[group], *const b_even = b_evens[group], *const b_odd = b_odds[group];
   const int wm = wave % Cfg::WAVES_M, wn = wave / Cfg::WAVES_M;
 
-  Loader<Cfg::WAVES> la, lb;
-  la.init(p.a_stride, wave, lane);
-  lb.init(p.b_stride, wave, lane);
   const int k = p.k_end ? min(p.k, max(0, p.k_end - w.batch * p.k)) : p.k;
-  auto bytes = [&](int rows, int64_t stride, int wrap) {
-    const int columns = k <= wrap ? k : max(wrap, k - wrap);
-    return (int)(((rows - 1) * stride + columns) * 2);
-  };
-  const int a_bytes = bytes(min(Cfg::BM, p.m - w.m0), p.a_stride, p.a_wrap);
-  const int b_bytes = bytes(min(Cfg::BN, p.n - w.n0), p.b_stride, p.b_wrap);
-  const T *const a_base = static_cast<const T *>(epilogue.operand(p, w.batch)) + w.m0 * p.a_stride;
-  const T *const b_base = static_cast<const T *>(p.b) + w.batch * p.b_batch + w.n0 * p.b_stride;
+  auto columns = [&](int wrap) { return k <= wrap ? k : max(wrap, k - wrap); };
+  Loader<T, Cfg::A_LOADS, Cfg::WAVES> la;
+  Loader<T, Cfg::B_LOADS, Cfg::WAVES> lb;
+  la.init(static_cast<const T *>(epilogue.operand(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
+  lb.init(static_cast<const T *>(p.b) + w.batch * p.b_batch + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
   // Stages of a group; those past the last k are zeros.
   const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
   int k0 = group * total * kStage;
   // The next stage's loads; past the last stage they read zeros.
   auto next_stage = [&](char *a, char *b) __attribute__((always_inline)) {
     const int left = k - k0;
-    const bool any = left > 0;
-    const Loads<Cfg> n{la, lb, rows_buffer<T>(a_base, any ? a_bytes : 0), rows_buffer<T>(b_base, any ? b_bytes : 0), a, b,
-                       k0 >= p.a_wrap ? k0 - p.a_wrap : k0, k0 >= p.b_wrap ? k0 - p.b_wrap : k0, wave};
+    const bool none = left <= 0;
+    const int from = none ? 0 : k0;  // a scalar offset past a buffer's end is not to be relied on
+    const Loads<T, Cfg> n{la, lb, a, b, from >= p.a_wrap ? from - p.a_wrap : from, from >= p.b_wrap ? from - p.b_wrap : from, none, wave};
     k0 += kStage;
-    if (any && left < kStage) la.cut(left), lb.cut(left);
+    if (!none && left < kStage) la.cut(left), lb.cut(left);
     return n;
   };
   auto load = [&](char *a, char *b) __attribute__((always_inline)) {
-    const Loads<Cfg> n = next_stage(a, b);
+    const Loads<T, Cfg> n = next_stage(a, b);
 #pragma unroll
-    for (int q = 0; q < Loads<Cfg>::kCount; ++q) n(q);
+    for (int q = 0; q < Loads<T, Cfg>::kCount; ++q) n(q);
   };
 
   f32x4 acc[Cfg::MI][Cfg::NI];
