@@ -274,6 +274,9 @@ struct LogitGradients : Piece {
   }
 };
 
+// Of a scale, a power of two.
+__device__ inline int exponent_of(const float *scale) { return __builtin_amdgcn_frexp_expf(scale[0]) - 1; }
+
 // A run of k of each product for itself: C of run b goes to sum[b], in 32 bits and unscaled, on top of what
 // an earlier piece left there.
 struct StoreSums : emrs_gemm::Operand {
@@ -286,7 +289,7 @@ struct StoreSums : emrs_gemm::Operand {
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4;
-    const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
+    const int by = exponent_of(scale_a) + exponent_of(scale_b);  // the product of the scales may be out of range
     float *const to = sum + w.batch * batch;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
@@ -305,7 +308,9 @@ struct StoreSums : emrs_gemm::Operand {
         const int at = m + i * 16;
         if (at >= p.m) continue;
         float *const o = to + n * stride + at;
-        const f32x4 c = acc[i][j] * by + before[i];
+        f32x4 c = before[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] += __builtin_amdgcn_ldexpf(acc[i][j][r], -by);
         if (wide) {
           *reinterpret_cast<f32x4 *>(o) = c;
           continue;
@@ -331,7 +336,7 @@ struct StoreRows : emrs_gemm::Operand {
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     using x4 = typename emrs_gemm::Vec<T>::x4;
     const int m = m0 + (lane >> 4) * 4;
-    const float by = 1.f / (scale_a[0] * scale_b[0]);  // powers of two
+    const int by = exponent_of(scale_a) + exponent_of(scale_b);  // the product of the scales may be out of range
     T *const to = static_cast<T *>(const_cast<void *>(out.p[w.batch]));
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
@@ -349,7 +354,9 @@ struct StoreRows : emrs_gemm::Operand {
         const int at = m + i * 16;
         if (at >= p.m) continue;
         const int64_t o = n * stride + at;
-        const f32x4 c = acc[i][j] * by + before[i];
+        f32x4 c = before[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] += __builtin_amdgcn_ldexpf(acc[i][j][r], -by);
         if (wide) {
           x4 v;
 #pragma unroll

@@ -270,6 +270,24 @@ def test_small_gradient_weights_in_fp16(gpu_device):
         assert (b.double() * 2 ** 10 - a.double()).abs().max() <= 2.0 ** -15  # the result's own smallest step
 
 
+@pytest.mark.parametrize("up,weight", [(-60, -40), (60, 45)])  # powers of two of hidden and of grad_loss
+@pytest.mark.parametrize("tokens,hidden,rows", [(40, 72, [130]), (600, 256, [3000, 3000])])
+def test_scales_far_from_one(gpu_device, tokens, hidden, rows, up, weight):
+    """hidden 2^up, weights 2^-up and grad_loss 2^weight of the plain ones: the same logits, and the same
+    gradients times a power of two each: to the last bit where that is in the range of normal numbers."""
+    h, w, target, g = _inputs(tokens, hidden, rows, torch.bfloat16)
+    lse, logit = training.vocab_statistics(h, w, target)
+    gh, gw = training.vocab_gradients(h, w, target, lse, g)
+    far_h, far_w, far_g = h * 2.0 ** up, [x * 2.0 ** -up for x in w], g * 2.0 ** weight
+    far_lse, far_logit = training.vocab_statistics(far_h, far_w, target)
+    assert torch.equal(lse, far_lse) and torch.equal(logit, far_logit)
+    far_gh, far_gw = training.vocab_gradients(far_h, far_w, target, far_lse, far_g)
+    for got, want, by in ((far_gh, gh, weight - up), *((a, b, weight + up) for a, b in zip(far_gw, gw))):
+        want = want.double() * 2.0 ** by
+        room = torch.where(want.abs() < 2.0 ** -126, 2.0 ** -126, 0.0)
+        assert (room == 0).any() and (got.double() - want).abs().le(room).all()
+
+
 def test_gradient_against_differences(gpu_device):
     """Loss differences over steps that bf16 holds exactly."""
     gen = torch.Generator(device="cuda").manual_seed(3)
