@@ -76,9 +76,12 @@ struct Tile {
 };
 
 // 256 x 256 with 8 waves of 128 x 64: a stage is 64 KB, and its 2^23 multiply-adds are 2048 cycles of the
-// CU's matrix units against 96 KB of fragment reads.  The smaller tiles are for products that would not
-// give every CU a large one.
+// CU's matrix units against 96 KB of fragment reads.  192 x 192 with 12 waves reads 1.33 times the bytes for a
+// multiply-add, and is for products whose large tiles would fill their last round badly: 253 of them take
+// 207 us where 136 large ones take 255 (4096 x 4096 by half, k 12288).  The smaller tiles are for products
+// that would not give every CU one of these.
 using Large = Tile<256, 256, 128, 64>;
+using Broad = Tile<192, 192, 64, 48>;
 using Medium = Tile<128, 128, 64, 64, 2>;
 using Small = Tile<64, 64, 32, 32, 4>;
 
@@ -100,6 +103,14 @@ struct Operand {
   }
 };
 
+// The row that holds place t of a triangle, whose row i holds i + 1.
+__device__ inline uint32_t triangle_row(uint32_t t) {
+  uint32_t i = (uint32_t)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
+  while (i * (i + 1) / 2 > t) --i;
+  while ((i + 1) * (i + 2) / 2 <= t) ++i;
+  return i;
+}
+
 // The tile of a workgroup.  Workgroups go to the XCDs in turn; each XCD gets a run of consecutive tiles,
 // and a run walks kGroup tiles of m for each n, so that its CUs share operand rows in the XCD's L2.
 template <class Cfg>
@@ -113,11 +124,18 @@ __device__ inline Where tile_of(const Product &p) {
   w.batch = t / per;
   t %= per;
   uint32_t i, j;
-  if (p.symmetric) {  // row i of the triangle holds i + 1 tiles
-    i = (uint32_t)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-    while (i * (i + 1) / 2 > t) --i;
-    while ((i + 1) * (i + 2) / 2 <= t) ++i;
-    j = t - i * (i + 1) / 2;
+  if (p.symmetric) {  // bands of kGroup rows: the columns left of the diagonal block, then that block
+    const uint32_t first = triangle_row(t) / kGroup * kGroup, rows = min((uint32_t)kGroup, tm - first);
+    uint32_t at = t - first * (first + 1) / 2;
+    if (at < first * rows) {
+      i = first + at % rows;
+      j = at / rows;
+    } else {
+      at -= first * rows;
+      const uint32_t r = triangle_row(at);
+      i = first + r;
+      j = first + at - r * (r + 1) / 2;
+    }
   } else {
     const uint32_t group = t / (kGroup * tn), first = group * kGroup, rows = min((uint32_t)kGroup, tm - first);
     const uint32_t at = t - group * kGroup * tn;
@@ -274,10 +292,11 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   // Stages of a group; those past the last k are zeros.
   const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
   int k0 = group * total * kStage;
+  const int k_to = min(k, k0 + total * kStage);
   // The next stage's loads; past the last stage they read zeros.
   auto next_stage = [&](char *a, char *b) __attribute__((always_inline)) {
     const int left = k - k0;
-    const bool none = left <= 0;
+    const bool none = k0 >= k_to;
     const int from = none ? 0 : k0;  // a scalar offset past a buffer's end is not to be relied on
     const Loads<T, Cfg> n{la, lb, a, b, from >= p.a_wrap ? from - p.a_wrap : from, from >= p.b_wrap ? from - p.b_wrap : from, none, wave};
     k0 += kStage;
@@ -371,11 +390,13 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p, own);
 }
 
-enum Shape { kLarge, kMedium, kSmall };
+enum Shape { kLarge, kBroad, kMedium, kSmall };
 
 // What a launch of one tile size takes, in microseconds, by its rounds of 256 workgroups (each has a CU's LDS
-// for itself): measured are 1.25 for a large tile's stage, 1.05 for the stage that each of a medium tile's
-// two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside its stages.
+// for itself): measured are 1.25 for a large tile's stage, 1.05 for a broad one's and for the stage that each
+// of a medium tile's two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside.
+// (A last round split along k instead, its pieces' sums joined by the last of them to end, was slower but for
+// the longest k: the sums of 240 pieces took 50 us on their way through memory.)
 template <class Cfg>
 inline double cost_of(const Product &p, double stage, double fixed) {
   const int64_t rounds = (tile_count<Cfg>(p) + 255) / 256, stages = (tiles_of(p.k, kStage) + Cfg::GROUPS - 1) / Cfg::GROUPS;
@@ -384,8 +405,11 @@ inline double cost_of(const Product &p, double stage, double fixed) {
 
 // Large tiles read the operands fewer times; smaller ones give more CUs work, and their waves share a long k.
 inline Shape shape_of(const Product &p) {
-  const double large = cost_of<Large>(p, 1.25, 8), medium = cost_of<Medium>(p, 1.05, 4), small = cost_of<Small>(p, 0.95, 3);
-  return large <= medium && large <= small ? kLarge : medium <= small ? kMedium : kSmall;
+  const double cost[4] = {cost_of<Large>(p, 1.25, 8), cost_of<Broad>(p, 1.05, 6), cost_of<Medium>(p, 1.05, 4), cost_of<Small>(p, 0.95, 3)};
+  int best = kLarge;
+  for (int i = kBroad; i <= kSmall; ++i)
+    if (cost[i] < cost[best]) best = i;
+  return (Shape)best;
 }
 
 template <class T, class Cfg, class Epilogue>
@@ -397,6 +421,7 @@ template <class T, class Epilogue>
 hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
   switch (shape_of(p)) {
     case kLarge: launch_as<T, Large>(p, e, stream); break;
+    case kBroad: launch_as<T, Broad>(p, e, stream); break;
     case kMedium: launch_as<T, Medium>(p, e, stream); break;
     case kSmall: launch_as<T, Small>(p, e, stream); break;
   }
@@ -407,6 +432,7 @@ hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
 inline int64_t wave_rows(const Product &p) {
   switch (shape_of(p)) {
     case kLarge: return tiles_of(p.m, Large::BM) * Large::WAVES_M;
+    case kBroad: return tiles_of(p.m, Broad::BM) * Broad::WAVES_M;
     case kMedium: return tiles_of(p.m, Medium::BM) * Medium::WAVES_M;
     default: return tiles_of(p.m, Small::BM) * Small::WAVES_M;
   }
