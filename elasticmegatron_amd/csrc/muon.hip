@@ -18,7 +18,7 @@
 // P = a I + b A + c A^2: near the end P is close to 0.7 I where b A + c A^2 is close to -2.7 I, and has a
 // quarter of its rounding; before, P's rounding on the diagonal would be such noise itself.  An error of A
 // enters by the polynomial's slope, b + 2 c A, of size 0.7 at the end.  Against 64 bits the result is then
-// below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 and 3e-3 for a matrix of rank one (4e-2 with one
+// below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 and 3.4e-3 for a matrix of rank one (4e-2 with one
 // part throughout, 3e-1 with bf16), about the rounding of the bf16 that it is written in.
 
 #include <hip/hip_runtime.h>
@@ -45,7 +45,7 @@ typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 constexpr float kGramScale = 64.f;  // of A and B: entries of a Gram matrix with spectrum in [0, 1.7]
 constexpr int kSide = 64;
 constexpr int kMaxMatrices = EMRS_MUON_MAX_MATRICES;
-constexpr int kMaxNormBlocks = 512;
+constexpr int kNormBlocks = 2048;  // of all matrices together
 
 template <class P>
 struct Table {
@@ -87,6 +87,15 @@ __device__ inline float block_sum(float v) {
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   return part[0] + part[1] + part[2] + part[3];
+}
+
+// The first part of a value, or a value whose parts are taken at two places, held in a register: the compiler
+// may otherwise round the product that it comes from to 16 bits at once in one place and by way of 32 in
+// another, and the first part that is stored is not always the one that the second part completes.
+template <class V>
+__device__ __forceinline__ V settled(V v) {
+  asm("" : "+v"(v));
+  return v;
 }
 
 // momentum = mu momentum + grad, and each workgroup's share of |update|^2.  Rows go to the workgroups in
@@ -133,43 +142,68 @@ struct Image {
   int64_t stride, batch, low;
 };
 
-// X_0 in both orientations, its two parts, and the padding's zeros.
+// X_0 in both orientations, its two parts, and the padding's zeros.  A workgroup turns a 64 x 64 tile over in
+// LDS; its elements are loaded before it adds up the norm.  Bound by its bytes: 1.07 GB
+// for four fp32 4096 x 4096 with momentum in 225 us, 4.7 TB/s, the rate of a copy.
+template <bool kWide>
 __global__ __launch_bounds__(256) void pack_kernel(Update u, const float *norms, int blocks, float eps, float scale, Image straight,
                                                    Image across, int parts) {
   __shared__ float tile[kSide][kSide + 1];
   const int b = blockIdx.z, r0 = blockIdx.y * kSide, c0 = blockIdx.x * kSide;
+  const int quad = threadIdx.x % 16 * 4, line = threadIdx.x / 16;
+  const void *grad = u.grad.p[b];
+  const float *buf = u.has_momentum ? u.momentum.p[b] : nullptr;
+  if (kWide) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t r = r0 + line + q * 16;
+      const int c = c0 + quad;
+      f32x4 v = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (r < u.rows && c < u.cols) {
+        if (!buf || u.nesterov) v = grad4_at(grad, u.grad_dtype, r * u.grad_stride + c);
+        if (buf) {
+          const f32x4 m = *reinterpret_cast<const f32x4 *>(buf + r * u.momentum_stride + c);
+          v = u.nesterov ? v + u.mu * m : m;
+        }
+      }
+      for (int i = 0; i < 4; ++i) tile[line + q * 16][quad + i] = v[i];
+    }
+  } else {
+    const int c = c0 + threadIdx.x % kSide;
+#pragma unroll 4
+    for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
+      const int64_t r = r0 + y;
+      float v = 0.f;
+      if (r < u.rows && c < u.cols) {
+        if (!buf || u.nesterov) v = grad_at(grad, u.grad_dtype, r * u.grad_stride + c);
+        if (buf) {
+          const float m = buf[r * u.momentum_stride + c];
+          v = u.nesterov ? v + u.mu * m : m;
+        }
+      }
+      tile[y][c - c0] = v;
+    }
+  }
   float norm = 0.f;
   for (int i = threadIdx.x; i < blocks; i += 256) norm += norms[b * blocks + i];
   norm = sqrtf(block_sum(norm));
   const float by = scale / (norm + eps);
-  const int x = threadIdx.x % kSide;
-  const void *grad = u.grad.p[b];
-  const float *buf = u.has_momentum ? u.momentum.p[b] : nullptr;
-  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
-    const int r = r0 + y, c = c0 + x;
-    float v = 0.f;
-    if (r < u.rows && c < u.cols) {
-      if (buf) {
-        v = buf[r * u.momentum_stride + c];
-        if (u.nesterov) v = grad_at(grad, u.grad_dtype, r * u.grad_stride + c) + u.mu * v;
-      } else {
-        v = grad_at(grad, u.grad_dtype, r * u.grad_stride + c);
-      }
-      v *= by;
-    }
-    tile[y][x] = v;
-    half *o = straight.p + b * straight.batch + r * straight.stride + c;
-    const half hi = (half)v;
-    o[0] = hi;
-    if (parts > 1) o[straight.low] = (half)(v - (float)hi);
-  }
+  auto store = [&](half *o, int64_t low, f32x4 x) __attribute__((always_inline)) {
+    half4 hi, lo;
+    for (int i = 0; i < 4; ++i) hi[i] = (half)x[i];
+    hi = settled(hi);
+    for (int i = 0; i < 4; ++i) lo[i] = (half)(x[i] - (float)hi[i]);
+    *reinterpret_cast<half4 *>(o) = hi;
+    if (parts > 1) *reinterpret_cast<half4 *>(o + low) = lo;
+  };
   __syncthreads();
-  for (int y = threadIdx.x / kSide; y < kSide; y += 256 / kSide) {
-    const float v = tile[x][y];
-    half *o = across.p + b * across.batch + (c0 + y) * across.stride + r0 + x;
-    const half hi = (half)v;
-    o[0] = hi;
-    if (parts > 1) o[across.low] = (half)(v - (float)hi);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int y = line + q * 16;
+    f32x4 v, t;
+    for (int i = 0; i < 4; ++i) v[i] = tile[y][quad + i], t[i] = tile[quad + i][y];
+    store(straight.p + b * straight.batch + (r0 + y) * straight.stride + c0 + quad, straight.low, v * by);
+    store(across.p + b * across.batch + (c0 + y) * across.stride + r0 + quad, across.low, t * by);
   }
 }
 
@@ -265,6 +299,7 @@ struct StoreSquare : emrs_gemm::Operand {
           const half4 hi = *reinterpret_cast<const half4 *>(x), lo = *reinterpret_cast<const half4 *>(x + low);
           for (int r = 0; r < 4; ++r) acc[i][j][r] += (m0 + m + r == n0 + n ? a : 0.f) + b * ((float)hi[r] + (float)lo[r]);
         }
+        acc[i][j] = settled(acc[i][j]);
         half4 v;
         for (int r = 0; r < 4; ++r) v[r] = (half)acc[i][j][r];
         emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
@@ -311,7 +346,7 @@ struct StoreIterate : emrs_gemm::Operand {
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int m = inside(i * 16 + (lane >> 4) * 4, m0, p.m - 4), n = inside(j * 16 + (lane & 15), n0, p.n - 1);
-        acc[i][j] = applied(x, n * step + m, low, in_parts, a, acc[i][j]);
+        acc[i][j] = settled(applied(x, n * step + m, low, in_parts, a, acc[i][j]));
         half4 v;
         for (int r = 0; r < 4; ++r) v[r] = (half)acc[i][j][r];
         Turn::put(own, i, j, lane, v);
@@ -512,7 +547,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(Small a) {
       const int at = from + i * kThreads, r = row_of(at, over_all), c = at - r * all_cols;
       if (at >= all) continue;
       const float v = (buf ? a.u.nesterov ? g[i] + a.u.mu * m[i] : m[i] : g[i]) * by;
-      const half h = (half)v;
+      const half h = settled((half)v);
       const int o = a.tall ? x_at(c, r) : x_at(r, c);
       hi[o] = h;
       lo[o] = (half)(v - (float)h);
@@ -655,7 +690,9 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(Small a) {
       for (int j = 0; j < ST; ++j) {
         const int o = x_at(j * 16 + t, l + q * 4);
         half4 x, y;
-        for (int i = 0; i < 4; ++i) x[i] = (half)acc[r][j][i], y[i] = (half)(acc[r][j][i] - (float)x[i]);
+        for (int i = 0; i < 4; ++i) x[i] = (half)acc[r][j][i];
+        x = settled(x);
+        for (int i = 0; i < 4; ++i) y[i] = (half)(acc[r][j][i] - (float)x[i]);
         *reinterpret_cast<half4 *>(hi + o) = x;
         *reinterpret_cast<half4 *>(lo + o) = y;
       }
@@ -722,7 +759,7 @@ Sizes sizes_of(const emrs_muon *a) {
   Sizes z{};
   z.s = round_up(std::min(a->rows, a->cols), kSide);
   z.l = round_up(std::max(a->rows, a->cols), kSide);
-  z.blocks = (uint32_t)std::min<uint64_t>(a->rows, kMaxNormBlocks);
+  z.blocks = (uint32_t)std::min<uint64_t>(a->rows, std::max<uint64_t>(kNormBlocks / a->count, 256));
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -877,7 +914,11 @@ int step(const emrs_muon *a, hipStream_t st) {
   const int64_t square = (int64_t)(z.s * z.s);
 
   const dim3 tiles(round_up(a->cols, kSide) / kSide, round_up(a->rows, kSide) / kSide, a->count);
-  pack_kernel<<<tiles, 256, 0, st>>>(u, norms, (int)z.blocks, a->eps, scale, tall ? xt(0) : x(0), tall ? x(0) : xt(0), parts_of(0));
+  const Image straight = tall ? xt(0) : x(0), across = tall ? x(0) : xt(0);
+  if (wide)
+    pack_kernel<true><<<tiles, 256, 0, st>>>(u, norms, (int)z.blocks, a->eps, scale, straight, across, parts_of(0));
+  else
+    pack_kernel<false><<<tiles, 256, 0, st>>>(u, norms, (int)z.blocks, a->eps, scale, straight, across, parts_of(0));
   TRY(hipGetLastError());
 
   int now = 0;
