@@ -96,10 +96,13 @@ struct Where {
   int m0, n0, batch;
 };
 
-// What an epilogue is beside its run(): where operand a of a matrix of the batch begins.
+// What an epilogue is beside its run(): where the operands of a matrix of the batch begin.
 struct Operand {
-  __device__ __forceinline__ const void *operand(const Product &p, int batch) const {
+  __device__ __forceinline__ const void *operand_a(const Product &p, int batch) const {
     return static_cast<const char *>(p.a) + batch * p.a_batch * 2;
+  }
+  __device__ __forceinline__ const void *operand_b(const Product &p, int batch) const {
+    return static_cast<const char *>(p.b) + batch * p.b_batch * 2;
   }
 };
 
@@ -287,8 +290,8 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   auto columns = [&](int wrap) { return k <= wrap ? k : max(wrap, k - wrap); };
   Loader<T, Cfg::A_LOADS, Cfg::WAVES> la;
   Loader<T, Cfg::B_LOADS, Cfg::WAVES> lb;
-  la.init(static_cast<const T *>(epilogue.operand(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
-  lb.init(static_cast<const T *>(p.b) + w.batch * p.b_batch + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
+  la.init(static_cast<const T *>(epilogue.operand_a(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
+  lb.init(static_cast<const T *>(epilogue.operand_b(p, w.batch)) + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
   // Stages of a group; those past the last k are zeros.
   const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
   int k0 = group * total * kStage;

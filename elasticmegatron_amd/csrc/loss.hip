@@ -54,7 +54,8 @@ struct Piece {
   int64_t first, shard;   // vocabulary index of the first shard's first row here; rows from a shard to the next
   int64_t vocab;          // rows from this vocabulary index on do not count
 
-  __device__ __forceinline__ const void *operand(const Product &, int batch) const { return weights.p[batch]; }
+  __device__ __forceinline__ const void *operand_a(const Product &, int batch) const { return weights.p[batch]; }
+  __device__ __forceinline__ const void *operand_b(const Product &p, int batch) const { return emrs_gemm::Operand{}.operand_b(p, batch); }
   __host__ __device__ int64_t first_of(int batch) const { return first + batch * shard; }
   __device__ __forceinline__ int valid(int batch, int rows) const {
     return (int)min((int64_t)rows, max((int64_t)0, vocab - first_of(batch)));

@@ -278,10 +278,19 @@ struct StorePolynomial : emrs_gemm::Operand {
 // A product of symmetric matrices that commute, in two parts like its operands (side by side in a row, the
 // second `stride` / 2 on): a I + b A + c A A for the polynomial, c alone for the others.
 struct StoreSquare : emrs_gemm::Operand {
-  half *out;
+  half *out, *second_out;
   const half *in;         // A, or NULL
+  const half *second;     // the first operand of matrices from `count` on, which share the second operand with
+  int32_t count;          // the first `count`, and whose product goes to second_out
   int64_t stride, batch;
   float a, b, c;
+
+  __device__ __forceinline__ const void *operand_a(const Product &p, int i) const {
+    return i < count ? static_cast<const half *>(p.a) + i * p.a_batch : second + (i - count) * p.a_batch;
+  }
+  __device__ __forceinline__ const void *operand_b(const Product &p, int i) const {
+    return static_cast<const half *>(p.b) + (i < count ? i : i - count) * p.b_batch;
+  }
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
@@ -305,7 +314,7 @@ struct StoreSquare : emrs_gemm::Operand {
         emrs_gemm::Turn<Cfg>::put(own, i, j, lane, v);
       }
     }
-    half *const to = out + w.batch * batch;
+    half *const to = w.batch < count ? out + w.batch * batch : second_out + (w.batch - count) * batch;
     store_symmetric<Cfg>(to, stride, w, m0, n0, lane, p, own);
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j)
@@ -929,14 +938,16 @@ int step(const emrs_muon *a, hipStream_t st) {
     auto matrix = [&](int i) { return squares + i * (int64_t)a->count * each; };
     half *gram_of = matrix(0), *const p_of = matrix(1), *spare = matrix(2), *q_of = matrix(3), *q_next = matrix(4);
     // hi hi + hi lo + lo hi
-    auto square = [&](const half *m, const half *n, half *out, const half *poly_of, float fa, float fb, float fc) {
+    // With a second m, its product with n too: launches of small matrices are bound by their number.
+    auto square = [&](const half *m, const half *n, half *out, const half *poly_of, float fa, float fb, float fc,
+                      const half *second = nullptr, half *second_out = nullptr) {
       Product g{};
       g.a = m, g.b = n;
       g.a_stride = g.b_stride = two, g.a_batch = g.b_batch = each;
       g.m = g.n = (int)z.s, g.k = 3 * (int)z.s;
       g.a_wrap = (int)z.s, g.b_wrap = 2 * (int)z.s;
-      g.batch = (int)a->count, g.symmetric = 1;
-      return emrs_gemm::launch<half>(g, StoreSquare{{}, out, poly_of, two, each, fa, fb, fc}, st);
+      g.batch = (int)a->count * (second ? 2 : 1), g.symmetric = 1;
+      return emrs_gemm::launch<half>(g, StoreSquare{{}, out, second_out, poly_of, second, (int)a->count, two, each, fa, fb, fc}, st);
     };
     const Image in = x(0), in_t = xt(0);
     Product g{};
@@ -945,19 +956,20 @@ int step(const emrs_muon *a, hipStream_t st) {
     g.m = g.n = (int)z.s, g.k = 3 * (int)z.l;
     g.a_wrap = (int)z.l, g.b_wrap = 2 * (int)z.l;
     g.batch = (int)a->count, g.symmetric = 1;
-    TRY((emrs_gemm::launch<half>(g, StoreSquare{{}, gram_of, nullptr, two, each, 0.f, 0.f, kGramScale / (scale * scale)}, st)));
+    TRY((emrs_gemm::launch<half>(g, StoreSquare{{}, gram_of, nullptr, nullptr, nullptr, (int)a->count, two, each, 0.f, 0.f, kGramScale / (scale * scale)}, st)));
     constexpr float one = 1.f / kGramScale;
     for (; parts_of(done) == 2; ++done) {
       const float *f = a->coefficients + 3 * done;
       half *const p = done == 0 ? q_of : p_of;
       TRY(square(gram_of, gram_of, p, gram_of, f[0] * kGramScale, f[1], f[2] * one));
-      if (parts_of(done + 1) == 2) {
-        TRY(square(p, gram_of, spare, nullptr, 0.f, 0.f, one));
-        TRY(square(spare, p, gram_of, nullptr, 0.f, 0.f, one));
+      const bool again = parts_of(done + 1) == 2;
+      if (done == 0) {
+        TRY(square(gram_of, p, spare, nullptr, 0.f, 0.f, one));
+      } else {
+        TRY(again ? square(q_of, p, q_next, nullptr, 0.f, 0.f, one, gram_of, spare) : square(q_of, p, q_next, nullptr, 0.f, 0.f, one));
+        std::swap(q_of, q_next);
       }
-      if (done == 0) continue;
-      TRY(square(p, q_of, q_next, nullptr, 0.f, 0.f, one));
-      std::swap(q_of, q_next);
+      if (again) TRY(square(spare, p, gram_of, nullptr, 0.f, 0.f, one));
     }
     Product r{};
     r.a = in_t.p, r.b = q_of;
