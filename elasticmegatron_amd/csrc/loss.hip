@@ -490,22 +490,33 @@ constexpr int kSide = 64;
 
 // out[c][r] = scale in[r][c] for the rows that count and every c, with zeros in the others, up to `padded` r
 // for each matrix, one beside the other.
+struct Turned {
+  Rows rows;
+  half *out;
+  int64_t out_stride;
+  int32_t padded;
+
+  __host__ __device__ uint32_t across() const { return (uint32_t)(padded + kSide - 1) / kSide; }
+  __host__ __device__ uint32_t tiles(int cols) const { return rows.count * across() * ((uint32_t)(cols + kSide - 1) / kSide); }
+};
+
+// Column c of the tile in row c of LDS; a row's 16-byte units of eight r are permuted by c, so that the eight
+// columns that a lane reads in one row meet no other lane's bank.
 template <class T>
-__global__ __launch_bounds__(256) void transpose_kernel(Rows a, int cols, half *out, int64_t out_stride, int padded) {
-  // Column c of the tile in row c of LDS; a row's 16-byte units of eight r are permuted by c, so that the
-  // eight columns that a lane reads in one row meet no other lane's bank.
-  __shared__ __attribute__((aligned(16))) half tile[kSide][kSide];
+__device__ __forceinline__ void turn(const Turned &to, uint32_t id, int cols, half (&tile)[kSide][kSide]) {
   using x8 = typename emrs_gemm::Vec<T>::x8;
-  const int r0 = blockIdx.x * kSide, c0 = blockIdx.y * kSide;
-  const T *in = static_cast<const T *>(a.piece.weights.p[blockIdx.z]);
-  const int valid = a.piece.valid(blockIdx.z, a.rows);
+  const Rows &a = to.rows;
+  const uint32_t matrix = id % (uint32_t)a.count, tile_at = id / (uint32_t)a.count;
+  const int r0 = (int)(tile_at % to.across()) * kSide, c0 = (int)(tile_at / to.across()) * kSide;
+  const T *in = static_cast<const T *>(a.piece.weights.p[matrix]);
+  const int valid = a.piece.valid(matrix, a.rows);
   float by = 1.f;
   if (a.blocks) {
     float top = 0.f;
     for (int i = threadIdx.x; i < a.count * a.blocks; i += 256) top = fmaxf(top, a.largest[i]);
     by = scale_of(block_max(top));
   }
-  if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) a.scale[0] = by;
+  if (id + threadIdx.x == 0) a.scale[0] = by;
   const bool wide = cols % 8 == 0 && a.stride % 8 == 0 && reinterpret_cast<uintptr_t>(in) % 16 == 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -529,10 +540,21 @@ __global__ __launch_bounds__(256) void transpose_kernel(Rows a, int cols, half *
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int at = threadIdx.x + h * 256, c = at / 8, unit = at % 8, r = r0 + unit * 8;
-    if (c0 + c < cols && r < padded)
-      *reinterpret_cast<emrs_gemm::fp16x8 *>(out + (c0 + c) * out_stride + (int64_t)blockIdx.z * padded + r) =
+    if (c0 + c < cols && r < to.padded)
+      *reinterpret_cast<emrs_gemm::fp16x8 *>(to.out + (c0 + c) * to.out_stride + (int64_t)matrix * to.padded + r) =
           *reinterpret_cast<const emrs_gemm::fp16x8 *>(&tile[c][(unit ^ (c / 8)) * 8]);
   }
+}
+
+// Both kinds in one launch.
+template <class T>
+__global__ __launch_bounds__(256) void transpose_kernel(Turned weights, Turned hidden, int cols) {
+  __shared__ __attribute__((aligned(16))) half tile[kSide][kSide];
+  const uint32_t firsts = weights.tiles(cols);
+  if (blockIdx.x < firsts)
+    turn<T>(weights, blockIdx.x, cols, tile);
+  else
+    turn<T>(hidden, blockIdx.x - firsts, cols, tile);
 }
 
 // out[r][c] = in[r][c], with zeros from `cols` up to the padded row: operands whose rows do not lie on 16 bytes.
@@ -745,14 +767,6 @@ Rows rows_of(const Piece &c, uint32_t count, int64_t stride, int64_t rows, const
 }
 
 template <class T>
-int transpose(const Rows &r, int64_t cols, half *out, int64_t out_stride, int64_t padded, hipStream_t st) {
-  const dim3 grid((padded + kSide - 1) / kSide, (cols + kSide - 1) / kSide, r.count);
-  transpose_kernel<T><<<grid, 256, 0, st>>>(r, (int)cols, out, out_stride, (int)padded);
-  TRY(hipGetLastError());
-  return EMRS_OK;
-}
-
-template <class T>
 int backward(const emrs_loss *a, hipStream_t st) {
   const Sizes s = sizes_of(a, true);
   char *ws = static_cast<char *>(a->workspace);
@@ -790,9 +804,11 @@ int backward(const emrs_loss *a, hipStream_t st) {
                                                   a->target, a->ignore_index, (int)tokens, d_scale);
         TRY(hipGetLastError());
       }
-      if (!scaled && a->grad_weights) {
-        rc = transpose<T>(h_rows, h, ht, (int64_t)s.tokens_padded, (int64_t)s.tokens_padded, st);
-        if (rc) return rc;
+      const Turned w_turned{a->grad_hidden ? w_rows : none, wt, (int64_t)(g.count * padded), (int32_t)padded};
+      const Turned h_turned{scaled || !a->grad_weights ? none : h_rows, ht, (int64_t)s.tokens_padded, (int32_t)s.tokens_padded};
+      if (const uint32_t tiles = w_turned.tiles((int)h) + h_turned.tiles((int)h)) {
+        transpose_kernel<T><<<tiles, 256, 0, st>>>(w_turned, h_turned, (int)h);
+        TRY(hipGetLastError());
       }
       scaled = true;
       Piece c = own;
@@ -803,8 +819,6 @@ int backward(const emrs_loss *a, hipStream_t st) {
       TRY((emrs_gemm::launch<T>(p, LogitGradients{c, a->grad_hidden ? d : nullptr, wanted ? dt : nullptr, (int32_t)(g.count * padded),
                                                   (int32_t)s.tokens_padded, (int32_t)padded, a->lse, a->grad_loss, a->target, a->ignore_index, d_scale}, st)));
       if (a->grad_hidden) {
-        rc = transpose<T>(w_rows, h, wt, (int64_t)(g.count * padded), (int64_t)padded, st);
-        if (rc) return rc;
         Product q{};
         q.a = wt, q.b = d;
         q.a_stride = q.b_stride = g.count * padded;
