@@ -12,6 +12,10 @@
 // c ^ swizzle(r): the 16 rows that a fragment read takes at one c then lie in 16 different slots of the
 // 64 banks.  Rows past the operand's last are past the buffer's end and read as zeros, and so are, by
 // their lane's offset, units past the last k.
+//
+// What bounds it is the card's power: in large products matrix instructions issue in 83% of the cycles, at 1.6
+// to 1.8 GHz.  Measured with what the epilogues do: statistics of 4096 x 32000 logits, k 4096, 780 us (1.38
+// PFLOP/s); d of 4096 x 16384, 450 us (1.22); the gradients' products of that d, 425 and 440 us (1.27).
 #ifndef EMRS_GEMM_H
 #define EMRS_GEMM_H
 

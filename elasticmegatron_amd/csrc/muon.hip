@@ -99,7 +99,8 @@ __device__ __forceinline__ V settled(V v) {
 }
 
 // momentum = mu momentum + grad, and each workgroup's share of |update|^2.  Rows go to the workgroups in
-// turn.  No atomics: the sums are the same on every run.
+// turn.  No atomics: the sums are the same on every run.  One pass: 805 MB for four fp32 4096 x 4096 in 155
+// us, 5.2 TB/s; with 512 workgroups in place of 2048, 3.0.
 template <bool kWide>
 __global__ __launch_bounds__(256) void momentum_kernel(Update u, float *norms) {
   const int b = blockIdx.y;
@@ -339,6 +340,8 @@ __device__ __forceinline__ f32x4 applied(const half *x, int at, int low, int par
 }
 
 // The next X (m: the longer side), in both orientations: its first part, then, where it has one, its second.
+// Units of 16 bytes through LDS (four elements a lane: 995 us for four 4096 x 4096 from two parts to two, 880
+// with, at the clock of that day); reading X and writing both orientations is a fifth of the time.
 struct StoreIterate : emrs_gemm::Operand {
   Image in, out, across;
   int32_t in_parts, out_parts;
@@ -459,7 +462,8 @@ struct StoreResult : emrs_gemm::Operand {
 // X lies [s][l] (s: the shorter side, padded to 32; l to 64), units of 16 bytes permuted by s; the product
 // X <- P X takes the columns of X as rows through the transposing LDS read.  LDS reads bound it, so a
 // wave of the S x S products computes 32 x 32, on or below the diagonal; where that leaves waves over, KS of
-// them share one over k.  For P X a wave has all S of every 16th 16 of L.
+// them share one over k.  For P X a wave has all S of every 16th 16 of L.  128 x 128 takes 41 us, one or two
+// of them; as launches of the large kernels, 108.
 
 struct Small {
   Update u;
