@@ -22,6 +22,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace emrs_gemm {
 
@@ -102,6 +103,7 @@ struct Where {
 
 // What an epilogue is beside its run(): where the operands of a matrix of the batch begin.
 struct Operand {
+  static constexpr bool kRowsOfK = false;  // whether operand a is [k][m]
   __device__ __forceinline__ const void *operand_a(const Product &p, int batch) const {
     return static_cast<const char *>(p.a) + batch * p.a_batch * 2;
   }
@@ -190,6 +192,36 @@ struct Loader {
   }
 };
 
+// The same of an operand a that is [k][m]: a stage is 64 of its rows, BM long each, 16-byte units permuted by
+// the row so that the transposing reads of 32 lanes, eight rows of 32 bytes, meet in different banks.  Rows
+// that do not count are past the end of their buffer.
+template <class T, class Cfg>
+struct RowLoader {
+  static constexpr int kUnits = Cfg::BM / 8, kRows = 64 / kUnits;  // of a row; of one load
+  int voffset, columns;
+  int64_t stride;
+  const T *first;  // the stage's first row, at the tile's first m
+  int rows;        // that count from there on
+  static __device__ __forceinline__ int permuted(int row) {
+    return Cfg::BM == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : (row & 3) | (row >> 3 & 1) << 2;
+  }
+  __device__ __forceinline__ void init(int64_t row_stride, int columns_here, int wave, int lane) {
+    static_assert(Cfg::BM == 128 || Cfg::BM == 64, "whole rows in a load");
+    static_assert(Cfg::WAVES * kRows % 16 == 0, "a wave's loads are permuted alike");
+    const int row = lane / kUnits, unit = lane % kUnits;
+    stride = row_stride, columns = columns_here;
+    voffset = (int)(row * stride * 2) + ((unit ^ permuted(wave * kRows + row) << 1) << 4);
+  }
+  __device__ __forceinline__ void cut(int) {}
+  __device__ __forceinline__ void load(char *lds, int j, int, bool none, int wave) const {
+    const int from = (wave + j * Cfg::WAVES) * kRows, here = min(rows - from, kRows);
+    const int bytes = none || here <= 0 ? 0 : (int)(((here - 1) * stride + columns) * 2);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(first + from * stride), 0, bytes, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * Cfg::WAVES) * 1024), 16,
+                                             voffset, 0, 0, 0);
+  }
+};
+
 // This wave's loads into LDS have landed and its LDS reads are in registers, and so are every other wave's:
 // a barrier alone waits for neither.
 __device__ __forceinline__ void arrive() {
@@ -202,10 +234,10 @@ __device__ __forceinline__ void arrive() {
 }
 
 // The loads of one stage, to be started one by one.
-template <class T, class Cfg>
+template <class T, class Cfg, class LoaderA>
 struct Loads {
   static constexpr int kCount = Cfg::A_LOADS + Cfg::B_LOADS;
-  const Loader<T, Cfg::A_LOADS, Cfg::WAVES> &loader_a;
+  const LoaderA &loader_a;
   const Loader<T, Cfg::B_LOADS, Cfg::WAVES> &loader_b;
   char *a, *b;
   int a_k, b_k;
@@ -223,6 +255,16 @@ struct NoLoads {
   static constexpr int kCount = 0;
   __device__ void operator()(int) const {}
 };
+
+// Eight consecutive k of a lane's m from rows of k: sixteen lanes read a block of 4 k x 16 m as it lies, twice.
+template <class X8>
+__device__ __forceinline__ X8 along_k(const char *at, int four_rows) {
+  typedef __attribute__((ext_vector_type(4))) short s16x4;
+  typedef __attribute__((address_space(3))) s16x4 *lds4;
+  char *const lo = const_cast<char *>(at);
+  const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)lo), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(lo + four_rows));
+  return __builtin_bit_cast(X8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+}
 
 // Where a group after the first leaves sum q of its lanes: the stages' arrays, one after the other.
 template <class Cfg>
@@ -292,9 +334,14 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
 
   const int k = p.k_end ? min(p.k, max(0, p.k_end - w.batch * p.k)) : p.k;
   auto columns = [&](int wrap) { return k <= wrap ? k : max(wrap, k - wrap); };
-  Loader<T, Cfg::A_LOADS, Cfg::WAVES> la;
+  constexpr bool rows_of_k = Epilogue::kRowsOfK;
+  typename std::conditional<rows_of_k, RowLoader<T, Cfg>, Loader<T, Cfg::A_LOADS, Cfg::WAVES>>::type la;
+  using NextLoads = Loads<T, Cfg, decltype(la)>;
   Loader<T, Cfg::B_LOADS, Cfg::WAVES> lb;
-  la.init(static_cast<const T *>(epilogue.operand_a(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
+  if constexpr (rows_of_k)
+    la.init(p.a_stride, min(Cfg::BM, ((p.m + 7) & ~7) - w.m0), wave, lane);
+  else
+    la.init(static_cast<const T *>(epilogue.operand_a(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
   lb.init(static_cast<const T *>(epilogue.operand_b(p, w.batch)) + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
   // Stages of a group; those past the last k are zeros.
   const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
@@ -305,15 +352,19 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
     const int left = k - k0;
     const bool none = k0 >= k_to;
     const int from = none ? 0 : k0;  // a scalar offset past a buffer's end is not to be relied on
-    const Loads<T, Cfg> n{la, lb, a, b, from >= p.a_wrap ? from - p.a_wrap : from, from >= p.b_wrap ? from - p.b_wrap : from, none, wave};
+    if constexpr (rows_of_k) {
+      epilogue.rows_from(p, w.batch * p.k + from, la.first, la.rows);
+      la.first += w.m0;
+    }
+    const NextLoads n{la, lb, a, b, from >= p.a_wrap ? from - p.a_wrap : from, from >= p.b_wrap ? from - p.b_wrap : from, none, wave};
     k0 += kStage;
     if (!none && left < kStage) la.cut(left), lb.cut(left);
     return n;
   };
   auto load = [&](char *a, char *b) __attribute__((always_inline)) {
-    const Loads<T, Cfg> n = next_stage(a, b);
+    const NextLoads n = next_stage(a, b);
 #pragma unroll
-    for (int q = 0; q < Loads<T, Cfg>::kCount; ++q) n(q);
+    for (int q = 0; q < NextLoads::kCount; ++q) n(q);
   };
 
   f32x4 acc[Cfg::MI][Cfg::NI];
@@ -325,12 +376,21 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   const int row = lane & 15, c = lane >> 4;
   const int unit[2] = {(c ^ swizzle(row)) << 4, ((4 + c) ^ swizzle(row)) << 4};
   const int a_at = (wm * Cfg::WM + row) * 128, b_at = (wn * Cfg::WN + row) * 128;
+  int a_rows[rows_of_k ? Cfg::MI : 1];
+  if constexpr (rows_of_k) {
+    const int k = c * 8 + (row >> 2);
+#pragma unroll
+    for (int i = 0; i < Cfg::MI; ++i)
+      a_rows[i] = k * Cfg::BM * 2 + ((wm * Cfg::MI + i) ^ RowLoader<T, Cfg>::permuted(k)) * 32 + (row & 3) * 8;
+  }
   struct Fragments {
     x8 a[Cfg::MI], b[Cfg::NI];
   } even, odd;  // of the first and the second 32 k of a stage
   auto read_one = [&](Fragments &f, const char *a, const char *b, int kk, int r) __attribute__((always_inline)) {
     if (r < Cfg::NI)
       f.b[r] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + r * 2048);
+    else if constexpr (rows_of_k)
+      f.a[r - Cfg::NI] = along_k<x8>(a + a_rows[r - Cfg::NI] + kk * 64 * Cfg::BM, 8 * Cfg::BM);
     else
       f.a[r - Cfg::NI] = *reinterpret_cast<const x8 *>(a + a_at + unit[kk] + (r - Cfg::NI) * 2048);
   };
@@ -432,6 +492,16 @@ hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
     case kMedium: launch_as<T, Medium>(p, e, stream); break;
     case kSmall: launch_as<T, Small>(p, e, stream); break;
   }
+  return hipGetLastError();
+}
+
+// With operand a [k][m]: the smaller tiles alone, since it is for products of few n.
+template <class T, class Epilogue>
+hipError_t launch_rows_of_k(const Product &p, const Epilogue &e, hipStream_t stream) {
+  if (cost_of<Medium>(p, 1.05, 4) <= cost_of<Small>(p, 0.95, 3))
+    launch_as<T, Medium>(p, e, stream);
+  else
+    launch_as<T, Small>(p, e, stream);
   return hipGetLastError();
 }
 
