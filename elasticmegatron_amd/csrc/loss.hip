@@ -38,8 +38,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kPieceBytes = 128ull << 20;  // of d in one orientation
 
 // Whether grad_hidden's product takes the weights as they lie: no search of their largest entry, no transposed
-// copy, but smaller tiles, and for bf16 a second part of d.  Of 32000 x 4096, bf16: 32 tokens 322 against 443
-// us, 512 tokens 764 against 724; fp16: 32 tokens 266 against 380, 1024 tokens 977 against 1040.
+// copy, but smaller tiles, and for bf16 twice the rows of d, in two parts.  All
+// gradients of 32000 x 4096 in bf16: 32 tokens 257 against 443 us, 384 tokens 719 against 657; in fp16: 32
+// tokens 246 against 380, 1024 tokens 923 against 989, 2048 tokens 1746 against 1669.
 bool takes_weights(uint32_t dtype, uint64_t tokens) { return tokens <= (dtype == EMRS_BF16 ? 256 : 1024); }
 
 
@@ -234,8 +235,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_statistics_kernel(const f
 
 // d of a piece, in both orientations, with zeros up to the padded sizes (the next products sum over them).  Its
 // 512 KB a large tile of exponentials and stores are what it is slower by than the statistics.
-// With kParts d is in two bf16 parts, side by side in a row: what the product with bf16 weights as they lie
-// takes.
+// With kParts d is in two bf16 parts, [2][tokens]: what the product with bf16 weights as they lie takes.
 template <bool kParts>
 struct LogitGradients : Piece {
   half *d;                // [tokens][shards x padded rows]: m contiguous; NULL: not wanted
@@ -300,14 +300,13 @@ struct LogitGradients : Piece {
             for (int r = 0; r < 4; ++r) acc[i][j][r] -= (float)v[r];
             Turn::put(own, i, j, lane, v);
           }
-        rows(to + (part ? d_stride / 2 : 0));
+        rows(to + part * (int64_t)p.n * d_stride);
       }
     }
   }
 };
 
-// A product with the weight's own rows as rows of k: of every shard in turn, padded, and once more from the
-// start for the second part of the other operand.
+// A product with the weight's own rows as rows of k: of every shard in turn, padded.
 template <class Base>
 struct OfWeights : Base {
   static constexpr bool kRowsOfK = true;
@@ -316,7 +315,6 @@ struct OfWeights : Base {
 
   template <class T>
   __device__ __forceinline__ void rows_from(const Product &p, int k, const T *&first, int &count) const {
-    k = k >= all ? k - all : k;
     const int shard = k < all ? k / padded : 0, row = k - shard * padded;
     first = static_cast<const T *>(piece.weights.p[shard]) + row * p.a_stride;
     count = k < all ? piece.valid(shard, rows) - row : 0;
@@ -372,18 +370,20 @@ struct StoreSums : emrs_gemm::Operand {
   }
 };
 
-// C as 16-bit rows out[n][m], on top of a sum of earlier pieces if there is one.
+// C as 16-bit rows out[n][m], on top of a sum of earlier pieces if there is one; through LDS, so that rows are
+// stored in whole lines (262 MB of gradients of few tokens: 87 us; with four elements a lane, 104).
 template <class T>
 struct StoreRows : emrs_gemm::Operand {
   Table out;              // of each matrix of the batch
   const float *sum;       // NULL: C alone (a batch of one)
   int64_t stride;         // elements between rows of out and of sum
-  int32_t wide;           // four elements can be stored at once
+  int32_t wide;           // eight elements can be stored at once
   const float *scale_a, *scale_b;
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     using x4 = typename emrs_gemm::Vec<T>::x4;
+    using Turn = emrs_gemm::Turn<Cfg>;
     const int m = m0 + (lane >> 4) * 4;
     const int by = exponent_of(scale_a) + exponent_of(scale_b);  // the product of the scales may be out of range
     T *const to = static_cast<T *>(const_cast<void *>(out.p[w.batch]));
@@ -397,12 +397,8 @@ struct StoreRows : emrs_gemm::Operand {
 #pragma unroll
         for (int i = 0; i < Cfg::MI; ++i)
           before[i] = *reinterpret_cast<const f32x4 *>(sum + min(n, p.n - 1) * stride + min(m + i * 16, p.m - 4));
-      if (n >= p.n) continue;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
-        const int at = m + i * 16;
-        if (at >= p.m) continue;
-        const int64_t o = n * stride + at;
         f32x4 c = before[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r) c[r] += __builtin_amdgcn_ldexpf(acc[i][j][r], -by);
@@ -410,14 +406,22 @@ struct StoreRows : emrs_gemm::Operand {
           x4 v;
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = (T)c[r];
-          *reinterpret_cast<x4 *>(to + o) = v;
+          Turn::put(own, i, j, lane, v);
           continue;
         }
+        const int at = m + i * 16;
+        const int64_t o = n * stride + at;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (at + r < p.m) to[o + r] = (T)(c[r] + (sum ? sum[o + r] : 0.f));
+          if (n < p.n && at + r < p.m) to[o + r] = (T)(c[r] + (sum ? sum[o + r] : 0.f));
       }
     }
+    if (!wide) return;
+    T *const corner = to + n0 * stride + m0;
+    const int step = (int)stride;  // 256 rows of 2^20 elements at most
+    Turn::along_m(own, lane, [&](int x, int y, emrs_gemm::fp16x8 v) __attribute__((always_inline)) {
+      if (m0 + x < p.m && n0 + y < p.n) *reinterpret_cast<emrs_gemm::fp16x8 *>(corner + (y * step + x)) = v;
+    });
   }
 };
 
@@ -633,6 +637,7 @@ struct Sizes {
   uint64_t tokens_padded;
   uint64_t splits;         // runs of k that grad_hidden's products are cut into
   bool direct;             // these take the weights as they lie
+  uint64_t parts, sums;    // of d there; partial sums of grad_hidden, splits x parts
   uint64_t pairs, hidden, weight, sum, d, dt, ht, wt, scales, largest, total;  // offsets
 };
 
@@ -702,8 +707,11 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   // grad_hidden's product has few tiles where there are few tokens: its sum over the vocabulary is cut into
   // runs of at least 1024 rows, as many as give every CU a tile.
   const uint64_t k = round_up(std::min(s.piece, most), 64) * shards;
-  const uint64_t tiles = ((a->hidden_size + 127) / 128) * ((a->tokens + 127) / 128);
+  s.direct = takes_weights(a->dtype, a->tokens);
+  s.parts = s.direct && a->dtype == EMRS_BF16 ? 2 : 1;
+  const uint64_t tiles = ((a->hidden_size + 127) / 128) * ((s.parts * a->tokens + 127) / 128);
   s.splits = std::max<uint64_t>(1, std::min(256 / std::max<uint64_t>(tiles, 1), k / 1024));
+  s.sums = s.splits * s.parts;
   uint64_t at = 0;
   auto take = [&](bool wanted, uint64_t bytes) {
     const uint64_t here = at;
@@ -713,9 +721,8 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   s.pairs = take(!backward, slots * a->tokens * sizeof(float2));
   s.hidden = take(s.pad_hidden, a->tokens * s.k * 2);
   s.weight = take(s.pad_weight, shards * s.piece * s.k * 2);
-  s.direct = takes_weights(a->dtype, a->tokens);
-  s.sum = take(backward && a->grad_hidden, s.splits * a->tokens * a->hidden_size * 4);
-  s.d = take(backward && a->grad_hidden, a->tokens * shards * s.piece * (s.direct && a->dtype == EMRS_BF16 ? 4 : 2));
+  s.sum = take(backward && a->grad_hidden, s.sums * a->tokens * a->hidden_size * 4);
+  s.d = take(backward && a->grad_hidden, s.parts * a->tokens * shards * s.piece * 2);
   s.wt = take(backward && a->grad_hidden && !s.direct, a->hidden_size * shards * s.piece * 2);
   s.dt = take(backward && a->grad_weights, shards * s.piece * s.tokens_padded * 2);
   s.ht = take(backward && a->grad_weights, a->hidden_size * s.tokens_padded * 2);
@@ -869,27 +876,25 @@ int backward(const emrs_loss *a, hipStream_t st) {
       Product p = logits_of(a, s, g, rows);
       p.b = hidden;
       const int32_t sum_k = (int32_t)(g.count * padded);
-      // d as the weights lie is of their type: in two parts where that is bf16.
-      const int parts = s.direct && std::is_same<T, __bf16>::value ? 2 : 1;
       auto gradients = [&](auto e) {
         static_cast<Piece &>(e) = c;
         e.d = a->grad_hidden ? d : nullptr, e.dt = wanted ? dt : nullptr;
-        e.d_stride = parts * sum_k, e.dt_stride = (int32_t)s.tokens_padded, e.padded = (int32_t)padded;
+        e.d_stride = sum_k, e.dt_stride = (int32_t)s.tokens_padded, e.padded = (int32_t)padded;
         e.lse = a->lse, e.grad_loss = a->grad_loss, e.target = a->target, e.ignore = a->ignore_index, e.scale = d_scale;
         return emrs_gemm::launch<T>(p, e, st);
       };
-      TRY(parts == 2 ? gradients(LogitGradients<true>{}) : gradients(LogitGradients<false>{}));
+      TRY(s.parts == 2 ? gradients(LogitGradients<true>{}) : gradients(LogitGradients<false>{}));
       if (a->grad_hidden) {
         Product q{};
         q.a = wt, q.b = d;
-        q.a_stride = s.direct ? p.a_stride : sum_k, q.b_stride = parts * sum_k;
-        q.m = h, q.n = tokens;
+        q.a_stride = s.direct ? p.a_stride : sum_k, q.b_stride = sum_k;
+        q.m = h, q.n = (int32_t)(s.parts * a->tokens);
         q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
         auto product = [&](const auto &e) {
           if (s.direct) return emrs_gemm::launch_rows_of_k<T>(q, OfWeights<std::decay_t<decltype(e)>>{e, c, (int32_t)padded, (int32_t)rows, sum_k}, st);
           return emrs_gemm::launch<half>(q, e, st);
         };
-        q.batch = 1, q.k = parts * sum_k;
+        q.batch = 1, q.k = sum_k;
         if (s.splits > 1) {
           // Runs of k as a batch: multiples of 64, the last one shorter (its stages past the end are zeros).
           q.k_end = q.k;
@@ -898,12 +903,12 @@ int backward(const emrs_loss *a, hipStream_t st) {
           q.a_batch = q.b_batch = q.k;
         }
         const float *const scale = s.direct ? nullptr : w_scale;
-        if (s.splits > 1 || left) {
-          TRY(product(StoreSums{{}, sum, h, tokens * h, begun, fours, d_scale, scale}));
+        if (s.sums > 1 || left) {
+          TRY(product(StoreSums{{}, sum, h, q.n * h, begun, fours, d_scale, scale}));
         } else {
           StoreRows<T> out{};
           out.out.p[0] = a->grad_hidden, out.sum = begun ? sum : nullptr, out.stride = h;
-          out.wide = fours && reinterpret_cast<uintptr_t>(a->grad_hidden) % 8 == 0;
+          out.wide = h % 8 == 0 && reinterpret_cast<uintptr_t>(a->grad_hidden) % 16 == 0;
           out.scale_a = d_scale, out.scale_b = scale;
           TRY(product(out));
         }
@@ -919,11 +924,11 @@ int backward(const emrs_loss *a, hipStream_t st) {
         q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
         q.batch = n;
         StoreRows<T> out{};
-        out.wide = fours;
+        out.wide = h % 8 == 0;
         for (uint32_t b = 0; b < n; ++b) {
           T *gw = static_cast<T *>(a->grad_weights[g.first + k + b]) + lo * h;
           out.out.p[b] = gw;
-          out.wide &= reinterpret_cast<uintptr_t>(gw) % 8 == 0;
+          out.wide &= reinterpret_cast<uintptr_t>(gw) % 16 == 0;
         }
         out.stride = h, out.scale_a = d_scale, out.scale_b = h_scale;
         TRY((emrs_gemm::launch<half>(q, out, st)));
@@ -931,8 +936,8 @@ int backward(const emrs_loss *a, hipStream_t st) {
     }
     first += all * g.count;
   }
-  if (a->grad_hidden && s.splits > 1) {
-    join_sums_kernel<T><<<(uint32_t)((tokens * h + 255) / 256), 256, 0, st>>>(sum, (int)s.splits, tokens * h, static_cast<T *>(a->grad_hidden));
+  if (a->grad_hidden && s.sums > 1) {
+    join_sums_kernel<T><<<(uint32_t)((tokens * h + 255) / 256), 256, 0, st>>>(sum, (int)s.sums, tokens * h, static_cast<T *>(a->grad_hidden));
     TRY(hipGetLastError());
   }
   return EMRS_OK;
