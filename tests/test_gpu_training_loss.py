@@ -93,6 +93,26 @@ def test_loss_and_gradients(gpu_device, tokens, hidden, rows, vocab, dtype):
         assert torch.equal(training.linear_cross_entropy(h, w, target, vocab_size=vocab, reduction="none"), loss)
 
 
+@pytest.mark.parametrize("tokens,hidden,rows,vocab,dtype", [
+    (256, 40, [270000], 269990, torch.bfloat16),       # more rows than one piece of d holds
+    (1000, 24, [35000, 35000], 69000, torch.float16),
+    (130, 1003, [4100, 4000], 8090, torch.bfloat16),   # rows that do not lie on 16 bytes, shards of two sizes
+    (1024, 200, [1500, 1500], None, torch.float16),
+])
+def test_few_tokens_and_many_rows(gpu_device, tokens, hidden, rows, vocab, dtype):
+    """grad_hidden's product takes the weights as they lie."""
+    vocab = sum(rows) if vocab is None else vocab
+    h, w, target, g = _inputs(tokens, hidden, rows, dtype, vocab=vocab)
+    for x in w:  # what does not count may hold anything
+        if sum(rows) > vocab and x is w[-1]:
+            x[vocab - sum(rows):] = math.nan
+    lse, logit = training.vocab_statistics(h, w, target, vocab_size=vocab)
+    gh, gw = training.vocab_gradients(h, w, target, lse, g, vocab_size=vocab)
+    clean = [x.nan_to_num(0.0) for x in w]
+    loss = torch.where(target >= 0, lse - logit, 0.0)
+    _check_gradients(h, clean, target, g, vocab, loss, gh, gw)
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 5, 15, 16, 31, 40, 63, 64, 100, 130])
 @pytest.mark.parametrize("hidden,rows,dtype", [(256, [1000], torch.bfloat16), (1000, [333, 512], torch.float16),
                                                (48, [70], torch.bfloat16)])
