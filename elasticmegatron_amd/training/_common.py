@@ -30,10 +30,19 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     return torch.empty(max(1, nbytes), dtype=torch.uint8, device=device)
 
 
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# The same without a Stream object on the way, where torch has it: 2 us less a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def run_on(device: torch.device, call, record) -> None:
     """``call(record, stream)`` with ``device`` current, on its current stream."""
+    stream = _raw_stream(device.index) if _raw_stream is not None else _stream(device)
     if torch.cuda.current_device() == device.index:
-        call(record, torch.cuda.current_stream(device).cuda_stream)
+        call(record, stream)
     else:
         with torch.cuda.device(device):
-            call(record, torch.cuda.current_stream(device).cuda_stream)
+            call(record, stream)

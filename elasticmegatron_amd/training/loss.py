@@ -23,10 +23,25 @@ Weight = Union[torch.Tensor, Sequence[torch.Tensor]]
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [n, h] with unit column stride and rows that do not overlap."""
-    n, h = t.shape
-    if (h > 1 and t.stride(1) != 1) or (n > 1 and not h <= t.stride(0) <= 1 << 21):
-        return t.contiguous()
+    (n, h), (over, along) = t.size(), t.stride()
+    if (h > 1 and along != 1) or (n > 1 and not h <= over <= 1 << 21):
+        return t.detach().contiguous()
     return t
+
+
+def _room_for(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous gradient of ``t``."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.size(), dtype=t.dtype, device=t.device)
+
+
+def _refuse(shards, device, dtype, h) -> None:
+    """Raises for the first shard that is not as it has to be."""
+    for i, w in enumerate(shards):
+        on_device(f"weight shard {i}", w, device)
+        if w.dtype != dtype:
+            raise TypeError(f"weight shard {i} is {w.dtype}, hidden {dtype}")
+        if w.dim() != 2 or w.shape[1] != h:
+            raise ValueError(f"weight shard {i} is {tuple(w.shape)}: [rows, {h}] is wanted")
 
 
 class _Call:
@@ -46,23 +61,21 @@ class _Call:
             raise TypeError(f"target is {target.dtype}: torch.int64 is wanted")
         if hidden.dim() < 1 or target.shape != hidden.shape[:-1]:
             raise ValueError(f"target {tuple(target.shape)} does not fit hidden {tuple(hidden.shape)}")
-        h = hidden.shape[-1]
-        for i, w in enumerate(shards):
-            on_device(f"weight shard {i}", w, self.device)
-            if w.dtype != hidden.dtype:
-                raise TypeError(f"weight shard {i} is {w.dtype}, hidden {hidden.dtype}")
-            if w.dim() != 2 or w.shape[1] != h:
-                raise ValueError(f"weight shard {i} is {tuple(w.shape)}: [rows, {h}] is wanted")
-        rows = [w.shape[0] for w in shards]
+        h, device, dtype = hidden.size(-1), self.device, hidden.dtype
+        for w in shards:  # one by one only where something is wrong: this is most of a small loss's host time
+            if not (isinstance(w, torch.Tensor) and w.dtype is dtype and w.device == device and w.dim() == 2 and w.size(1) == h):
+                _refuse(shards, device, dtype, h)
+        rows = [w.size(0) for w in shards]
         if vocab_start < 0:
             raise ValueError("vocab_start is negative")
         if vocab_size is None:
             vocab_size = vocab_start + sum(rows)
         if vocab_size < 0:
             raise ValueError("vocab_size is negative")
-        self.hidden = _rows(hidden.detach().reshape(-1, h))
-        self.shards = [_rows(w.detach()) for w in shards]
-        self.target = target.reshape(-1).contiguous()
+        self.hidden = _rows(hidden if hidden.dim() == 2 else hidden.detach().reshape(-1, h))
+        self.shards = [_rows(w) for w in shards]
+        self.shape = target.size()
+        self.target = target if target.dim() == 1 and target.is_contiguous() else target.reshape(-1).contiguous()
         n = len(shards)
         pointers, strides, counts = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
         for i, w in enumerate(self.shards):
@@ -76,22 +89,24 @@ class _Call:
         a.target, a.ignore_index = self.target.data_ptr(), ignore_index
 
     def forward(self, with_loss: bool) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+        """``(lse, target logits, losses or None)``, the losses in the target's shape."""
         a, t = self.record, self.target.numel()
-        out = torch.empty(3 if with_loss else 2, t, dtype=torch.float32, device=self.device)
-        lse, logit, loss = out[0], out[1], out[2] if with_loss else None
+        out = torch.empty((2, t), dtype=torch.float32, device=self.device)
+        loss = torch.empty(self.shape, dtype=torch.float32, device=self.device) if with_loss else None
         if t:
-            a.lse, a.target_logit, a.loss = lse.data_ptr(), logit.data_ptr(), loss.data_ptr() if with_loss else None
+            at = out.data_ptr()
+            a.lse, a.target_logit, a.loss = at, at + 4 * t, loss.data_ptr() if with_loss else None
             scratch = workspace(_native.loss_workspace(a, False), self.device)
             a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
             run_on(self.device, _native.loss_forward, a)
+        lse, logit = out.unbind()
         return lse, logit, loss
 
     def backward(self, lse, grad_loss, want_hidden: bool, want_weights: Sequence[bool]):
         a = self.record
-        gh = torch.empty(self.hidden.shape, dtype=self.hidden.dtype, device=self.device) if want_hidden else None
-        gw = [torch.empty(w.shape, dtype=w.dtype, device=self.device) if want else None
-              for w, want in zip(self.shards, want_weights)]
-        if not self.target.numel() or not any(w.shape[0] for w in self.shards):  # sums over nothing
+        gh = _room_for(self.hidden) if want_hidden else None
+        gw = [_room_for(w) if want else None for w, want in zip(self.shards, want_weights)]
+        if not a.tokens or not any(self._tables[2]):  # sums over nothing
             for g in (gh, *gw):
                 if g is not None:
                     g.zero_()
@@ -113,15 +128,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
         lse, _, loss = call.forward(True)
         ctx.save_for_backward(hidden, target, lse, *shards)
         ctx.call = call  # views of the same inputs, checked already
-        return loss.view(target.shape)
+        return loss  # no view: users may scale it in place
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         hidden, _, lse, *_ = ctx.saved_tensors  # raises where an input was changed in place
-        grad_loss = grad_loss.reshape(-1).to(torch.float32).contiguous()
+        if grad_loss.dim() != 1 or grad_loss.dtype != torch.float32 or not grad_loss.is_contiguous():
+            grad_loss = grad_loss.reshape(-1).to(torch.float32).contiguous()
         gh, gw = ctx.call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
-        return (None if gh is None else gh.view(hidden.shape), None, None, None, *gw)
+        return (gh if gh is None or hidden.dim() == 2 else gh.view(hidden.shape), None, None, None, *gw)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, *, vocab_size: Optional[int] = None,
@@ -141,7 +157,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Ten
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (hidden, *shards)):
         loss = _LinearCrossEntropy.apply(hidden, target, vocab_size, ignore_index, *shards)
     else:
-        loss = _Call(hidden, shards, target, 0, vocab_size, ignore_index).forward(True)[2].view(target.shape)
+        loss = _Call(hidden, shards, target, 0, vocab_size, ignore_index).forward(True)[2]
     if reduction == "none":
         return loss
     total = loss.sum()

@@ -150,6 +150,18 @@ def test_reductions_and_shapes(gpu_device):
     assert torch.equal(got, h.grad)
 
 
+@pytest.mark.parametrize("shape", [(24,), (2, 12)])
+def test_losses_scaled_in_place(gpu_device, shape):
+    h, w, target, _ = _inputs(24, 64, [100], torch.bfloat16)
+    h, target = h.view(*shape, 64).requires_grad_(), target.view(shape)
+    loss = training.linear_cross_entropy(h, w[0], target, reduction="none")
+    want, = torch.autograd.grad((loss * 0.5).sum(), h)
+    loss = training.linear_cross_entropy(h, w[0], target, reduction="none")
+    loss *= 0.5
+    got, = torch.autograd.grad(loss.sum(), h)
+    assert torch.equal(got, want)
+
+
 def test_no_tokens_no_rows_and_nothing_that_counts(gpu_device):
     h, w, target, g = _inputs(8, 64, [100], torch.bfloat16)
     empty = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
