@@ -198,24 +198,25 @@ struct Loader {
 template <class T, class Cfg>
 struct RowLoader {
   static constexpr int kUnits = Cfg::BM / 8, kRows = 64 / kUnits;  // of a row; of one load
-  int voffset, columns;
-  int64_t stride;
+  int voffset, columns, stride;
   const T *first;  // the stage's first row, at the tile's first m
   int rows;        // that count from there on
   static __device__ __forceinline__ int permuted(int row) {
     return Cfg::BM == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : (row & 3) | (row >> 3 & 1) << 2;
   }
   __device__ __forceinline__ void init(int64_t row_stride, int columns_here, int wave, int lane) {
-    static_assert(Cfg::BM == 128 || Cfg::BM == 64, "whole rows in a load");
+    static_assert(Cfg::BM == 256 || Cfg::BM == 128 || Cfg::BM == 64, "whole rows in a load");
     static_assert(Cfg::WAVES * kRows % 16 == 0, "a wave's loads are permuted alike");
     const int row = lane / kUnits, unit = lane % kUnits;
-    stride = row_stride, columns = columns_here;
+    stride = (int)row_stride, columns = columns_here;
     voffset = (int)(row * stride * 2) + ((unit ^ permuted(wave * kRows + row) << 1) << 4);
   }
   __device__ __forceinline__ void cut(int) {}
   __device__ __forceinline__ void load(char *lds, int j, int, bool none, int wave) const {
-    const int from = (wave + j * Cfg::WAVES) * kRows, here = min(rows - from, kRows);
-    const int bytes = none || here <= 0 ? 0 : (int)(((here - 1) * stride + columns) * 2);
+    // No branches: the loads are started between matrix instructions.  (columns <= stride.)  The median is a
+    // vector instruction; a buffer that might differ between lanes would cost the load a loop.
+    const int from = (wave + j * Cfg::WAVES) * kRows, here = __builtin_amdgcn_readfirstlane(none ? 0 : min(max(rows - from, 0), kRows));
+    const int bytes = max(0, (here - 1) * stride + columns) * 2;
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(first + from * stride), 0, bytes, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * Cfg::WAVES) * 1024), 16,
                                              voffset, 0, 0, 0);
@@ -376,13 +377,10 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   const int row = lane & 15, c = lane >> 4;
   const int unit[2] = {(c ^ swizzle(row)) << 4, ((4 + c) ^ swizzle(row)) << 4};
   const int a_at = (wm * Cfg::WM + row) * 128, b_at = (wn * Cfg::WN + row) * 128;
-  int a_rows[rows_of_k ? Cfg::MI : 1];
-  if constexpr (rows_of_k) {
-    const int k = c * 8 + (row >> 2);
-#pragma unroll
-    for (int i = 0; i < Cfg::MI; ++i)
-      a_rows[i] = k * Cfg::BM * 2 + ((wm * Cfg::MI + i) ^ RowLoader<T, Cfg>::permuted(k)) * 32 + (row & 3) * 8;
-  }
+  // The first of the wave's 32-byte pieces of its rows of k; piece i lies where i is added to it before the
+  // permutation, and both are exclusive ors: the wave's first piece is a multiple of MI.
+  const int a_k = c * 8 + (row >> 2);
+  int a_piece = rows_of_k ? a_k * Cfg::BM * 2 + ((wm * Cfg::MI) ^ RowLoader<T, Cfg>::permuted(a_k)) * 32 + (row & 3) * 8 : 0;
   struct Fragments {
     x8 a[Cfg::MI], b[Cfg::NI];
   } even, odd;  // of the first and the second 32 k of a stage
@@ -390,7 +388,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
     if (r < Cfg::NI)
       f.b[r] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + r * 2048);
     else if constexpr (rows_of_k)
-      f.a[r - Cfg::NI] = along_k<x8>(a + a_rows[r - Cfg::NI] + kk * 64 * Cfg::BM, 8 * Cfg::BM);
+      f.a[r - Cfg::NI] = along_k<x8>(a + (a_piece ^ (r - Cfg::NI) << 5) + kk * 64 * Cfg::BM, 8 * Cfg::BM);
     else
       f.a[r - Cfg::NI] = *reinterpret_cast<const x8 *>(a + a_at + unit[kk] + (r - Cfg::NI) * 2048);
   };
@@ -400,6 +398,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   auto half = [&](const Fragments &now, Fragments &next, const char *a, const char *b, int kk, auto start) __attribute__((always_inline)) {
     constexpr int products = Cfg::MI * Cfg::NI, reads = Cfg::MI + Cfg::NI, loads = decltype(start)::kCount;
     constexpr int per = products * 3 / 4 / reads > 0 ? products * 3 / 4 / reads : 1;
+    if constexpr (rows_of_k) asm("" : "+v"(a_piece));  // its MI exclusive ors are taken again: registers
 #pragma unroll
     for (int q = 0; q < products; ++q) {
       acc[q / Cfg::NI][q % Cfg::NI] = mfma(now.a[q / Cfg::NI], now.b[q % Cfg::NI], acc[q / Cfg::NI][q % Cfg::NI]);
@@ -461,7 +460,8 @@ enum Shape { kLarge, kBroad, kMedium, kSmall };
 
 // What a launch of one tile size takes, in microseconds, by its rounds of 256 workgroups (each has a CU's LDS
 // for itself): measured are 1.25 for a large tile's stage, 1.05 for a broad one's and for the stage that each
-// of a medium tile's two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside.
+// of a medium tile's two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside; 1.7
+// for a large tile's with rows of k, whose reads leave it short of registers.
 // (A last round split along k instead, its pieces' sums joined by the last of them to end, was slower but for
 // the longest k: the sums of 240 pieces took 50 us on their way through memory.)
 template <class Cfg>
@@ -471,13 +471,18 @@ inline double cost_of(const Product &p, double stage, double fixed) {
 }
 
 // Large tiles read the operands fewer times; smaller ones give more CUs work, and their waves share a long k.
-inline Shape shape_of(const Product &p) {
-  const double cost[4] = {cost_of<Large>(p, 1.25, 8), cost_of<Broad>(p, 1.05, 6), cost_of<Medium>(p, 1.05, 4), cost_of<Small>(p, 0.95, 3)};
+struct Choice {
+  Shape shape;
+  double cost;
+};
+inline Choice choice_of(const Product &p, bool rows_of_k) {
+  const double cost[4] = {cost_of<Large>(p, rows_of_k ? 1.7 : 1.25, 8), cost_of<Broad>(p, 1.05, 6), cost_of<Medium>(p, 1.05, 4), cost_of<Small>(p, 0.95, 3)};
   int best = kLarge;
   for (int i = kBroad; i <= kSmall; ++i)
-    if (cost[i] < cost[best]) best = i;
-  return (Shape)best;
+    if (cost[i] < cost[best] && !(rows_of_k && i == kBroad)) best = i;
+  return {(Shape)best, cost[best]};
 }
+inline Shape shape_of(const Product &p) { return choice_of(p, false).shape; }
 
 template <class T, class Cfg, class Epilogue>
 void launch_as(const Product &p, const Epilogue &e, hipStream_t stream) {
@@ -486,22 +491,14 @@ void launch_as(const Product &p, const Epilogue &e, hipStream_t stream) {
 
 template <class T, class Epilogue>
 hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
-  switch (shape_of(p)) {
+  switch (choice_of(p, Epilogue::kRowsOfK).shape) {
     case kLarge: launch_as<T, Large>(p, e, stream); break;
-    case kBroad: launch_as<T, Broad>(p, e, stream); break;
+    case kBroad:  // rows of 192 are no whole loads
+      if constexpr (!Epilogue::kRowsOfK) launch_as<T, Broad>(p, e, stream);
+      break;
     case kMedium: launch_as<T, Medium>(p, e, stream); break;
     case kSmall: launch_as<T, Small>(p, e, stream); break;
   }
-  return hipGetLastError();
-}
-
-// With operand a [k][m]: the smaller tiles alone, since it is for products of few n.
-template <class T, class Epilogue>
-hipError_t launch_rows_of_k(const Product &p, const Epilogue &e, hipStream_t stream) {
-  if (cost_of<Medium>(p, 1.05, 4) <= cost_of<Small>(p, 0.95, 3))
-    launch_as<T, Medium>(p, e, stream);
-  else
-    launch_as<T, Small>(p, e, stream);
   return hipGetLastError();
 }
 

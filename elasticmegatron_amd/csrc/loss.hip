@@ -39,9 +39,9 @@ constexpr uint64_t kPieceBytes = 128ull << 20;  // of d in one orientation
 
 // Whether grad_hidden's product takes the weights as they lie: no search of their largest entry, no transposed
 // copy, but smaller tiles, and for bf16 twice the rows of d, in two parts.  All
-// gradients of 32000 x 4096 in bf16: 32 tokens 257 against 443 us, 384 tokens 719 against 657; in fp16: 32
-// tokens 246 against 380, 1024 tokens 923 against 989, 2048 tokens 1746 against 1669.
-bool takes_weights(uint32_t dtype, uint64_t tokens) { return tokens <= (dtype == EMRS_BF16 ? 256 : 1024); }
+// gradients of 32000 x 4096 in bf16: 8 tokens 238 against 409 us, 512 tokens 699 against 647; in fp16: 8 tokens
+// 239 against 350, 512 tokens 542 against 589, 2048 tokens 1667 against 1567.
+bool takes_weights(uint32_t dtype, uint64_t tokens) { return tokens <= (dtype == EMRS_BF16 ? 256 : 768); }
 
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
@@ -705,12 +705,19 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
     for (uint64_t lo = 0; lo < a->shard_rows[s.groups[i].first]; lo += s.piece)
       slots += slots_of(a, logits_of(a, s, s.groups[i], std::min(s.piece, a->shard_rows[s.groups[i].first] - lo))) * s.groups[i].count;
   // grad_hidden's product has few tiles where there are few tokens: its sum over the vocabulary is cut into
-  // runs of at least 1024 rows, as many as give every CU a tile.
+  // runs of at least 1024 rows, as many as the product and the sums' way through memory take least time with.
   const uint64_t k = round_up(std::min(s.piece, most), 64) * shards;
   s.direct = takes_weights(a->dtype, a->tokens);
   s.parts = s.direct && a->dtype == EMRS_BF16 ? 2 : 1;
-  const uint64_t tiles = ((a->hidden_size + 127) / 128) * ((s.parts * a->tokens + 127) / 128);
-  s.splits = std::max<uint64_t>(1, std::min(256 / std::max<uint64_t>(tiles, 1), k / 1024));
+  s.splits = 1;
+  double best = 0;
+  for (uint64_t n = 1; n <= std::min<uint64_t>(256, std::max<uint64_t>(1, k / 1024)); n += n < 16 ? 1 : n / 8) {
+    Product q{};
+    q.m = (int32_t)a->hidden_size, q.n = (int32_t)(s.parts * a->tokens), q.k = (int32_t)round_up((k + n - 1) / n, 64);
+    q.batch = (int32_t)n;
+    const double cost = emrs_gemm::choice_of(q, s.direct).cost + (n * s.parts > 1 ? 6 + 8e-6 * n * q.m * q.n / 4 : 0);
+    if (n == 1 || cost < best) best = cost, s.splits = n;
+  }
   s.sums = s.splits * s.parts;
   uint64_t at = 0;
   auto take = [&](bool wanted, uint64_t bytes) {
@@ -891,7 +898,7 @@ int backward(const emrs_loss *a, hipStream_t st) {
         q.m = h, q.n = (int32_t)(s.parts * a->tokens);
         q.a_wrap = q.b_wrap = emrs_gemm::kNoWrap;
         auto product = [&](const auto &e) {
-          if (s.direct) return emrs_gemm::launch_rows_of_k<T>(q, OfWeights<std::decay_t<decltype(e)>>{e, c, (int32_t)padded, (int32_t)rows, sum_k}, st);
+          if (s.direct) return emrs_gemm::launch<T>(q, OfWeights<std::decay_t<decltype(e)>>{e, c, (int32_t)padded, (int32_t)rows, sum_k}, st);
           return emrs_gemm::launch<half>(q, e, st);
         };
         q.batch = 1, q.k = sum_k;
