@@ -101,25 +101,27 @@ int launch(const emrs_adamw *a, const Factors &f, hipStream_t st) {
 }  // namespace
 
 extern "C" int emrs_adamw_step(const emrs_adamw *a, void *stream) {
-  emrs_internal::clear_error();
-  if (!a) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: NULL argument");
-  if (a->grad_dtype > EMRS_FP16) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: gradients are fp32, bf16 or fp16");
-  if (a->step == 0) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: steps count from 1");
-  if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1))
-    return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: betas lie in [0, 1)");
-  if (a->n == 0) return EMRS_OK;
-  if (a->n > (1ull << 38)) return fail(EMRS_ERR_TOO_LARGE, "adamw: at most 2^38 elements");
-  if (!a->main || !a->exp_avg || !a->exp_avg_sq || !a->grad) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: NULL buffer");
-  const uint64_t grad_bytes = a->grad_dtype == EMRS_FP32 ? 4 : 2;
-  if (!on(a->main, 4) || !on(a->exp_avg, 4) || !on(a->exp_avg_sq, 4) || !on(a->grad, grad_bytes) || !on(a->image, 2))
-    return fail(EMRS_ERR_MISALIGNED, "adamw: a buffer off its type's alignment");
-  const int rc = emrs_internal::need_device();
-  if (rc) return rc;
-  const double c1 = 1.0 - std::pow(a->beta1, (double)a->step), c2 = 1.0 - std::pow(a->beta2, (double)a->step);
-  const Factors f{(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps,
-                  (float)(1.0 - a->lr * a->weight_decay), (float)(a->lr / c1), (float)(1.0 / c2)};
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  return a->grad_dtype == EMRS_FP32   ? launch<float>(a, f, st)
-         : a->grad_dtype == EMRS_BF16 ? launch<__bf16>(a, f, st)
-                                      : launch<_Float16>(a, f, st);
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    if (!a) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: NULL argument");
+    if (a->grad_dtype > EMRS_FP16) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: gradients are fp32, bf16 or fp16");
+    if (a->step == 0) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: steps count from 1");
+    if (!(a->beta1 >= 0 && a->beta1 < 1 && a->beta2 >= 0 && a->beta2 < 1))
+      return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: betas lie in [0, 1)");
+    if (a->n == 0) return EMRS_OK;
+    if (a->n > (1ull << 38)) return fail(EMRS_ERR_TOO_LARGE, "adamw: at most 2^38 elements");
+    if (!a->main || !a->exp_avg || !a->exp_avg_sq || !a->grad) return fail(EMRS_ERR_INVALID_ARGUMENT, "adamw: NULL buffer");
+    const uint64_t grad_bytes = a->grad_dtype == EMRS_FP32 ? 4 : 2;
+    if (!on(a->main, 4) || !on(a->exp_avg, 4) || !on(a->exp_avg_sq, 4) || !on(a->grad, grad_bytes) || !on(a->image, 2))
+      return fail(EMRS_ERR_MISALIGNED, "adamw: a buffer off its type's alignment");
+    const int rc = emrs_internal::need_device();
+    if (rc) return rc;
+    const double c1 = 1.0 - std::pow(a->beta1, (double)a->step), c2 = 1.0 - std::pow(a->beta2, (double)a->step);
+    const Factors f{(float)a->beta1, (float)(1.0 - a->beta1), (float)a->beta2, (float)(1.0 - a->beta2), (float)a->eps,
+                    (float)(1.0 - a->lr * a->weight_decay), (float)(a->lr / c1), (float)(1.0 / c2)};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return a->grad_dtype == EMRS_FP32   ? launch<float>(a, f, st)
+           : a->grad_dtype == EMRS_BF16 ? launch<__bf16>(a, f, st)
+                                        : launch<_Float16>(a, f, st);
+  });
 }

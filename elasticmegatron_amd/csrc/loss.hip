@@ -964,43 +964,49 @@ int check_workspace(const emrs_loss *a, bool backward) {
 extern "C" {
 
 int emrs_loss_workspace(const emrs_loss *a, int backward, uint64_t *bytes) {
-  emrs_internal::clear_error();
-  const int rc = check(a);
-  if (rc) return rc;
-  if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: NULL argument");
-  *bytes = sizes_of(a, backward != 0).total;
-  return EMRS_OK;
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    const int rc = check(a);
+    if (rc) return rc;
+    if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: NULL argument");
+    *bytes = sizes_of(a, backward != 0).total;
+    return EMRS_OK;
+  });
 }
 
 int emrs_loss_forward(const emrs_loss *a, void *stream) {
-  emrs_internal::clear_error();
-  int rc = check(a);
-  if (rc) return rc;
-  if (a->tokens == 0) return EMRS_OK;
-  if (!a->lse || !a->target_logit) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: forward wants lse and target_logit");
-  rc = check_workspace(a, false);
-  if (rc) return rc;
-  rc = emrs_internal::need_device();
-  if (rc) return rc;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  return a->dtype == EMRS_BF16 ? forward<__bf16>(a, st) : forward<_Float16>(a, st);
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    int rc = check(a);
+    if (rc) return rc;
+    if (a->tokens == 0) return EMRS_OK;
+    if (!a->lse || !a->target_logit) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: forward wants lse and target_logit");
+    rc = check_workspace(a, false);
+    if (rc) return rc;
+    rc = emrs_internal::need_device();
+    if (rc) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return a->dtype == EMRS_BF16 ? forward<__bf16>(a, st) : forward<_Float16>(a, st);
+  });
 }
 
 int emrs_loss_backward(const emrs_loss *a, void *stream) {
-  emrs_internal::clear_error();
-  int rc = check(a);
-  if (rc) return rc;
-  if (a->tokens && (!a->lse || !a->grad_loss)) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: backward wants lse and grad_loss");
-  uint64_t rows = 0;
-  for (uint32_t i = 0; i < a->n_shards; ++i) rows += a->shard_rows[i];
-  if (a->tokens == 0 || rows == 0)
-    return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: no tokens or no vocabulary rows: the gradients are zeros, which the caller fills");
-  rc = check_workspace(a, true);
-  if (rc) return rc;
-  rc = emrs_internal::need_device();
-  if (rc) return rc;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  return a->dtype == EMRS_BF16 ? backward<__bf16>(a, st) : backward<_Float16>(a, st);
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    int rc = check(a);
+    if (rc) return rc;
+    if (a->tokens && (!a->lse || !a->grad_loss)) return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: backward wants lse and grad_loss");
+    uint64_t rows = 0;
+    for (uint32_t i = 0; i < a->n_shards; ++i) rows += a->shard_rows[i];
+    if (a->tokens == 0 || rows == 0)
+      return fail(EMRS_ERR_INVALID_ARGUMENT, "loss: no tokens or no vocabulary rows: the gradients are zeros, which the caller fills");
+    rc = check_workspace(a, true);
+    if (rc) return rc;
+    rc = emrs_internal::need_device();
+    if (rc) return rc;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return a->dtype == EMRS_BF16 ? backward<__bf16>(a, st) : backward<_Float16>(a, st);
+  });
 }
 
 }  // extern "C"

@@ -1033,27 +1033,31 @@ int step(const emrs_muon *a, hipStream_t st) {
 extern "C" {
 
 int emrs_muon_workspace(const emrs_muon *a, uint64_t *bytes) {
-  emrs_internal::clear_error();
-  const int rc = check(a);
-  if (rc) return rc;
-  if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: NULL argument");
-  *bytes = sizes_of(a).total;
-  return EMRS_OK;
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    const int rc = check(a);
+    if (rc) return rc;
+    if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "muon: NULL argument");
+    *bytes = sizes_of(a).total;
+    return EMRS_OK;
+  });
 }
 
 int emrs_muon_step(const emrs_muon *a, void *stream) {
-  emrs_internal::clear_error();
-  int rc = check(a);
-  if (!rc) rc = check_matrices(a);
-  if (rc) return rc;
-  const uint64_t want = sizes_of(a).total;
-  if (!a->workspace || a->workspace_bytes < want)
-    return fail(EMRS_ERR_INVALID_ARGUMENT,
-                "muon: the workspace holds " + std::to_string(a->workspace_bytes) + " bytes of " + std::to_string(want));
-  if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(EMRS_ERR_MISALIGNED, "muon: the workspace is off 256 bytes");
-  rc = emrs_internal::need_device();
-  if (rc) return rc;
-  return step(a, static_cast<hipStream_t>(stream));
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    int rc = check(a);
+    if (!rc) rc = check_matrices(a);
+    if (rc) return rc;
+    const uint64_t want = sizes_of(a).total;
+    if (!a->workspace || a->workspace_bytes < want)
+      return fail(EMRS_ERR_INVALID_ARGUMENT,
+                  "muon: the workspace holds " + std::to_string(a->workspace_bytes) + " bytes of " + std::to_string(want));
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail(EMRS_ERR_MISALIGNED, "muon: the workspace is off 256 bytes");
+    rc = emrs_internal::need_device();
+    if (rc) return rc;
+    return step(a, static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"
