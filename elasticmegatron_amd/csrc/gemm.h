@@ -84,11 +84,14 @@ struct Tile {
 // CU's matrix units against 96 KB of fragment reads.  192 x 192 with 12 waves reads 1.33 times the bytes for a
 // multiply-add, and is for products whose large tiles would fill their last round badly: 253 of them take
 // 207 us where 136 large ones take 255 (4096 x 4096 by half, k 12288).  The smaller tiles are for products
-// that would not give every CU one of these.
+// that would not give every CU one of these: what bounds them is how often a stage's loads are waited for, so
+// the smaller a tile, the more groups of waves share its k (Newton-Schulz on 512 x 512: 112 us, with tiles of
+// 64 at the least 147).
 using Large = Tile<256, 256, 128, 64>;
 using Broad = Tile<192, 192, 64, 48>;
 using Medium = Tile<128, 128, 64, 64, 2>;
 using Small = Tile<64, 64, 32, 32, 4>;
+using Tiny = Tile<32, 32, 32, 32, 8>;
 
 __host__ __device__ inline int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
 template <class Cfg>
@@ -104,6 +107,7 @@ struct Where {
 // What an epilogue is beside its run(): where the operands of a matrix of the batch begin.
 struct Operand {
   static constexpr bool kRowsOfK = false;  // whether operand a is [k][m]
+  static constexpr bool kBy32 = true;      // whether tiles of 32 will do; else they reach the next multiples of 64
   __device__ __forceinline__ const void *operand_a(const Product &p, int batch) const {
     return static_cast<const char *>(p.a) + batch * p.a_batch * 2;
   }
@@ -165,16 +169,17 @@ __device__ inline int swizzle(int row) { return (row ^ ((row >> 3) & 1)) & 7; }
 // (where k goes), so what places a row must not be scalar.
 template <class T, int LOADS, int WAVES>
 struct Loader {
-  int voffset;
-  int unit;  // first k, within a stage, of the 16 bytes
+  int voffset[2];  // a wave's groups are all even or all odd ([0]), or (one wave) both in turn
+  int unit;        // first k, within a stage, of the 16 bytes of [0]; its neighbour's of [1]
   const T *base[LOADS];
   int bytes[LOADS];  // 0: no row of the group is the operand's
   // first: the tile's first row; rows: how many of its rows there are; columns: what a row holds.
   __device__ __forceinline__ void init(const T *first, int64_t stride, int rows, int columns, int wave, int lane) {
-    static_assert(WAVES % 2 == 0, "a wave's groups of eight rows are all even or all odd");
+    static_assert(WAVES % 2 == 0 || WAVES == 1, "see voffset");
     const int row = lane >> 3, c = (lane & 7) ^ swizzle(wave * 8 + row);
     unit = c * 8;
-    voffset = (int)(row * stride * 2) + (c << 4);
+    voffset[0] = (int)(row * stride * 2) + (c << 4);
+    voffset[1] = (int)(row * stride * 2) + ((c ^ 1) << 4);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int at = (wave + j * WAVES) * 8, here = rows - at;
@@ -183,12 +188,15 @@ struct Loader {
     }
   }
   // Fewer than a stage's k are left: lanes whose 16 bytes are past them go past the buffer's end instead.
-  __device__ __forceinline__ void cut(int left) { voffset = unit < left ? voffset : (int)0x80000000; }
+  __device__ __forceinline__ void cut(int left) {
+    voffset[0] = unit < left ? voffset[0] : (int)0x80000000;
+    if (WAVES == 1) voffset[1] = (unit ^ 8) < left ? voffset[1] : (int)0x80000000;
+  }
   // Load j of the stage from k0 on; none: zeros.
   __device__ __forceinline__ void load(char *lds, int j, int k0, bool none, int wave) const {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base[j]), 0, none ? 0 : bytes[j], 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * WAVES) * 1024), 16,
-                                             voffset, k0 * 2, 0, 0);
+                                             voffset[WAVES == 1 ? j & 1 : 0], k0 * 2, 0, 0);
   }
 };
 
@@ -456,11 +464,11 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   epilogue.template run<Cfg>(acc, w, w.m0 + wm * Cfg::WM, w.n0 + wn * Cfg::WN, wm, lane, p, own);
 }
 
-enum Shape { kLarge, kBroad, kMedium, kSmall };
+enum Shape { kLarge, kBroad, kMedium, kSmall, kTiny };
 
 // What a launch of one tile size takes, in microseconds, by its rounds of 256 workgroups (each has a CU's LDS
 // for itself): measured are 1.25 for a large tile's stage, 1.05 for a broad one's and for the stage that each
-// of a medium tile's two groups works on, 0.95 for a small tile's four, and what a workgroup takes beside; 1.7
+// of a medium tile's two groups works on, 0.95 for a small tile's four, 0.9 for the smallest's eight, and what a workgroup takes beside; 1.7
 // for a large tile's with rows of k, whose reads leave it short of registers.
 // (A last round split along k instead, its pieces' sums joined by the last of them to end, was slower but for
 // the longest k: the sums of 240 pieces took 50 us on their way through memory.)
@@ -475,14 +483,15 @@ struct Choice {
   Shape shape;
   double cost;
 };
-inline Choice choice_of(const Product &p, bool rows_of_k) {
-  const double cost[4] = {cost_of<Large>(p, rows_of_k ? 1.7 : 1.25, 8), cost_of<Broad>(p, 1.05, 6), cost_of<Medium>(p, 1.05, 4), cost_of<Small>(p, 0.95, 3)};
+inline Choice choice_of(const Product &p, bool rows_of_k, bool by_32) {
+  const double cost[5] = {cost_of<Large>(p, rows_of_k ? 1.7 : 1.25, 8), cost_of<Broad>(p, 1.05, 6), cost_of<Medium>(p, 1.05, 4), cost_of<Small>(p, 0.95, 3),
+                          cost_of<Tiny>(p, 0.9, 3)};
   int best = kLarge;
-  for (int i = kBroad; i <= kSmall; ++i)
-    if (cost[i] < cost[best] && !(rows_of_k && i == kBroad)) best = i;
+  for (int i = kBroad; i <= kTiny; ++i)
+    if (cost[i] < cost[best] && !(rows_of_k && i == kBroad) && (by_32 || i != kTiny)) best = i;
   return {(Shape)best, cost[best]};
 }
-inline Shape shape_of(const Product &p) { return choice_of(p, false).shape; }
+inline Shape shape_of(const Product &p) { return choice_of(p, false, true).shape; }
 
 template <class T, class Cfg, class Epilogue>
 void launch_as(const Product &p, const Epilogue &e, hipStream_t stream) {
@@ -491,13 +500,16 @@ void launch_as(const Product &p, const Epilogue &e, hipStream_t stream) {
 
 template <class T, class Epilogue>
 hipError_t launch(const Product &p, const Epilogue &e, hipStream_t stream) {
-  switch (choice_of(p, Epilogue::kRowsOfK).shape) {
+  switch (choice_of(p, Epilogue::kRowsOfK, Epilogue::kBy32).shape) {
     case kLarge: launch_as<T, Large>(p, e, stream); break;
     case kBroad:  // rows of 192 are no whole loads
       if constexpr (!Epilogue::kRowsOfK) launch_as<T, Broad>(p, e, stream);
       break;
     case kMedium: launch_as<T, Medium>(p, e, stream); break;
     case kSmall: launch_as<T, Small>(p, e, stream); break;
+    case kTiny:
+      if constexpr (Epilogue::kBy32) launch_as<T, Tiny>(p, e, stream);
+      break;
   }
   return hipGetLastError();
 }
@@ -508,6 +520,7 @@ inline int64_t wave_rows(const Product &p) {
     case kLarge: return tiles_of(p.m, Large::BM) * Large::WAVES_M;
     case kBroad: return tiles_of(p.m, Broad::BM) * Broad::WAVES_M;
     case kMedium: return tiles_of(p.m, Medium::BM) * Medium::WAVES_M;
+    case kTiny: return tiles_of(p.m, Tiny::BM) * Tiny::WAVES_M;
     default: return tiles_of(p.m, Small::BM) * Small::WAVES_M;
   }
 }

@@ -57,7 +57,7 @@ struct Table {
 
 // A piece of the vocabulary: the same `rows` rows of every shard of a group.
 struct Piece {
-  static constexpr bool kRowsOfK = false;
+  static constexpr bool kRowsOfK = false, kBy32 = true;
   Table weights;          // first row of the piece in each shard
   int64_t first, shard;   // vocabulary index of the first shard's first row here; rows from a shard to the next
   int64_t vocab;          // rows from this vocabulary index on do not count
@@ -238,6 +238,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_statistics_kernel(const f
 // With kParts d is in two bf16 parts, [2][tokens]: what the product with bf16 weights as they lie takes.
 template <bool kParts>
 struct LogitGradients : Piece {
+  static constexpr bool kBy32 = false;  // writes zeros up to multiples of 64
   half *d;                // [tokens][shards x padded rows]: m contiguous; NULL: not wanted
   half *dt;               // [shards x padded rows][padded tokens]: n contiguous; NULL: not wanted
   int32_t d_stride, dt_stride, padded;
@@ -309,7 +310,7 @@ struct LogitGradients : Piece {
 // A product with the weight's own rows as rows of k: of every shard in turn, padded.
 template <class Base>
 struct OfWeights : Base {
-  static constexpr bool kRowsOfK = true;
+  static constexpr bool kRowsOfK = true, kBy32 = false;
   Piece piece;
   int32_t padded, rows, all;  // of a shard; of all of them, padded
 
@@ -715,7 +716,7 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
     Product q{};
     q.m = (int32_t)a->hidden_size, q.n = (int32_t)(s.parts * a->tokens), q.k = (int32_t)round_up((k + n - 1) / n, 64);
     q.batch = (int32_t)n;
-    const double cost = emrs_gemm::choice_of(q, s.direct).cost + (n * s.parts > 1 ? 6 + 8e-6 * n * q.m * q.n / 4 : 0);
+    const double cost = emrs_gemm::choice_of(q, s.direct, !s.direct).cost + (n * s.parts > 1 ? 6 + 8e-6 * n * q.m * q.n / 4 : 0);
     if (n == 1 || cost < best) best = cost, s.splits = n;
   }
   s.sums = s.splits * s.parts;
