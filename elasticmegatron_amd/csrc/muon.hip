@@ -17,7 +17,7 @@
 // step but the last two, where the noise has two steps at most to grow.  There a X goes into the polynomial,
 // P = a I + b A + c A^2: near the end P is close to 0.7 I where b A + c A^2 is close to -2.7 I, and has a
 // quarter of its rounding; before, P's rounding on the diagonal would be such noise itself.  An error of A
-// enters by the polynomial's slope, b + 2 c A, of size 0.7 at the end.  Against 64 bits the result is then
+// enters by the polynomial's slope, b + 2 c A, of size 0.7 at the end.  Against 64 bits five steps' result is then
 // below 2e-3 off in norm for spectra from flat to s_i ~ i^-3 and 3.4e-3 for a matrix of rank one (4e-2 with one
 // part throughout, 3e-1 with bf16), about the rounding of the bf16 that it is written in.
 
@@ -762,10 +762,45 @@ uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 // 4.5 r + 13.5 products of S S S for three steps in place of 10.5 r + 6, by the multiply-adds; where two more
 // launches and triangles that fill their last round badly count too, it pays from r = 2.5 on.  (Not for the
 // steps with one part: there the rounding of A, which grows by a^2 a step, would double the error.)
+//
+// Q's size is the product of the polynomials' largest values, and where there are no singular values that is
+// the product of the a: held times 64 in fp16 it must stay under 65504.  (The default triple's product is 41
+// in five steps, 485 in seven, 1669 in eight.)  Steps on X itself have no such growth: past a product of 512
+// they run instead.
 constexpr int kSquares = 5;
+constexpr double kMostGrowth = 512;
+
+// The largest values of the polynomials of the steps with two parts, multiplied: of the first step over
+// singular values in [0, 1], of each later one over what the step before can make of them.
+double growth(const emrs_muon *a) {
+  double product = 1, top = 1;  // of singular values
+  for (uint32_t k = 0; k + 2 < a->steps; ++k) {
+    const double c0 = a->coefficients[3 * k], c1 = a->coefficients[3 * k + 1], c2 = a->coefficients[3 * k + 2];
+    const double end = top * top;
+    auto p = [&](double t) { return std::abs(c0 + t * (c1 + t * c2)); };  // of t = s s
+    // Both extremes lie at an end or where the derivative is 0: of p at -c1 / 2 c2, of s p at 0 = c0 + 3 c1 t + 5 c2 t t.
+    double most = std::max(p(0), p(end)), next = top * p(end);
+    auto inner = [&](double t) {
+      if (t > 0 && t < end) most = std::max(most, p(t)), next = std::max(next, std::sqrt(t) * p(t));
+    };
+    if (c2 != 0) {
+      inner(-c1 / (2 * c2));
+      const double root = std::sqrt(std::max(0.0, 9 * c1 * c1 - 20 * c0 * c2));
+      inner((-3 * c1 + root) / (10 * c2));
+      inner((-3 * c1 - root) / (10 * c2));
+    } else if (c1 != 0) {
+      inner(-c0 / (3 * c1));
+    }
+    product *= std::max(1.0, most);
+    top = next;
+  }
+  return product;
+}
+
+// Without coefficients (a workspace may be asked for before they are known) what the shape alone allows.
 bool by_squares(const emrs_muon *a) {
   const uint64_t s = std::min(a->rows, a->cols), l = std::max(a->rows, a->cols);
-  return a->steps > 3 && 2 * l >= 5 * s;
+  return a->steps > 3 && 2 * l >= 5 * s && (!a->coefficients || growth(a) <= kMostGrowth);
 }
 
 Sizes sizes_of(const emrs_muon *a) {

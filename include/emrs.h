@@ -523,6 +523,7 @@ typedef struct emrs_muon {
 #define EMRS_MUON_MAX_MATRICES 32u
 #define EMRS_MUON_MAX_STEPS 16u
 
+/* Bytes of workspace that emrs_muon_step wants.  Depends on the coefficients too: NULL asks for as much as any want. */
 int emrs_muon_workspace(const emrs_muon *muon, uint64_t *bytes);
 int emrs_muon_step(const emrs_muon *muon, void *stream);
 
