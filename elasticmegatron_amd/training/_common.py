@@ -38,6 +38,12 @@ def _stream(device: torch.device) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def written(*tensors: torch.Tensor) -> None:
+    """Counts ``tensors`` as changed in place, which kernels behind an address do not do by themselves: a graph
+    that saved one of them, or an arena that it is a view of, then refuses to run backward."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def run_on(device: torch.device, call, record) -> None:
     """``call(record, stream)`` with ``device`` current, on its current stream."""
     stream = _raw_stream(device.index) if _raw_stream is not None else _stream(device)

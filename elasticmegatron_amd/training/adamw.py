@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._common import DTYPE_CODES, dtype_code, on_device, run_on
+from ._common import DTYPE_CODES, dtype_code, on_device, run_on, written
 
 
 def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, grad: torch.Tensor, *,
@@ -39,6 +39,7 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
     grad = grad.detach().contiguous()
     a = _native.AdamW(n, main.data_ptr(), exp_avg.data_ptr(), exp_avg_sq.data_ptr(), grad.data_ptr(), DTYPE_CODES[grad.dtype], step,
                       None if model is None else model.data_ptr(), lr, beta1, beta2, eps, weight_decay)
+    written(*((main, exp_avg, exp_avg_sq) if model is None else (main, exp_avg, exp_avg_sq, model)))
     run_on(device, _native.adamw_step, a)
 
 

@@ -15,7 +15,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, run_on, workspace
+from ._common import dtype_code, on_device, run_on, workspace, written
 
 Matrices = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -111,6 +111,7 @@ def _run(kinds, *, steps, coefficients, eps, mu, nesterov, decay, rate) -> None:
     size = _native.muon_workspace(a)
     scratch = workspace(size, grad.device)
     a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
+    written(*(t for name, k in kinds.items() if name != "grad" for t in k.tensors))
     for lo in range(0, grad.count, at_once):
         hi = min(grad.count, lo + at_once)
         a.count = hi - lo
