@@ -21,17 +21,23 @@ from ._common import dtype_code, on_device, run_on, workspace
 Weight = Union[torch.Tensor, Sequence[torch.Tensor]]
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [n, h] with unit column stride and rows that do not overlap."""
-    (n, h), (over, along) = t.size(), t.stride()
+def _rows(t: torch.Tensor):
+    """``t`` [n, h] with unit column stride and rows that do not overlap; its sizes and strides."""
+    size, stride = t.size(), t.stride()
+    (n, h), (over, along) = size, stride
     if (h > 1 and along != 1) or (n > 1 and not h <= over <= 1 << 21):
-        return t.detach().contiguous()
-    return t
+        t = t.detach().contiguous()
+        stride = t.stride()
+    return t, size, stride
 
 
 def _room_for(t: torch.Tensor) -> torch.Tensor:
     """A contiguous gradient of ``t``."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.size(), dtype=t.dtype, device=t.device)
+
+
+def _table(values):
+    return (ctypes.c_uint64 * len(values))(*values)
 
 
 def _refuse(shards, device, dtype, h) -> None:
@@ -62,31 +68,28 @@ class _Call:
         if hidden.dim() < 1 or target.shape != hidden.shape[:-1]:
             raise ValueError(f"target {tuple(target.shape)} does not fit hidden {tuple(hidden.shape)}")
         h, device, dtype = hidden.size(-1), self.device, hidden.dtype
+        laid, pointers, strides, rows, lie = [], [], [], [], []
         for w in shards:  # one by one only where something is wrong: this is most of a small loss's host time
-            if not (isinstance(w, torch.Tensor) and w.dtype is dtype and w.device == device and w.dim() == 2 and w.size(1) == h):
+            if not (isinstance(w, torch.Tensor) and w.dtype is dtype and w.device == device and w.dim() == 2):
                 _refuse(shards, device, dtype, h)
-        rows = [w.size(0) for w in shards]
+            w, size, stride = _rows(w)
+            if size[1] != h:
+                _refuse(shards, device, dtype, h)
+            laid.append(w), pointers.append(w.data_ptr()), strides.append(stride[0]), rows.append(size[0]), lie.append((size, stride))
         if vocab_start < 0:
             raise ValueError("vocab_start is negative")
         if vocab_size is None:
             vocab_size = vocab_start + sum(rows)
         if vocab_size < 0:
             raise ValueError("vocab_size is negative")
-        self.hidden = _rows(hidden if hidden.dim() == 2 else hidden.detach().reshape(-1, h))
-        self.shards = [_rows(w) for w in shards]
-        self.shape = target.size()
+        self.hidden, size, stride = _rows(hidden if hidden.dim() == 2 else hidden.detach().reshape(-1, h))
+        self.shards, self.shape, self.rows = laid, target.size(), sum(rows)
         self.target = target if target.dim() == 1 and target.is_contiguous() else target.reshape(-1).contiguous()
-        n = len(shards)
-        pointers, strides, counts = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
-        for i, w in enumerate(self.shards):
-            pointers[i], strides[i], counts[i] = w.data_ptr(), w.stride(0), rows[i]
-        self._tables = (pointers, strides, counts)
-        a = self.record = _native.Loss()
-        a.dtype, a.n_shards, a.tokens, a.hidden_size = code, n, self.target.numel(), h
-        a.hidden, a.hidden_stride = self.hidden.data_ptr(), self.hidden.stride(0)
-        a.weights, a.weight_strides, a.shard_rows = (ctypes.addressof(x) for x in self._tables)
-        a.vocab_start, a.vocab_size = vocab_start, vocab_size
-        a.target, a.ignore_index = self.target.data_ptr(), ignore_index
+        self._lie, self._dtype, count = [*lie, (size, stride)], dtype, len(laid)
+        self._tables = (_table([*pointers, *strides, *rows]),)
+        at = ctypes.addressof(self._tables[0])
+        self.record = _native.Loss(code, count, size[0], h, self.hidden.data_ptr(), stride[0], at, at + 8 * count, at + 16 * count,
+                                   vocab_start, vocab_size, self.target.data_ptr(), ignore_index)
 
     def forward(self, with_loss: bool) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
         """``(lse, target logits, losses or None)``, the losses in the target's shape."""
@@ -102,16 +105,35 @@ class _Call:
         lse, logit = out.unbind()
         return lse, logit, loss
 
+    def again(self, hidden, target, shards) -> "_Call":
+        """The same call on tensors that autograd hands back: at their own addresses, and checked anew where they
+        do not lie as the first did."""
+        a, device = self.record, self.device
+        lie = [(t.size(), t.stride()) for t in shards if t.dtype is self._dtype and t.device == device]
+        lie.append((hidden.size(), hidden.stride()))
+        if not (lie == self._lie and hidden.dtype is self._dtype and hidden.device == device and target.dtype is torch.int64 and
+                target.device == device and target.size() == (a.tokens,) and target.is_contiguous()):
+            return _Call(hidden, shards, target, a.vocab_start, a.vocab_size, a.ignore_index)
+        call = object.__new__(_Call)
+        call.device, call.rows, call.hidden, call.target, call.shards = device, self.rows, hidden, target, shards
+        call._tables = (_table([w.data_ptr() for w in shards]), *self._tables)
+        a = call.record = _native.Loss.from_buffer_copy(a)
+        a.hidden, a.target, a.weights = hidden.data_ptr(), target.data_ptr(), ctypes.addressof(call._tables[0])
+        return call
+
+    def release(self) -> None:
+        self.hidden = self.target = self.shards = None
+
     def backward(self, lse, grad_loss, want_hidden: bool, want_weights: Sequence[bool]):
         a = self.record
         gh = _room_for(self.hidden) if want_hidden else None
         gw = [_room_for(w) if want else None for w, want in zip(self.shards, want_weights)]
-        if not a.tokens or not any(self._tables[2]):  # sums over nothing
+        if not a.tokens or not self.rows:  # sums over nothing
             for g in (gh, *gw):
                 if g is not None:
                     g.zero_()
             return gh, gw
-        table = (ctypes.c_uint64 * len(gw))(*(0 if g is None else g.data_ptr() for g in gw))
+        table = _table([0 if g is None else g.data_ptr() for g in gw])
         a.lse, a.grad_loss = lse.data_ptr(), grad_loss.data_ptr()
         a.grad_hidden = None if gh is None else gh.data_ptr()
         a.grad_weights = ctypes.addressof(table) if any(want_weights) else None
@@ -126,18 +148,24 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, hidden, target, vocab_size, ignore_index, *shards):
         call = _Call(hidden, shards, target, 0, vocab_size, ignore_index)
         lse, _, loss = call.forward(True)
-        ctx.save_for_backward(hidden, target, lse, *shards)
-        ctx.call = call  # views of the same inputs, checked already
+        # What the kernels read: the inputs, or the copies that had to be made of them.  The graph alone keeps them.
+        ctx.save_for_backward(call.hidden, call.target, lse, *call.shards)
+        ctx.call, ctx.shape = call, hidden.size()
+        call.release()
         return loss  # no view: users may scale it in place
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        hidden, _, lse, *_ = ctx.saved_tensors  # raises where an input was changed in place
+        hidden, target, lse, *shards = ctx.saved_tensors  # raises where one was changed in place
+        call = ctx.call.again(hidden, target, shards)
+        if not (lse.device == call.device and lse.is_contiguous()):
+            on_device("lse", lse, call.device)
+            lse = lse.contiguous()
         if grad_loss.dim() != 1 or grad_loss.dtype != torch.float32 or not grad_loss.is_contiguous():
             grad_loss = grad_loss.reshape(-1).to(torch.float32).contiguous()
-        gh, gw = ctx.call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
-        return (gh if gh is None or hidden.dim() == 2 else gh.view(hidden.shape), None, None, None, *gw)
+        gh, gw = call.backward(lse, grad_loss, ctx.needs_input_grad[0], ctx.needs_input_grad[4:])
+        return (gh if gh is None or len(ctx.shape) == 2 else gh.view(ctx.shape), None, None, None, *gw)
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, *, vocab_size: Optional[int] = None,
