@@ -10,8 +10,10 @@
 //
 // d is an operand of the matrix instructions, and so rounded to 16 bits: to fp16, whose 11 bits leave the
 // gradients with the rounding of their own type alone (in bf16, d's rounding would be as large as theirs).
-// fp16's range is met by powers of two: d is scaled by the largest |g|, and copies of w and h, which the
-// products want transposed anyway, by their largest entry; bf16's 8 bits lose nothing in them.
+// fp16's range is met by powers of two: each token's d is scaled by its own |g|, and copies of w and h, which the
+// products want transposed anyway, by their largest entry; bf16's 8 bits lose nothing in them.  grad_h takes a
+// token's scale off its row.  grad_w sums over tokens: h carries there what a token's |g| is below the largest, so
+// that h's entries keep all bits down to 2^-27 of the largest |g| times the largest |h|, and below 2^-38 are lost.
 //
 // Equal vocabulary shards (those of tensor parallelism are) go through every kernel together, as a batch.
 
@@ -233,6 +235,17 @@ __global__ __launch_bounds__(kMergeThreads) void merge_statistics_kernel(const f
 
 // ---- backward ----
 
+// Of a scale, a power of two; NULL: 1.
+__device__ inline int exponent_of(const float *scale) { return scale ? __builtin_amdgcn_frexp_expf(scale[0]) - 1 : 0; }
+
+// The power of two that brings |x| to [2^13, 2^14); `otherwise` for 0 and for what is not finite.
+__device__ inline int exponent_for(float x, int otherwise) {
+  x = fabsf(x);
+  return x > 0.f && x < INFINITY ? min(max(14 - __builtin_amdgcn_frexp_expf(x), -120), 120) : otherwise;
+}
+
+__device__ inline float scale_of(float top) { return __builtin_amdgcn_ldexpf(1.f, exponent_for(top, 14)); }
+
 // d of a piece, in both orientations, with zeros up to the padded sizes (the next products sum over them).  Its
 // 512 KB a large tile of exponentials and stores are what it is slower by than the statistics.
 // With kParts d is in two bf16 parts, [2][tokens]: what the product with bf16 weights as they lie takes.
@@ -245,13 +258,13 @@ struct LogitGradients : Piece {
   const float *lse, *grad_loss;
   const int64_t *target;
   int64_t ignore;
-  const float *scale;     // of d
+  const float *scale;     // of the largest |grad_loss|
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4, valid = this->valid(w.batch, p.m);
     const int64_t first = first_of(w.batch);
-    const float by = scale[0];
+    const int largest = exponent_of(scale);
     using Turn = emrs_gemm::Turn<Cfg>;
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
@@ -259,7 +272,7 @@ struct LogitGradients : Piece {
       const int64_t label = t < p.n ? target[t] : ignore;
       const bool counts = label != ignore;
       const int64_t at = label - first;
-      const float g = counts ? grad_loss[t] * by : 0.f, l = counts ? lse[t] * kLog2e : 0.f;
+      const float weight = counts ? grad_loss[t] : 0.f, g = __builtin_amdgcn_ldexpf(weight, exponent_for(weight, largest)), l = counts ? lse[t] * kLog2e : 0.f;
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) {
         const int v = m + i * 16;
@@ -322,8 +335,22 @@ struct OfWeights : Base {
   }
 };
 
-// Of a scale, a power of two; NULL: 1.
-__device__ inline int exponent_of(const float *scale) { return scale ? __builtin_amdgcn_frexp_expf(scale[0]) - 1 : 0; }
+// What the sums are to be divided by, as a power of two: the scales of both operands, and where row n is a token's
+// (or that of its second part), the token's own in place of the largest.
+struct Scales {
+  const float *a, *b;
+  const float *grad_loss;  // NULL: no tokens
+  int32_t tokens;
+
+  // Both read once, before a tile's stores.  The product of the scales may be out of range: exponents.
+  struct Exponents {
+    int a, b;
+  };
+  __device__ __forceinline__ Exponents exponents() const { return {exponent_of(a), exponent_of(b)}; }
+  __device__ __forceinline__ int of(int n, const Exponents &e) const {
+    return e.b + (grad_loss ? exponent_for(grad_loss[min(n < tokens ? n : n - tokens, tokens - 1)], e.a) : e.a);
+  }
+};
 
 // A run of k of each product for itself: C of run b goes to sum[b], in 32 bits and unscaled, on top of what
 // an earlier piece left there.
@@ -332,16 +359,16 @@ struct StoreSums : emrs_gemm::Operand {
   int64_t stride, batch;
   int32_t add;
   int32_t wide;
-  const float *scale_a, *scale_b;
+  Scales scales;
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     const int m = m0 + (lane >> 4) * 4;
-    const int by = exponent_of(scale_a) + exponent_of(scale_b);  // the product of the scales may be out of range
     float *const to = sum + w.batch * batch;
+    const auto exponents = scales.exponents();
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
-      const int n = n0 + j * 16 + (lane & 15);
+      const int n = n0 + j * 16 + (lane & 15), by = scales.of(n, exponents);
       // What lies outside reads the last element inside: with no branch, these loads are on their way together.
       f32x4 before[Cfg::MI];
 #pragma unroll
@@ -379,18 +406,18 @@ struct StoreRows : emrs_gemm::Operand {
   const float *sum;       // NULL: C alone (a batch of one)
   int64_t stride;         // elements between rows of out and of sum
   int32_t wide;           // eight elements can be stored at once
-  const float *scale_a, *scale_b;
+  Scales scales;
 
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
     using x4 = typename emrs_gemm::Vec<T>::x4;
     using Turn = emrs_gemm::Turn<Cfg>;
     const int m = m0 + (lane >> 4) * 4;
-    const int by = exponent_of(scale_a) + exponent_of(scale_b);  // the product of the scales may be out of range
     T *const to = static_cast<T *>(const_cast<void *>(out.p[w.batch]));
+    const auto exponents = scales.exponents();
 #pragma unroll
     for (int j = 0; j < Cfg::NI; ++j) {
-      const int n = n0 + j * 16 + (lane & 15);
+      const int n = n0 + j * 16 + (lane & 15), by = scales.of(n, exponents);
       f32x4 before[Cfg::MI];
 #pragma unroll
       for (int i = 0; i < Cfg::MI; ++i) before[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -436,7 +463,7 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float *sum, int su
   out[i] = (T)v;
 }
 
-// ---- scales: powers of two that bring the largest finite entry to [2^13, 2^14), and |grad_loss| likewise ----
+// ---- scales: powers of two that bring the largest finite entry, or |grad_loss|, to [2^13, 2^14) ----
 
 constexpr int kScaleBlocks = 1024;  // workgroups that look for the largest entries of one kind
 
@@ -449,20 +476,16 @@ __device__ inline float block_max(float v) {
   return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
 }
 
-__device__ inline float scale_of(float top) {
-  int e = 0;
-  if (top > 0.f && top < INFINITY) frexpf(top, &e);
-  return ldexpf(1.f, min(max(14 - e, -100), 100));
-}
-
 // Rows of one kind that become a transposed operand: a group's weight rows, or the hidden states.
 struct Rows {
   Piece piece;
   int64_t stride;
   int32_t rows, count;    // of each matrix; matrices
-  int32_t blocks;         // workgroups that look for a matrix's largest entry; 0: fp16, copied unscaled
+  int32_t blocks;         // workgroups that look for a matrix's largest entry; 0: copied unscaled
   const int64_t *target;  // NULL, or: rows whose target is `ignore` do not count
   int64_t ignore;
+  const float *grad_loss; // NULL, or: a row carries what its |grad_loss| is below the largest, whose scale is d_scale
+  const float *d_scale;
   float *largest;         // [count x blocks]
   float *scale;           // written by the transposition
 };
@@ -564,6 +587,7 @@ __device__ __forceinline__ void turn(const Turned &to, uint32_t id, int cols, ha
   const T *in = static_cast<const T *>(a.piece.weights.p[matrix]);
   const int valid = a.piece.valid(matrix, a.rows);
   float by = 1.f;
+  const int largest = exponent_of(a.d_scale);
   if (a.blocks) {
     float top = 0.f;
     for (int i = threadIdx.x; i < a.count * a.blocks; i += 256) top = fmaxf(top, a.largest[i]);
@@ -575,6 +599,8 @@ __device__ __forceinline__ void turn(const Turned &to, uint32_t id, int cols, ha
   for (int h = 0; h < 2; ++h) {
     const int at = threadIdx.x + h * 256, r = at / 8, c = at % 8 * 8;
     const bool keep = r0 + r < valid && !(a.target && a.target[r0 + r] == a.ignore);
+    float own = by;
+    if (a.grad_loss && keep) own = __builtin_amdgcn_ldexpf(by, min(0, largest - exponent_for(a.grad_loss[r0 + r], largest)));
     const T *row = in + (r0 + r) * a.stride + c0 + c;
     x8 v;
 #pragma unroll
@@ -587,7 +613,7 @@ __device__ __forceinline__ void turn(const Turned &to, uint32_t id, int cols, ha
         if (c0 + c + i < cols) v[i] = row[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tile[c + i][((r / 8 ^ (c / 8)) * 8) + r % 8] = (half)((float)v[i] * by);
+    for (int i = 0; i < 8; ++i) tile[c + i][((r / 8 ^ (c / 8)) * 8) + r % 8] = (half)((float)v[i] * own);
   }
   __syncthreads();
 #pragma unroll
@@ -822,12 +848,10 @@ int forward(const emrs_loss *a, hipStream_t st) {
   return EMRS_OK;
 }
 
-template <class T>
-Rows rows_of(const Piece &c, uint32_t count, int64_t stride, int64_t rows, const int64_t *target, int64_t ignore, float *largest, float *scale) {
+Rows rows_of(const Piece &c, uint32_t count, int64_t stride, int64_t rows, bool scaled, float *largest, float *scale) {
   Rows r{};
   r.piece = c, r.stride = stride, r.rows = (int32_t)rows, r.count = (int32_t)count;
-  r.blocks = std::is_same<T, half>::value ? 0 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(rows, kScaleBlocks / count));
-  r.target = target, r.ignore = ignore;
+  r.blocks = scaled ? (int32_t)std::max<int64_t>(1, std::min<int64_t>(rows, kScaleBlocks / count)) : 0;
   r.largest = largest, r.scale = scale;
   return r;
 }
@@ -846,7 +870,9 @@ int backward(const emrs_loss *a, hipStream_t st) {
   if (rc) return rc;
   Piece every{};
   every.weights.p[0] = a->hidden, every.vocab = tokens;
-  const Rows h_rows = rows_of<T>(every, 1, (int64_t)a->hidden_stride, tokens, a->target, a->ignore_index, largest + kScaleBlocks, h_scale);
+  Rows h_rows = rows_of(every, 1, (int64_t)a->hidden_stride, tokens, true, largest + kScaleBlocks, h_scale);
+  h_rows.target = a->target, h_rows.ignore = a->ignore_index;
+  h_rows.grad_loss = a->grad_loss, h_rows.d_scale = d_scale;
   const bool fours = h % 4 == 0;
   uint64_t first = a->vocab_start, left = 0;
   for (uint32_t i = 0; i < s.n_groups; ++i) left += (a->shard_rows[s.groups[i].first] + s.piece - 1) / s.piece;
@@ -861,7 +887,7 @@ int backward(const emrs_loss *a, hipStream_t st) {
       --left;
       if (!a->grad_hidden && !wanted) continue;
       const Piece own = piece_of(a, g, first, lo);
-      const Rows w_rows = rows_of<T>(own, g.count, (int64_t)a->weight_strides[g.first], (int64_t)rows, nullptr, 0, largest, w_scale);
+      const Rows w_rows = rows_of(own, g.count, (int64_t)a->weight_strides[g.first], (int64_t)rows, !std::is_same<T, half>::value, largest, w_scale);
       Rows none = h_rows;
       none.count = 0;
       const bool copied = a->grad_hidden && !s.direct;
@@ -910,14 +936,14 @@ int backward(const emrs_loss *a, hipStream_t st) {
           q.k = (int32_t)round_up((q.k + s.splits - 1) / s.splits, 64);
           q.a_batch = q.b_batch = q.k;
         }
-        const float *const scale = s.direct ? nullptr : w_scale;
+        const Scales scales{d_scale, s.direct ? nullptr : w_scale, a->grad_loss, (int32_t)tokens};
         if (s.sums > 1 || left) {
-          TRY(product(StoreSums{{}, sum, h, q.n * h, begun, fours, d_scale, scale}));
+          TRY(product(StoreSums{{}, sum, h, q.n * h, begun, fours, scales}));
         } else {
           StoreRows<T> out{};
           out.out.p[0] = a->grad_hidden, out.sum = begun ? sum : nullptr, out.stride = h;
           out.wide = h % 8 == 0 && reinterpret_cast<uintptr_t>(a->grad_hidden) % 16 == 0;
-          out.scale_a = d_scale, out.scale_b = scale;
+          out.scales = scales;
           TRY(product(out));
         }
         begun = true;
@@ -938,7 +964,7 @@ int backward(const emrs_loss *a, hipStream_t st) {
           out.out.p[b] = gw;
           out.wide &= reinterpret_cast<uintptr_t>(gw) % 16 == 0;
         }
-        out.stride = h, out.scale_a = d_scale, out.scale_b = h_scale;
+        out.stride = h, out.scales = Scales{d_scale, h_scale, nullptr, 0};
         TRY((emrs_gemm::launch<half>(q, out, st)));
       }
     }
