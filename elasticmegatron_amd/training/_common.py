@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -22,6 +23,18 @@ def on_device(what: str, t: torch.Tensor, device: torch.device) -> None:
         raise ValueError(f"{what} is on {t.device}: a GPU is wanted")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the others on {device}")
+
+
+def refuse_tangents(*arguments) -> None:
+    """Raises where a tensor, alone or in a sequence, carries a forward-mode tangent: no operator here has such a
+    derivative, and a kernel that reads the tensor's memory would drop it."""
+    if forward_ad._current_level < 0:  # none is being taken
+        return
+    for t in arguments:
+        if isinstance(t, (list, tuple)):
+            refuse_tangents(*t)
+        elif isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the operators of a training step have no forward-mode derivatives")
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -7,7 +7,7 @@ from typing import Optional
 import torch
 
 from .. import _native
-from ._common import DTYPE_CODES, dtype_code, on_device, run_on, written
+from ._common import DTYPE_CODES, dtype_code, on_device, refuse_tangents, run_on, written
 
 
 def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, grad: torch.Tensor, *,
@@ -22,6 +22,7 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
     ``main``, ``exp_avg`` and ``exp_avg_sq`` are fp32, ``grad`` fp32, bf16 or fp16, all contiguous and of one
     size: a parameter's, a rank's shard of it, or a whole arena.  ``step`` counts from 1.
     """
+    refuse_tangents(main, exp_avg, exp_avg_sq, grad, model)
     n = main.numel() if isinstance(main, torch.Tensor) else 0
     for t in (main, exp_avg, exp_avg_sq):
         if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.is_cuda and t.numel() == n and t.is_contiguous()):

@@ -16,7 +16,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, run_on, workspace
+from ._common import dtype_code, on_device, refuse_tangents, run_on, workspace
 
 Weight = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -59,6 +59,7 @@ class _Call:
             raise ValueError(f"{len(shards)} vocabulary shards: 1 to {_native.EMRS_LOSS_MAX_SHARDS} are wanted")
         if not isinstance(hidden, torch.Tensor):
             raise TypeError("hidden is no tensor")
+        refuse_tangents(hidden, shards)
         self.device = hidden.device
         on_device("hidden", hidden, self.device)
         on_device("target", target, self.device)
@@ -182,6 +183,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Ten
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction {reduction!r}: 'none', 'sum' or 'mean' is wanted")
     shards = [weight] if isinstance(weight, torch.Tensor) else list(weight)
+    refuse_tangents(hidden, shards)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (hidden, *shards)):
         loss = _LinearCrossEntropy.apply(hidden, target, vocab_size, ignore_index, *shards)
     else:
@@ -214,6 +216,7 @@ def vocab_gradients(hidden: torch.Tensor, weight: Weight, target: torch.Tensor, 
     ``hidden`` (the whole is the sum over the processes) and the gradients of its own shards.
 
     ``lse`` is of the whole vocabulary; ``grad_loss`` is the loss's gradient for each token."""
+    refuse_tangents(lse, grad_loss)
     call = _Call(hidden, weight, target, vocab_start, vocab_size, ignore_index)
     for what, t in (("lse", lse), ("grad_loss", grad_loss)):
         on_device(what, t, call.device)

@@ -15,7 +15,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from .. import _native
-from ._common import dtype_code, on_device, run_on, workspace, written
+from ._common import dtype_code, on_device, refuse_tangents, run_on, workspace, written
 
 Matrices = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -44,6 +44,7 @@ class _Stack:
                     raise TypeError(f"{what} is no tensor")
                 if t.dim() != 2:
                     raise ValueError(f"{what} has a member of {t.dim()} dimensions: matrices are wanted")
+        refuse_tangents(self.tensors)
         if self.count:
             self.shape = self.tensors[0].shape[-2:]
             self.dtype, self.device = self.tensors[0].dtype, self.tensors[0].device
