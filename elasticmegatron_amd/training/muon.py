@@ -16,6 +16,7 @@ import torch
 
 from .. import _native
 from ._common import dtype_code, on_device, refuse_tangents, run_on, workspace, written
+from ._overlap import first_conflict, rows_of
 
 Matrices = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -74,12 +75,16 @@ class _Stack:
         if len(self.tensors) == 1 and self.tensors[0].dim() == 3:
             t = self.tensors[0]
             step = t.stride(0) * t.element_size()
-            if not copy and self.count > 1 and step < ((rows - 1) * self.stride + cols) * t.element_size():
-                raise ValueError(f"{self.what} is written in place: its matrices overlap")
             base = t.data_ptr()
             self.addresses = [base + i * step for i in range(self.count)]
         else:
             self.addresses = [t.data_ptr() for t in self.tensors]
+
+    def in_memory(self, written: bool):
+        rows, cols = self.shape
+        size = self.tensors[0].element_size()
+        stride = (self.stride if rows > 1 else cols) * size
+        return [rows_of(base, rows, stride, cols * size, self.what, i, written) for i, base in enumerate(self.addresses)]
 
     def table(self, lo: int, hi: int):
         return (ctypes.c_uint64 * (hi - lo))(*self.addresses[lo:hi])
@@ -99,6 +104,11 @@ def _run(kinds, *, steps, coefficients, eps, mu, nesterov, decay, rate) -> None:
     grad = kinds["grad"]
     for name, k in kinds.items():
         k.lay_out(copy=name == "grad")
+    if "main" in kinds:  # matrices are worked on side by side
+        conflict = first_conflict(m for name, k in kinds.items() for m in k.in_memory(name != "grad"))
+        if conflict:
+            a, b = conflict
+            raise ValueError(f"{a.what} [{a.index}] and {b.what} [{b.index}] share memory, which is written in place")
     a = _native.Muon()
     a.grad_dtype = dtype_code(grad.tensors[0], "grad")
     a.rows, a.cols, a.steps, a.nesterov = *grad.shape, steps, int(nesterov)
@@ -160,7 +170,8 @@ def muon_step(main: Matrices, momentum_buffer: Matrices, grad: Matrices, *, mode
 
     ``main`` and ``momentum_buffer`` are fp32 (a state's main and exp_avg), ``grad`` fp32, bf16 or fp16.
     Entries of an orthogonal matrix are 1 / sqrt(max(rows, cols)), so an update's are about
-    ``lr * rms_scale``, as AdamW's are with 0.2.  A matrix is taken as it is given: one that tensor
+    ``lr * rms_scale``, as AdamW's are with 0.2.  No two matrices may share memory that is written (a tied one is
+    listed once); ``grad`` may be that of its own ``main`` or ``model``.  A matrix is taken as it is given: one that tensor
     parallelism or a distributed optimizer has cut is to be gathered first.
     """
     g, w, b = _Stack("grad", grad), _Stack("main", main), _Stack("momentum_buffer", momentum_buffer)

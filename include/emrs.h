@@ -501,7 +501,8 @@ int emrs_loss_backward(const emrs_loss *loss, void *stream);
  *   X = update / (|update|_F + eps); per step with its (a, b, c): A = X X^T, X = a X + (b A + c A A) X
  *   out = X                                                   (out != NULL, bf16)
  *   main = main (1 - decay) - rate X, image = main as bf16    (main != NULL)
- * Matrices are row-major with unit column stride; *_stride: elements between rows. */
+ * Matrices are row-major with unit column stride; *_stride: elements between rows.  They are worked on side by
+ * side: what is written may share no memory with another matrix, nor momentum with its gradient. */
 typedef struct emrs_muon {
   uint32_t count;                 /* 1 to EMRS_MUON_MAX_MATRICES */
   uint32_t grad_dtype;            /* EMRS_FP32, EMRS_BF16 or EMRS_FP16 */
