@@ -46,7 +46,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(uint64_t fours, uint64_
                                                          Factors f) {
   using g4 = typename Four<G>::type;
   using h4 = typename Four<__bf16>::type;
-  uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+  uint64_t i = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x;
   if (kWide && i < fours) {
     f32x4 a = stream_in(reinterpret_cast<const f32x4 *>(w) + i), b = stream_in(reinterpret_cast<const f32x4 *>(m) + i);
     f32x4 c = stream_in(reinterpret_cast<const f32x4 *>(v) + i);
@@ -84,7 +84,10 @@ int launch(const emrs_adamw *a, const Factors &f, hipStream_t st) {
   __bf16 *image = static_cast<__bf16 *>(a->image);
   const bool wide = on(a->main, 16) && on(a->exp_avg, 16) && on(a->exp_avg_sq, 16) && on(g, 4 * sizeof(G)) && on(image, 8);
   const uint64_t fours = wide ? a->n / 4 : 0, lanes = fours + (a->n - fours * 4);
-  const uint32_t blocks = (uint32_t)((lanes + kThreads - 1) / kThreads);
+  // A row of the grid holds less than 2^32 lanes; rows of equal length, so that the last one is not empty for the most part.
+  constexpr uint64_t most = 0xffffffffull / kThreads;
+  const uint64_t all = (lanes + kThreads - 1) / kThreads, rows = (all + most - 1) / most;
+  const dim3 blocks((uint32_t)((all + rows - 1) / rows), (uint32_t)rows);
   if (wide)
     adamw_kernel<G, kImage, true><<<blocks, kThreads, 0, st>>>(fours, a->n, a->main, a->exp_avg, a->exp_avg_sq, g, image, f);
   else
