@@ -20,7 +20,8 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
         model = main as bf16   (``model`` given)
 
     ``main``, ``exp_avg`` and ``exp_avg_sq`` are fp32, ``grad`` fp32, bf16 or fp16, all contiguous and of one
-    size: a parameter's, a rank's shard of it, or a whole arena.  ``step`` counts from 1.
+    size: a parameter's, a rank's shard of it, or a whole arena.  Shapes may differ as views of one flat run do; a
+    ``grad`` with ``main``'s sides in another order is refused.  ``step`` counts from 1.
     """
     refuse_tangents(main, exp_avg, exp_avg_sq, grad, model)
     n = main.numel() if isinstance(main, torch.Tensor) else 0
@@ -29,6 +30,8 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
             _refuse(main, exp_avg, exp_avg_sq, grad, model)
     if not (isinstance(grad, torch.Tensor) and grad.dtype in DTYPE_CODES and grad.is_cuda and grad.numel() == n):
         _refuse(main, exp_avg, exp_avg_sq, grad, model)
+    if grad.size() != main.size() and _turned(grad.size(), main.size()):
+        raise ValueError(f"grad is {tuple(grad.size())}, main {tuple(main.size())}: its elements are in another order")
     if model is not None and not (isinstance(model, torch.Tensor) and model.dtype is torch.bfloat16 and model.is_cuda and
                                   model.numel() == n and model.is_contiguous()):
         _refuse(main, exp_avg, exp_avg_sq, grad, model)
@@ -42,6 +45,12 @@ def adamw_step(main: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tens
                       None if model is None else model.data_ptr(), lr, beta1, beta2, eps, weight_decay)
     written(*((main, exp_avg, exp_avg_sq) if model is None else (main, exp_avg, exp_avg_sq, model)))
     run_on(device, _native.adamw_step, a)
+
+
+def _turned(a, b) -> bool:
+    """Whether ``a`` has the sides of ``b`` in another order: a transposed tensor, no flat run of the same one."""
+    a, b = ([n for n in x if n != 1] for x in (a, b))
+    return a != b and sorted(a) == sorted(b)
 
 
 def _refuse(main, exp_avg, exp_avg_sq, grad, model) -> None:
