@@ -38,6 +38,10 @@ using emrs_internal::fail;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kPieceBytes = 128ull << 20;  // of d in one orientation
+// Of a copy of weights, transposed or padded: with few tokens a piece of d would let it be the whole weight
+// (128256 x 4096, 512 tokens: 1.32 GB of workspace; bounded to this 388 MB, and 2614 us against 2350; to half of
+// it 180 MB and 3080).
+constexpr uint64_t kCopyBytes = 256ull << 20;
 
 // Whether grad_hidden's product takes the weights as they lie: no search of their largest entry, no transposed
 // copy, but smaller tiles, and for bf16 twice the rows of d, in two parts.  All
@@ -727,6 +731,9 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   s.piece = round_up(most, 256);
   if (backward || s.pad_weight)
     s.piece = std::min(s.piece, std::max<uint64_t>(kPieceBytes / 2 / s.tokens_padded / shards / 256, 1) * 256);
+  s.direct = takes_weights(a->dtype, a->tokens);
+  if (s.pad_weight || (backward && a->grad_hidden && !s.direct))
+    s.piece = std::min(s.piece, std::max<uint64_t>(kCopyBytes / 2 / s.k / shards / 256, 1) * 256);
   uint64_t slots = 0;
   for (uint32_t i = 0; i < s.n_groups; ++i)
     for (uint64_t lo = 0; lo < a->shard_rows[s.groups[i].first]; lo += s.piece)
@@ -734,7 +741,6 @@ Sizes sizes_of(const emrs_loss *a, bool backward) {
   // grad_hidden's product has few tiles where there are few tokens: its sum over the vocabulary is cut into
   // runs of at least 1024 rows, as many as the product and the sums' way through memory take least time with.
   const uint64_t k = round_up(std::min(s.piece, most), 64) * shards;
-  s.direct = takes_weights(a->dtype, a->tokens);
   s.parts = s.direct && a->dtype == EMRS_BF16 ? 2 : 1;
   s.splits = 1;
   double best = 0;
