@@ -13,9 +13,10 @@
 // 64 banks.  Rows past the operand's last are past the buffer's end and read as zeros, and so are, by
 // their lane's offset, units past the last k.
 //
-// What bounds it is the card's power: in large products matrix instructions issue in 83% of the cycles, at 1.6
-// to 1.8 GHz.  Measured with what the epilogues do: statistics of 4096 x 32000 logits, k 4096, 780 us (1.38
-// PFLOP/s); d of 4096 x 16384, 450 us (1.22); the gradients' products of that d, 425 and 440 us (1.27).
+// In large products matrix instructions issue in 63 to 66% of the cycles that a CU is busy, start and epilogue
+// included (75% where k is 12288, 54% where the epilogue reads X and writes it twice), at 1.9 to 2.0 GHz of 2.4.
+// Measured with what the epilogues do, on two cards: statistics of 4096 x 32000 logits, k 4096, 780 and 832 us (1.38 and 1.29 PFLOP/s); d
+// of 4096 x 16384, 450 and 472 us; the gradients' products of that d, 425 to 458 us.
 #ifndef EMRS_GEMM_H
 #define EMRS_GEMM_H
 

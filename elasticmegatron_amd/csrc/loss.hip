@@ -14,6 +14,7 @@
 // products want transposed anyway, by their largest entry; bf16's 8 bits lose nothing in them.  grad_h takes a
 // token's scale off its row.  grad_w sums over tokens: h carries there what a token's |g| is below the largest, so
 // that h's entries keep all bits down to 2^-27 of the largest |g| times the largest |h|, and below 2^-38 are lost.
+// So do d's: where a probability is below 2^-27 bits of it are lost, and below 2^-38 all.
 //
 // Equal vocabulary shards (those of tensor parallelism are) go through every kernel together, as a batch.
 
@@ -39,16 +40,20 @@ using emrs_internal::fail;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint64_t kPieceBytes = 128ull << 20;  // of d in one orientation
 // Of a copy of weights, transposed or padded: with few tokens a piece of d would let it be the whole weight
-// (128256 x 4096, 512 tokens: 1.32 GB of workspace; bounded to this 388 MB, and 2614 us against 2350; to half of
-// it 180 MB and 3080).
+// (128256 x 4096, 512 tokens: 1321 MiB of workspace; bounded to this 388, and 2614 us against 2350; to half of it
+// 180 and 3080).
 constexpr uint64_t kCopyBytes = 256ull << 20;
 
 // Whether grad_hidden's product takes the weights as they lie: no search of their largest entry, no transposed
-// copy, but smaller tiles, and for bf16 twice the rows of d, in two parts.  All
-// gradients of 32000 x 4096 in bf16: 8 tokens 238 against 409 us, 512 tokens 699 against 647; in fp16: 8 tokens
-// 239 against 350, 512 tokens 542 against 589, 2048 tokens 1667 against 1567.
+// copy, but smaller tiles, and for bf16 twice the rows of d, in two parts.  What both read and compute grows alike
+// with rows and hidden size, so that tokens decide.  All gradients, this against the other, us:
+//   bf16       64 tokens   256          512          1024            fp16  256 tokens   512          1024
+//   32000 x 512     69/76    102/100      123/113      208/165              89/95        102/109      161/163
+//   8000 x 4096     86/108   141/152      192/178      342/259             132/140       157/169      246/253
+//   32000 x 4096   253/423   486/559      698/641     1220/950             399/504       543/589      902/896
+//   128256 x 4096  914/1744 1550/2278    2578/2594    4781/3789           1259/2035     1961/2361    3507/3584
+//   32000 x 8192   510/866   890/1104    1316/1384    2351/1832            746/982      1010/1270    1745/1725
 bool takes_weights(uint32_t dtype, uint64_t tokens) { return tokens <= (dtype == EMRS_BF16 ? 256 : 768); }
-
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 

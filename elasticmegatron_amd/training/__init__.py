@@ -13,7 +13,8 @@ these read and write: the output layer's bf16 vocabulary shards, and main / exp_
 
 Kernels run on the current stream of the tensors' device, as torch's own operators do; outputs and
 workspaces come from torch's caching allocator.  There is no fallback: without a GPU and the built
-library every call raises.
+library every call raises.  The loss has reverse-mode derivatives, once; nothing has forward-mode ones, and tensors
+that carry a tangent are refused.  What an update writes counts as changed in place.
 """
 
 from .adamw import adamw_step

@@ -179,6 +179,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: Weight, target: torch.Ten
     to any gradient, whatever their hidden state holds.  A target outside the vocabulary has loss inf.
     ``reduction``: ``"none"`` (fp32, the shape of ``target``), ``"sum"``, or ``"mean"`` over the tokens that
     count (NaN where none does).  Differentiable once, to ``hidden`` and to every shard.
+
+    A token's gradient to ``hidden`` is as exact whatever the other tokens' loss counts for.  Gradients to the shards
+    sum over tokens: what one adds there keeps fewer bits from 2^-27 of the largest |gradient of a loss| times
+    |hidden| on, and nothing below 2^-38.
     """
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction {reduction!r}: 'none', 'sum' or 'mean' is wanted")
