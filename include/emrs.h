@@ -463,6 +463,8 @@ int emrs_ipc_open_count(void);
  * 0 where target[t] == ignore_index.  A target in none of these rows has target_logit -inf and loss +inf.
  * Backward: d = grad_loss[t] (exp(x - lse[t]) - [v == target[t]]), 0 for ignored tokens;
  *   grad_hidden[t] = sum_v d w[v], grad_weights[v] = sum_t d hidden[t]; rows >= vocab_size get zeros.
+ * d is rounded to 16 bits under a power of two of each token's own; in grad_weights a token's share keeps all its
+ * bits down to 2^-27 of the largest |grad_loss| times the largest |hidden|.
  * The hidden states of ignored tokens and the rows >= vocab_size may hold anything, NaN included. */
 typedef struct emrs_loss {
   uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16: hidden, weights and their gradients */
