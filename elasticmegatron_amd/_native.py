@@ -110,7 +110,53 @@ class AdamW(ctypes.Structure):
                 ("weight_decay", ctypes.c_double)]
 
 
+class Norm(ctypes.Structure):
+    """struct emrs_norm"""
+
+    _fields_ = [("dtype", ctypes.c_uint32), ("residual_dtype", ctypes.c_uint32), ("gate_kind", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32), ("tokens", ctypes.c_uint64), ("hidden", ctypes.c_uint64),
+                ("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_uint64), ("branch", ctypes.c_void_p),
+                ("branch_stride", ctypes.c_uint64), ("gate", ctypes.c_void_p), ("gate_stride", ctypes.c_uint64),
+                ("branch_weight", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("residual_scale", ctypes.c_float),
+                ("eps", ctypes.c_float), ("stream", ctypes.c_void_p), ("stream_stride", ctypes.c_uint64),
+                ("normed", ctypes.c_void_p), ("stream_rms", ctypes.c_void_p), ("branch_rms", ctypes.c_void_p),
+                ("grad_stream", ctypes.c_void_p), ("grad_normed", ctypes.c_void_p), ("grad_residual", ctypes.c_void_p),
+                ("grad_branch", ctypes.c_void_p), ("grad_gate", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p),
+                ("grad_branch_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class Experts(ctypes.Structure):
+    """struct emrs_experts"""
+
+    _fields_ = [("dtype", ctypes.c_uint32), ("n_experts", ctypes.c_uint32), ("rows", ctypes.c_uint64),
+                ("n_in", ctypes.c_uint64), ("n_out", ctypes.c_uint64), ("counts", ctypes.c_void_p),
+                ("counts_bytes", ctypes.c_uint32), ("reserved", ctypes.c_uint32), ("x", ctypes.c_void_p),
+                ("x_stride", ctypes.c_uint64), ("weights", ctypes.c_void_p), ("weight_stride", ctypes.c_uint64),
+                ("y", ctypes.c_void_p), ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_uint64),
+                ("grad_x", ctypes.c_void_p), ("grad_weights", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class Attention(ctypes.Structure):
+    """struct emrs_attention"""
+
+    _fields_ = [("dtype", ctypes.c_uint32), ("causal", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("kv_heads", ctypes.c_uint32), ("dim", ctypes.c_uint32), ("offset_bytes", ctypes.c_uint32),
+                ("rows", ctypes.c_uint64), ("key_rows", ctypes.c_uint64), ("documents", ctypes.c_uint64),
+                ("offsets", ctypes.c_void_p), ("key_offsets", ctypes.c_void_p),
+                ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("q_strides", ctypes.c_uint64 * 2), ("k_strides", ctypes.c_uint64 * 2), ("v_strides", ctypes.c_uint64 * 2),
+                ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("grad_out", ctypes.c_void_p), ("grad_out_strides", ctypes.c_uint64 * 2), ("grad_q", ctypes.c_void_p),
+                ("grad_k", ctypes.c_void_p), ("grad_v", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
 EMRS_FP32, EMRS_BF16, EMRS_FP16 = 0, 1, 2
+EMRS_NORM_GATE_NONE, EMRS_NORM_GATE_CHANNEL, EMRS_NORM_GATE_TOKEN = 0, 1, 2
+EMRS_NORM_MAX_HIDDEN = 16384
+EMRS_EXPERTS_MAX = 256
+EMRS_ATTENTION_MAX_DIM = 128
 EMRS_LOSS_MAX_SHARDS = 64
 EMRS_MUON_MAX_MATRICES = 32
 EMRS_MUON_MAX_STEPS = 16
@@ -169,8 +215,10 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.emrs_loss_workspace.argtypes = [ctypes.POINTER(Loss), I, ctypes.POINTER(U64)]
     lib.emrs_muon_workspace.restype = I
     lib.emrs_muon_workspace.argtypes = [ctypes.POINTER(Muon), ctypes.POINTER(U64)]
+    lib.emrs_norm_workspace.restype = I
+    lib.emrs_norm_workspace.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(U64)]
     for fn, record in ((lib.emrs_loss_forward, Loss), (lib.emrs_loss_backward, Loss), (lib.emrs_muon_step, Muon),
-                       (lib.emrs_adamw_step, AdamW)):
+                       (lib.emrs_adamw_step, AdamW), (lib.emrs_norm_forward, Norm), (lib.emrs_norm_backward, Norm)):
         fn.restype = I
         fn.argtypes = [ctypes.POINTER(record), P]
     if lib.emrs_abi_version() != 8:
@@ -404,3 +452,18 @@ def muon_step(a: Muon, stream: int = 0) -> None:
 
 def adamw_step(a: AdamW, stream: int = 0) -> None:
     _check(load().emrs_adamw_step(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_adamw_step")
+
+
+def norm_workspace(a: Norm) -> int:
+    """emrs_norm_workspace: bytes of workspace that backward wants."""
+    n = ctypes.c_uint64()
+    _check(load().emrs_norm_workspace(ctypes.byref(a), ctypes.byref(n)), "emrs_norm_workspace")
+    return int(n.value)
+
+
+def norm_forward(a: Norm, stream: int = 0) -> None:
+    _check(load().emrs_norm_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_norm_forward")
+
+
+def norm_backward(a: Norm, stream: int = 0) -> None:
+    _check(load().emrs_norm_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_norm_backward")

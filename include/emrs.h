@@ -546,6 +546,50 @@ typedef struct emrs_adamw {
 
 int emrs_adamw_step(const emrs_adamw *adamw, void *stream);
 
+/* What joins a block to the residual stream and the norm before the next block, in one pass.  With n(b) =
+ * b / rms(b) branch_weight (branch_weight == NULL: b), rms(x) = sqrt(mean x^2 + eps):
+ *   stream = residual_scale residual + gate n(branch)       (branch == NULL: the residual's part alone)
+ *   normed = stream / rms(stream) weight                    (of the stream before its rounding)
+ * stream and normed are contiguous; NULL: not wanted.  stream_rms and branch_rms get 1 / rms of every token (NULL:
+ * not wanted).  Backward reads them, the stream that forward wrote (without a branch: the residual, where
+ * residual_scale is 1), and the gradients of stream and normed, either of which may be NULL.  The gradients that it
+ * writes are contiguous, of their input's type; NULL: not wanted.  A gate for each channel is [hidden], one for each
+ * token [tokens][hidden].  Operands, normed and all but the stream's gradients are of `dtype`. */
+#define EMRS_NORM_GATE_NONE 0u
+#define EMRS_NORM_GATE_CHANNEL 1u
+#define EMRS_NORM_GATE_TOKEN 2u
+
+typedef struct emrs_norm {
+  uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16 */
+  uint32_t residual_dtype;        /* of residual, stream and their gradients: dtype or EMRS_FP32 */
+  uint32_t gate_kind;
+  uint32_t reserved;              /* must be 0 */
+  uint64_t tokens;                /* may be 0 */
+  uint64_t hidden;                /* 1 to 16384 */
+  const void *residual;           /* [tokens][hidden], rows *_stride elements apart: forward */
+  uint64_t residual_stride;
+  const void *branch;
+  uint64_t branch_stride;
+  const void *gate;
+  uint64_t gate_stride;           /* of a gate for each token */
+  const void *branch_weight;      /* [hidden] */
+  const void *weight;             /* [hidden] */
+  float residual_scale, eps;
+  void *stream;                   /* written by forward (contiguous), read by backward */
+  uint64_t stream_stride;         /* backward */
+  void *normed;
+  float *stream_rms, *branch_rms;
+  const void *grad_stream, *grad_normed;
+  void *grad_residual, *grad_branch, *grad_gate, *grad_weight, *grad_branch_weight;
+  void *workspace;                /* 256-byte aligned: backward with a gradient that sums over tokens */
+  uint64_t workspace_bytes;
+} emrs_norm;
+
+/* Bytes of workspace that emrs_norm_backward wants. */
+int emrs_norm_workspace(const emrs_norm *norm, uint64_t *bytes);
+int emrs_norm_forward(const emrs_norm *norm, void *stream);
+int emrs_norm_backward(const emrs_norm *norm, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
