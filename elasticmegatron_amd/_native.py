@@ -44,7 +44,8 @@ EXPORTS = (
     "emrs_set_tuning", "emrs_synth_fill", "emrs_synth_verify", "emrs_plan_compare", "emrs_xor_checksum",
     "emrs_plan_compare_static", "emrs_plan_prepare", "emrs_ipc_export", "emrs_ipc_open", "emrs_ipc_close",
     "emrs_ipc_open_count", "emrs_loss_workspace", "emrs_loss_forward", "emrs_loss_backward", "emrs_muon_workspace",
-    "emrs_muon_step", "emrs_adamw_step",
+    "emrs_muon_step", "emrs_adamw_step", "emrs_norm_workspace", "emrs_norm_forward", "emrs_norm_backward",
+    "emrs_experts_workspace", "emrs_experts_forward", "emrs_experts_backward",
 )
 
 # struct emrs_compare_stats
@@ -217,8 +218,11 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.emrs_muon_workspace.argtypes = [ctypes.POINTER(Muon), ctypes.POINTER(U64)]
     lib.emrs_norm_workspace.restype = I
     lib.emrs_norm_workspace.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(U64)]
+    lib.emrs_experts_workspace.restype = I
+    lib.emrs_experts_workspace.argtypes = [ctypes.POINTER(Experts), I, ctypes.POINTER(U64)]
     for fn, record in ((lib.emrs_loss_forward, Loss), (lib.emrs_loss_backward, Loss), (lib.emrs_muon_step, Muon),
-                       (lib.emrs_adamw_step, AdamW), (lib.emrs_norm_forward, Norm), (lib.emrs_norm_backward, Norm)):
+                       (lib.emrs_adamw_step, AdamW), (lib.emrs_norm_forward, Norm), (lib.emrs_norm_backward, Norm),
+                       (lib.emrs_experts_forward, Experts), (lib.emrs_experts_backward, Experts)):
         fn.restype = I
         fn.argtypes = [ctypes.POINTER(record), P]
     if lib.emrs_abi_version() != 8:
@@ -467,3 +471,18 @@ def norm_forward(a: Norm, stream: int = 0) -> None:
 
 def norm_backward(a: Norm, stream: int = 0) -> None:
     _check(load().emrs_norm_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_norm_backward")
+
+
+def experts_workspace(a: Experts, backward: bool) -> int:
+    """emrs_experts_workspace: bytes of workspace that the call wants, 0 for none."""
+    n = ctypes.c_uint64()
+    _check(load().emrs_experts_workspace(ctypes.byref(a), 1 if backward else 0, ctypes.byref(n)), "emrs_experts_workspace")
+    return int(n.value)
+
+
+def experts_forward(a: Experts, stream: int = 0) -> None:
+    _check(load().emrs_experts_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_experts_forward")
+
+
+def experts_backward(a: Experts, stream: int = 0) -> None:
+    _check(load().emrs_experts_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_experts_backward")

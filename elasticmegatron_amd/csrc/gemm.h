@@ -103,6 +103,7 @@ __host__ inline int64_t tile_count(const Product &p) {
 
 struct Where {
   int m0, n0, batch;
+  int first;  // where place() found the tile's rows: the first of them
 };
 
 // What an epilogue is beside its run(): where the operands of a matrix of the batch begin.
@@ -115,6 +116,18 @@ struct Operand {
   __device__ __forceinline__ const void *operand_b(const Product &p, int batch) const {
     return static_cast<const char *>(p.b) + batch * p.b_batch * 2;
   }
+};
+
+// What an epilogue may have besides.  kColumnsOfK: operand b is [k][n].  kPlaced: place() finds the workgroup's tile
+// and may narrow the product to a part of it (rows of n, or k), or says that there is none; rows of k then come from
+// rows_from() and columns_from() by that tile.
+template <class E, class = void>
+struct Extras {
+  static constexpr bool kColumnsOfK = false, kPlaced = false;
+};
+template <class E>
+struct Extras<E, std::void_t<decltype(E::kPlaced)>> {
+  static constexpr bool kColumnsOfK = E::kColumnsOfK, kPlaced = E::kPlaced;
 };
 
 // The row that holds place t of a triangle, whose row i holds i + 1.
@@ -201,21 +214,21 @@ struct Loader {
   }
 };
 
-// The same of an operand a that is [k][m]: a stage is 64 of its rows, BM long each, 16-byte units permuted by
-// the row so that the transposing reads of 32 lanes, eight rows of 32 bytes, meet in different banks.  Rows
-// that do not count are past the end of their buffer.
-template <class T, class Cfg>
+// The same of an operand that is [k][m] or [k][n]: a stage is 64 of its rows, B (a tile's m or n) long each, 16-byte
+// units permuted by the row so that the transposing reads of 32 lanes, eight rows of 32 bytes, meet in different
+// banks.  Rows that do not count are past the end of their buffer.
+template <class T, int B, int WAVES>
 struct RowLoader {
-  static constexpr int kUnits = Cfg::BM / 8, kRows = 64 / kUnits;  // of a row; of one load
+  static constexpr int kUnits = B / 8, kRows = 64 / kUnits;  // of a row; of one load
   int voffset, columns, stride;
   const T *first;  // the stage's first row, at the tile's first m
   int rows;        // that count from there on
   static __device__ __forceinline__ int permuted(int row) {
-    return Cfg::BM == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : (row & 3) | (row >> 3 & 1) << 2;
+    return B == 64 ? (row >> 1 & 1) | (row >> 3 & 1) << 1 : (row & 3) | (row >> 3 & 1) << 2;
   }
   __device__ __forceinline__ void init(int64_t row_stride, int columns_here, int wave, int lane) {
-    static_assert(Cfg::BM == 256 || Cfg::BM == 128 || Cfg::BM == 64, "whole rows in a load");
-    static_assert(Cfg::WAVES * kRows % 16 == 0, "a wave's loads are permuted alike");
+    static_assert(B == 256 || B == 128 || B == 64, "whole rows in a load");
+    static_assert(WAVES * kRows % 16 == 0, "a wave's loads are permuted alike");
     const int row = lane / kUnits, unit = lane % kUnits;
     stride = (int)row_stride, columns = columns_here;
     voffset = (int)(row * stride * 2) + ((unit ^ permuted(wave * kRows + row) << 1) << 4);
@@ -224,10 +237,10 @@ struct RowLoader {
   __device__ __forceinline__ void load(char *lds, int j, int, bool none, int wave) const {
     // No branches: the loads are started between matrix instructions.  (columns <= stride.)  The median is a
     // vector instruction; a buffer that might differ between lanes would cost the load a loop.
-    const int from = (wave + j * Cfg::WAVES) * kRows, here = __builtin_amdgcn_readfirstlane(none ? 0 : min(max(rows - from, 0), kRows));
+    const int from = (wave + j * WAVES) * kRows, here = __builtin_amdgcn_readfirstlane(none ? 0 : min(max(rows - from, 0), kRows));
     const int bytes = max(0, (here - 1) * stride + columns) * 2;
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(first + from * stride), 0, bytes, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * Cfg::WAVES) * 1024), 16,
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (wave + j * WAVES) * 1024), 16,
                                              voffset, 0, 0, 0);
   }
 };
@@ -244,11 +257,11 @@ __device__ __forceinline__ void arrive() {
 }
 
 // The loads of one stage, to be started one by one.
-template <class T, class Cfg, class LoaderA>
+template <class Cfg, class LoaderA, class LoaderB>
 struct Loads {
   static constexpr int kCount = Cfg::A_LOADS + Cfg::B_LOADS;
   const LoaderA &loader_a;
-  const Loader<T, Cfg::B_LOADS, Cfg::WAVES> &loader_b;
+  const LoaderB &loader_b;
   char *a, *b;
   int a_k, b_k;
   bool none;
@@ -336,7 +349,13 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   __shared__ __attribute__((aligned(1024))) char a_odds[Cfg::GROUPS][Cfg::BM * 128];
   __shared__ __attribute__((aligned(1024))) char b_evens[Cfg::GROUPS][Cfg::BN * 128];
   __shared__ __attribute__((aligned(1024))) char b_odds[Cfg::GROUPS][Cfg::BN * 128];
-  const Where w = tile_of<Cfg>(p);
+  constexpr bool rows_of_k = Epilogue::kRowsOfK, columns_of_k = Extras<Epilogue>::kColumnsOfK;
+  Where w;
+  if constexpr (Extras<Epilogue>::kPlaced) {
+    if (!epilogue.template place<Cfg>(p, w)) return;
+  } else {
+    w = tile_of<Cfg>(p);
+  }
   const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = Cfg::GROUPS > 1 ? all / Cfg::WAVES : 0, wave = Cfg::GROUPS > 1 ? all % Cfg::WAVES : all;
   char *const a_even = a_evens[group], *const a_odd = a_odds[group], *const b_even = b_evens[group], *const b_odd = b_odds[group];
@@ -344,15 +363,17 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
 
   const int k = p.k_end ? min(p.k, max(0, p.k_end - w.batch * p.k)) : p.k;
   auto columns = [&](int wrap) { return k <= wrap ? k : max(wrap, k - wrap); };
-  constexpr bool rows_of_k = Epilogue::kRowsOfK;
-  typename std::conditional<rows_of_k, RowLoader<T, Cfg>, Loader<T, Cfg::A_LOADS, Cfg::WAVES>>::type la;
-  using NextLoads = Loads<T, Cfg, decltype(la)>;
-  Loader<T, Cfg::B_LOADS, Cfg::WAVES> lb;
+  typename std::conditional<rows_of_k, RowLoader<T, Cfg::BM, Cfg::WAVES>, Loader<T, Cfg::A_LOADS, Cfg::WAVES>>::type la;
+  typename std::conditional<columns_of_k, RowLoader<T, Cfg::BN, Cfg::WAVES>, Loader<T, Cfg::B_LOADS, Cfg::WAVES>>::type lb;
+  using NextLoads = Loads<Cfg, decltype(la), decltype(lb)>;
   if constexpr (rows_of_k)
     la.init(p.a_stride, min(Cfg::BM, ((p.m + 7) & ~7) - w.m0), wave, lane);
   else
     la.init(static_cast<const T *>(epilogue.operand_a(p, w.batch)) + w.m0 * p.a_stride, p.a_stride, min(Cfg::BM, p.m - w.m0), columns(p.a_wrap), wave, lane);
-  lb.init(static_cast<const T *>(epilogue.operand_b(p, w.batch)) + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
+  if constexpr (columns_of_k)
+    lb.init(p.b_stride, min(Cfg::BN, ((p.n + 7) & ~7) - w.n0), wave, lane);
+  else
+    lb.init(static_cast<const T *>(epilogue.operand_b(p, w.batch)) + w.n0 * p.b_stride, p.b_stride, min(Cfg::BN, p.n - w.n0), columns(p.b_wrap), wave, lane);
   // Stages of a group; those past the last k are zeros.
   const int total = ((p.k + kStage - 1) / kStage + Cfg::GROUPS - 1) / Cfg::GROUPS;
   int k0 = group * total * kStage;
@@ -363,8 +384,15 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
     const bool none = k0 >= k_to;
     const int from = none ? 0 : k0;  // a scalar offset past a buffer's end is not to be relied on
     if constexpr (rows_of_k) {
-      epilogue.rows_from(p, w.batch * p.k + from, la.first, la.rows);
+      if constexpr (Extras<Epilogue>::kPlaced)
+        epilogue.rows_from(p, w, from, la.first, la.rows);
+      else
+        epilogue.rows_from(p, w.batch * p.k + from, la.first, la.rows);
       la.first += w.m0;
+    }
+    if constexpr (columns_of_k) {
+      epilogue.columns_from(p, w, from, lb.first, lb.rows);
+      lb.first += w.n0;
     }
     const NextLoads n{la, lb, a, b, from >= p.a_wrap ? from - p.a_wrap : from, from >= p.b_wrap ? from - p.b_wrap : from, none, wave};
     k0 += kStage;
@@ -389,14 +417,18 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
   // The first of the wave's 32-byte pieces of its rows of k; piece i lies where i is added to it before the
   // permutation, and both are exclusive ors: the wave's first piece is a multiple of MI.
   const int a_k = c * 8 + (row >> 2);
-  int a_piece = rows_of_k ? a_k * Cfg::BM * 2 + ((wm * Cfg::MI) ^ RowLoader<T, Cfg>::permuted(a_k)) * 32 + (row & 3) * 8 : 0;
+  int a_piece = rows_of_k ? a_k * Cfg::BM * 2 + ((wm * Cfg::MI) ^ RowLoader<T, rows_of_k ? Cfg::BM : 64, Cfg::WAVES>::permuted(a_k)) * 32 + (row & 3) * 8 : 0;
+  int b_piece = columns_of_k ? a_k * Cfg::BN * 2 + ((wn * Cfg::NI) ^ RowLoader<T, columns_of_k ? Cfg::BN : 64, Cfg::WAVES>::permuted(a_k)) * 32 + (row & 3) * 8 : 0;
   struct Fragments {
     x8 a[Cfg::MI], b[Cfg::NI];
   } even, odd;  // of the first and the second 32 k of a stage
   auto read_one = [&](Fragments &f, const char *a, const char *b, int kk, int r) __attribute__((always_inline)) {
-    if (r < Cfg::NI)
-      f.b[r] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + r * 2048);
-    else if constexpr (rows_of_k)
+    if (r < Cfg::NI) {
+      if constexpr (columns_of_k)
+        f.b[r] = along_k<x8>(b + (b_piece ^ r << 5) + kk * 64 * Cfg::BN, 8 * Cfg::BN);
+      else
+        f.b[r] = *reinterpret_cast<const x8 *>(b + b_at + unit[kk] + r * 2048);
+    } else if constexpr (rows_of_k)
       f.a[r - Cfg::NI] = along_k<x8>(a + (a_piece ^ (r - Cfg::NI) << 5) + kk * 64 * Cfg::BM, 8 * Cfg::BM);
     else
       f.a[r - Cfg::NI] = *reinterpret_cast<const x8 *>(a + a_at + unit[kk] + (r - Cfg::NI) * 2048);
@@ -408,6 +440,7 @@ __global__ __launch_bounds__(Cfg::THREADS) void product_kernel(Product p, Epilog
     constexpr int products = Cfg::MI * Cfg::NI, reads = Cfg::MI + Cfg::NI, loads = decltype(start)::kCount;
     constexpr int per = products * 3 / 4 / reads > 0 ? products * 3 / 4 / reads : 1;
     if constexpr (rows_of_k) asm("" : "+v"(a_piece));  // its MI exclusive ors are taken again: registers
+    if constexpr (columns_of_k) asm("" : "+v"(b_piece));
 #pragma unroll
     for (int q = 0; q < products; ++q) {
       acc[q / Cfg::NI][q % Cfg::NI] = mfma(now.a[q / Cfg::NI], now.b[q % Cfg::NI], acc[q / Cfg::NI][q % Cfg::NI]);

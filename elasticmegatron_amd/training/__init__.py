@@ -6,6 +6,7 @@ main / exp_avg / exp_avg_sq.
 
   rms_norm                  the norm before a block
   residual_norm             a block's output into the residual stream, and the norm behind it
+  expert_linear             products of tokens with their experts' matrices
   linear_cross_entropy      loss of every token from hidden states and vocabulary shards, with its gradient
   vocab_statistics          one process's part of that loss, where its shards are on several
   merge_vocab_statistics    the whole loss's statistics from every process's part
@@ -16,14 +17,16 @@ main / exp_avg / exp_avg_sq.
 
 Kernels run on the current stream of the tensors' device, as torch's own operators do; outputs and
 workspaces come from torch's caching allocator.  There is no fallback: without a GPU and the built
-library every call raises.  The loss and the layers' operators have reverse-mode derivatives, once; nothing has forward-mode ones, and tensors
-that carry a tangent are refused.  What an update writes counts as changed in place.
+library every call raises.  The loss and the layers' operators have reverse-mode derivatives, once; nothing
+has forward-mode ones, and tensors that carry a tangent are refused.  What an update writes counts as changed
+in place.
 """
 
 from .adamw import adamw_step
+from .experts import expert_linear
 from .loss import linear_cross_entropy, merge_vocab_statistics, vocab_gradients, vocab_statistics
 from .muon import MUON_COEFFICIENTS, muon_step, orthogonalise
 from .norm import residual_norm, rms_norm
 
-__all__ = ["rms_norm", "residual_norm", "linear_cross_entropy", "vocab_statistics", "merge_vocab_statistics", "vocab_gradients", "orthogonalise",
-           "muon_step", "adamw_step", "MUON_COEFFICIENTS"]
+__all__ = ["rms_norm", "residual_norm", "expert_linear", "linear_cross_entropy", "vocab_statistics", "merge_vocab_statistics",
+           "vocab_gradients", "orthogonalise", "muon_step", "adamw_step", "MUON_COEFFICIENTS"]

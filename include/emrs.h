@@ -590,6 +590,39 @@ int emrs_norm_workspace(const emrs_norm *norm, uint64_t *bytes);
 int emrs_norm_forward(const emrs_norm *norm, void *stream);
 int emrs_norm_backward(const emrs_norm *norm, void *stream);
 
+/* Products of every row with its expert's weight matrix.  Rows lie by expert: the first counts[0] rows are expert
+ * 0's, and so on.  The counts are on the device; those below 0 count as 0, and rows end at `rows`.  Rows behind the
+ * last expert's belong to none: their y and grad_x are zeros.
+ *   y[t] = W[e] x[t]
+ *   grad_x[t] = W[e]^T grad_y[t],  grad_weights[e] = sum_t grad_y[t] x[t]^T  (zeros where e has no rows) */
+typedef struct emrs_experts {
+  uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16 */
+  uint32_t n_experts;             /* 1 to EMRS_EXPERTS_MAX */
+  uint64_t rows;                  /* may be 0 */
+  uint64_t n_in, n_out;           /* 1 to 2^20 */
+  const void *counts;             /* [n_experts], on the device */
+  uint32_t counts_bytes;          /* of a count: 4 or 8 */
+  uint32_t reserved;              /* must be 0 */
+  const void *x;                  /* [rows][n_in], rows x_stride elements apart (at most 2^21) */
+  uint64_t x_stride;
+  const void *const *weights;     /* per expert [n_out][n_in], rows weight_stride elements apart */
+  uint64_t weight_stride;
+  void *y;                        /* [rows][n_out], contiguous: forward */
+  const void *grad_y;             /* [rows][n_out]: backward */
+  uint64_t grad_y_stride;
+  void *grad_x;                   /* [rows][n_in], contiguous; NULL: not wanted */
+  void *const *grad_weights;      /* per expert, contiguous; NULL: not wanted */
+  void *workspace;                /* 256-byte aligned: copies of operands whose rows lie off 16 bytes */
+  uint64_t workspace_bytes;
+} emrs_experts;
+
+#define EMRS_EXPERTS_MAX 256u
+
+/* Bytes of workspace that emrs_experts_forward (backward = 0) or emrs_experts_backward (1) wants; may be 0. */
+int emrs_experts_workspace(const emrs_experts *experts, int backward, uint64_t *bytes);
+int emrs_experts_forward(const emrs_experts *experts, void *stream);
+int emrs_experts_backward(const emrs_experts *experts, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
