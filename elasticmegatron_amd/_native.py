@@ -46,6 +46,7 @@ EXPORTS = (
     "emrs_ipc_open_count", "emrs_loss_workspace", "emrs_loss_forward", "emrs_loss_backward", "emrs_muon_workspace",
     "emrs_muon_step", "emrs_adamw_step", "emrs_norm_workspace", "emrs_norm_forward", "emrs_norm_backward",
     "emrs_experts_workspace", "emrs_experts_forward", "emrs_experts_backward",
+    "emrs_attention_workspace", "emrs_attention_forward", "emrs_attention_backward",
 )
 
 # struct emrs_compare_stats
@@ -218,11 +219,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.emrs_muon_workspace.argtypes = [ctypes.POINTER(Muon), ctypes.POINTER(U64)]
     lib.emrs_norm_workspace.restype = I
     lib.emrs_norm_workspace.argtypes = [ctypes.POINTER(Norm), ctypes.POINTER(U64)]
+    lib.emrs_attention_workspace.restype = I
+    lib.emrs_attention_workspace.argtypes = [ctypes.POINTER(Attention), I, ctypes.POINTER(U64)]
     lib.emrs_experts_workspace.restype = I
     lib.emrs_experts_workspace.argtypes = [ctypes.POINTER(Experts), I, ctypes.POINTER(U64)]
     for fn, record in ((lib.emrs_loss_forward, Loss), (lib.emrs_loss_backward, Loss), (lib.emrs_muon_step, Muon),
                        (lib.emrs_adamw_step, AdamW), (lib.emrs_norm_forward, Norm), (lib.emrs_norm_backward, Norm),
-                       (lib.emrs_experts_forward, Experts), (lib.emrs_experts_backward, Experts)):
+                       (lib.emrs_experts_forward, Experts), (lib.emrs_experts_backward, Experts),
+                       (lib.emrs_attention_forward, Attention), (lib.emrs_attention_backward, Attention)):
         fn.restype = I
         fn.argtypes = [ctypes.POINTER(record), P]
     if lib.emrs_abi_version() != 8:
@@ -486,3 +490,18 @@ def experts_forward(a: Experts, stream: int = 0) -> None:
 
 def experts_backward(a: Experts, stream: int = 0) -> None:
     _check(load().emrs_experts_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_experts_backward")
+
+
+def attention_workspace(a: Attention, backward: bool) -> int:
+    """emrs_attention_workspace: bytes of workspace that the call wants, 0 for none."""
+    n = ctypes.c_uint64()
+    _check(load().emrs_attention_workspace(ctypes.byref(a), 1 if backward else 0, ctypes.byref(n)), "emrs_attention_workspace")
+    return int(n.value)
+
+
+def attention_forward(a: Attention, stream: int = 0) -> None:
+    _check(load().emrs_attention_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_attention_forward")
+
+
+def attention_backward(a: Attention, stream: int = 0) -> None:
+    _check(load().emrs_attention_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_attention_backward")

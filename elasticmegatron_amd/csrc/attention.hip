@@ -1,0 +1,979 @@
+// Attention within documents, and its gradients, which compute the probabilities again.
+//
+// For every query i of a document with n queries and m keys (causal: i sees the keys j <= i + m - n):
+//   s_ij = scale q_i . k_j,  lse_i = log sum_j exp(s_ij),  p_ij = exp(s_ij - lse_i),  out_i = sum_j p_ij v_j
+//   delta_i = grad_out_i . out_i,  d_ij = p_ij (grad_out_i . v_j - delta_i)
+//   grad_q_i = scale sum_j d_ij k_j,  grad_k_j = scale sum_i d_ij q_i,  grad_v_j = sum_i p_ij grad_out_i
+// where keys of a head get the sums over all query heads that share it.  Nothing of size queries x keys is written.
+//
+// All three kernels are one scheme.  A wave owns 32 rows of one side (queries; for grad_k and grad_v keys), whose
+// operands and sums stay in its registers, and the workgroup walks the other side in tiles that buffer loads put into
+// LDS, the next one while this one is worked on.  The product with the tile's rows as m and the wave's as n (32x32x16)
+// leaves each lane with 16 values of its own row: softmax sums need one exchange with the other half of the wave, and
+// the values, rounded to 16 bits, are where the next product wants its operand b, if that product's k (the tile's
+// rows) is taken in the order 0..3, 8..11 | 4..7, 12..15 of each 16.  Operand a, the tile's columns, comes through
+// transposing LDS reads in the same order.  So probabilities never leave registers.
+//
+// Statistics and sums are in 32 bits; p and d are rounded to the operands' type, as the matrix instructions take
+// them.  fp16 holds p and d scaled by powers of two (p by 2^7 or 2^15, d by what its largest possible value allows),
+// so that only what is 2^-29 of the largest or less loses bits.  No result passes through atomics but the largest
+// entries that choose that scale: the same call gives the same bits.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <type_traits>
+
+#include "emrs.h"
+#include "gemm.h"
+#include "internal.h"
+
+namespace {
+
+using emrs_gemm::arrive;
+using emrs_gemm::kXcds;
+using emrs_internal::fail;
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+constexpr int kWaves = 4, kThreads = kWaves * 64;
+constexpr int kOwn = 32 * kWaves;  // rows of a workgroup's own side
+constexpr int kTile = 64;          // rows of the other side in LDS
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ inline f32x16 mfma(emrs_gemm::bf16x8 a, emrs_gemm::bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ inline f32x16 mfma(emrs_gemm::fp16x8 a, emrs_gemm::fp16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ int lane_of() { return threadIdx.x & 63; }
+// The row, among a product's 32, of a lane's value r.
+__device__ __forceinline__ int row_of(int r) { return (r >> 2) * 8 + (lane_of() >> 5) * 4 + (r & 3); }
+
+// ---- documents ----
+
+// Where documents begin and end in one side's rows.  Segment 0 are the rows before the first document, segment i the
+// i-th document, the last one the rows behind all documents; those of no document see nothing.
+struct Bounds {
+  const void *offsets;  // [documents + 1]; NULL: documents of equal length
+  int32_t bytes, documents, rows, each;
+
+  __device__ __forceinline__ int at(int i) const {  // i <= documents
+    if (!offsets) return i * each;
+    if (bytes == 8) return (int)min(max(static_cast<const int64_t *>(offsets)[i], (int64_t)0), (int64_t)rows);
+    return min(max(static_cast<const int32_t *>(offsets)[i], 0), rows);
+  }
+};
+
+struct Span {
+  int first, end;
+};
+
+// This lane's segment of a run of 64: ends that never go back, and tiles up to and with it.
+struct Walk {
+  int first, end, tiles, end_before, tiles_before;
+
+  __device__ __forceinline__ void begin() { end_before = tiles_before = 0; }
+  __device__ __forceinline__ void step(const Bounds &b, int from) {
+    const int e = from + lane_of();
+    end = e <= b.documents ? b.at(e) : b.rows;
+    end = max(end, end_before);
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int before = __shfl_up(end, o);
+      if (lane_of() >= o) end = max(end, before);
+    }
+    const int below = __shfl_up(end, 1);
+    first = lane_of() ? below : end_before;
+    tiles = (end - first + kOwn - 1) / kOwn;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+      const int before = __shfl_up(tiles, o);
+      if (lane_of() >= o) tiles += before;
+    }
+    tiles += tiles_before;
+    end_before = __builtin_amdgcn_readlane(end, 63);
+    tiles_before = __builtin_amdgcn_readlane(tiles, 63);
+  }
+};
+
+// Segment `segment` of a side, a document.
+__device__ __forceinline__ Span span_of(const Bounds &b, int segment) {
+  if (!b.offsets) return {b.at(segment - 1), b.at(segment)};
+  Walk walk;
+  walk.begin();
+  for (int from = 0; from <= segment; from += 64) walk.step(b, from);
+  const int lane = segment & 63;
+  return {__builtin_amdgcn_readlane(walk.first, lane), __builtin_amdgcn_readlane(walk.end, lane)};
+}
+
+struct Place {
+  Span own, other;  // the document's rows on both sides
+  int row;          // the workgroup's first row, from the document's first
+  int head, split;
+};
+
+// The workgroup's rows, head and share of the other side; false: there are none for it.  Each XCD gets a run of
+// consecutive places, heads that share keys one after the other: whole heads where they divide by the XCDs.  Within
+// it the last rows come first, whose causal work is the longest (grad_k: the first).
+template <bool kLastFirst>
+__device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, int heads, int splits, Place &at) {
+  const int segments = own.documents + 2;
+  Walk walk;
+  walk.begin();
+  for (int from = 0; from < segments; from += 64) walk.step(own, from);
+  const uint32_t tiles = (uint32_t)walk.tiles_before, total = tiles * heads * splits;
+  const uint32_t q = total / kXcds, r = total % kXcds, x = blockIdx.x % kXcds, nth = blockIdx.x / kXcds;
+  if (nth >= q + (x < r ? 1 : 0)) return false;
+  uint32_t t = x * q + min(x, r) + nth;
+  const uint32_t chunk = (heads % kXcds ? 1 : heads / kXcds) * splits, each = chunk * tiles;
+  const uint32_t first_head = t / each * chunk;
+  t -= t / each * each;
+  uint32_t tile = t / chunk;
+  const uint32_t unit = first_head + t % chunk;
+  at.head = unit / splits, at.split = unit % splits;
+  if (kLastFirst) tile = tiles - 1 - tile;
+  if (segments > 64) walk.begin();
+  for (int from = 0;; from += 64) {
+    if (segments > 64) walk.step(own, from);
+    const uint64_t past = __ballot(tile < (uint32_t)walk.tiles);
+    if (!past) continue;  // never of the last 64: tile < tiles
+    const int lane = __builtin_ctzll(past), segment = from + lane;
+    at.own.first = __builtin_amdgcn_readlane(walk.first, lane);
+    at.own.end = __builtin_amdgcn_readlane(walk.end, lane);
+    const int rows = at.own.end - at.own.first;
+    at.row = ((int)tile - __builtin_amdgcn_readlane(walk.tiles, lane) + (rows + kOwn - 1) / kOwn) * kOwn;
+    if (segment > 0 && segment <= own.documents) {
+      at.other = own.offsets == other.offsets && own.offsets && own.rows == other.rows ? at.own : span_of(other, segment);
+    } else {
+      at.other.first = at.other.end = 0;
+    }
+    return true;
+  }
+}
+
+// ---- tiles ----
+
+// A tile's rows in LDS: DIM 16-bit elements each, in units of 16 bytes that are permuted by the row.  Both kinds of
+// reads then meet 16 different units of the 64 banks: 16 rows at one unit (a product's operand of rows), and four rows
+// at four units (one of columns).
+template <int DIM>
+__device__ __forceinline__ int permuted(int row) {
+  return DIM == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
+}
+
+// What a lane loads of every tile of an operand: 16 bytes of every (kWaves x 1 KB)-th row.
+template <class T, int DIM>
+struct TileLoader {
+  static constexpr int kUnits = DIM / 8, kRows = 64 / kUnits, kLoads = kTile / (kRows * kWaves);
+  int offset, step, stride, dim;
+  __device__ __forceinline__ void init(int64_t row_stride, int dim_, int wave) {
+    const int row = wave * kRows + lane_of() / kUnits, unit = lane_of() % kUnits ^ permuted<DIM>(row);
+    static_assert(kRows * kWaves % 16 == 0, "a lane's rows are permuted alike");
+    stride = (int)row_stride * 2, dim = dim_ * 2, step = kRows * kWaves * stride;
+    offset = unit * 8 < dim_ ? row * stride + unit * 16 : (int)0x80000000;  // past the end: zeros
+  }
+  // `rows` rows from `first` on (more than a tile's: a tile's; less: zeros behind them; none: zeros).
+  __device__ __forceinline__ void load(char *lds, const T *first, int rows, int wave) const {
+    rows = min(rows, kTile);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(first), 0, rows > 0 ? (rows - 1) * stride + dim : 0, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (j * kWaves + wave) * 1024), 16,
+                                               offset < 0 ? offset : offset + j * step, 0, 0, 0);
+  }
+};
+
+// A lane's places in a tile for the reads of both kinds.
+template <class T, int DIM>
+struct TileReader {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  static constexpr int kRow = DIM * 2;
+  int by_rows, by_columns;
+  __device__ __forceinline__ void init() {
+    const int lane = lane_of(), row = lane & 31, half = lane >> 5, t = lane & 15;
+    by_rows = row * kRow + ((half ^ permuted<DIM>(row)) << 4);
+    const int four = half * 4 + (t >> 2);  // the row of the first four; those of the second four are 8 further
+    by_columns = four * kRow + ((((lane >> 4 & 1) * 2 + (t >> 1 & 1)) ^ permuted<DIM>(four)) << 4) + (t & 1) * 8;
+  }
+  // Rows block * 32 .. + 31 as operand a, 16 of their elements from 16 c on.
+  __device__ __forceinline__ x8 rows(const char *tile, int block, int c) const {
+    return *reinterpret_cast<const x8 *>(tile + (by_rows ^ c << 5) + block * 32 * kRow);
+  }
+  // Columns 32 d .. + 31 as operand a: 16 rows from 16 c on, in the order in which a lane holds its values.
+  __device__ __forceinline__ x8 columns(const char *tile, int d, int c) const {
+    typedef __attribute__((ext_vector_type(4))) short s16x4;
+    typedef __attribute__((address_space(3))) s16x4 *lds4;
+    char *const at = const_cast<char *>(tile) + c * 16 * kRow;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + (by_columns ^ d << 6)));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * kRow + (by_columns ^ d << 6 ^ 32)));
+    return __builtin_bit_cast(x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// A wave's own rows as operand b: row lane % 32, eight elements from 16 c + 8 (lane / 32) on.
+template <class T, int DIM>
+struct OwnRows {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  x8 v[DIM / 16];
+  __device__ __forceinline__ void load(const T *row, bool valid, int dim) {
+#pragma unroll
+    for (int c = 0; c < DIM / 16; ++c) {
+      const int at = c * 16 + (lane_of() >> 5) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = (T)0.f;
+      if (valid && at < dim) v[c] = *reinterpret_cast<const x8 *>(row + at);
+    }
+  }
+};
+
+// Eight of a lane's 16 values, in 16 bits, as operand b of the next product.
+template <class T>
+__device__ __forceinline__ typename emrs_gemm::Vec<T>::x8 eight_of(const f32x16 &v, int half) {
+  typename emrs_gemm::Vec<T>::x8 o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = (T)v[half * 8 + e];
+  return o;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+struct Strides {
+  int64_t row, head;
+};
+
+struct Attention {
+  Bounds queries, keys;
+  const void *q, *k, *v, *grad_out;
+  Strides q_at, k_at, v_at, grad_out_at;
+  int32_t heads, group, dim, real_dim, causal, splits;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
+  float scale;           // of the scores
+  void *out;             // [rows][heads][real_dim]
+  float *lse;            // [heads][rows]
+  float *exponent, *delta;  // the same, backward: lse in units of log 2 (infinity where a query sees nothing), and delta
+  void *grad_q, *grad_k, *grad_v;
+  float *parts, *parts2, *part_lse;  // of every split, where there are several
+  const uint32_t *largest;  // fp16: the largest |grad_out| and |v|, as bits
+};
+
+// A wave's sums, held as [column][row], to rows of the output or of its part.
+template <class T, int DIM>
+__device__ __forceinline__ void store_own(const f32x16 (&acc)[DIM / 32], T *to, float *part, bool valid, int dim, float by) {
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int at = d * 32 + row_of(r);
+      if (!valid) continue;
+      if (part) {
+        if (dim % 4 == 0) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[d][r + e] * by;
+          if (at < dim) *reinterpret_cast<f32x4 *>(part + at) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (at + e < dim) part[at + e] = acc[d][r + e] * by;
+        }
+      } else if (dim % 4 == 0) {
+        typename emrs_gemm::Vec<T>::x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[d][r + e] * by);
+        if (at < dim) *reinterpret_cast<typename emrs_gemm::Vec<T>::x4 *>(to + at) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at + e < dim) to[at + e] = (T)(acc[d][r + e] * by);
+      }
+    }
+}
+
+// A split's run of tiles.
+__device__ __forceinline__ Span share_of(int tiles, int split, int splits) {
+  return {(int)((int64_t)tiles * split / splits), (int)((int64_t)tiles * (split + 1) / splits)};
+}
+
+// ---- forward ----
+
+template <class T, int DIM>
+__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attention p) {
+  constexpr int kBytes = kTile * DIM * 2;
+  __shared__ __attribute__((aligned(1024))) char k_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char k_odd[kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_odd[kBytes];
+  Place at;
+  if (!find<true>(p.queries, p.keys, p.heads, p.splits, at)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
+  const int queries = at.own.end - at.own.first, keys = at.other.end - at.other.first;
+  const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = at.head / p.group;
+  const bool valid = query < queries;
+  const int64_t row = at.own.first + query;
+
+  OwnRows<T, DIM> q;
+  q.load(static_cast<const T *>(p.q) + row * p.q_at.row + at.head * p.q_at.head, valid, p.dim);
+
+  // Keys that the workgroup's, the wave's and the lane's last query sees.
+  const int shift = keys - queries;
+  auto seen_by = [&](int i) { return p.causal ? min(max(min(i, queries - 1) + shift + 1, 0), keys) : keys; };
+  const int seen = seen_by(at.row + kOwn - 1), seen_wave = mine < queries ? seen_by(mine + 31) : 0, seen_lane = seen_by(query), seen_by_all = seen_by(mine);
+  const Span tiles = share_of((seen + kTile - 1) / kTile, at.split, p.splits);
+
+  TileLoader<T, DIM> k_loader, v_loader;
+  k_loader.init(p.k_at.row, p.dim, wave);
+  v_loader.init(p.v_at.row, p.dim, wave);
+  TileReader<T, DIM> reader;
+  reader.init();
+  const T *const k = static_cast<const T *>(p.k) + at.other.first * p.k_at.row + kv_head * p.k_at.head;
+  const T *const v = static_cast<const T *>(p.v) + at.other.first * p.v_at.row + kv_head * p.v_at.head;
+  auto load = [&](char *to_k, char *to_v, int t) __attribute__((always_inline)) {
+    const int rows = t < tiles.end ? keys - t * kTile : 0;
+    const int64_t from = rows > 0 ? t * kTile : 0;
+    k_loader.load(to_k, k + from * p.k_at.row, rows, wave);
+    v_loader.load(to_v, v + from * p.v_at.row, rows, wave);
+  };
+
+  const float by = p.scale * kLog2e;
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  constexpr float kLift = kHalf ? 7.f : 0.f, kSlack = 8.f;  // exponents are kept below kLift + kSlack
+  f32x16 out[DIM / 32];
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) out[d][r] = 0.f;
+  float top = -INFINITY, sum = 0.f;  // top: what exponents are taken off, in units of log 2; sum: this lane's part
+
+  auto work = [&](const char *kt, const char *vt, int t) __attribute__((always_inline)) {
+    const int from = t * kTile;
+    if (from >= seen_wave) return;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c) s[b] = mfma(reader.rows(kt, b, c), q.v[c], s[b]);
+    }
+    if (from + kTile > seen_by_all) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (from + b * 32 + row_of(r) >= seen_lane) s[b][r] = -INFINITY;
+    }
+    float most = s[0][0];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][r]);
+    most = fmaxf(most, other_half(most)) * by;
+    // The sums are brought to a new maximum only where exponents would grow past the slack.
+    if (__any(most > top + kSlack)) {
+      const float next = fmaxf(top, most), less = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+      sum *= less;
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) out[d][r] *= less;
+      top = next;
+    }
+    const float off = (top == -INFINITY ? 0.f : top) - kLift;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], by, -off));
+        sum += s[b][r];
+      }
+#pragma unroll
+    for (int c = 0; c < kTile / 16; ++c) {
+      const auto prob = eight_of<T>(s[c >> 1], c & 1);
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d) out[d] = mfma(reader.columns(vt, d, c), prob, out[d]);
+    }
+  };
+
+  load(k_even, v_even, tiles.first);
+  for (int t = tiles.first; t < tiles.end; t += 2) {
+    arrive();
+    load(k_odd, v_odd, t + 1);
+    work(k_even, v_even, t);
+    if (t + 1 >= tiles.end) break;
+    arrive();
+    load(k_even, v_even, t + 2);
+    work(k_odd, v_odd, t + 1);
+  }
+  arrive();  // no load may still be on its way into LDS that another workgroup gets
+
+  sum += other_half(sum);
+  const float lse = sum == 0.f ? -INFINITY : (top - kLift) * kLn2 + logf(sum);
+  const float norm = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t place = (row * p.heads + at.head) * p.real_dim;
+  if (p.splits > 1) {
+    if (valid && lane < 32) p.part_lse[((int64_t)at.split * p.heads + at.head) * p.queries.rows + row] = lse;
+    store_own<T, DIM>(out, nullptr, p.parts + (int64_t)at.split * p.queries.rows * p.heads * p.real_dim + place, valid, p.real_dim, norm);
+  } else {
+    if (valid && lane < 32 && p.lse) p.lse[(int64_t)at.head * p.queries.rows + row] = lse;
+    store_own<T, DIM>(out, static_cast<T *>(p.out) + place, nullptr, valid, p.real_dim, norm);
+  }
+}
+
+// Joins the splits of one row of one head: 64 lanes of a wave, a row a wave.
+template <class T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const float *parts, const float *part_lse, int splits, int64_t rows, int heads, int dim, T *out,
+                                                             float *lse) {
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // row * heads + head
+  if (unit >= rows * heads) return;
+  const int64_t row = unit / heads, head = unit % heads;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_lse[(s * heads + head) * rows + row]);
+  const float shift = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int s = 0; s < splits; ++s) sum += expf(part_lse[(s * heads + head) * rows + row] - shift);
+  const float norm = sum == 0.f ? 0.f : 1.f / sum;
+  for (int c = lane_of(); c < dim; c += 64) {
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      const float w = expf(part_lse[(s * heads + head) * rows + row] - shift) * norm;
+      if (w != 0.f) v += w * parts[(s * rows * heads + unit) * dim + c];  // NaN is not 0
+    }
+    out[unit * dim + c] = (T)v;
+  }
+  if (lane_of() == 0 && lse) lse[head * rows + row] = sum == 0.f ? -INFINITY : shift + logf(sum);
+}
+
+// Sums of every split's part.
+template <class T>
+__global__ __launch_bounds__(256) void attention_sum_kernel(const float *parts, int splits, int64_t each, T *out) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= each) return;
+  float v = parts[i];
+  for (int s = 1; s < splits; ++s) v += parts[s * each + i];
+  out[i] = (T)v;
+}
+
+// ---- backward ----
+
+// fp16: 2^e that brings the largest possible |d| (2 dim |grad_out| |v| of the largest entries) below 2^15.
+__device__ __forceinline__ float lift_of(const uint32_t *largest, int dim) {
+  const float a = __uint_as_float(largest[0]), b = __uint_as_float(largest[1]);
+  if (!(a > 0.f) || !(b > 0.f)) return 1.f;
+  const int e = 14 - __builtin_amdgcn_frexp_expf(a) - __builtin_amdgcn_frexp_expf(b) - __builtin_amdgcn_frexp_expf((float)dim);
+  return __builtin_amdgcn_ldexpf(1.f, min(max(e, -100), 100));
+}
+
+__global__ void attention_clear_kernel(uint32_t *largest) { largest[threadIdx.x] = 0; }
+
+// The largest finite |entry| of an operand's rows, joined over the workgroups by an unsigned maximum of the bits.
+template <class T>
+__global__ __launch_bounds__(256) void attention_largest_kernel(const T *x, Strides at, int64_t rows, int heads, int dim, uint32_t *largest) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  const int units = dim / 8;
+  float top = 0.f;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * heads * units; u += (int64_t)gridDim.x * 256) {
+    const int64_t row = u / (heads * units);
+    const int rest = (int)(u % (heads * units));
+    const x8 v = *reinterpret_cast<const x8 *>(x + row * at.row + rest / units * at.head + rest % units * 8);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf((float)v[e]);
+      top = a < INFINITY ? fmaxf(top, a) : top;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane_of() == 0 && top > 0.f) atomicMax(largest, __float_as_uint(top));
+}
+
+// grad_q, and on the way delta and the exponent (split 0 leaves them for grad_k).
+template <class T, int DIM>
+__global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention p) {
+  constexpr int kBytes = kTile * DIM * 2;
+  __shared__ __attribute__((aligned(1024))) char k_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char k_odd[kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_odd[kBytes];
+  Place at;
+  if (!find<true>(p.queries, p.keys, p.heads, p.splits, at)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
+  const int queries = at.own.end - at.own.first, keys = at.other.end - at.other.first;
+  const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = at.head / p.group;
+  const bool valid = query < queries;
+  const int64_t row = at.own.first + query, place = (row * p.heads + at.head) * p.real_dim;
+
+  OwnRows<T, DIM> q, g;
+  q.load(static_cast<const T *>(p.q) + row * p.q_at.row + at.head * p.q_at.head, valid, p.dim);
+  g.load(static_cast<const T *>(p.grad_out) + row * p.grad_out_at.row + at.head * p.grad_out_at.head, valid, p.dim);
+  float delta = 0.f, lse = INFINITY;
+  if (valid) {
+    const T *const out = static_cast<const T *>(p.out) + place;
+#pragma unroll
+    for (int c = 0; c < DIM / 16; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = c * 16 + (lane >> 5) * 8 + e;
+        if (d < p.real_dim) delta = fmaf((float)g.v[c][e], (float)out[d], delta);
+      }
+    lse = p.lse[(int64_t)at.head * p.queries.rows + row] * kLog2e;
+    if (lse == -INFINITY) lse = INFINITY;  // sees nothing: probabilities of 0
+  }
+  delta += other_half(delta);
+  if (valid && lane < 32 && at.split == 0) {
+    p.exponent[(int64_t)at.head * p.queries.rows + row] = lse;
+    p.delta[(int64_t)at.head * p.queries.rows + row] = delta;
+  }
+
+  const int shift = keys - queries;
+  auto seen_by = [&](int i) { return p.causal ? min(max(min(i, queries - 1) + shift + 1, 0), keys) : keys; };
+  const int seen = seen_by(at.row + kOwn - 1), seen_wave = mine < queries ? seen_by(mine + 31) : 0, seen_lane = seen_by(query), seen_by_all = seen_by(mine);
+  const Span tiles = share_of((seen + kTile - 1) / kTile, at.split, p.splits);
+
+  TileLoader<T, DIM> k_loader, v_loader;
+  k_loader.init(p.k_at.row, p.dim, wave);
+  v_loader.init(p.v_at.row, p.dim, wave);
+  TileReader<T, DIM> reader;
+  reader.init();
+  const T *const k = static_cast<const T *>(p.k) + at.other.first * p.k_at.row + kv_head * p.k_at.head;
+  const T *const v = static_cast<const T *>(p.v) + at.other.first * p.v_at.row + kv_head * p.v_at.head;
+  auto load = [&](char *to_k, char *to_v, int t) __attribute__((always_inline)) {
+    const int rows = t < tiles.end ? keys - t * kTile : 0;
+    const int64_t from = rows > 0 ? t * kTile : 0;
+    k_loader.load(to_k, k + from * p.k_at.row, rows, wave);
+    v_loader.load(to_v, v + from * p.v_at.row, rows, wave);
+  };
+  const float by = p.scale * kLog2e;
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  const float lift = kHalf ? lift_of(p.largest, p.real_dim) : 1.f;
+
+  f32x16 acc[DIM / 32];
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+
+  auto work = [&](const char *kt, const char *vt, int t) __attribute__((always_inline)) {
+    const int from = t * kTile;
+    if (from >= seen_wave) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c) {
+        s = mfma(reader.rows(kt, b, c), q.v[c], s);
+        dp = mfma(reader.rows(vt, b, c), g.v[c], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float d = __builtin_amdgcn_exp2f(fmaf(s[r], by, -lse)) * (dp[r] - delta);
+        if (kHalf) d *= lift;
+        s[r] = d;
+      }
+      if (from + kTile > seen_by_all) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (from + b * 32 + row_of(r) >= seen_lane) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const auto ds = eight_of<T>(s, c);
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) acc[d] = mfma(reader.columns(kt, d, b * 2 + c), ds, acc[d]);
+      }
+    }
+  };
+
+  load(k_even, v_even, tiles.first);
+  for (int t = tiles.first; t < tiles.end; t += 2) {
+    arrive();
+    load(k_odd, v_odd, t + 1);
+    work(k_even, v_even, t);
+    if (t + 1 >= tiles.end) break;
+    arrive();
+    load(k_even, v_even, t + 2);
+    work(k_odd, v_odd, t + 1);
+  }
+  arrive();
+  if (!p.grad_q && !p.parts) return;
+  store_own<T, DIM>(acc, static_cast<T *>(p.grad_q) + place,
+                    p.splits > 1 ? p.parts + (int64_t)at.split * p.queries.rows * p.heads * p.real_dim + place : nullptr, valid, p.real_dim, p.scale / lift);
+}
+
+// grad_k and grad_v of one head of keys: the sums over the queries of every head that shares it, or, with splits, of
+// a run of these heads.
+template <class T, int DIM>
+__global__ __launch_bounds__(kThreads, 1) void attention_grad_kv_kernel(Attention p) {
+  constexpr int kBytes = kTile * DIM * 2;
+  __shared__ __attribute__((aligned(1024))) char q_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char q_odd[kBytes];
+  __shared__ __attribute__((aligned(1024))) char g_even[kBytes];
+  __shared__ __attribute__((aligned(1024))) char g_odd[kBytes];
+  __shared__ __attribute__((aligned(256))) float sums_even[2][kTile];  // exponent and delta of the tile's queries
+  __shared__ __attribute__((aligned(256))) float sums_odd[2][kTile];
+  const int kv_heads = p.heads / p.group;
+  Place at;
+  if (!find<false>(p.keys, p.queries, kv_heads, p.splits, at)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
+  const int keys = at.own.end - at.own.first, queries = at.other.end - at.other.first;
+  const int mine = at.row + wave * 32, key = mine + (lane & 31);
+  const bool valid = key < keys;
+  const int64_t row = at.own.first + key;
+
+  OwnRows<T, DIM> k, v;
+  k.load(static_cast<const T *>(p.k) + row * p.k_at.row + at.head * p.k_at.head, valid, p.dim);
+  v.load(static_cast<const T *>(p.v) + row * p.v_at.row + at.head * p.v_at.head, valid, p.dim);
+
+  // The first query that sees the workgroup's, the wave's and the lane's key, and the one from which on all of the
+  // wave's are seen.
+  const int shift = keys - queries;
+  auto first_for = [&](int j) { return p.causal ? min(max(j - shift, 0), queries) : 0; };
+  const int first = first_for(at.row), first_wave = mine < keys ? first_for(mine) : queries, first_lane = first_for(key), all_from = first_for(mine + 31);
+  const int from_tile = first / kTile, tiles = (queries + kTile - 1) / kTile - from_tile;  // of a head
+  const Span heads = share_of(p.group, at.split, p.splits);
+  const int total = max(tiles, 0) * (heads.end - heads.first);
+
+  TileLoader<T, DIM> q_loader, g_loader;
+  q_loader.init(p.q_at.row, p.dim, wave);
+  g_loader.init(p.grad_out_at.row, p.dim, wave);
+  TileReader<T, DIM> reader;
+  reader.init();
+  const T *const q = static_cast<const T *>(p.q) + at.other.first * p.q_at.row;
+  const T *const g = static_cast<const T *>(p.grad_out) + at.other.first * p.grad_out_at.row;
+  const int first_head = at.head * p.group + heads.first;
+  auto load = [&](char *to_q, char *to_g, float (*sums)[kTile], int n) __attribute__((always_inline)) {
+    const int t = n < total ? n % tiles + from_tile : 0, head = first_head + (n < total ? n / tiles : 0);
+    const int rows = n < total ? queries - t * kTile : 0;
+    const int64_t from = t * kTile;
+    q_loader.load(to_q, q + from * p.q_at.row + head * p.q_at.head, rows, wave);
+    g_loader.load(to_g, g + from * p.grad_out_at.row + head * p.grad_out_at.head, rows, wave);
+    if (wave < 2) {  // zeros where there is no query: its operands are zeros
+      const float *const of = (wave ? p.delta : p.exponent) + (int64_t)head * p.queries.rows + at.other.first + from;
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(of), 0, max(0, min(rows, kTile)) * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)sums[wave], 4, lane * 4, 0, 0, 0);
+    }
+  };
+  const float by = p.scale * kLog2e;
+  constexpr bool kHalf = std::is_same<T, _Float16>::value;
+  const float lift = kHalf ? lift_of(p.largest, p.real_dim) : 1.f;
+
+  f32x16 grad_k[DIM / 32], grad_v[DIM / 32];
+#pragma unroll
+  for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) grad_k[d][r] = grad_v[d][r] = 0.f;
+
+  auto work = [&](const char *qt, const char *gt, const float (*sums)[kTile], int n) __attribute__((always_inline)) {
+    const int from = (n % tiles + from_tile) * kTile;
+    if (from + kTile <= first_wave) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c) {
+        s = mfma(reader.rows(qt, b, c), k.v[c], s);
+        dp = mfma(reader.rows(gt, b, c), v.v[c], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 lse = *reinterpret_cast<const f32x4 *>(&sums[0][b * 32 + row_of(i * 4)]);
+        const f32x4 delta = *reinterpret_cast<const f32x4 *>(&sums[1][b * 32 + row_of(i * 4)]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -lse[e]));
+          float d = x * (dp[i * 4 + e] - delta[e]);
+          if (kHalf) d *= lift;
+          s[i * 4 + e] = kHalf ? x * 32768.f : x;
+          dp[i * 4 + e] = d;
+        }
+      }
+      if (from < all_from || !__all(valid)) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (from + b * 32 + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const auto prob = eight_of<T>(s, c), ds = eight_of<T>(dp, c);
+#pragma unroll
+        for (int d = 0; d < DIM / 32; ++d) {
+          grad_v[d] = mfma(reader.columns(gt, d, b * 2 + c), prob, grad_v[d]);
+          grad_k[d] = mfma(reader.columns(qt, d, b * 2 + c), ds, grad_k[d]);
+        }
+      }
+    }
+  };
+
+  load(q_even, g_even, sums_even, 0);
+  for (int n = 0; n < total; n += 2) {
+    arrive();
+    load(q_odd, g_odd, sums_odd, n + 1);
+    work(q_even, g_even, sums_even, n);
+    if (n + 1 >= total) break;
+    arrive();
+    load(q_even, g_even, sums_even, n + 2);
+    work(q_odd, g_odd, sums_odd, n + 1);
+  }
+  arrive();
+  const int64_t place = (row * kv_heads + at.head) * p.real_dim, each = (int64_t)p.keys.rows * kv_heads * p.real_dim;
+  const bool split = p.splits > 1;
+  store_own<T, DIM>(grad_k, static_cast<T *>(p.grad_k) + place, split ? p.parts + at.split * each + place : nullptr, valid, p.real_dim, p.scale / lift);
+  store_own<T, DIM>(grad_v, static_cast<T *>(p.grad_v) + place, split ? p.parts2 + at.split * each + place : nullptr, valid, p.real_dim,
+                    kHalf ? 1.f / 32768.f : 1.f);
+}
+
+// Rows as operands want them: on 16 bytes, with zeros up to the next multiple of eight.
+template <class T>
+__global__ __launch_bounds__(256) void attention_pad_kernel(const T *from, Strides at, int64_t rows, int heads, int dim, int padded, T *to) {
+  typedef __attribute__((ext_vector_type(8))) T x8;
+  const int units = padded / 8;
+  const int64_t all = rows * heads * units;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < all; u += (int64_t)gridDim.x * 256) {
+    const int64_t row = u / (heads * units);
+    const int rest = (int)(u % (heads * units)), c = rest % units * 8;
+    const T *const in = from + row * at.row + rest / units * at.head;
+    x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = c + e < dim ? in[c + e] : (T)0.f;
+    reinterpret_cast<x8 *>(to)[u] = v;
+  }
+}
+
+// ---- calls ----
+
+uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+bool on(const void *p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// Workgroups that a launch ought to have: two for each CU, twice over, so that their ends even out.
+constexpr uint64_t kWanted = 1024;
+
+// Splits of the keys that queries walk: as many as fill the card, with four tiles for each at the least.
+uint32_t key_splits(const emrs_attention *a) {
+  const uint64_t units = std::max<uint64_t>(1, (a->rows + kOwn - 1) / kOwn) * a->heads, each = a->key_rows / std::max<uint64_t>(1, a->documents);
+  if (units * 2 > kWanted) return 1;
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kWanted / units, each / (4 * kTile), 32}));
+}
+// Of the heads that share a key's.
+uint32_t head_splits(const emrs_attention *a) {
+  const uint32_t group = a->heads / a->kv_heads;
+  const uint64_t units = std::max<uint64_t>(1, (a->key_rows + kOwn - 1) / kOwn) * a->kv_heads;
+  uint32_t splits = 1;
+  while (splits < group && units * splits < kWanted) {
+    do ++splits;
+    while (group % splits);
+  }
+  return splits;
+}
+
+// What lies in the workspace, and where.
+struct Room {
+  bool pad_q, pad_k, pad_v, pad_g;
+  uint64_t q, k, v, g, parts, parts2, part_lse, exponent, delta, largest, bytes;
+};
+
+// Rows that a tile's loads cannot take as they lie: off 16 bytes, too far apart, or (expanded tensors) one over the
+// other, so that what is past the last of them is not past the end of their buffer.
+bool off_units(const emrs_attention *a, const void *p, const uint64_t *strides) {
+  return a->dim % 8 || strides[0] < a->dim || strides[0] % 8 || strides[1] % 8 || !on(p, 16) || strides[0] > (1u << 23);
+}
+
+Room room_of(const emrs_attention *a, bool backward) {
+  Room r{};
+  const uint64_t dim8 = round_up(a->dim, 8), own = a->rows * a->heads, other = a->key_rows * a->kv_heads;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  r.pad_q = off_units(a, a->q, a->q_strides), r.pad_k = off_units(a, a->k, a->k_strides), r.pad_v = off_units(a, a->v, a->v_strides);
+  r.pad_g = backward && off_units(a, a->grad_out, a->grad_out_strides);
+  if (r.pad_q) r.q = take(own * dim8 * 2);
+  if (r.pad_k) r.k = take(other * dim8 * 2);
+  if (r.pad_v) r.v = take(other * dim8 * 2);
+  if (r.pad_g) r.g = take(own * dim8 * 2);
+  if (backward) {
+    r.exponent = take(own * 4);
+    r.delta = take(own * 4);
+    r.largest = take(8);
+  }
+  const uint64_t keys = key_splits(a), heads = backward ? head_splits(a) : 1;
+  // grad_q's parts are summed before grad_k's and grad_v's are written.
+  const uint64_t parts = std::max(keys > 1 ? keys * own * a->dim * 4 : 0, heads > 1 ? heads * other * a->dim * 4 : 0);
+  r.parts = take(parts);
+  if (heads > 1) r.parts2 = take(heads * other * a->dim * 4);
+  if (!backward && keys > 1) r.part_lse = take(keys * own * 4);
+  r.bytes = at;
+  return r;
+}
+
+int check_sizes(const emrs_attention *a) {
+  if (!a) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL argument");
+  if (a->dtype != EMRS_BF16 && a->dtype != EMRS_FP16) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: operands are bf16 or fp16");
+  if (a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: heads are a multiple of kv_heads");
+  if (a->heads > 4096) return fail(EMRS_ERR_TOO_LARGE, "attention: at most 4096 heads");
+  if (a->dim < 1 || a->dim > EMRS_ATTENTION_MAX_DIM) return fail(EMRS_ERR_TOO_LARGE, "attention: heads of 1 to 128 elements");
+  if (a->documents < 1 || a->documents > (1u << 20)) return fail(EMRS_ERR_TOO_LARGE, "attention: 1 to 2^20 documents");
+  if (a->rows > (1u << 28) || a->key_rows > (1u << 28)) return fail(EMRS_ERR_TOO_LARGE, "attention: at most 2^28 rows");
+  const uint64_t heads = (uint64_t)a->heads * 32;
+  if ((a->rows / kOwn + a->documents + 2) * heads > 0x3fffffffull || (a->key_rows / kOwn + a->documents + 2) * heads > 0x3fffffffull)
+    return fail(EMRS_ERR_TOO_LARGE, "attention: too many tiles for one launch");
+  return EMRS_OK;
+}
+
+uint32_t grid_of(uint64_t rows, uint64_t documents, uint64_t heads, uint64_t splits) {
+  return (uint32_t)(std::min(rows, rows / kOwn + documents + 2) * heads * splits);
+}
+
+template <class T>
+const T *pad(const void *from, const uint64_t *strides, uint64_t rows, uint32_t heads, uint32_t dim, char *to, Strides &at, hipStream_t st) {
+  const uint32_t dim8 = (uint32_t)round_up(dim, 8);
+  const uint64_t units = rows * heads * (dim8 / 8);
+  if (units)
+    attention_pad_kernel<T><<<(uint32_t)std::min<uint64_t>((units + 255) / 256, 8192), 256, 0, st>>>(
+        static_cast<const T *>(from), Strides{(int64_t)strides[0], (int64_t)strides[1]}, (int64_t)rows, (int)heads, (int)dim, (int)dim8, reinterpret_cast<T *>(to));
+  at = {(int64_t)heads * dim8, (int64_t)dim8};
+  return reinterpret_cast<const T *>(to);
+}
+
+template <class T>
+void sum_parts(const float *parts, uint32_t splits, uint64_t each, void *out, hipStream_t st) {
+  if (each) attention_sum_kernel<T><<<(uint32_t)((each + 255) / 256), 256, 0, st>>>(parts, (int)splits, (int64_t)each, static_cast<T *>(out));
+}
+
+template <class T, int DIM>
+int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
+  const Room room = room_of(a, backward);
+  char *const w = static_cast<char *>(a->workspace);
+  const uint32_t dim8 = (uint32_t)round_up(a->dim, 8);
+  Attention p{};
+  const bool uniform = !a->offsets;
+  p.queries = {a->offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->rows, uniform ? (int32_t)(a->rows / a->documents) : 0};
+  p.keys = {a->key_offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->key_rows, uniform ? (int32_t)(a->key_rows / a->documents) : 0};
+  auto strides = [](const uint64_t *s) { return Strides{(int64_t)s[0], (int64_t)s[1]}; };
+  p.q = a->q, p.k = a->k, p.v = a->v, p.grad_out = a->grad_out;
+  p.q_at = strides(a->q_strides), p.k_at = strides(a->k_strides), p.v_at = strides(a->v_strides), p.grad_out_at = strides(a->grad_out_strides);
+  if (room.pad_q) p.q = pad<T>(a->q, a->q_strides, a->rows, a->heads, a->dim, w + room.q, p.q_at, st);
+  if (room.pad_k) p.k = pad<T>(a->k, a->k_strides, a->key_rows, a->kv_heads, a->dim, w + room.k, p.k_at, st);
+  if (room.pad_v) p.v = pad<T>(a->v, a->v_strides, a->key_rows, a->kv_heads, a->dim, w + room.v, p.v_at, st);
+  if (room.pad_g) p.grad_out = pad<T>(a->grad_out, a->grad_out_strides, a->rows, a->heads, a->dim, w + room.g, p.grad_out_at, st);
+  p.heads = (int32_t)a->heads, p.group = (int32_t)(a->heads / a->kv_heads), p.dim = (int32_t)dim8, p.real_dim = (int32_t)a->dim, p.causal = a->causal != 0;
+  p.scale = a->scale, p.out = a->out, p.lse = a->lse;
+  p.splits = (int32_t)key_splits(a);
+  p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
+  if (!backward) {
+    if (a->rows == 0) return EMRS_OK;
+    p.part_lse = reinterpret_cast<float *>(w + room.part_lse);
+    attention_forward_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
+    if (p.splits > 1)
+      attention_join_kernel<T><<<(uint32_t)((a->rows * a->heads + 3) / 4), 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,
+                                                                                        (int)a->dim, static_cast<T *>(a->out), a->lse);
+  } else {
+    p.exponent = reinterpret_cast<float *>(w + room.exponent);
+    p.delta = reinterpret_cast<float *>(w + room.delta);
+    if (std::is_same<T, _Float16>::value && a->rows && a->key_rows) {
+      uint32_t *const largest = reinterpret_cast<uint32_t *>(w + room.largest);
+      attention_clear_kernel<<<1, 2, 0, st>>>(largest);
+      auto grid = [&](uint64_t n) { return (uint32_t)std::min<uint64_t>((n * (dim8 / 8) + 255) / 256, 1024); };
+      attention_largest_kernel<T><<<grid(a->rows * a->heads), 256, 0, st>>>(static_cast<const T *>(p.grad_out), p.grad_out_at, (int64_t)a->rows, (int)a->heads,
+                                                                           (int)dim8, largest);
+      attention_largest_kernel<T><<<grid(a->key_rows * a->kv_heads), 256, 0, st>>>(static_cast<const T *>(p.v), p.v_at, (int64_t)a->key_rows, (int)a->kv_heads,
+                                                                                  (int)dim8, largest + 1);
+      p.largest = largest;
+    }
+    // delta and exponent come out of grad_q's kernel, so that it runs in any case.
+    p.grad_q = a->grad_q;
+    if (!a->grad_q && p.splits > 1) p.splits = 1, p.parts = nullptr;
+    if (a->rows) {
+      attention_grad_q_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
+      if (p.splits > 1) sum_parts<T>(p.parts, p.splits, a->rows * a->heads * a->dim, a->grad_q, st);
+    }
+    if (a->grad_k && a->key_rows) {
+      p.grad_k = a->grad_k, p.grad_v = a->grad_v;
+      p.splits = (int32_t)head_splits(a);
+      p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
+      p.parts2 = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts2) : nullptr;
+      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
+      if (p.splits > 1) {
+        sum_parts<T>(p.parts, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_k, st);
+        sum_parts<T>(p.parts2, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_v, st);
+      }
+    }
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? EMRS_OK : fail(EMRS_ERR_HIP, std::string("attention: ") + hipGetErrorString(e));
+}
+
+int run(const emrs_attention *a, bool backward, hipStream_t st) {
+  int rc = check_sizes(a);
+  if (rc) return rc;
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: the scale is positive and finite");
+  if (!a->offsets != !a->key_offsets) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: offsets of both sides, or of none");
+  if (a->offsets) {
+    if (a->offset_bytes != 4 && a->offset_bytes != 8) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: offsets are of 4 or 8 bytes");
+    if (!on(a->offsets, a->offset_bytes) || !on(a->key_offsets, a->offset_bytes))
+      return fail(EMRS_ERR_MISALIGNED, "attention: offsets off their type's alignment");
+  } else if (a->rows % a->documents || a->key_rows % a->documents) {
+    return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: documents of equal length do not fill the rows");
+  }
+  auto operand = [&](const void *p, uint64_t rows, const uint64_t *strides) {
+    if (!rows) return EMRS_OK;
+    if (!p) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL operand");
+    if (!on(p, 2)) return fail(EMRS_ERR_MISALIGNED, "attention: an operand off its type's alignment");
+    if (strides[0] > (1ull << 40) || strides[1] > (1ull << 40)) return fail(EMRS_ERR_TOO_LARGE, "attention: strides are at most 2^40");
+    return (int)EMRS_OK;
+  };
+  if ((rc = operand(a->q, a->rows, a->q_strides)) || (rc = operand(a->k, a->key_rows, a->k_strides)) || (rc = operand(a->v, a->key_rows, a->v_strides)))
+    return rc;
+  if (a->rows && !a->out) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL out");
+  if (!on(a->out, 8) || !on(a->lse, 4)) return fail(EMRS_ERR_MISALIGNED, "attention: out is off 8 bytes");
+  if (backward) {
+    if ((rc = operand(a->grad_out, a->rows, a->grad_out_strides))) return rc;
+    if (a->rows && !a->lse) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL lse");
+    if (!a->grad_q && !a->grad_k) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: no gradient is wanted");
+    if (!a->grad_k != !a->grad_v) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: grad_k and grad_v come together");
+    if (!on(a->grad_q, 8) || !on(a->grad_k, 8) || !on(a->grad_v, 8)) return fail(EMRS_ERR_MISALIGNED, "attention: a gradient is off 8 bytes");
+  }
+  const uint64_t wanted = room_of(a, backward).bytes;
+  if (wanted) {
+    if (!a->workspace || a->workspace_bytes < wanted) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: the workspace is too small");
+    if (!on(a->workspace, 256)) return fail(EMRS_ERR_MISALIGNED, "attention: the workspace is off 256 bytes");
+  }
+  if (!a->rows && (!backward || !a->grad_k || !a->key_rows)) return EMRS_OK;
+  rc = emrs_internal::need_device();
+  if (rc) return rc;
+  if (a->dtype == EMRS_BF16) return a->dim <= 64 ? run_as<__bf16, 64>(a, backward, st) : run_as<__bf16, 128>(a, backward, st);
+  return a->dim <= 64 ? run_as<_Float16, 64>(a, backward, st) : run_as<_Float16, 128>(a, backward, st);
+}
+
+}  // namespace
+
+extern "C" int emrs_attention_workspace(const emrs_attention *a, int backward, uint64_t *bytes) {
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    if (!bytes) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL argument");
+    const int rc = check_sizes(a);
+    if (rc) return rc;
+    *bytes = room_of(a, backward != 0).bytes;
+    return EMRS_OK;
+  });
+}
+
+extern "C" int emrs_attention_forward(const emrs_attention *a, void *stream) {
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    return run(a, false, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int emrs_attention_backward(const emrs_attention *a, void *stream) {
+  return emrs_internal::guarded([&]() -> int {
+    emrs_internal::clear_error();
+    return run(a, true, static_cast<hipStream_t>(stream));
+  });
+}

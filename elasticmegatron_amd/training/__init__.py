@@ -6,6 +6,7 @@ main / exp_avg / exp_avg_sq.
 
   rms_norm                  the norm before a block
   residual_norm             a block's output into the residual stream, and the norm behind it
+  attention                 attention within packed documents
   expert_linear             products of tokens with their experts' matrices
   linear_cross_entropy      loss of every token from hidden states and vocabulary shards, with its gradient
   vocab_statistics          one process's part of that loss, where its shards are on several
@@ -27,6 +28,7 @@ from .experts import expert_linear
 from .loss import linear_cross_entropy, merge_vocab_statistics, vocab_gradients, vocab_statistics
 from .muon import MUON_COEFFICIENTS, muon_step, orthogonalise
 from .norm import residual_norm, rms_norm
+from .packed_attention import attention
 
-__all__ = ["rms_norm", "residual_norm", "expert_linear", "linear_cross_entropy", "vocab_statistics", "merge_vocab_statistics",
-           "vocab_gradients", "orthogonalise", "muon_step", "adamw_step", "MUON_COEFFICIENTS"]
+__all__ = ["rms_norm", "residual_norm", "attention", "expert_linear", "linear_cross_entropy", "vocab_statistics",
+           "merge_vocab_statistics", "vocab_gradients", "orthogonalise", "muon_step", "adamw_step", "MUON_COEFFICIENTS"]

@@ -623,6 +623,43 @@ int emrs_experts_workspace(const emrs_experts *experts, int backward, uint64_t *
 int emrs_experts_forward(const emrs_experts *experts, void *stream);
 int emrs_experts_backward(const emrs_experts *experts, void *stream);
 
+/* Attention within documents.  Document d has the queries offsets[d] .. offsets[d + 1] - 1 and the keys key_offsets[d]
+ * .. key_offsets[d + 1] - 1; query i of n sees all m keys, or (causal) those j <= i + m - n, so that the last query
+ * sees the last key.  Head h reads the keys and values of head h / (heads / kv_heads).
+ *   s = scale q . k over the keys seen,  lse = log sum exp(s),  out = sum exp(s - lse) v
+ * A query that sees nothing, or belongs to no document, has out 0 and lse -inf.
+ * Backward reads out and lse, and writes the gradients of q, k and v; keys that nothing sees have gradients of 0.
+ * Offsets are on the device; they are held within the rows, and one that goes back counts as the one before. */
+typedef struct emrs_attention {
+  uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16 */
+  uint32_t causal;
+  uint32_t heads, kv_heads;       /* heads a multiple of kv_heads */
+  uint32_t dim;                   /* of a head, 1 to EMRS_ATTENTION_MAX_DIM */
+  uint32_t offset_bytes;          /* of an offset: 4 or 8 */
+  uint64_t rows, key_rows;        /* may be 0 */
+  uint64_t documents;             /* >= 1 */
+  const void *offsets, *key_offsets; /* [documents + 1]; both NULL: documents of equal length that fill the rows */
+  const void *q, *k, *v;          /* [rows][heads][dim], [key_rows][kv_heads][dim], unit stride along dim */
+  uint64_t q_strides[2], k_strides[2], v_strides[2]; /* elements between rows and between heads */
+  float scale;                    /* > 0 */
+  uint32_t reserved;              /* must be 0 */
+  void *out;                      /* [rows][heads][dim], contiguous */
+  float *lse;                     /* [heads][rows]; forward: may be NULL */
+  const void *grad_out;
+  uint64_t grad_out_strides[2];
+  void *grad_q;                   /* contiguous; NULL: not wanted */
+  void *grad_k, *grad_v;          /* contiguous; both NULL: not wanted */
+  void *workspace;                /* 256-byte aligned */
+  uint64_t workspace_bytes;
+} emrs_attention;
+
+#define EMRS_ATTENTION_MAX_DIM 128u
+
+/* Bytes of workspace that emrs_attention_forward (backward = 0) or emrs_attention_backward (1) wants; may be 0. */
+int emrs_attention_workspace(const emrs_attention *attention, int backward, uint64_t *bytes);
+int emrs_attention_forward(const emrs_attention *attention, void *stream);
+int emrs_attention_backward(const emrs_attention *attention, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
