@@ -32,6 +32,8 @@ using emrs_gemm::Where;
 using emrs_internal::fail;
 
 constexpr uint64_t kMaxRows = 1u << 30;
+constexpr uint64_t kCutFrom = 8192;  // k from which on the tiles of a last round are cut along it
+constexpr uint64_t kFew = 2;         // rows up to which weights are read by rows, in vector arithmetic
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
@@ -89,23 +91,36 @@ struct Walk {
   }
 };
 
-// A tile of the experts' rows (n) and of the weights' side m; false: there is none for this workgroup.
+// Tiles that fill no round of 256 workgroups, cut along a long k: `whole` tiles go as they are, and each of the others
+// is as many parts as there are workgroups for, whose sums a second kernel joins.  The same in both kernels.
+struct Cut {
+  uint32_t total, whole, parts;
+};
+constexpr uint32_t kRound = 256, kLeastStages = 16;
+
+__device__ __forceinline__ Cut cut_of(uint32_t total, int k, bool cuts) {
+  const uint32_t rest = total % kRound, stages = (k + emrs_gemm::kStage - 1) / emrs_gemm::kStage;
+  const uint32_t parts = cuts && rest ? min(kRound / rest, stages / kLeastStages) : 1;
+  return parts > 1 ? Cut{total, total - rest, parts} : Cut{total, total, 1};
+}
+
+// Tiles along n of all segments; `walk` is then at the last 64.
 template <class Cfg>
-__device__ __forceinline__ bool find(const Counts &c, const Product &p, Where &w, Segment &s) {
-  const uint32_t tm = (p.m + Cfg::BM - 1) / Cfg::BM;
-  Walk walk;
+__device__ __forceinline__ uint32_t tiles_of(const Counts &c, Walk &walk) {
   walk.begin();
   for (int from = 0; from <= c.experts; from += 64) walk.step<true>(c, from, Cfg::BN);
-  const uint32_t total = (uint32_t)walk.tiles_before * tm;  // checked on the host to fit
-  // Each XCD has a run of consecutive tiles.
-  const uint32_t q = total / kXcds, r = total % kXcds, x = blockIdx.x % kXcds, at = blockIdx.x / kXcds;
-  if (at >= q + (x < r ? 1 : 0)) return false;
-  uint32_t t = x * q + min(x, r) + at;
+  return (uint32_t)walk.tiles_before;
+}
+
+// Tile t of the experts' rows (n) and of the weights' side m.
+template <class Cfg>
+__device__ __forceinline__ void locate(const Counts &c, const Product &p, Walk &walk, uint32_t t, Where &w, Segment &s) {
+  const uint32_t tm = (p.m + Cfg::BM - 1) / Cfg::BM;
   if (c.experts >= 64) walk.begin();  // of more than one 64, find the one
   for (int from = 0;; from += 64) {
     if (c.experts >= 64) walk.step<true>(c, from, Cfg::BN);
     const uint64_t past = __ballot(t < (uint32_t)walk.tiles * tm);
-    if (!past) continue;  // never of the last 64: t < total
+    if (!past) continue;  // never of the last 64: t is less than all tiles
     const int lane = __builtin_ctzll(past);
     s.expert = from + lane;
     s.first = __builtin_amdgcn_readlane(walk.first, lane);
@@ -118,7 +133,30 @@ __device__ __forceinline__ bool find(const Counts &c, const Product &p, Where &w
   const uint32_t in = t - group * kGroup * tn;
   w.m0 = (int)(first + in % rows) * Cfg::BM;
   w.n0 = (int)(in / rows) * Cfg::BN;
-  w.batch = 0;
+  w.first = s.first;
+}
+
+// The workgroup's tile, or its part of one; false: there is none.  Each XCD has a run of consecutive tiles.
+template <class Cfg>
+__device__ __forceinline__ bool find(const Counts &c, Product &p, bool cuts, Where &w, Segment &s) {
+  Walk walk;
+  const uint32_t tm = (p.m + Cfg::BM - 1) / Cfg::BM;
+  const Cut cut = cut_of(tiles_of<Cfg>(c, walk) * tm, p.k, cuts);  // checked on the host to fit
+  const bool whole = blockIdx.x < cut.whole;
+  const uint32_t id = whole ? blockIdx.x : blockIdx.x - cut.whole, units = whole ? cut.whole : (cut.total - cut.whole) * cut.parts;
+  const uint32_t q = units / kXcds, r = units % kXcds, x = id % kXcds, at = id / kXcds;
+  if (at >= q + (x < r ? 1 : 0)) return false;
+  const uint32_t unit = x * q + min(x, r) + at;
+  locate<Cfg>(c, p, walk, whole ? unit : cut.whole + unit / cut.parts, w, s);
+  w.k_from = 0;
+  w.part = -1;
+  if (!whole) {
+    const int stages = (p.k + emrs_gemm::kStage - 1) / emrs_gemm::kStage, part = unit % cut.parts;
+    w.k_from = stages * part / (int)cut.parts * emrs_gemm::kStage;
+    w.part = unit;
+    p.k = min(p.k, stages * (part + 1) / (int)cut.parts * emrs_gemm::kStage) - w.k_from;
+  }
+  if (s.expert == c.experts) p.k = 0;  // zeros
   return true;
 }
 
@@ -173,30 +211,130 @@ struct OfTokens {
   Counts counts;
   int32_t wide, n_out;    // n_out: rows of a weight
   T *out;                 // [rows][m]
+  float *parts;           // [part][BN][BM], where tiles may be cut along k; NULL: they are not
 
   template <class Cfg>
   __device__ __forceinline__ bool place(Product &p, Where &w) const {
     Segment s;
-    if (!find<Cfg>(counts, p, w, s)) return false;
+    if (!find<Cfg>(counts, p, parts != nullptr, w, s)) return false;
     p.n = s.end - s.first;
-    p.b = static_cast<const T *>(p.b) + s.first * p.b_stride;
-    if (s.expert == counts.experts) p.k = 0;  // zeros
+    p.b = static_cast<const T *>(p.b) + s.first * p.b_stride + w.k_from;
     w.batch = min(s.expert, counts.experts - 1);
-    w.first = s.first;
+    p.a = static_cast<const T *>(weights.p[w.batch]) + w.k_from * (kTransposed ? p.a_stride : 1);
     return true;
   }
-  __device__ __forceinline__ const void *operand_a(const Product &, int expert) const { return weights.p[expert]; }
+  __device__ __forceinline__ const void *operand_a(const Product &p, int) const { return p.a; }
   __device__ __forceinline__ const void *operand_b(const Product &p, int) const { return p.b; }
   template <class U>
   __device__ __forceinline__ void rows_from(const Product &p, const Where &w, int k, const U *&first, int &count) const {
-    first = static_cast<const U *>(weights.p[w.batch]) + k * p.a_stride;
-    count = n_out - k;
+    first = static_cast<const U *>(p.a) + k * p.a_stride;
+    count = n_out - w.k_from - k;
   }
   template <class Cfg>
   __device__ __forceinline__ void run(f32x4 (&acc)[Cfg::MI][Cfg::NI], const Where &w, int m0, int n0, int, int lane, const Product &p, char *own) const {
-    store_rows<T, Cfg>(acc, out + (int64_t)w.first * p.m, p.m, wide, m0, n0, lane, p, own);
+    if (w.part < 0) return store_rows<T, Cfg>(acc, out + (int64_t)w.first * p.m, p.m, wide, m0, n0, lane, p, own);
+    float *const to = parts + (int64_t)w.part * (Cfg::BN * Cfg::BM);
+#pragma unroll
+    for (int j = 0; j < Cfg::NI; ++j)
+#pragma unroll
+      for (int i = 0; i < Cfg::MI; ++i) {
+        const int n = n0 - w.n0 + j * 16 + (lane & 15), m = m0 - w.m0 + i * 16 + (lane >> 4) * 4;
+        *reinterpret_cast<f32x4 *>(to + n * Cfg::BM + m) = acc[i][j];
+      }
   }
 };
+
+// Joins the parts of the tiles that were cut: 32 of a tile's rows to a workgroup, in the order of k.
+constexpr int kJoinRows = 32;
+
+template <class T, class Cfg>
+__global__ __launch_bounds__(256) void join_tiles_kernel(Product p, Counts counts, const float *parts, T *out) {
+  constexpr int each = Cfg::BN / kJoinRows;
+  Walk walk;
+  const uint32_t tm = (p.m + Cfg::BM - 1) / Cfg::BM;
+  const Cut cut = cut_of(tiles_of<Cfg>(counts, walk) * tm, p.k, true);
+  const uint32_t nth = blockIdx.x / each;
+  if (nth >= cut.total - cut.whole) return;
+  Where w;
+  Segment s;
+  locate<Cfg>(counts, p, walk, cut.whole + nth, w, s);
+  static_assert(Cfg::BM == 256, "a row of a tile is four elements of each lane of a wave");
+  const int m = (threadIdx.x & 63) * 4, n0 = blockIdx.x % each * kJoinRows + (threadIdx.x >> 6) * (kJoinRows / 4);
+  const float *const from = parts + (int64_t)nth * cut.parts * (Cfg::BN * Cfg::BM) + m;
+#pragma unroll 1
+  for (int n = n0; n < n0 + kJoinRows / 4 && w.n0 + n < s.end - s.first; ++n) {
+    f32x4 v = *reinterpret_cast<const f32x4 *>(from + n * Cfg::BM);
+#pragma unroll 4
+    for (uint32_t i = 1; i < cut.parts; ++i) v += *reinterpret_cast<const f32x4 *>(from + (int64_t)i * (Cfg::BN * Cfg::BM) + n * Cfg::BM);
+    T *const to = out + (int64_t)(s.first + w.n0 + n) * p.m + w.m0 + m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (w.m0 + m + e < p.m) to[e] = (T)v[e];
+  }
+}
+
+// Few rows: a token's experts are read once, in vector arithmetic.  A wave takes four of a weight's rows, each in whole
+// consecutive kilobytes and many of them on their way at a time, for up to two of the expert's rows.
+constexpr int kFewRows = 2, kFewWeights = 4, kFewWaves = 4;
+
+template <class T>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(Table weights, int64_t weight_stride, Counts counts, const T *x, int64_t x_stride, int k,
+                                                                  int n_out, T *y) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
+  Walk walk;
+  walk.begin();
+  Segment s{};
+  int at = 0;
+  bool found = false;
+  for (int from = 0; from <= counts.experts && !found; from += 64) {
+    walk.step<true>(counts, from, kFewRows);
+    const uint64_t past = __ballot((int)blockIdx.y < walk.tiles);
+    if (!past) continue;
+    const int lane = __builtin_ctzll(past);
+    s = {from + lane, __builtin_amdgcn_readlane(walk.first, lane), __builtin_amdgcn_readlane(walk.end, lane)};
+    at = s.first + ((int)blockIdx.y - __builtin_amdgcn_readlane(walk.tiles, lane) + (s.end - s.first + kFewRows - 1) / kFewRows) * kFewRows;
+    found = true;
+  }
+  const int m0 = ((int)blockIdx.x * kFewWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kFewWeights, lane = lane_of();
+  if (!found || m0 >= n_out) return;
+  const int count = min(kFewRows, s.end - at);
+  const T *const w = static_cast<const T *>(weights.p[min(s.expert, counts.experts - 1)]);
+  const T *const row = x + at * x_stride, *const second = row + (count > 1 ? x_stride : 0);
+  float acc[kFewRows][kFewWeights];
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+    for (int i = 0; i < kFewWeights; ++i) acc[r][i] = 0.f;
+  if (s.expert < counts.experts)
+#pragma unroll 4
+    for (int c = lane * 8; c < k; c += 64 * 8) {
+      x8 a[kFewWeights];  // rows past the last one read it again, and are left out below
+#pragma unroll
+      for (int i = 0; i < kFewWeights; ++i) a[i] = __builtin_nontemporal_load(reinterpret_cast<const x8 *>(w + min(m0 + i, n_out - 1) * weight_stride + c));
+      const x8 b = *reinterpret_cast<const x8 *>(row + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int i = 0; i < kFewWeights; ++i) acc[0][i] = fmaf((float)a[i][e], (float)b[e], acc[0][i]);
+      if (count > 1) {
+        const x8 d = *reinterpret_cast<const x8 *>(second + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int i = 0; i < kFewWeights; ++i) acc[1][i] = fmaf((float)a[i][e], (float)d[e], acc[1][i]);
+      }
+    }
+#pragma unroll
+  for (int r = 0; r < kFewRows; ++r)
+#pragma unroll
+    for (int i = 0; i < kFewWeights; ++i) {
+      if (r >= count) continue;
+      float v = acc[r][i];
+#pragma unroll
+      for (int o = 32; o; o /= 2) v += __shfl_xor(v, o);
+      if (lane == 0 && m0 + i < n_out) y[(int64_t)(at + r) * n_out + m0 + i] = (T)v;
+    }
+}
 
 // grad_W: both operands are rows of k.
 template <class T>
@@ -208,7 +346,15 @@ struct OfWeights {
 
   template <class Cfg>
   __device__ __forceinline__ bool place(Product &p, Where &w) const {
-    w = emrs_gemm::tile_of<Cfg>(p);
+    // One expert after the other, each over all XCDs: how long a tile takes is its expert's rows.
+    const uint32_t tm = (p.m + Cfg::BM - 1) / Cfg::BM, tn = (p.n + Cfg::BN - 1) / Cfg::BN, each = (tm * tn + kXcds - 1) / kXcds;
+    const uint32_t t = blockIdx.x % kXcds * each + blockIdx.x / kXcds % each;
+    if (t >= tm * tn) return false;
+    w.batch = blockIdx.x / (each * kXcds);
+    const uint32_t group = t / (kGroup * tn), first = group * kGroup, rows = min((uint32_t)kGroup, tm - first);
+    const uint32_t in = t - group * kGroup * tn;
+    w.m0 = (int)(first + in % rows) * Cfg::BM;
+    w.n0 = (int)(in / rows) * Cfg::BN;
     const Segment s = rows_of(counts, w.batch);
     p.k = s.end - s.first;
     p.a = static_cast<const T *>(p.a) + s.first * p.a_stride;
@@ -251,10 +397,14 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(Table from, int64_t strid
 
 bool on(const void *p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// Of the three inputs, which have to be copied, and where in the workspace the copies lie.
+// Whether a product over k may cut the tiles of its last round, and the room that their parts take.
+bool may_cut(uint64_t k, uint64_t rows) { return k >= kCutFrom && rows >= emrs_gemm::Large::BN; }
+constexpr uint64_t kPartsBytes = (uint64_t)kRound * emrs_gemm::Large::BN * emrs_gemm::Large::BM * 4;
+
+// Of the three inputs, which have to be copied, and where in the workspace the copies and the tiles' parts lie.
 struct Copies {
-  bool x, weights, grad_y;
-  uint64_t at_weights, at_grad_y, bytes;
+  bool x, weights, grad_y, cuts;
+  uint64_t at_weights, at_grad_y, at_parts, bytes;
 };
 
 Copies copies_of(const emrs_experts *a, bool backward) {
@@ -267,7 +417,9 @@ Copies copies_of(const emrs_experts *a, bool backward) {
   c.grad_y = backward && (a->n_out % 8 || a->grad_y_stride % 8 || !on(a->grad_y, 16));
   c.at_weights = c.x ? round_up(a->rows * in8 * 2, 256) : 0;
   c.at_grad_y = c.at_weights + (c.weights ? round_up((uint64_t)a->n_experts * a->n_out * in8 * 2, 256) : 0);
-  c.bytes = c.at_grad_y + (c.grad_y ? a->rows * out8 * 2 : 0);
+  c.cuts = (!backward && may_cut(a->n_in, a->rows)) || (backward && a->grad_x && may_cut(a->n_out, a->rows));
+  c.at_parts = c.at_grad_y + (c.grad_y ? round_up(a->rows * out8 * 2, 256) : 0);
+  c.bytes = c.at_parts + (c.cuts ? kPartsBytes : 0);
   return c;
 }
 
@@ -289,17 +441,21 @@ double tiles_expected(const Product &p, uint64_t rows, uint64_t experts) {
 }
 
 template <class Cfg>
-double cost_of(double tiles, double k, double stage, double fixed) {
-  const double rounds = std::max(1.0, tiles / 256), stages = std::ceil(std::ceil(k / emrs_gemm::kStage) / Cfg::GROUPS);
-  return (rounds < 4 ? std::ceil(rounds) : rounds) * (fixed + stage * stages);
+double cost_of(double tiles, double k, double stage, double fixed, bool cuts = false) {
+  const double rounds = std::max(1.0, tiles / kRound), stages = std::ceil(std::ceil(k / emrs_gemm::kStage) / Cfg::GROUPS);
+  return (rounds < 4 && !cuts ? std::ceil(rounds) : rounds) * (fixed + stage * stages) + (cuts ? 40 : 0);
 }
 
-template <class T, class Cfg, class Epilogue>
-int launch_tokens(const Product &p, const Epilogue &e, uint64_t rows, uint64_t experts, hipStream_t st) {
+template <class Cfg, class T, bool kTransposed>
+int launch_tokens(const Product &p, OfTokens<T, kTransposed> e, uint64_t rows, uint64_t experts, hipStream_t st) {
   // Every segment, that of the rows of none among them, may have one tile that is not full.
   const uint64_t tiles = std::min(rows, rows / Cfg::BN + experts + 1) * (uint64_t)emrs_gemm::tiles_of(p.m, Cfg::BM);
   if (tiles > 0x3fffffff) return fail(EMRS_ERR_TOO_LARGE, "experts: too many tiles for one launch");
-  emrs_gemm::product_kernel<T, Cfg><<<(uint32_t)tiles, Cfg::THREADS, 0, st>>>(p, e);
+  constexpr bool cuts = std::is_same<Cfg, emrs_gemm::Large>::value;
+  if (!cuts) e.parts = nullptr;
+  emrs_gemm::product_kernel<T, Cfg><<<(uint32_t)tiles + (e.parts ? kRound : 0), Cfg::THREADS, 0, st>>>(p, e);
+  if constexpr (cuts)
+    if (e.parts) join_tiles_kernel<T, Cfg><<<(kRound - 1) * (Cfg::BN / kJoinRows), 256, 0, st>>>(p, e.counts, e.parts, e.out);
   return EMRS_OK;
 }
 
@@ -307,38 +463,41 @@ template <class T, bool kTransposed>
 int launch(const Product &p, const OfTokens<T, kTransposed> &e, uint64_t rows, uint64_t experts, hipStream_t st) {
   using namespace emrs_gemm;
   const double k = p.k;
-  const double cost[5] = {cost_of<Large>(tiles_expected<Large>(p, rows, experts), k, kTransposed ? 1.7 : 1.25, 8),
-                          cost_of<Broad>(tiles_expected<Broad>(p, rows, experts), k, 1.05, 6),
-                          cost_of<Medium>(tiles_expected<Medium>(p, rows, experts), k, 1.05, 4),
-                          cost_of<Small>(tiles_expected<Small>(p, rows, experts), k, 0.95, 3),
-                          cost_of<Tiny>(tiles_expected<Tiny>(p, rows, experts), k, 0.9, 3)};
+  const double cost[5] = {cost_of<Large>(tiles_expected<Large>(p, rows, experts), k, 1.6, 8, e.parts),
+                          cost_of<Broad>(tiles_expected<Broad>(p, rows, experts), k, 1.2, 6),
+                          cost_of<Medium>(tiles_expected<Medium>(p, rows, experts), k, kTransposed ? 1.5 : 1.35, 4),
+                          cost_of<Small>(tiles_expected<Small>(p, rows, experts), k, kTransposed ? 1.3 : 1.15, 3),
+                          cost_of<Tiny>(tiles_expected<Tiny>(p, rows, experts), k, 1.0, 3)};
   int best = kLarge;
   for (int i = kBroad; i <= kTiny; ++i)
     if (cost[i] < cost[best] && !(kTransposed && (i == kBroad || i == kTiny))) best = i;
-  if (best == kLarge) return launch_tokens<T, Large>(p, e, rows, experts, st);
+  if (best == kLarge) return launch_tokens<Large>(p, e, rows, experts, st);
   if constexpr (!kTransposed) {
-    if (best == kBroad) return launch_tokens<T, Broad>(p, e, rows, experts, st);
-    if (best == kTiny) return launch_tokens<T, Tiny>(p, e, rows, experts, st);
+    if (best == kBroad) return launch_tokens<Broad>(p, e, rows, experts, st);
+    if (best == kTiny) return launch_tokens<Tiny>(p, e, rows, experts, st);
   }
-  if (best == kMedium) return launch_tokens<T, Medium>(p, e, rows, experts, st);
-  return launch_tokens<T, Small>(p, e, rows, experts, st);
+  if (best == kMedium) return launch_tokens<Medium>(p, e, rows, experts, st);
+  return launch_tokens<Small>(p, e, rows, experts, st);
+}
+
+template <class Cfg, class T>
+int launch_weights(const Product &p, const OfWeights<T> &e, hipStream_t st) {
+  const int64_t each = emrs_gemm::tiles_of(emrs_gemm::tiles_of(p.m, Cfg::BM) * emrs_gemm::tiles_of(p.n, Cfg::BN), kXcds) * kXcds;
+  if (each * p.batch > 0x3fffffff) return fail(EMRS_ERR_TOO_LARGE, "experts: too many tiles for one launch");
+  emrs_gemm::product_kernel<T, Cfg><<<(uint32_t)(each * p.batch), Cfg::THREADS, 0, st>>>(p, e);
+  return EMRS_OK;
 }
 
 template <class T>
 int launch(const Product &p, const OfWeights<T> &e, uint64_t rows, hipStream_t st) {
   using namespace emrs_gemm;
   const double k = (double)rows / p.batch;
-  const double cost[3] = {cost_of<Large>((double)tile_count<Large>(p), k, 1.7, 8), cost_of<Medium>((double)tile_count<Medium>(p), k, 1.05, 4),
-                          cost_of<Small>((double)tile_count<Small>(p), k, 0.95, 3)};
+  const double cost[3] = {cost_of<Large>((double)tile_count<Large>(p), k, 1.7, 8), cost_of<Medium>((double)tile_count<Medium>(p), k, 1.8, 4),
+                          cost_of<Small>((double)tile_count<Small>(p), k, 2.1, 3)};
   const int best = (int)(std::min_element(cost, cost + 3) - cost);
-  const int64_t tiles = best == 0 ? tile_count<Large>(p) : best == 1 ? tile_count<Medium>(p) : tile_count<Small>(p);
-  if (tiles > 0x3fffffff) return fail(EMRS_ERR_TOO_LARGE, "experts: too many tiles for one launch");
-  switch (best) {
-    case 0: launch_as<T, Large>(p, e, st); break;
-    case 1: launch_as<T, Medium>(p, e, st); break;
-    default: launch_as<T, Small>(p, e, st);
-  }
-  return EMRS_OK;
+  if (best == 0) return launch_weights<Large>(p, e, st);
+  if (best == 1) return launch_weights<Medium>(p, e, st);
+  return launch_weights<Small>(p, e, st);
 }
 
 template <class T>
@@ -374,15 +533,22 @@ int run_as(const emrs_experts *a, bool backward, hipStream_t st) {
     pad<T>(Table{{grad_y}}, 1, grad_y_stride, a->rows, a->n_out, to, st);
     grad_y = to, grad_y_stride = (int64_t)out8;
   }
+  float *const parts = copies.cuts ? reinterpret_cast<float *>(room + copies.at_parts) : nullptr;
   int rc = EMRS_OK;
   if (!backward && a->rows) {
     const Product p{nullptr, x, weight_stride, x_stride, 0, 0, (int32_t)a->n_out, 0, (int32_t)in8, emrs_gemm::kNoWrap, emrs_gemm::kNoWrap, 0, 1, 0};
-    const OfTokens<T, false> e{weights, counts, a->n_out % 8 == 0 && on(a->y, 16), (int32_t)a->n_out, static_cast<T *>(a->y)};
-    rc = launch<T, false>(p, e, a->rows, a->n_experts, st);
+    const OfTokens<T, false> e{weights, counts, a->n_out % 8 == 0 && on(a->y, 16), (int32_t)a->n_out, static_cast<T *>(a->y), parts};
+    if (a->rows <= kFew) {
+      const uint64_t groups = std::min<uint64_t>(a->rows, a->rows / kFewRows + a->n_experts + 1);
+      few_rows_kernel<T><<<dim3((uint32_t)((a->n_out + kFewWeights * kFewWaves - 1) / (kFewWeights * kFewWaves)), (uint32_t)groups), 64 * kFewWaves, 0, st>>>(
+          weights, weight_stride, counts, x, x_stride, (int)in8, (int)a->n_out, static_cast<T *>(a->y));
+    } else {
+      rc = launch<T, false>(p, e, a->rows, a->n_experts, st);
+    }
   }
   if (backward && a->grad_x && a->rows) {
     const Product p{nullptr, grad_y, weight_stride, grad_y_stride, 0, 0, (int32_t)a->n_in, 0, (int32_t)out8, emrs_gemm::kNoWrap, emrs_gemm::kNoWrap, 0, 1, 0};
-    const OfTokens<T, true> e{weights, counts, a->n_in % 8 == 0 && on(a->grad_x, 16), (int32_t)a->n_out, static_cast<T *>(a->grad_x)};
+    const OfTokens<T, true> e{weights, counts, a->n_in % 8 == 0 && on(a->grad_x, 16), (int32_t)a->n_out, static_cast<T *>(a->grad_x), parts};
     rc = launch<T, true>(p, e, a->rows, a->n_experts, st);
   }
   if (rc == EMRS_OK && backward && a->grad_weights) {

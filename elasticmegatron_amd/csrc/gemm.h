@@ -103,7 +103,8 @@ __host__ inline int64_t tile_count(const Product &p) {
 
 struct Where {
   int m0, n0, batch;
-  int first;  // where place() found the tile's rows: the first of them
+  // Of place(): the tile's first row, the first k, and which part of a tile's k it is (-1: the whole).
+  int first, k_from, part;
 };
 
 // What an epilogue is beside its run(): where the operands of a matrix of the batch begin.

@@ -86,7 +86,21 @@ CASES = [
     ([5000], 200, 264, FP16, 0),
     ([2100, 1900, 96], 2048, 768, BF16, 0),
     ([12, 20], 8200, 72, BF16, 0),
+    ([0, 1, 0, 0, 0, 1], 4096, 1000, BF16, 0),     # one token's experts: weights read by rows
+    ([2], 520, 37, FP16, 0),
+    ([0, 1], 1001, 130, BF16, 1),                  # and a row of none
+    ([0] * 70 + [1], 264, 64, BF16, 1),
 ]
+
+
+@pytest.mark.parametrize("counts,n_in,n_out,spare", [([2100, 1999], 8200, 4360, 7), ([3000, 1, 1090], 4352, 8192, 0)])
+def test_long_sums_are_cut(gpu_device, counts, n_in, n_out, spare):
+    """The tiles of the last round are cut along a long k: of y where n_in is long, of grad_x where n_out is."""
+    x, w, c, g = _inputs(counts, n_in, n_out, BF16, spare)
+    got = _run(x, w, c, g)
+    _check(x, w, c, g, *got)
+    again = _run(x, w, c, g)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
 
 
 @pytest.mark.parametrize("counts,n_in,n_out,dtype,spare", CASES)
