@@ -148,8 +148,8 @@ class Attention(ctypes.Structure):
                 ("offsets", ctypes.c_void_p), ("key_offsets", ctypes.c_void_p),
                 ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
                 ("q_strides", ctypes.c_uint64 * 2), ("k_strides", ctypes.c_uint64 * 2), ("v_strides", ctypes.c_uint64 * 2),
-                ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-                ("grad_out", ctypes.c_void_p), ("grad_out_strides", ctypes.c_uint64 * 2), ("grad_q", ctypes.c_void_p),
+                ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32), ("out", ctypes.c_void_p), ("out_rest", ctypes.c_void_p),
+                ("lse", ctypes.c_void_p), ("grad_out", ctypes.c_void_p), ("grad_out_strides", ctypes.c_uint64 * 2), ("grad_q", ctypes.c_void_p),
                 ("grad_k", ctypes.c_void_p), ("grad_v", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
                 ("workspace_bytes", ctypes.c_uint64)]
 

@@ -248,9 +248,9 @@ struct Attention {
   Bounds queries, keys;
   const void *q, *k, *v, *grad_out;
   Strides q_at, k_at, v_at, grad_out_at;
-  int32_t heads, group, dim, real_dim, causal, splits;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
+  int32_t heads, group, dim, real_dim, causal, splits, wide_out;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
   float scale;           // of the scores
-  void *out;             // [rows][heads][real_dim]
+  void *out, *rest;      // [rows][heads][real_dim]: the output, and what its rounding left over
   float *lse;            // [heads][rows]
   float *exponent, *delta;  // the same, backward: lse in units of log 2 (infinity where a query sees nothing), and delta
   void *grad_q, *grad_k, *grad_v;
@@ -258,9 +258,16 @@ struct Attention {
   const uint32_t *largest;  // fp16: the largest |grad_out| and |v|, as bits
 };
 
+// What rounding x to `rounded` left over (nothing of infinities and NaN).
+template <class T>
+__device__ __forceinline__ T rest_of(float x, T rounded) {
+  const float left = x - (float)rounded;
+  return fabsf(left) < INFINITY ? (T)left : (T)0.f;
+}
+
 // A wave's sums, held as [column][row], to rows of the output or of its part.
 template <class T, int DIM>
-__device__ __forceinline__ void store_own(const f32x16 (&acc)[DIM / 32], T *to, float *part, bool valid, int dim, float by) {
+__device__ __forceinline__ void store_own(const f32x16 (&acc)[DIM / 32], T *to, float *part, bool valid, int dim, float by, T *rest = nullptr) {
 #pragma unroll
   for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
@@ -279,14 +286,22 @@ __device__ __forceinline__ void store_own(const f32x16 (&acc)[DIM / 32], T *to, 
             if (at + e < dim) part[at + e] = acc[d][r + e] * by;
         }
       } else if (dim % 4 == 0) {
-        typename emrs_gemm::Vec<T>::x4 v;
+        using x4 = typename emrs_gemm::Vec<T>::x4;
+        x4 v, left;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(acc[d][r + e] * by);
-        if (at < dim) *reinterpret_cast<typename emrs_gemm::Vec<T>::x4 *>(to + at) = v;
+        for (int e = 0; e < 4; ++e) {
+          v[e] = (T)(acc[d][r + e] * by);
+          left[e] = rest_of<T>(acc[d][r + e] * by, v[e]);
+        }
+        if (at < dim) *reinterpret_cast<x4 *>(to + at) = v;
+        if (rest && at < dim) *reinterpret_cast<x4 *>(rest + at) = left;
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (at + e < dim) to[at + e] = (T)(acc[d][r + e] * by);
+          if (at + e < dim) {
+            to[at + e] = (T)(acc[d][r + e] * by);
+            if (rest) rest[at + e] = rest_of<T>(acc[d][r + e] * by, (T)(acc[d][r + e] * by));
+          }
       }
     }
 }
@@ -417,14 +432,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
     store_own<T, DIM>(out, nullptr, p.parts + (int64_t)at.split * p.queries.rows * p.heads * p.real_dim + place, valid, p.real_dim, norm);
   } else {
     if (valid && lane < 32 && p.lse) p.lse[(int64_t)at.head * p.queries.rows + row] = lse;
-    store_own<T, DIM>(out, static_cast<T *>(p.out) + place, nullptr, valid, p.real_dim, norm);
+    store_own<T, DIM>(out, static_cast<T *>(p.out) + place, nullptr, valid, p.real_dim, norm, p.rest ? static_cast<T *>(p.rest) + place : nullptr);
   }
 }
 
 // Joins the splits of one row of one head: 64 lanes of a wave, a row a wave.
 template <class T>
 __global__ __launch_bounds__(256) void attention_join_kernel(const float *parts, const float *part_lse, int splits, int64_t rows, int heads, int dim, T *out,
-                                                             float *lse) {
+                                                             T *rest, float *lse) {
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // row * heads + head
   if (unit >= rows * heads) return;
   const int64_t row = unit / heads, head = unit % heads;
@@ -441,6 +456,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float *parts,
       if (w != 0.f) v += w * parts[(s * rows * heads + unit) * dim + c];  // NaN is not 0
     }
     out[unit * dim + c] = (T)v;
+    if (rest) rest[unit * dim + c] = rest_of<T>(v, (T)v);
   }
   if (lane_of() == 0 && lse) lse[head * rows + row] = sum == 0.f ? -INFINITY : shift + logf(sum);
 }
@@ -509,14 +525,25 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention
   g.load(static_cast<const T *>(p.grad_out) + row * p.grad_out_at.row + at.head * p.grad_out_at.head, valid, p.dim);
   float delta = 0.f, lse = INFINITY;
   if (valid) {
-    const T *const out = static_cast<const T *>(p.out) + place;
+    // Of the output before its rounding, as far as it was kept: delta's error is one of every d of the row.
+    const T *const out = static_cast<const T *>(p.out) + place, *const rest = p.rest ? static_cast<const T *>(p.rest) + place : nullptr;
+    if (p.wide_out) {
+      OwnRows<T, DIM> a, b;
+      a.load(out, true, p.real_dim);
+      b.load(rest, rest != nullptr, p.real_dim);
 #pragma unroll
-    for (int c = 0; c < DIM / 16; ++c)
+      for (int c = 0; c < DIM / 16; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = c * 16 + (lane >> 5) * 8 + e;
-        if (d < p.real_dim) delta = fmaf((float)g.v[c][e], (float)out[d], delta);
-      }
+        for (int e = 0; e < 8; ++e) delta = fmaf((float)g.v[c][e], (float)a.v[c][e] + (float)b.v[c][e], delta);
+    } else {
+#pragma unroll
+      for (int c = 0; c < DIM / 16; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = c * 16 + (lane >> 5) * 8 + e;
+          if (d < p.real_dim) delta = fmaf((float)g.v[c][e], (float)out[d] + (rest ? (float)rest[d] : 0.f), delta);
+        }
+    }
     lse = p.lse[(int64_t)at.head * p.queries.rows + row] * kLog2e;
     if (lse == -INFINITY) lse = INFINITY;  // sees nothing: probabilities of 0
   }
@@ -863,7 +890,8 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   if (room.pad_v) p.v = pad<T>(a->v, a->v_strides, a->key_rows, a->kv_heads, a->dim, w + room.v, p.v_at, st);
   if (room.pad_g) p.grad_out = pad<T>(a->grad_out, a->grad_out_strides, a->rows, a->heads, a->dim, w + room.g, p.grad_out_at, st);
   p.heads = (int32_t)a->heads, p.group = (int32_t)(a->heads / a->kv_heads), p.dim = (int32_t)dim8, p.real_dim = (int32_t)a->dim, p.causal = a->causal != 0;
-  p.scale = a->scale, p.out = a->out, p.lse = a->lse;
+  p.scale = a->scale, p.out = a->out, p.rest = a->out_rest, p.lse = a->lse;
+  p.wide_out = a->dim % 8 == 0 && on(a->out, 16) && on(a->out_rest, 16);
   p.splits = (int32_t)key_splits(a);
   p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
   if (!backward) {
@@ -872,7 +900,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
     attention_forward_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
     if (p.splits > 1)
       attention_join_kernel<T><<<(uint32_t)((a->rows * a->heads + 3) / 4), 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,
-                                                                                        (int)a->dim, static_cast<T *>(a->out), a->lse);
+                                                                                        (int)a->dim, static_cast<T *>(a->out), static_cast<T *>(a->out_rest), a->lse);
   } else {
     p.exponent = reinterpret_cast<float *>(w + room.exponent);
     p.delta = reinterpret_cast<float *>(w + room.delta);
@@ -931,7 +959,7 @@ int run(const emrs_attention *a, bool backward, hipStream_t st) {
   if ((rc = operand(a->q, a->rows, a->q_strides)) || (rc = operand(a->k, a->key_rows, a->k_strides)) || (rc = operand(a->v, a->key_rows, a->v_strides)))
     return rc;
   if (a->rows && !a->out) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL out");
-  if (!on(a->out, 8) || !on(a->lse, 4)) return fail(EMRS_ERR_MISALIGNED, "attention: out is off 8 bytes");
+  if (!on(a->out, 8) || !on(a->out_rest, 8) || !on(a->lse, 4)) return fail(EMRS_ERR_MISALIGNED, "attention: out is off 8 bytes");
   if (backward) {
     if ((rc = operand(a->grad_out, a->rows, a->grad_out_strides))) return rc;
     if (a->rows && !a->lse) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: NULL lse");

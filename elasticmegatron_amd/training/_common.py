@@ -37,6 +37,11 @@ def refuse_tangents(*arguments) -> None:
             raise NotImplementedError("the operators of a training step have no forward-mode derivatives")
 
 
+def lies(*tensors) -> tuple:
+    """Where tensors (or None) are and how: what a record of their addresses holds good for."""
+    return tuple([None if t is None else (t.data_ptr(), t.size(), t.stride(), t.dtype) for t in tensors])
+
+
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """Scratch of one call.  The caching allocator's blocks lie on 512 bytes, and one that is freed after the
     call is reused by later work of the same stream only."""

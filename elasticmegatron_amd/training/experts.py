@@ -13,7 +13,7 @@ from typing import Sequence, Union
 import torch
 
 from .. import _native
-from ._common import DTYPE_CODES, dtype_code, on_device, refuse_tangents, run_on, workspace
+from ._common import DTYPE_CODES, dtype_code, lies, on_device, refuse_tangents, run_on, workspace
 
 Weights = Union[torch.Tensor, Sequence[torch.Tensor]]
 
@@ -28,7 +28,7 @@ def _rows(t: torch.Tensor):
 
 
 def _same_rows(weights):
-    """The same of every expert's matrix, all with one stride."""
+    """The same of every expert's matrix, all with one stride: tensors, addresses, stride."""
     if len(weights) == 1 and weights[0].dim() == 3:
         t = weights[0]
         (_, n, k), (_, over, along) = t.size(), t.stride()
@@ -37,15 +37,38 @@ def _same_rows(weights):
             over = k
         base, step = t.data_ptr(), t.stride(0) * t.element_size()
         return [t], [base + i * step for i in range(t.shape[0])], over if n > 1 else k
-    laid = [_rows(w) for w in weights]
-    strides = {over for _, over in laid}
-    if len(strides) > 1:
-        laid = [(w.detach().contiguous(), w.shape[1]) for w, _ in laid]
-    return [w for w, _ in laid], [w.data_ptr() for w, _ in laid], laid[0][1]
+    n, k = weights[0].size()
+    first = weights[0].stride()
+    if (first[1] == 1 or k == 1) and (n == 1 or k <= first[0] <= 1 << 21) and all(w.stride() == first for w in weights):
+        return weights, [w.data_ptr() for w in weights], first[0] if n > 1 else k
+    laid = [w.detach().contiguous() for w in weights]
+    return laid, [w.data_ptr() for w in laid], k
 
 
 def _table(values):
     return (ctypes.c_uint64 * len(values))(*values)
+
+
+def _refuse(x, counts, weights) -> None:
+    """Raises for the first argument that is not as it has to be."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x is no tensor")
+    device = x.device
+    on_device("x", x, device)
+    dtype_code(x, "x", (torch.bfloat16, torch.float16))
+    if x.dim() != 2:
+        raise ValueError(f"x is {tuple(x.shape)}: [rows, n_in] is wanted")
+    on_device("counts", counts, device)
+    if counts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"counts is {counts.dtype}: torch.int32 or torch.int64 is wanted")
+    for i, w in enumerate(weights):
+        on_device(f"weight {i}", w, device)
+        if w.dtype != x.dtype:
+            raise TypeError(f"weight {i} is {w.dtype}, x {x.dtype}")
+        if w.dim() != (3 if len(weights) == 1 and w.dim() == 3 else 2):
+            raise ValueError(f"weight {i} has {w.dim()} dimensions: a matrix for every expert, or all of them stacked, is wanted")
+        if w.shape[-1] != x.shape[1] or w.shape[-2:] != weights[0].shape[-2:]:
+            raise ValueError(f"weight {i} is {tuple(w.shape[-2:])}: [{weights[0].shape[-2]}, {x.shape[1]}] is wanted")
 
 
 class _Call:
@@ -54,41 +77,46 @@ class _Call:
     ``weights``: one tensor [experts, n_out, n_in], or one matrix [n_out, n_in] for every expert."""
 
     def __init__(self, x, counts, weights):
-        if not isinstance(x, torch.Tensor):
-            raise TypeError("x is no tensor")
-        device = self.device = x.device
-        on_device("x", x, device)
-        dtype_code(x, "x", (torch.bfloat16, torch.float16))
-        if x.dim() != 2:
-            raise ValueError(f"x is {tuple(x.shape)}: [rows, n_in] is wanted")
-        on_device("counts", counts, device)
-        if counts.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"counts is {counts.dtype}: torch.int32 or torch.int64 is wanted")
-        for i, w in enumerate(weights):
-            on_device(f"weight {i}", w, device)
-            if w.dtype != x.dtype:
-                raise TypeError(f"weight {i} is {w.dtype}, x {x.dtype}")
-            if w.dim() != (3 if len(weights) == 1 and w.dim() == 3 else 2):
-                raise ValueError(f"weight {i} has {w.dim()} dimensions: a matrix for every expert, or all of them stacked, is wanted")
-            if w.shape[-1] != x.shape[1] or w.shape[-2:] != weights[0].shape[-2:]:
-                raise ValueError(f"weight {i} is {tuple(w.shape[-2:])}: [{weights[0].shape[-2]}, {x.shape[1]}] is wanted")
-        experts = weights[0].shape[0] if len(weights) == 1 and weights[0].dim() == 3 else len(weights)
+        stacked = len(weights) == 1 and isinstance(weights[0], torch.Tensor) and weights[0].dim() == 3
+        if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.dim() == 2 and
+                isinstance(weights[0], torch.Tensor)):
+            _refuse(x, counts, weights)
+        device, dtype, size = x.device, x.dtype, weights[0].size()
+        for w in weights:  # one by one only where something is wrong
+            if not (isinstance(w, torch.Tensor) and w.dtype is dtype and w.device == device and w.size() == size):
+                _refuse(x, counts, weights)
+        if not (isinstance(counts, torch.Tensor) and counts.device == device and counts.dtype in (torch.int32, torch.int64) and
+                len(size) == (3 if stacked else 2) and size[-1] == x.size(1)):
+            _refuse(x, counts, weights)
+        experts = size[0] if stacked else len(weights)
         if not 1 <= experts <= _native.EMRS_EXPERTS_MAX:
             raise ValueError(f"{experts} experts: 1 to {_native.EMRS_EXPERTS_MAX} are wanted")
         if counts.shape != (experts,):
             raise ValueError(f"counts is {tuple(counts.shape)}: [{experts}] is wanted")
-        n_out, n_in = weights[0].shape[-2:]
+        n_out, n_in = size[-2:]
         if not n_in or not n_out:
             raise ValueError(f"weights of {n_out} x {n_in}: no side may be 0")
-        rows, x_stride = _rows(x)
-        counts = counts.contiguous()
-        laid, addresses, weight_stride = _same_rows(weights)
-        self._keep = [rows, counts, laid, _table(addresses)]
-        self.experts, self.n_out, self.shape, self.dtype = experts, n_out, x.size(), x.dtype
-        a = self.record = _native.Experts()
-        a.dtype, a.n_experts, a.rows, a.n_in, a.n_out = DTYPE_CODES[x.dtype], experts, x.shape[0], n_in, n_out
-        a.counts, a.counts_bytes = counts.data_ptr(), counts.element_size()
-        a.x, a.x_stride, a.weights, a.weight_stride = rows.data_ptr(), x_stride, ctypes.addressof(self._keep[3]), weight_stride
+        self.x, x_stride = _rows(x)
+        self.counts = counts if counts.is_contiguous() else counts.contiguous()
+        self.weights, addresses, weight_stride = _same_rows(weights)
+        self.device, self.dtype, self.experts, self.shape, self.size, self.n_out = device, dtype, experts, x.size(), size, n_out
+        self._table = _table(addresses)
+        self.record = _native.Experts(DTYPE_CODES[dtype], experts, x.shape[0], n_in, n_out, self.counts.data_ptr(), counts.element_size(), 0,
+                                      self.x.data_ptr(), x_stride, ctypes.addressof(self._table), weight_stride)
+
+    def again(self, x, counts, weights) -> "_Call":
+        """The same call on tensors that autograd hands back: itself where they are where they were, and checked anew where not."""
+        if lies(x, counts, *weights) != self.lies:
+            return _Call(x, counts, weights)
+        call = object.__new__(_Call)
+        call.__dict__.update(self.__dict__)
+        call.record = _native.Experts.from_buffer_copy(self.record)
+        return call
+
+    def release(self) -> None:
+        """What is left knows where its tensors were, and does not keep them."""
+        self.lies = lies(self.x, self.counts, *self.weights)
+        self.x = self.counts = self.weights = None
 
     def _run(self, call, backward):
         a = self.record
@@ -105,16 +133,24 @@ class _Call:
             self._run(_native.experts_forward, False)
         return y
 
-    def backward(self, grad_y, want_x, weights, want_weights):
+    def backward(self, grad_y, want_x, want_weights):
+        """``(grad_x, gradients of the weights)``; each may be None."""
         a = self.record
-        rows, a.grad_y_stride = _rows(grad_y.to(self.dtype))
-        a.grad_y = rows.data_ptr()
+        if grad_y.size() != (self.shape[0], self.n_out):
+            raise ValueError(f"a gradient of {tuple(grad_y.shape)} for {self.shape[0]} rows of {self.n_out}")
+        rows, a.grad_y_stride = _rows(grad_y if grad_y.dtype is self.dtype else grad_y.to(self.dtype))
+        a.grad_y, a.y = rows.data_ptr(), None
         gx = torch.empty(self.shape, dtype=self.dtype, device=self.device) if want_x else None
-        gw = [torch.empty(w.size(), dtype=self.dtype, device=self.device) for w in weights] if want_weights else None
+        gw = None
         a.grad_x = None if gx is None else gx.data_ptr()
-        if gw:
-            step = gw[0].element_size() * self.n_out * self.shape[1]
-            table = _table([gw[0].data_ptr() + i * step for i in range(self.experts)] if gw[0].dim() == 3 else [g.data_ptr() for g in gw])
+        if want_weights:
+            if len(self.size) == 3:
+                gw = [torch.empty(self.size, dtype=self.dtype, device=self.device)]
+                step = gw[0].element_size() * self.n_out * self.shape[1]
+                table = _table([gw[0].data_ptr() + i * step for i in range(self.experts)])
+            else:
+                gw = [torch.empty(self.size, dtype=self.dtype, device=self.device) for _ in range(self.experts)]
+                table = _table([g.data_ptr() for g in gw])
             a.grad_weights = ctypes.addressof(table)
         if gw or (want_x and self.shape[0]):
             self._run(_native.experts_backward, True)
@@ -124,8 +160,12 @@ class _Call:
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, counts, *weights):
-        y = _Call(x, counts, weights).forward()
-        ctx.save_for_backward(x, counts, *weights)
+        call = _Call(x, counts, weights)
+        y = call.forward()
+        # What the kernels read: the inputs, or the copies that had to be made of them.  The graph alone keeps them.
+        ctx.save_for_backward(call.x, call.counts, *call.weights)
+        ctx.call = call
+        call.release()
         return y
 
     @staticmethod
@@ -133,7 +173,7 @@ class _ExpertLinear(torch.autograd.Function):
     def backward(ctx, grad_y):
         x, counts, *weights = ctx.saved_tensors  # raises where one was changed in place
         need = ctx.needs_input_grad
-        gx, gw = _Call(x, counts, weights).backward(grad_y, need[0], weights, any(need[2:]))
+        gx, gw = ctx.call.again(x, counts, weights).backward(grad_y, need[0], any(need[2:]))
         return (gx, None, *((g if want else None for g, want in zip(gw, need[2:])) if gw else [None] * len(weights)))
 
 

@@ -628,7 +628,7 @@ int emrs_experts_backward(const emrs_experts *experts, void *stream);
  * sees the last key.  Head h reads the keys and values of head h / (heads / kv_heads).
  *   s = scale q . k over the keys seen,  lse = log sum exp(s),  out = sum exp(s - lse) v
  * A query that sees nothing, or belongs to no document, has out 0 and lse -inf.
- * Backward reads out and lse, and writes the gradients of q, k and v; keys that nothing sees have gradients of 0.
+ * Backward reads out, out_rest and lse, and writes the gradients of q, k and v; keys that nothing sees have gradients of 0.
  * Offsets are on the device; they are held within the rows, and one that goes back counts as the one before. */
 typedef struct emrs_attention {
   uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16 */
@@ -644,6 +644,7 @@ typedef struct emrs_attention {
   float scale;                    /* > 0 */
   uint32_t reserved;              /* must be 0 */
   void *out;                      /* [rows][heads][dim], contiguous */
+  void *out_rest;                 /* the same: what out's rounding left over, rounded; may be NULL */
   float *lse;                     /* [heads][rows]; forward: may be NULL */
   const void *grad_out;
   uint64_t grad_out_strides[2];

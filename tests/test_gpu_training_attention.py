@@ -10,8 +10,8 @@ from elasticmegatron_amd import training
 pytestmark = pytest.mark.gpu
 
 BF16, FP16 = torch.bfloat16, torch.float16
-UNIT = {BF16: 2.0 ** -8, FP16: 2.0 ** -11}  # half a step, relative
-STEP = {BF16: 2.0 ** -134, FP16: 2.0 ** -25}  # half the smallest number
+UNIT = {BF16: 2.0 ** -8, FP16: 2.0 ** -11, torch.double: 2.0 ** -53}  # half a step, relative
+STEP = {BF16: 2.0 ** -134, FP16: 2.0 ** -25, torch.double: 0.0}  # half the smallest number
 
 
 def _bounds(lengths):
@@ -33,10 +33,10 @@ def _formula(q, k, v, g, q_at, k_at, causal, scale):
     """out, gradients and what bounds their errors but for the last rounding, in 64 bits.
 
     Scores sum ``dim`` products in 32 bits, and their exponents are off by that and by a few roundings of themselves.  Probabilities and their
-    gradients have one rounding to the type (fp16 holds them scaled: a step of 2^-31 of the largest), and delta comes from the rounded output.
+    gradients have one rounding to the type (fp16 holds them scaled: a step of 2^-31 of the largest), and delta comes from the output with what its rounding left over.
     An exponential below 2^-126, the smallest normal number of 32 bits, may be 0: p is off by as much there, and its gradient by that times
     |grad_out . v - delta|."""
-    u, f = UNIT[q.dtype], 2.0 ** -24
+    u, f, unit = UNIT[q.dtype], 2.0 ** -24, STEP[q.dtype]
     dim, share = q.shape[2], q.shape[1] // k.shape[1]
     tiny = 2.0 ** -31 if q.dtype == FP16 else 0.0
     q, k, v, g = (t.double() for t in (q, k, v, g))
@@ -62,7 +62,7 @@ def _formula(q, k, v, g, q_at, k_at, causal, scale):
             o = p @ c
             out[0][lo:hi, h] = o
             err[0][lo:hi, h] = e_p @ c.abs() + f * m * (p @ c.abs())
-            delta, e_delta = (d * o).sum(1, keepdim=True), (d.abs() * (err[0][lo:hi, h] + u * o.abs() + f * dim * o.abs())).sum(1, keepdim=True)
+            delta, e_delta = (d * o).sum(1, keepdim=True), (d.abs() * (err[0][lo:hi, h] + (u * u + f * dim) * o.abs() + unit)).sum(1, keepdim=True)
             dp, e_dp = d @ c.t(), f * dim * (d.abs() @ c.abs().t())
             ds = p * (dp - delta)
             e_ds = p * (e_dp + e_delta + f * (dp.abs() + delta.abs())) + ds.abs() * (e_s + u) + (tiny * biggest * 2.0 ** -6 + 2.0 ** -126 * (dp.abs() + delta.abs())) * see
@@ -241,9 +241,8 @@ def test_against_differences(gpu_device):
     gen = torch.Generator(device="cuda").manual_seed(5)
 
     def value(x):
-        return float((_formula(*x, g.double(), at, at, True, 40 ** -0.5)[0][0] * g.double()).sum()) if x[0].dtype != FP16 else 0.0
+        return float((_formula(*x, g.double(), at, at, True, 40 ** -0.5)[0][0] * g.double()).sum())
 
-    UNIT[torch.double] = 0.0
     base = [t.double() for t in (q, k, v)]
     for i, grad in enumerate(got):
         d = torch.randn(base[i].shape, generator=gen, device="cuda").double()
