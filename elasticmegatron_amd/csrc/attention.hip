@@ -164,24 +164,24 @@ __device__ __forceinline__ int permuted(int row) {
   return DIM == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
 }
 
-// What a lane loads of every tile of an operand: 16 bytes of every (kWaves x 1 KB)-th row.
-template <class T, int DIM>
+// What a lane loads of every tile of ROWS rows of an operand: 16 bytes of each of its wave's kilobytes.
+template <class T, int DIM, int WAVES = kWaves, int ROWS = kTile>
 struct TileLoader {
-  static constexpr int kUnits = DIM / 8, kRows = 64 / kUnits, kLoads = kTile / (kRows * kWaves);
+  static constexpr int kUnits = DIM / 8, kRows = 64 / kUnits, kLoads = ROWS / (kRows * WAVES);
   int offset, step, stride, dim;
   __device__ __forceinline__ void init(int64_t row_stride, int dim_, int wave) {
     const int row = wave * kRows + lane_of() / kUnits, unit = lane_of() % kUnits ^ permuted<DIM>(row);
-    static_assert(kRows * kWaves % 16 == 0, "a lane's rows are permuted alike");
-    stride = (int)row_stride * 2, dim = dim_ * 2, step = kRows * kWaves * stride;
+    static_assert(kRows * WAVES % 16 == 0 && kLoads * kRows * WAVES == ROWS, "a lane's rows are permuted alike");
+    stride = (int)row_stride * 2, dim = dim_ * 2, step = kRows * WAVES * stride;
     offset = unit * 8 < dim_ ? row * stride + unit * 16 : (int)0x80000000;  // past the end: zeros
   }
   // `rows` rows from `first` on (more than a tile's: a tile's; less: zeros behind them; none: zeros).
   __device__ __forceinline__ void load(char *lds, const T *first, int rows, int wave) const {
-    rows = min(rows, kTile);
+    rows = min(rows, ROWS);
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(first), 0, rows > 0 ? (rows - 1) * stride + dim : 0, 0x00020000);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (j * kWaves + wave) * 1024), 16,
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)(lds + (j * WAVES + wave) * 1024), 16,
                                                offset < 0 ? offset : offset + j * step, 0, 0, 0);
   }
 };
@@ -248,7 +248,7 @@ struct Attention {
   Bounds queries, keys;
   const void *q, *k, *v, *grad_out;
   Strides q_at, k_at, v_at, grad_out_at;
-  int32_t heads, group, dim, real_dim, causal, splits, wide_out;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
+  int32_t heads, group, dim, real_dim, causal, splits, wide_out, wide_grads;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
   float scale;           // of the scores
   void *out, *rest;      // [rows][heads][real_dim]: the output, and what its rounding left over
   float *lse;            // [heads][rows]
@@ -265,46 +265,45 @@ __device__ __forceinline__ T rest_of(float x, T rounded) {
   return fabsf(left) < INFINITY ? (T)left : (T)0.f;
 }
 
-// A wave's sums, held as [column][row], to rows of the output or of its part.
-template <class T, int DIM>
-__device__ __forceinline__ void store_own(const f32x16 (&acc)[DIM / 32], T *to, float *part, bool valid, int dim, float by, T *rest = nullptr) {
+// A wave's sums, held as [column][row], to the rows of an output: turned over in the wave's own part of LDS, whose
+// units of 16 bytes are permuted by the row, so that rows are stored in whole lines (straight from registers, eight
+// bytes a lane, the two outputs of 8192 x 32 x 128 took 25 us longer).
+template <class V, int DIM>
+struct RowStore {
+  static constexpr int kEach = 16 / sizeof(V), kUnits = DIM / kEach, kMask = kUnits < 16 ? kUnits - 1 : 15;
+  static __device__ __forceinline__ int at(int row, int unit) { return (row * kUnits + (unit ^ (row & kMask))) * 16; }
+  // value(d, r): of the lane's row, in 32 bits.  rows: how many of the wave's rows there are.
+  template <class Value>
+  static __device__ __forceinline__ void store(char *room, Value value, V *to, int64_t stride, int rows, int dim, bool wide) {
+    typedef __attribute__((ext_vector_type(4))) V v4;
+    typedef __attribute__((ext_vector_type(kEach))) V unit_t;
+    const int lane = lane_of();
 #pragma unroll
-  for (int d = 0; d < DIM / 32; ++d)
+    for (int d = 0; d < DIM / 32; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const int at = d * 32 + row_of(r);
-      if (!valid) continue;
-      if (part) {
-        if (dim % 4 == 0) {
-          f32x4 v;
+      for (int r = 0; r < 16; r += 4) {
+        v4 v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[d][r + e] * by;
-          if (at < dim) *reinterpret_cast<f32x4 *>(part + at) = v;
-        } else {
+        for (int e = 0; e < 4; ++e) v[e] = (V)value(d, r + e);
+        const int column = d * 32 + row_of(r);
+        *reinterpret_cast<v4 *>(room + at(lane & 31, column / kEach) + column % kEach * sizeof(V)) = v;
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (at + e < dim) part[at + e] = acc[d][r + e] * by;
-        }
-      } else if (dim % 4 == 0) {
-        using x4 = typename emrs_gemm::Vec<T>::x4;
-        x4 v, left;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = (T)(acc[d][r + e] * by);
-          left[e] = rest_of<T>(acc[d][r + e] * by, v[e]);
-        }
-        if (at < dim) *reinterpret_cast<x4 *>(to + at) = v;
-        if (rest && at < dim) *reinterpret_cast<x4 *>(rest + at) = left;
+    for (int pass = 0; pass < kUnits / 2; ++pass) {
+      const int row = pass * (64 / kUnits) + lane / kUnits, unit = lane % kUnits;
+      const unit_t v = *reinterpret_cast<const unit_t *>(room + at(row, unit));
+      V *const out = to + row * stride + unit * kEach;
+      if (row >= rows || unit * kEach >= dim) continue;
+      if (wide) {
+        *reinterpret_cast<unit_t *>(out) = v;
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at + e < dim) {
-            to[at + e] = (T)(acc[d][r + e] * by);
-            if (rest) rest[at + e] = rest_of<T>(acc[d][r + e] * by, (T)(acc[d][r + e] * by));
-          }
+        for (int e = 0; e < kEach; ++e)
+          if (unit * kEach + e < dim) out[e] = v[e];
       }
     }
-}
+  }
+};
 
 // A split's run of tiles.
 __device__ __forceinline__ Span share_of(int tiles, int split, int splits) {
@@ -426,49 +425,73 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
   sum += other_half(sum);
   const float lse = sum == 0.f ? -INFINITY : (top - kLift) * kLn2 + logf(sum);
   const float norm = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t place = (row * p.heads + at.head) * p.real_dim;
+  const int64_t place = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
+  char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
+  const int rows = queries - mine;
+  auto value = [&](int d, int r) { return out[d][r] * norm; };
   if (p.splits > 1) {
     if (valid && lane < 32) p.part_lse[((int64_t)at.split * p.heads + at.head) * p.queries.rows + row] = lse;
-    store_own<T, DIM>(out, nullptr, p.parts + (int64_t)at.split * p.queries.rows * p.heads * p.real_dim + place, valid, p.real_dim, norm);
-  } else {
-    if (valid && lane < 32 && p.lse) p.lse[(int64_t)at.head * p.queries.rows + row] = lse;
-    store_own<T, DIM>(out, static_cast<T *>(p.out) + place, nullptr, valid, p.real_dim, norm, p.rest ? static_cast<T *>(p.rest) + place : nullptr);
+    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride + place, stride, rows, p.real_dim, p.real_dim % 4 == 0);
+    return;
   }
+  if (valid && lane < 32 && p.lse) p.lse[(int64_t)at.head * p.queries.rows + row] = lse;
+  RowStore<T, DIM>::store(room, value, static_cast<T *>(p.out) + place, stride, rows, p.real_dim, p.wide_out);
+  if (p.rest)
+    RowStore<T, DIM>::store(room, [&](int d, int r) { return (float)rest_of<T>(value(d, r), (T)value(d, r)); }, static_cast<T *>(p.rest) + place, stride, rows,
+                            p.real_dim, p.wide_out);
 }
 
-// Joins the splits of one row of one head: 64 lanes of a wave, a row a wave.
-template <class T>
+// Joins the splits' outputs: four elements a thread where heads are whole units of four, and one else.
+template <class T, int E>
 __global__ __launch_bounds__(256) void attention_join_kernel(const float *parts, const float *part_lse, int splits, int64_t rows, int heads, int dim, T *out,
                                                              T *rest, float *lse) {
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // row * heads + head
-  if (unit >= rows * heads) return;
+  typedef __attribute__((ext_vector_type(E))) float fE;
+  typedef __attribute__((ext_vector_type(E))) T tE;
+  const int units = dim / E;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = rows * heads * units, unit = i / units;  // row * heads + head
+  if (i >= all) return;
   const int64_t row = unit / heads, head = unit % heads;
   float top = -INFINITY;
   for (int s = 0; s < splits; ++s) top = fmaxf(top, part_lse[(s * heads + head) * rows + row]);
   const float shift = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  for (int s = 0; s < splits; ++s) sum += expf(part_lse[(s * heads + head) * rows + row] - shift);
-  const float norm = sum == 0.f ? 0.f : 1.f / sum;
-  for (int c = lane_of(); c < dim; c += 64) {
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float w = expf(part_lse[(s * heads + head) * rows + row] - shift) * norm;
-      if (w != 0.f) v += w * parts[(s * rows * heads + unit) * dim + c];  // NaN is not 0
-    }
-    out[unit * dim + c] = (T)v;
-    if (rest) rest[unit * dim + c] = rest_of<T>(v, (T)v);
+  fE v;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float w = __builtin_amdgcn_exp2f((part_lse[(s * heads + head) * rows + row] - shift) * kLog2e);
+    const fE x = *reinterpret_cast<const fE *>(parts + (s * all + i) * E);
+    sum += w;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = w == 0.f ? v[e] : fmaf(w, x[e], v[e]);  // NaN is not 0
   }
-  if (lane_of() == 0 && lse) lse[head * rows + row] = sum == 0.f ? -INFINITY : shift + logf(sum);
+  const float norm = sum == 0.f ? 0.f : 1.f / sum;
+  tE o, left;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    o[e] = (T)(v[e] * norm);
+    left[e] = rest_of<T>(v[e] * norm, o[e]);
+  }
+  *reinterpret_cast<tE *>(out + i * E) = o;
+  if (rest) *reinterpret_cast<tE *>(rest + i * E) = left;
+  if (i % units == 0 && lse) lse[head * rows + row] = sum == 0.f ? -INFINITY : shift + logf(sum);
 }
 
-// Sums of every split's part.
-template <class T>
+// Sums of every split's part, E elements a thread.
+template <class T, int E>
 __global__ __launch_bounds__(256) void attention_sum_kernel(const float *parts, int splits, int64_t each, T *out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  typedef __attribute__((ext_vector_type(E))) float fE;
+  typedef __attribute__((ext_vector_type(E))) T tE;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * E;
   if (i >= each) return;
-  float v = parts[i];
-  for (int s = 1; s < splits; ++s) v += parts[s * each + i];
-  out[i] = (T)v;
+  fE v = *reinterpret_cast<const fE *>(parts + i);
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const fE *>(parts + s * each + i);
+  tE o;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = (T)v[e];
+  *reinterpret_cast<tE *>(out + i) = o;
 }
 
 // ---- backward ----
@@ -626,55 +649,71 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention
   }
   arrive();
   if (!p.grad_q && !p.parts) return;
-  store_own<T, DIM>(acc, static_cast<T *>(p.grad_q) + place,
-                    p.splits > 1 ? p.parts + (int64_t)at.split * p.queries.rows * p.heads * p.real_dim + place : nullptr, valid, p.real_dim, p.scale / lift);
+  const int64_t corner = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
+  char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
+  const float back = p.scale / lift;
+  auto value = [&](int d, int r) { return acc[d][r] * back; };
+  if (p.splits > 1)
+    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride + corner, stride, queries - mine, p.real_dim, p.real_dim % 4 == 0);
+  else
+    RowStore<T, DIM>::store(room, value, static_cast<T *>(p.grad_q) + corner, stride, queries - mine, p.real_dim, p.wide_grads);
 }
 
 // grad_k and grad_v of one head of keys: the sums over the queries of every head that shares it, or, with splits, of
-// a run of these heads.
+// a run of these heads.  Two waves share 32 keys, each with its own half of a tile's queries, and add their sums at the
+// end: that makes two waves for each SIMD, whose turns at the matrix units and at everything else fill each other's
+// waits.  What a wave holds of its keys and both sums leaves no registers for v, which stays in LDS.
+constexpr int kPairs = 2 * kWaves;
+
 template <class T, int DIM>
-__global__ __launch_bounds__(kThreads, 1) void attention_grad_kv_kernel(Attention p) {
+__global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Attention p) {
   constexpr int kBytes = kTile * DIM * 2;
   __shared__ __attribute__((aligned(1024))) char q_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char q_odd[kBytes];
   __shared__ __attribute__((aligned(1024))) char g_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char g_odd[kBytes];
+  __shared__ __attribute__((aligned(1024))) char v_own[kOwn * DIM * 2];
   __shared__ __attribute__((aligned(256))) float sums_even[2][kTile];  // exponent and delta of the tile's queries
   __shared__ __attribute__((aligned(256))) float sums_odd[2][kTile];
   const int kv_heads = p.heads / p.group;
   Place at;
   if (!find<false>(p.keys, p.queries, kv_heads, p.splits, at)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of(), half = wave / kWaves, block = wave % kWaves;
   const int keys = at.own.end - at.own.first, queries = at.other.end - at.other.first;
-  const int mine = at.row + wave * 32, key = mine + (lane & 31);
+  const int mine = at.row + block * 32, key = mine + (lane & 31);
   const bool valid = key < keys;
   const int64_t row = at.own.first + key;
 
-  OwnRows<T, DIM> k, v;
+  {
+    TileLoader<T, DIM, kPairs, kOwn> loader;
+    loader.init(p.v_at.row, p.dim, wave);
+    loader.load(v_own, static_cast<const T *>(p.v) + (int64_t)(at.own.first + at.row) * p.v_at.row + at.head * p.v_at.head, keys - at.row, wave);
+  }
+  OwnRows<T, DIM> k;
   k.load(static_cast<const T *>(p.k) + row * p.k_at.row + at.head * p.k_at.head, valid, p.dim);
-  v.load(static_cast<const T *>(p.v) + row * p.v_at.row + at.head * p.v_at.head, valid, p.dim);
 
   // The first query that sees the workgroup's, the wave's and the lane's key, and the one from which on all of the
   // wave's are seen.
   const int shift = keys - queries;
   auto first_for = [&](int j) { return p.causal ? min(max(j - shift, 0), queries) : 0; };
   const int first = first_for(at.row), first_wave = mine < keys ? first_for(mine) : queries, first_lane = first_for(key), all_from = first_for(mine + 31);
+  const bool all_valid = mine + 32 <= keys;
   const int from_tile = first / kTile, tiles = (queries + kTile - 1) / kTile - from_tile;  // of a head
   const Span heads = share_of(p.group, at.split, p.splits);
   const int total = max(tiles, 0) * (heads.end - heads.first);
 
-  TileLoader<T, DIM> q_loader, g_loader;
+  TileLoader<T, DIM, kPairs> q_loader, g_loader;
   q_loader.init(p.q_at.row, p.dim, wave);
   g_loader.init(p.grad_out_at.row, p.dim, wave);
   TileReader<T, DIM> reader;
   reader.init();
   const T *const q = static_cast<const T *>(p.q) + at.other.first * p.q_at.row;
   const T *const g = static_cast<const T *>(p.grad_out) + at.other.first * p.grad_out_at.row;
-  const int first_head = at.head * p.group + heads.first;
-  auto load = [&](char *to_q, char *to_g, float (*sums)[kTile], int n) __attribute__((always_inline)) {
-    const int t = n < total ? n % tiles + from_tile : 0, head = first_head + (n < total ? n / tiles : 0);
-    const int rows = n < total ? queries - t * kTile : 0;
-    const int64_t from = t * kTile;
+  // The next tile to be loaded and the one that is worked on: tile of a head, head.
+  int load_tile = 0, load_head = at.head * p.group + heads.first, work_tile = 0;
+  auto load = [&](char *to_q, char *to_g, float (*sums)[kTile], bool any) __attribute__((always_inline)) {
+    const int64_t from = any ? (from_tile + load_tile) * kTile : 0;
+    const int rows = any ? queries - (int)from : 0, head = any ? load_head : 0;
     q_loader.load(to_q, q + from * p.q_at.row + head * p.q_at.head, rows, wave);
     g_loader.load(to_g, g + from * p.grad_out_at.row + head * p.grad_out_at.head, rows, wave);
     if (wave < 2) {  // zeros where there is no query: its operands are zeros
@@ -682,6 +721,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_kv_kernel(Attentio
       const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(of), 0, max(0, min(rows, kTile)) * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)sums[wave], 4, lane * 4, 0, 0, 0);
     }
+    if (++load_tile == tiles) load_tile = 0, ++load_head;
   };
   const float by = p.scale * kLog2e;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
@@ -693,65 +733,96 @@ __global__ __launch_bounds__(kThreads, 1) void attention_grad_kv_kernel(Attentio
 #pragma unroll
     for (int r = 0; r < 16; ++r) grad_k[d][r] = grad_v[d][r] = 0.f;
 
-  auto work = [&](const char *qt, const char *gt, const float (*sums)[kTile], int n) __attribute__((always_inline)) {
-    const int from = (n % tiles + from_tile) * kTile;
-    if (from + kTile <= first_wave) return;
+  auto work = [&](const char *qt, const char *gt, const float (*sums)[kTile]) __attribute__((always_inline)) {
+    const int from = (from_tile + work_tile) * kTile + half * 32;
+    if (++work_tile == tiles) work_tile = 0;
+    if (from + 32 <= first_wave || from >= queries) return;
+    f32x16 s, dp;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      f32x16 s, dp;
+    for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+    for (int c = 0; c < DIM / 16; ++c) {
+      s = mfma(reader.rows(qt, half, c), k.v[c], s);
+      dp = mfma(reader.rows(gt, half, c), reader.rows(v_own, block, c), dp);
+    }
 #pragma unroll
-      for (int c = 0; c < DIM / 16; ++c) {
-        s = mfma(reader.rows(qt, b, c), k.v[c], s);
-        dp = mfma(reader.rows(gt, b, c), v.v[c], dp);
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 exponent = *reinterpret_cast<const f32x4 *>(&sums[0][half * 32 + row_of(i * 4)]);
+      const f32x4 delta = *reinterpret_cast<const f32x4 *>(&sums[1][half * 32 + row_of(i * 4)]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -exponent[e]));
+        float d = x * (dp[i * 4 + e] - delta[e]);
+        if (kHalf) d *= lift;
+        s[i * 4 + e] = kHalf ? x * 32768.f : x;
+        dp[i * 4 + e] = d;
       }
+    }
+    if (from < all_from || !all_valid) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f32x4 lse = *reinterpret_cast<const f32x4 *>(&sums[0][b * 32 + row_of(i * 4)]);
-        const f32x4 delta = *reinterpret_cast<const f32x4 *>(&sums[1][b * 32 + row_of(i * 4)]);
+      for (int r = 0; r < 16; ++r)
+        if (from + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -lse[e]));
-          float d = x * (dp[i * 4 + e] - delta[e]);
-          if (kHalf) d *= lift;
-          s[i * 4 + e] = kHalf ? x * 32768.f : x;
-          dp[i * 4 + e] = d;
-        }
-      }
-      if (from < all_from || !__all(valid)) {
+    for (int c = 0; c < 2; ++c) {
+      const auto prob = eight_of<T>(s, c), ds = eight_of<T>(dp, c);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (from + b * 32 + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const auto prob = eight_of<T>(s, c), ds = eight_of<T>(dp, c);
-#pragma unroll
-        for (int d = 0; d < DIM / 32; ++d) {
-          grad_v[d] = mfma(reader.columns(gt, d, b * 2 + c), prob, grad_v[d]);
-          grad_k[d] = mfma(reader.columns(qt, d, b * 2 + c), ds, grad_k[d]);
-        }
+      for (int d = 0; d < DIM / 32; ++d) {
+        grad_v[d] = mfma(reader.columns(gt, d, half * 2 + c), prob, grad_v[d]);
+        grad_k[d] = mfma(reader.columns(qt, d, half * 2 + c), ds, grad_k[d]);
       }
     }
   };
 
-  load(q_even, g_even, sums_even, 0);
+  load(q_even, g_even, sums_even, total > 0);
   for (int n = 0; n < total; n += 2) {
     arrive();
-    load(q_odd, g_odd, sums_odd, n + 1);
-    work(q_even, g_even, sums_even, n);
+    load(q_odd, g_odd, sums_odd, n + 1 < total);
+    work(q_even, g_even, sums_even);
     if (n + 1 >= total) break;
     arrive();
-    load(q_even, g_even, sums_even, n + 2);
-    work(q_odd, g_odd, sums_odd, n + 1);
+    load(q_even, g_even, sums_even, n + 2 < total);
+    work(q_odd, g_odd, sums_odd);
   }
   arrive();
-  const int64_t place = (row * kv_heads + at.head) * p.real_dim, each = (int64_t)p.keys.rows * kv_heads * p.real_dim;
-  const bool split = p.splits > 1;
-  store_own<T, DIM>(grad_k, static_cast<T *>(p.grad_k) + place, split ? p.parts + at.split * each + place : nullptr, valid, p.real_dim, p.scale / lift);
-  store_own<T, DIM>(grad_v, static_cast<T *>(p.grad_v) + place, split ? p.parts2 + at.split * each + place : nullptr, valid, p.real_dim,
-                    kHalf ? 1.f / 32768.f : 1.f);
+
+  // The second halves' sums pass through the tiles' LDS.
+  char *const room = block == 0 ? q_even : block == 1 ? q_odd : block == 2 ? g_even : g_odd;
+  auto join = [&](f32x16 (&acc)[DIM / 32]) __attribute__((always_inline)) {
+    f32x4 *const part = reinterpret_cast<f32x4 *>(room) + lane;
+    if (half) {
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part[(d * 4 + i) * 64] = f32x4{acc[d][i * 4], acc[d][i * 4 + 1], acc[d][i * 4 + 2], acc[d][i * 4 + 3]};
+    }
+    arrive();
+    if (!half) {
+#pragma unroll
+      for (int d = 0; d < DIM / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 v = part[(d * 4 + i) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[d][i * 4 + e] += v[e];
+        }
+    }
+    arrive();
+  };
+  join(grad_k);
+  join(grad_v);
+  if (half) return;
+  const int64_t stride = (int64_t)kv_heads * p.real_dim, corner = (int64_t)(at.own.first + mine) * stride + at.head * p.real_dim, part = at.split * (p.keys.rows * stride);
+  const float back_k = p.scale / lift, back_v = kHalf ? 1.f / 32768.f : 1.f;
+  auto value_k = [&](int d, int r) { return grad_k[d][r] * back_k; };
+  auto value_v = [&](int d, int r) { return grad_v[d][r] * back_v; };
+  if (p.splits > 1) {
+    RowStore<float, DIM>::store(room, value_k, p.parts + part + corner, stride, keys - mine, p.real_dim, p.real_dim % 4 == 0);
+    RowStore<float, DIM>::store(room, value_v, p.parts2 + part + corner, stride, keys - mine, p.real_dim, p.real_dim % 4 == 0);
+  } else {
+    RowStore<T, DIM>::store(room, value_k, static_cast<T *>(p.grad_k) + corner, stride, keys - mine, p.real_dim, p.wide_grads);
+    RowStore<T, DIM>::store(room, value_v, static_cast<T *>(p.grad_v) + corner, stride, keys - mine, p.real_dim, p.wide_grads);
+  }
 }
 
 // Rows as operands want them: on 16 bytes, with zeros up to the next multiple of eight.
@@ -806,7 +877,7 @@ struct Room {
 // Rows that a tile's loads cannot take as they lie: off 16 bytes, too far apart, or (expanded tensors) one over the
 // other, so that what is past the last of them is not past the end of their buffer.
 bool off_units(const emrs_attention *a, const void *p, const uint64_t *strides) {
-  return a->dim % 8 || strides[0] < a->dim || strides[0] % 8 || strides[1] % 8 || !on(p, 16) || strides[0] > (1u << 23);
+  return a->dim % 8 || strides[0] < a->dim || strides[0] % 8 || strides[1] % 8 || !on(p, 16) || strides[0] > (1u << 22);
 }
 
 Room room_of(const emrs_attention *a, bool backward) {
@@ -870,7 +941,10 @@ const T *pad(const void *from, const uint64_t *strides, uint64_t rows, uint32_t 
 
 template <class T>
 void sum_parts(const float *parts, uint32_t splits, uint64_t each, void *out, hipStream_t st) {
-  if (each) attention_sum_kernel<T><<<(uint32_t)((each + 255) / 256), 256, 0, st>>>(parts, (int)splits, (int64_t)each, static_cast<T *>(out));
+  if (each % 4 == 0)  // outputs lie on 8 bytes
+    attention_sum_kernel<T, 4><<<(uint32_t)((each / 4 + 255) / 256), 256, 0, st>>>(parts, (int)splits, (int64_t)each, static_cast<T *>(out));
+  else
+    attention_sum_kernel<T, 1><<<(uint32_t)((each + 255) / 256), 256, 0, st>>>(parts, (int)splits, (int64_t)each, static_cast<T *>(out));
 }
 
 template <class T, int DIM>
@@ -892,15 +966,18 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   p.heads = (int32_t)a->heads, p.group = (int32_t)(a->heads / a->kv_heads), p.dim = (int32_t)dim8, p.real_dim = (int32_t)a->dim, p.causal = a->causal != 0;
   p.scale = a->scale, p.out = a->out, p.rest = a->out_rest, p.lse = a->lse;
   p.wide_out = a->dim % 8 == 0 && on(a->out, 16) && on(a->out_rest, 16);
+  p.wide_grads = a->dim % 8 == 0 && on(a->grad_q, 16) && on(a->grad_k, 16) && on(a->grad_v, 16);
   p.splits = (int32_t)key_splits(a);
   p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
   if (!backward) {
     if (a->rows == 0) return EMRS_OK;
     p.part_lse = reinterpret_cast<float *>(w + room.part_lse);
     attention_forward_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
-    if (p.splits > 1)
-      attention_join_kernel<T><<<(uint32_t)((a->rows * a->heads + 3) / 4), 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,
-                                                                                        (int)a->dim, static_cast<T *>(a->out), static_cast<T *>(a->out_rest), a->lse);
+    if (p.splits > 1) {
+      const uint32_t e = a->dim % 4 ? 1 : 4, blocks = (uint32_t)((a->rows * a->heads * (a->dim / e) + 255) / 256);
+      (e == 4 ? attention_join_kernel<T, 4> : attention_join_kernel<T, 1>)<<<blocks, 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,
+                                                                                                 (int)a->dim, static_cast<T *>(a->out), static_cast<T *>(a->out_rest), a->lse);
+    }
   } else {
     p.exponent = reinterpret_cast<float *>(w + room.exponent);
     p.delta = reinterpret_cast<float *>(w + room.delta);
@@ -926,7 +1003,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
       p.splits = (int32_t)head_splits(a);
       p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
       p.parts2 = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts2) : nullptr;
-      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
+      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), 64 * kPairs, 0, st>>>(p);
       if (p.splits > 1) {
         sum_parts<T>(p.parts, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_k, st);
         sum_parts<T>(p.parts2, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_v, st);
