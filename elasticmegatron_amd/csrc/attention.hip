@@ -229,6 +229,29 @@ struct OwnRows {
   }
 };
 
+// Products in a row: use(i, fragment) of each, with what comes D products later read right behind it, so that no
+// product waits for its own read.  The order is pinned: left to itself, where registers are short, the compiler reads
+// every fragment just before its product.  first(): the reads of the first D, to be started earlier.
+template <int N, int D, class F>
+struct Products {
+  F f[D];
+  template <class Read>
+  __device__ __forceinline__ void first(Read read) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) f[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  template <class Read, class Use>
+  __device__ __forceinline__ void run(Read read, Use use) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      use(i, f[i % D]);
+      if (i + D < N) f[i % D] = read(i + D);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
 // Eight of a lane's 16 values, in 16 bits, as operand b of the next product.
 template <class T>
 __device__ __forceinline__ typename emrs_gemm::Vec<T>::x8 eight_of(const f32x16 &v, int half) {
@@ -313,7 +336,8 @@ __device__ __forceinline__ Span share_of(int tiles, int split, int splits) {
 // ---- forward ----
 
 template <class T, int DIM>
-__global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attention p) {
+__global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward_kernel(Attention p) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
   constexpr int kBytes = kTile * DIM * 2;
   __shared__ __attribute__((aligned(1024))) char k_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char k_odd[kBytes];
@@ -363,14 +387,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
   auto work = [&](const char *kt, const char *vt, int t) __attribute__((always_inline)) {
     const int from = t * kTile;
     if (from >= seen_wave) return;
+    constexpr int kC = DIM / 16, kD = DIM / 32;
     f32x16 s[2];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = 0.f;
-#pragma unroll
-      for (int c = 0; c < DIM / 16; ++c) s[b] = mfma(reader.rows(kt, b, c), q.v[c], s[b]);
-    }
+    Products<2 * kC, 4, x8> scores;
+    auto key_rows = [&](int i) __attribute__((always_inline)) { return reader.rows(kt, i % 2, i / 2); };
+    scores.first(key_rows);
+    scores.run(key_rows, [&](int i, const x8 &f) __attribute__((always_inline)) { s[i % 2] = mfma(f, q.v[i / 2], s[i % 2]); });
+    Products<4 * kD, 4, x8> sums;
+    auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(vt, i % kD, i / kD); };
+    sums.first(columns);
     if (from + kTile > seen_by_all) {
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -395,19 +424,26 @@ __global__ __launch_bounds__(kThreads, 2) void attention_forward_kernel(Attentio
       top = next;
     }
     const float off = (top == -INFINITY ? 0.f : top) - kLift;
+    // Values 2 n and 2 n + 1 of the tile: the first eight before any product with v, the others between them, eight ahead.
+    auto exponentials = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], by, -off));
-        sum += s[b][r];
+      for (int e = 0; e < 2; ++e) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[n / 8][n % 8 * 2 + e], by, -off));
+        s[n / 8][n % 8 * 2 + e] = x;
+        sum += x;
       }
+    };
 #pragma unroll
-    for (int c = 0; c < kTile / 16; ++c) {
-      const auto prob = eight_of<T>(s[c >> 1], c & 1);
+    for (int n = 0; n < 4; ++n) exponentials(n);
+    x8 prob = eight_of<T>(s[0], 0);
+    sums.run(columns, [&](int i, const x8 &f) __attribute__((always_inline)) {
+      const int c = i / kD, d = i % kD;
+      if (i && d == 0) prob = eight_of<T>(s[c >> 1], c & 1);
+      out[d] = mfma(f, prob, out[d]);
+      if (c < 3)
 #pragma unroll
-      for (int d = 0; d < DIM / 32; ++d) out[d] = mfma(reader.columns(vt, d, c), prob, out[d]);
-    }
+        for (int n = 0; n < 4 / kD; ++n) exponentials((c + 1) * 4 + d * (4 / kD) + n);
+    });
   };
 
   load(k_even, v_even, tiles.first);
@@ -529,7 +565,8 @@ __global__ __launch_bounds__(256) void attention_largest_kernel(const T *x, Stri
 
 // grad_q, and on the way delta and the exponent (split 0 leaves them for grad_k).
 template <class T, int DIM>
-__global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention p) {
+__global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_grad_q_kernel(Attention p) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
   constexpr int kBytes = kTile * DIM * 2;
   __shared__ __attribute__((aligned(1024))) char k_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char k_odd[kBytes];
@@ -607,16 +644,24 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention
   auto work = [&](const char *kt, const char *vt, int t) __attribute__((always_inline)) {
     const int from = t * kTile;
     if (from >= seen_wave) return;
+    constexpr int kC = DIM / 16, kD = DIM / 32;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
-#pragma unroll
-      for (int c = 0; c < DIM / 16; ++c) {
-        s = mfma(reader.rows(kt, b, c), q.v[c], s);
-        dp = mfma(reader.rows(vt, b, c), g.v[c], dp);
-      }
+      Products<2 * kC, 4, x8> scores;
+      auto rows = [&](int i) __attribute__((always_inline)) { return reader.rows(i % 2 ? vt : kt, b, i / 2); };
+      scores.first(rows);
+      scores.run(rows, [&](int i, const x8 &f) __attribute__((always_inline)) {
+        if (i % 2)
+          dp = mfma(f, g.v[i / 2], dp);
+        else
+          s = mfma(f, q.v[i / 2], s);
+      });
+      Products<2 * kD, 4, x8> sums;
+      auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(kt, i % kD, b * 2 + i / kD); };
+      sums.first(columns);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float d = __builtin_amdgcn_exp2f(fmaf(s[r], by, -lse)) * (dp[r] - delta);
@@ -628,12 +673,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_q_kernel(Attention
         for (int r = 0; r < 16; ++r)
           if (from + b * 32 + row_of(r) >= seen_lane) s[r] = 0.f;
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const auto ds = eight_of<T>(s, c);
-#pragma unroll
-        for (int d = 0; d < DIM / 32; ++d) acc[d] = mfma(reader.columns(kt, d, b * 2 + c), ds, acc[d]);
-      }
+      const x8 ds[2] = {eight_of<T>(s, 0), eight_of<T>(s, 1)};
+      sums.run(columns, [&](int i, const x8 &f) __attribute__((always_inline)) { acc[i % kD] = mfma(f, ds[i / kD], acc[i % kD]); });
     }
   };
 
@@ -667,6 +708,7 @@ constexpr int kPairs = 2 * kWaves;
 
 template <class T, int DIM>
 __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Attention p) {
+  using x8 = typename emrs_gemm::Vec<T>::x8;
   constexpr int kBytes = kTile * DIM * 2;
   __shared__ __attribute__((aligned(1024))) char q_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char q_odd[kBytes];
@@ -737,41 +779,55 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
     const int from = (from_tile + work_tile) * kTile + half * 32;
     if (++work_tile == tiles) work_tile = 0;
     if (from + 32 <= first_wave || from >= queries) return;
+    asm("" : "+v"(reader.by_rows), "+v"(reader.by_columns));  // their exclusive ors are taken again: registers
     f32x16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
-#pragma unroll
-    for (int c = 0; c < DIM / 16; ++c) {
-      s = mfma(reader.rows(qt, half, c), k.v[c], s);
-      dp = mfma(reader.rows(gt, half, c), reader.rows(v_own, block, c), dp);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 exponent = *reinterpret_cast<const f32x4 *>(&sums[0][half * 32 + row_of(i * 4)]);
-      const f32x4 delta = *reinterpret_cast<const f32x4 *>(&sums[1][half * 32 + row_of(i * 4)]);
+    constexpr int kC = DIM / 16, kD = DIM / 32;
+    struct Rows {
+      x8 q, g, v;
+    };
+    Products<kC, 2, Rows> scores;
+    auto rows = [&](int c) __attribute__((always_inline)) { return Rows{reader.rows(qt, half, c), reader.rows(gt, half, c), reader.rows(v_own, block, c)}; };
+    scores.first(rows);
+    scores.run(rows, [&](int c, const Rows &f) __attribute__((always_inline)) {
+      s = mfma(f.q, k.v[c], s);
+      dp = mfma(f.g, f.v, dp);
+    });
+    struct Sums {
+      f32x4 exponent, delta;
+    };
+    Products<4, 2, Sums> values;
+    auto sums_of = [&](int i) __attribute__((always_inline)) {
+      return Sums{*reinterpret_cast<const f32x4 *>(&sums[0][half * 32 + row_of(i * 4)]), *reinterpret_cast<const f32x4 *>(&sums[1][half * 32 + row_of(i * 4)])};
+    };
+    values.first(sums_of);
+    Products<4 * kD, 4, x8> products;
+    auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(i % 2 ? qt : gt, i / 2 % kD, half * 2 + i / (2 * kD)); };
+    products.first(columns);
+    values.run(sums_of, [&](int i, const Sums &f) __attribute__((always_inline)) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -exponent[e]));
-        float d = x * (dp[i * 4 + e] - delta[e]);
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -f.exponent[e]));
+        float d = x * (dp[i * 4 + e] - f.delta[e]);
         if (kHalf) d *= lift;
         s[i * 4 + e] = kHalf ? x * 32768.f : x;
         dp[i * 4 + e] = d;
       }
-    }
+    });
     if (from < all_from || !all_valid) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (from + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
     }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const auto prob = eight_of<T>(s, c), ds = eight_of<T>(dp, c);
-#pragma unroll
-      for (int d = 0; d < DIM / 32; ++d) {
-        grad_v[d] = mfma(reader.columns(gt, d, half * 2 + c), prob, grad_v[d]);
-        grad_k[d] = mfma(reader.columns(qt, d, half * 2 + c), ds, grad_k[d]);
-      }
-    }
+    const x8 prob[2] = {eight_of<T>(s, 0), eight_of<T>(s, 1)}, ds[2] = {eight_of<T>(dp, 0), eight_of<T>(dp, 1)};
+    products.run(columns, [&](int i, const x8 &f) __attribute__((always_inline)) {
+      const int c = i / (2 * kD), d = i / 2 % kD;
+      if (i % 2)
+        grad_k[d] = mfma(f, ds[c], grad_k[d]);
+      else
+        grad_v[d] = mfma(f, prob[c], grad_v[d]);
+    });
   };
 
   load(q_even, g_even, sums_even, total > 0);
