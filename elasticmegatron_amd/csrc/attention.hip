@@ -127,7 +127,10 @@ __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, int
   const uint32_t tiles = (uint32_t)walk.tiles_before, total = tiles * heads * splits;
   const uint32_t q = total / kXcds, r = total % kXcds, x = blockIdx.x % kXcds, nth = blockIdx.x / kXcds;
   if (nth >= q + (x < r ? 1 : 0)) return false;
-  uint32_t t = x * q + min(x, r) + nth;
+  // Causal work falls along the places: of those that fill a XCD's CUs twice, the second half goes backwards, so that
+  // each CU begins with the same sum (4096 rows, 32 heads: 157 us against 161, grad_q 207 against 214).
+  constexpr uint32_t kCus = 32;
+  uint32_t t = x * q + min(x, r) + (kLastFirst && q >= 2 * kCus && nth >= kCus && nth < 2 * kCus ? 3 * kCus - 1 - nth : nth);
   const uint32_t chunk = (heads % kXcds ? 1 : heads / kXcds) * splits, each = chunk * tiles;
   const uint32_t first_head = t / each * chunk;
   t -= t / each * each;
@@ -261,7 +264,19 @@ __device__ __forceinline__ typename emrs_gemm::Vec<T>::x8 eight_of(const f32x16 
   return o;
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// Both halves of the wave's values, exchanged without a way through LDS.
+__device__ __forceinline__ float2 both_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+  const float2 x = both_halves(v);
+  return x.x + x.y;
+}
+__device__ __forceinline__ float most_of_halves(float v) {
+  const float2 x = both_halves(v);
+  return fmaxf(x.x, x.y);
+}
 
 struct Strides {
   int64_t row, head;
@@ -407,12 +422,14 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward
         for (int r = 0; r < 16; ++r)
           if (from + b * 32 + row_of(r) >= seen_lane) s[b][r] = -INFINITY;
     }
-    float most = s[0][0];
+    float tops[4];  // in four chains: one would be 16 dependent instructions
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int i = 0; i < 4; ++i) {
+      tops[i] = s[i >> 1][(i & 1) * 8];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][r]);
-    most = fmaxf(most, other_half(most)) * by;
+      for (int r = 1; r < 8; ++r) tops[i] = fmaxf(tops[i], s[i >> 1][(i & 1) * 8 + r]);
+    }
+    const float most = most_of_halves(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * by;
     // The sums are brought to a new maximum only where exponents would grow past the slack.
     if (__any(most > top + kSlack)) {
       const float next = fmaxf(top, most), less = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
@@ -458,7 +475,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward
   }
   arrive();  // no load may still be on its way into LDS that another workgroup gets
 
-  sum += other_half(sum);
+  sum = sum_of_halves(sum);
   const float lse = sum == 0.f ? -INFINITY : (top - kLift) * kLn2 + logf(sum);
   const float norm = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t place = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
@@ -565,7 +582,7 @@ __global__ __launch_bounds__(256) void attention_largest_kernel(const T *x, Stri
 
 // grad_q, and on the way delta and the exponent (split 0 leaves them for grad_k).
 template <class T, int DIM>
-__global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_grad_q_kernel(Attention p) {
+__global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_kernel(Attention p) {
   using x8 = typename emrs_gemm::Vec<T>::x8;
   constexpr int kBytes = kTile * DIM * 2;
   __shared__ __attribute__((aligned(1024))) char k_even[kBytes];
@@ -607,7 +624,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_grad_q_
     lse = p.lse[(int64_t)at.head * p.queries.rows + row] * kLog2e;
     if (lse == -INFINITY) lse = INFINITY;  // sees nothing: probabilities of 0
   }
-  delta += other_half(delta);
+  delta = sum_of_halves(delta);
   if (valid && lane < 32 && at.split == 0) {
     p.exponent[(int64_t)at.head * p.queries.rows + row] = lse;
     p.delta[(int64_t)at.head * p.queries.rows + row] = delta;
@@ -747,8 +764,13 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
   TileLoader<T, DIM, kPairs> q_loader, g_loader;
   q_loader.init(p.q_at.row, p.dim, wave);
   g_loader.init(p.grad_out_at.row, p.dim, wave);
-  TileReader<T, DIM> reader;
+  // Of the wave's half of a tile, and of its keys: the places are far above the bits that exclusive ors change.
+  TileReader<T, DIM> reader, own_reader;
   reader.init();
+  own_reader = reader;
+  reader.by_rows += half * 32 * reader.kRow;
+  reader.by_columns += half * 32 * reader.kRow;
+  own_reader.by_rows += block * 32 * reader.kRow;
   const T *const q = static_cast<const T *>(p.q) + at.other.first * p.q_at.row;
   const T *const g = static_cast<const T *>(p.grad_out) + at.other.first * p.grad_out_at.row;
   // The next tile to be loaded and the one that is worked on: tile of a head, head.
@@ -779,7 +801,7 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
     const int from = (from_tile + work_tile) * kTile + half * 32;
     if (++work_tile == tiles) work_tile = 0;
     if (from + 32 <= first_wave || from >= queries) return;
-    asm("" : "+v"(reader.by_rows), "+v"(reader.by_columns));  // their exclusive ors are taken again: registers
+    asm("" : "+v"(reader.by_rows), "+v"(reader.by_columns), "+v"(own_reader.by_rows));  // their exclusive ors are taken again: registers
     f32x16 s, dp;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
@@ -788,12 +810,15 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
       x8 q, g, v;
     };
     Products<kC, 2, Rows> scores;
-    auto rows = [&](int c) __attribute__((always_inline)) { return Rows{reader.rows(qt, half, c), reader.rows(gt, half, c), reader.rows(v_own, block, c)}; };
+    auto rows = [&](int c) __attribute__((always_inline)) { return Rows{reader.rows(qt, 0, c), reader.rows(gt, 0, c), own_reader.rows(v_own, 0, c)}; };
+    // What the matrix units wait for goes first: the other wave's arithmetic fills what is left (2.5%).
+    __builtin_amdgcn_s_setprio(1);
     scores.first(rows);
     scores.run(rows, [&](int c, const Rows &f) __attribute__((always_inline)) {
       s = mfma(f.q, k.v[c], s);
       dp = mfma(f.g, f.v, dp);
     });
+    __builtin_amdgcn_s_setprio(0);
     struct Sums {
       f32x4 exponent, delta;
     };
@@ -802,8 +827,8 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
       return Sums{*reinterpret_cast<const f32x4 *>(&sums[0][half * 32 + row_of(i * 4)]), *reinterpret_cast<const f32x4 *>(&sums[1][half * 32 + row_of(i * 4)])};
     };
     values.first(sums_of);
-    Products<4 * kD, 4, x8> products;
-    auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(i % 2 ? qt : gt, i / 2 % kD, half * 2 + i / (2 * kD)); };
+    Products<4 * kD, 3, x8> products;
+    auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(i % 2 ? qt : gt, i / 2 % kD, i / (2 * kD)); };
     products.first(columns);
     values.run(sums_of, [&](int i, const Sums &f) __attribute__((always_inline)) {
 #pragma unroll
@@ -821,6 +846,7 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
         if (from + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
     }
     const x8 prob[2] = {eight_of<T>(s, 0), eight_of<T>(s, 1)}, ds[2] = {eight_of<T>(dp, 0), eight_of<T>(dp, 1)};
+    __builtin_amdgcn_s_setprio(1);
     products.run(columns, [&](int i, const x8 &f) __attribute__((always_inline)) {
       const int c = i / (2 * kD), d = i / 2 % kD;
       if (i % 2)
@@ -828,6 +854,7 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
       else
         grad_v[d] = mfma(f, prob[c], grad_v[d]);
     });
+    __builtin_amdgcn_s_setprio(0);
   };
 
   load(q_even, g_even, sums_even, total > 0);
