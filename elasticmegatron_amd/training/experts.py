@@ -149,7 +149,8 @@ class _Call:
                 step = gw[0].element_size() * self.n_out * self.shape[1]
                 table = _table([gw[0].data_ptr() + i * step for i in range(self.experts)])
             else:
-                gw = [torch.empty(self.size, dtype=self.dtype, device=self.device) for _ in range(self.experts)]
+                # One allocation: that of each for itself is most of a small call's host time.
+                gw = torch.empty((self.experts, *self.size), dtype=self.dtype, device=self.device).unbind(0)
                 table = _table([g.data_ptr() for g in gw])
             a.grad_weights = ctypes.addressof(table)
         if gw or (want_x and self.shape[0]):
@@ -186,8 +187,8 @@ def expert_linear(x: torch.Tensor, weights: Weights, counts: torch.Tensor) -> to
     more than there are rows, rows end first.
 
     ``weights``: one matrix [n_out, n_in] for every expert (1 to 256), as a state holds them, or a tensor
-    [experts, n_out, n_in]; of ``x``'s type.  Differentiable once, to ``x`` and to every matrix; an expert without
-    rows has a gradient of zeros.  Rows that lie off 16 bytes, or whose length is no multiple of 8, are copied first."""
+    [experts, n_out, n_in]; of ``x``'s type.  Differentiable once, to ``x`` and to every matrix (whose gradients share
+    one allocation); an expert without rows has a gradient of zeros.  Rows that lie off 16 bytes, or whose length is no multiple of 8, are copied first."""
     weights = [weights] if isinstance(weights, torch.Tensor) else list(weights)
     if not weights:
         raise ValueError("no weights are given")

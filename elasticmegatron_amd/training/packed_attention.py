@@ -71,7 +71,7 @@ class _Call:
         if not 0 < scale < math.inf:
             raise ValueError(f"scale is {scale}: a positive number is wanted")
         a = self.record = _native.Attention()
-        (q, a.q_strides[:]), (k, a.k_strides[:]), (v, a.v_strides[:]) = (_operand(t if t.dim() == 3 else t.flatten(0, 1)) for t in (q, k, v))
+        (q, a.q_strides[:]), (k, a.k_strides[:]), (v, a.v_strides[:]) = (_operand(t if t.dim() == 3 else t.detach().flatten(0, 1)) for t in (q, k, v))
         a.dtype, a.causal, a.heads, a.kv_heads, a.dim = DTYPE_CODES[self.dtype], 1 if causal else 0, heads, kv_heads, dim
         a.rows, a.key_rows, a.scale = q.shape[0], k.shape[0], scale
         a.documents = max(1, self.shape[0]) if len(self.shape) == 4 else 1

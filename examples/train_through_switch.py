@@ -3,14 +3,13 @@
     python examples/train_through_switch.py [--steps 12] [--switch-at 6]
 
 Every rank's state lives on one GPU, as the resharding manager holds it.  A step runs the model forward and
-backward (plain torch; the loss over the output layer's vocabulary shards as the state holds them is
-``training.linear_cross_entropy``), then updates the state: ``training.muon_step`` on the matrices of the
+backward (norms, attention and the loss over the output layer's vocabulary shards as the state holds them are
+``training``'s, projections torch's), then updates the state: ``training.muon_step`` on the matrices of the
 layers, gathered from their shards, ``training.adamw_step`` on every rank's own shard of the rest.  In the
 middle the job switches from TP1 to TP2 with ``ElasticMegatronManager.reshard``, and training goes on.
 """
 
 import argparse
-import math
 import os
 import sys
 
@@ -98,29 +97,27 @@ def is_matrix_of_a_layer(vp):
     return len(vp.full_shape) == 2 and "embedding" not in vp.param_def.name and "output_layer" not in vp.param_def.name
 
 
-def rms_norm(x, weight):
-    return (x.float() * torch.rsqrt(x.float().square().mean(-1, keepdim=True) + 1e-5) * weight.float()).to(x.dtype)
-
-
 def attention(x, qkv, proj, heads):
     b, n, h = x.shape
-    q, k, v = (x @ qkv.t()).view(b, n, heads, 3, h // heads).float().permute(3, 0, 2, 1, 4).contiguous().unbind(0)
-    scores = (q @ k.transpose(-1, -2).contiguous()) / math.sqrt(h // heads)
-    scores = scores.masked_fill(torch.ones(n, n, dtype=torch.bool, device=x.device).triu(1), -math.inf)
-    out = (scores.softmax(-1) @ v).to(x.dtype)
-    return out.transpose(1, 2).reshape(b, n, h) @ proj.t()
+    q, k, v = (x @ qkv.t()).view(b, n, heads, 3, h // heads).unbind(3)
+    return training.attention(q, k, v).view(b, n, h) @ proj.t()
+
+
+def feed_forward(x, fc1, fc2):
+    gate, up = (x @ fc1.t()).chunk(2, -1)
+    return (torch.nn.functional.silu(gate) * up) @ fc2.t()
 
 
 def hidden_states(spec, weights, tokens):
     x = weights["embedding.word_embeddings.weight"][tokens]
+    y = training.rms_norm(x, weights["0.self_attention.linear_qkv.layer_norm_weight"])
     for layer in range(spec.num_layers):
         w = lambda name: weights[f"{layer}.{name}"]  # noqa: E731
-        y = rms_norm(x, w("self_attention.linear_qkv.layer_norm_weight"))
-        x = x + attention(y, w("self_attention.linear_qkv.weight"), w("self_attention.linear_proj.weight"), spec.num_attention_heads)
-        y = rms_norm(x, w("mlp.linear_fc1.layer_norm_weight")) @ w("mlp.linear_fc1.weight").t()
-        gate, up = y.chunk(2, -1)
-        x = x + (torch.nn.functional.silu(gate) * up) @ w("mlp.linear_fc2.weight").t()
-    return rms_norm(x, weights["decoder.final_layernorm.weight"])
+        branch = attention(y, w("self_attention.linear_qkv.weight"), w("self_attention.linear_proj.weight"), spec.num_attention_heads)
+        x, y = training.residual_norm(x, branch, w("mlp.linear_fc1.layer_norm_weight"))
+        after = f"{layer + 1}.self_attention.linear_qkv.layer_norm_weight" if layer + 1 < spec.num_layers else "decoder.final_layernorm.weight"
+        x, y = training.residual_norm(x, feed_forward(y, w("mlp.linear_fc1.weight"), w("mlp.linear_fc2.weight")), weights[after])
+    return y
 
 
 def key_of(vp):
