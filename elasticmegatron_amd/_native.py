@@ -470,11 +470,15 @@ def norm_workspace(a: Norm) -> int:
 
 
 def norm_forward(a: Norm, stream: int = 0) -> None:
-    _check(load().emrs_norm_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_norm_forward")
+    rc = (_lib or load()).emrs_norm_forward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_norm_forward")
 
 
 def norm_backward(a: Norm, stream: int = 0) -> None:
-    _check(load().emrs_norm_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_norm_backward")
+    rc = (_lib or load()).emrs_norm_backward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_norm_backward")
 
 
 def experts_workspace(a: Experts, backward: bool) -> int:
@@ -485,11 +489,15 @@ def experts_workspace(a: Experts, backward: bool) -> int:
 
 
 def experts_forward(a: Experts, stream: int = 0) -> None:
-    _check(load().emrs_experts_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_experts_forward")
+    rc = (_lib or load()).emrs_experts_forward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_experts_forward")
 
 
 def experts_backward(a: Experts, stream: int = 0) -> None:
-    _check(load().emrs_experts_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_experts_backward")
+    rc = (_lib or load()).emrs_experts_backward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_experts_backward")
 
 
 def attention_workspace(a: Attention, backward: bool) -> int:
@@ -500,8 +508,12 @@ def attention_workspace(a: Attention, backward: bool) -> int:
 
 
 def attention_forward(a: Attention, stream: int = 0) -> None:
-    _check(load().emrs_attention_forward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_attention_forward")
+    rc = (_lib or load()).emrs_attention_forward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_attention_forward")
 
 
 def attention_backward(a: Attention, stream: int = 0) -> None:
-    _check(load().emrs_attention_backward(ctypes.byref(a), ctypes.c_void_p(int(stream))), "emrs_attention_backward")
+    rc = (_lib or load()).emrs_attention_backward(ctypes.byref(a), stream)
+    if rc:
+        _check(rc, "emrs_attention_backward")

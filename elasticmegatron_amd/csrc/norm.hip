@@ -45,14 +45,14 @@ int run(const emrs_norm *a, bool backward, hipStream_t st) {
   if (rc) return rc;
   if (a->gate_kind > EMRS_NORM_GATE_TOKEN) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: unknown kind of gate");
   const uint64_t h = a->hidden;
-  if (!a->branch && (a->gate_kind || a->branch_weight || a->grad_branch || a->grad_gate || a->grad_branch_weight))
+  const bool full = a->gate_kind || a->branch_weight;
+  if (!a->branch && (full || a->grad_gate || a->grad_branch_weight))
     return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: a gate or a branch's norm without a branch");
   if (a->gate_kind && !a->gate) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: NULL gate");
   if (a->grad_gate && !a->gate_kind) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: a gradient of no gate");
   if (a->grad_branch_weight && !a->branch_weight) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: a gradient of no branch weight");
   if ((a->branch && a->branch_stride < h) || (a->gate_kind == EMRS_NORM_GATE_TOKEN && a->gate_stride < h))
     return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: rows overlap");
-  const bool full = a->branch && (a->gate_kind || a->branch_weight);
   if (!backward) {
     if (!a->stream && !a->normed) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: nothing is wanted");
     if (a->normed && !a->weight) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: NULL weight");

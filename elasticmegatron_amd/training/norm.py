@@ -17,6 +17,8 @@ from ._common import DTYPE_CODES, dtype_code, lies, on_device, refuse_tangents, 
 
 def _rows(t: torch.Tensor, h: int):
     """``t`` as rows [n, h] with unit column stride that do not overlap, and the stride between them."""
+    if t.is_contiguous():
+        return t, h
     if t.dim() != 2:
         t = t.detach().reshape(-1, h)
     (n, _), (over, along) = t.size(), t.stride()
@@ -32,8 +34,8 @@ def _vector(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() else t.detach().contiguous()
 
 
-def _check(residual, branch, gate, branch_weight, weight) -> int:
-    """Raises for the first argument that is not as it has to be; the kind of gate."""
+def _refuse(residual, branch, gate, branch_weight, weight) -> None:
+    """Raises for the first argument that is not as it has to be."""
     if not isinstance(residual, torch.Tensor):
         raise TypeError("residual is no tensor")
     device = residual.device
@@ -42,50 +44,59 @@ def _check(residual, branch, gate, branch_weight, weight) -> int:
     if residual.dim() < 1 or not 1 <= residual.shape[-1] <= _native.EMRS_NORM_MAX_HIDDEN:
         raise ValueError(f"residual is {tuple(residual.shape)}: [..., h] with h from 1 to {_native.EMRS_NORM_MAX_HIDDEN} is wanted")
     size, first = residual.size(), None
-    vector = size[-1:]
     for what, t in (("branch", branch), ("weight", weight), ("branch_weight", branch_weight), ("gate", gate)):
         if t is None:
             continue
-        if not (isinstance(t, torch.Tensor) and t.device == device):
-            on_device(what, t, device)
+        on_device(what, t, device)
         first = first or (what, t.dtype)
-        if t.dtype != first[1] or t.dtype not in (torch.bfloat16, torch.float16):
-            dtype_code(t, what, (torch.bfloat16, torch.float16))
+        dtype_code(t, what, (torch.bfloat16, torch.float16))
+        if t.dtype != first[1]:
             raise TypeError(f"{what} is {t.dtype}, {first[0]} {first[1]}")
         if what == "branch" and t.size() != size:
             raise ValueError(f"branch {tuple(t.shape)} does not fit residual {tuple(size)}")
-        if what in ("weight", "branch_weight") and t.size() != vector:
+        if what in ("weight", "branch_weight") and t.size() != size[-1:]:
             raise ValueError(f"{what} is {tuple(t.shape)}: [{size[-1]}] is wanted")
     if first is None:
         raise ValueError("neither a branch nor a weight is given")
     if residual.dtype not in (torch.float32, first[1]):
         raise TypeError(f"residual is {residual.dtype}: torch.float32 or {first[0]}'s {first[1]} is wanted")
-    if gate is None:
-        return _native.EMRS_NORM_GATE_NONE
-    if branch is None:
+    if gate is not None and branch is None:
         raise ValueError("a gate without a branch")
-    if gate.size() == size:
-        return _native.EMRS_NORM_GATE_TOKEN
-    if gate.size() != vector:
+    if gate is not None and gate.size() not in (size, size[-1:]):
         raise ValueError(f"gate is {tuple(gate.shape)}: [{size[-1]}] or branch's {tuple(size)} is wanted")
-    return _native.EMRS_NORM_GATE_CHANNEL
 
 
-def _address(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+_HALVES = (torch.bfloat16, torch.float16)
+
+
+def _fits(t, device, dtype, size) -> bool:
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == device and t.size() == size
 
 
 def _record(residual, branch, gate, branch_weight, weight, scale, eps):
-    """The record with what both passes read, and those tensors: rows and vectors as the kernels take them."""
-    kind = _check(residual, branch, gate, branch_weight, weight)
-    h = residual.shape[-1]
-    a = _native.Norm(DTYPE_CODES[(weight if branch is None else branch).dtype], DTYPE_CODES[residual.dtype], kind, 0, residual.numel() // h, h)
+    """The record with what both passes read, and those tensors: rows and vectors as the kernels take them.
+
+    Small calls are host time for the most part: what is right is found at once, and what is not, one by one."""
+    model = weight if branch is None else branch
+    if not (isinstance(residual, torch.Tensor) and isinstance(model, torch.Tensor) and residual.is_cuda and residual.dim()):
+        _refuse(residual, branch, gate, branch_weight, weight)
+    device, size, dtype = residual.device, residual.size(), model.dtype
+    h, vector = size[-1], size[-1:]
+    if not (dtype in _HALVES and (residual.dtype is dtype or residual.dtype is torch.float32) and 1 <= h <= _native.EMRS_NORM_MAX_HIDDEN and
+            (branch is None or _fits(branch, device, dtype, size)) and (weight is None or _fits(weight, device, dtype, vector)) and
+            (branch_weight is None or _fits(branch_weight, device, dtype, vector)) and
+            (gate is None or branch is not None and (_fits(gate, device, dtype, size) or _fits(gate, device, dtype, vector)))):
+        _refuse(residual, branch, gate, branch_weight, weight)
+    a = _native.Norm(DTYPE_CODES[dtype], DTYPE_CODES[residual.dtype], _native.EMRS_NORM_GATE_NONE, 0, residual.numel() // h, h)
     a.residual_scale, a.eps = scale, eps
     if branch is not None:
         branch, a.branch_stride = _rows(branch, h)
         a.branch = branch.data_ptr()
         if gate is not None:
-            gate, a.gate_stride = _rows(gate, h) if kind == _native.EMRS_NORM_GATE_TOKEN else (_vector(gate), h)
+            if gate.size() == size:
+                a.gate_kind, (gate, a.gate_stride) = _native.EMRS_NORM_GATE_TOKEN, _rows(gate, h)
+            else:
+                a.gate_kind, gate = _native.EMRS_NORM_GATE_CHANNEL, _vector(gate)
             a.gate = gate.data_ptr()
         if branch_weight is not None:
             branch_weight = _vector(branch_weight)
@@ -93,24 +104,32 @@ def _record(residual, branch, gate, branch_weight, weight, scale, eps):
     if weight is not None:
         weight = _vector(weight)
         a.weight = weight.data_ptr()
-    return a, (branch, gate, branch_weight, weight)
+    return a, branch, gate, branch_weight, weight
 
 
 def _forward(residual, branch, gate, branch_weight, weight, scale, eps, statistics):
-    """``(stream or None, normed or None, statistics or None, the record, the tensors that it points to)``."""
-    a, read = _record(residual, branch, gate, branch_weight, weight, scale, eps)
+    """``(stream or None, normed or None, statistics or None, the record, what backward reads of the others)``."""
+    a, rows, gate, branch_weight, weight = _record(residual, branch, gate, branch_weight, weight, scale, eps)
     size, device, tokens = residual.size(), residual.device, a.tokens
-    stream = None if branch is None else torch.empty(size, dtype=residual.dtype, device=device)
-    normed = None if weight is None else torch.empty(size, dtype=weight.dtype, device=device)
-    rms = torch.empty((2, tokens), dtype=torch.float32, device=device) if statistics else None
+    stream = normed = rms = None
+    if branch is not None:
+        stream = torch.empty(size, dtype=residual.dtype, device=device)
+        a.stream = stream.data_ptr()
+    if weight is not None:
+        normed = torch.empty(size, dtype=weight.dtype, device=device)
+        a.normed = normed.data_ptr()
+    if statistics:
+        rms = torch.empty((2, tokens), dtype=torch.float32, device=device)
+        a.stream_rms = at = rms.data_ptr()
+        a.branch_rms = at + 4 * tokens
     if tokens:
-        rows, a.residual_stride = _rows(residual, a.hidden)
-        a.residual, a.stream, a.normed = rows.data_ptr(), _address(stream), _address(normed)
-        if statistics:
-            a.stream_rms = rms.data_ptr()
-            a.branch_rms = a.stream_rms + 4 * tokens
+        flat, a.residual_stride = _rows(residual, a.hidden)
+        a.residual = flat.data_ptr()
         run_on(device, _native.norm_forward, a)
-    return stream, normed, rms, a, read
+    # With nothing between the branch and the stream, backward does not read it, and the graph does not keep it.
+    if gate is None and branch_weight is None:
+        rows = a.branch = None
+    return stream, normed, rms, a, (rows, gate, branch_weight, weight)
 
 
 class _ResidualNorm(torch.autograd.Function):
@@ -118,10 +137,9 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, residual, branch, gate, branch_weight, weight, scale, eps):
         stream, normed, rms, a, read = _forward(residual, branch, gate, branch_weight, weight, scale, eps, True)
         # What the kernels read: the inputs, or the copies that had to be made of them.
-        saved = (residual if stream is None else stream, *read, rms)
+        saved = [residual if stream is None else stream, rms, *[t for t in read if t is not None]]
         ctx.save_for_backward(*saved)
-        ctx.record, ctx.lies = a, lies(*saved)
-        ctx.likes = [None if t is None else t.size() for t in (residual, branch, gate, branch_weight, weight)]
+        ctx.record, ctx.lies, ctx.has, ctx.size = a, lies(*saved), [t is not None for t in read], residual.size()
         ctx.set_materialize_grads(False)
         if stream is None:
             return normed
@@ -130,51 +148,53 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        saved = ctx.saved_tensors  # raises where one was changed in place
-        stream, branch, gate, branch_weight, weight, rms = saved
-        a, likes, need = ctx.record, ctx.likes, ctx.needs_input_grad
-        grad_stream = None if branch is None else grads[0]
-        grad_normed = None if weight is None else grads[-1]
+        stream, rms, *others = saved = ctx.saved_tensors  # raises where one was changed in place
+        need, size, has = ctx.needs_input_grad, ctx.size, ctx.has
+        # Without a branch there is no stream to be differentiated to, without a weight no norm.
+        grad_normed = grads[-1] if has[3] else None
+        grad_stream = grads[0] if len(grads) > 1 or not has[3] else None
         if grad_stream is None and grad_normed is None:
             return (None,) * 7
-        device, shape, h = stream.device, likes[0], likes[0][-1]
         if lies(*saved) == ctx.lies:
-            a = _native.Norm.from_buffer_copy(a)
-        else:  # hooks on saved tensors handed back others
-            on_device("the statistics", rms, device)
-            if rms.size() != (2, a.tokens) or rms.dtype != torch.float32:
-                raise ValueError("the saved statistics are not those of the forward pass")
-            rms = rms.contiguous()
-            back = [None if t is None else t.reshape(like) for t, like in zip((stream, branch, gate, branch_weight, weight), likes)]
-            a, (branch, gate, branch_weight, weight) = _record(*back, a.residual_scale, a.eps)
-            stream = back[0]
-        tokens, dtype = a.tokens, (weight if branch is None else branch).dtype
+            a = _native.Norm.from_buffer_copy(ctx.record)
+        else:
+            a, stream, rms, *others = _again(ctx, stream, rms, others)
+        device, tokens, h, dtype = stream.device, a.tokens, size[-1], others[0].dtype if others else None
+        dtype = dtype or _DTYPES[a.dtype]
+        out = torch.empty
         # With nothing between them, residual and branch have one gradient, as those of a sum have.
-        one = need[0] and need[1] and gate is None and branch_weight is None and a.residual_scale == 1.0 and stream.dtype == dtype
-        sums = need[3] or (need[4] and grad_normed is not None) or (need[2] and a.gate_kind == _native.EMRS_NORM_GATE_CHANNEL)
-        gr = torch.empty(shape, dtype=stream.dtype, device=device) if need[0] else None
-        gb = torch.empty(shape, dtype=dtype, device=device) if need[1] and not one else None
-        gg = torch.empty(likes[2], dtype=dtype, device=device) if need[2] else None
-        gbw = torch.empty(likes[3], dtype=dtype, device=device) if need[3] else None
-        gw = torch.empty(likes[4], dtype=dtype, device=device) if need[4] and grad_normed is not None else None
+        one = need[0] and need[1] and not has[0] and a.residual_scale == 1.0 and stream.dtype is dtype
+        gr = out(size, dtype=stream.dtype, device=device) if need[0] else None
+        gb = out(size, dtype=dtype, device=device) if need[1] and not one else None
+        gg = gbw = gw = None
+        if need[2]:
+            gg = out(size if a.gate_kind == _native.EMRS_NORM_GATE_TOKEN else size[-1:], dtype=dtype, device=device)
+        if need[3]:
+            gbw = out(size[-1:], dtype=dtype, device=device)
+        if need[4] and grad_normed is not None:
+            gw = out(size[-1:], dtype=dtype, device=device)
         if tokens:
-            keep = []
-            a.stream = a.grad_stream = a.grad_normed = a.normed = None
+            a.stream = a.normed = None
             if grad_normed is not None:
                 rows, a.stream_stride = _rows(stream, h)
                 if not (grad_normed.dtype is dtype and grad_normed.is_contiguous()):
                     grad_normed = grad_normed.to(dtype).contiguous()
-                keep += [rows, grad_normed]
                 a.stream, a.grad_normed = rows.data_ptr(), grad_normed.data_ptr()
             if grad_stream is not None:
                 if not (grad_stream.dtype is stream.dtype and grad_stream.is_contiguous()):
                     grad_stream = grad_stream.to(stream.dtype).contiguous()
                 a.grad_stream = grad_stream.data_ptr()
-            a.stream_rms = rms.data_ptr()
-            a.branch_rms = a.stream_rms + 4 * tokens
-            a.grad_residual, a.grad_branch, a.grad_gate = _address(gr), _address(gb), _address(gg)
-            a.grad_branch_weight, a.grad_weight = _address(gbw), _address(gw)
-            if sums:
+            if gr is not None:
+                a.grad_residual = gr.data_ptr()
+            if gb is not None:
+                a.grad_branch = gb.data_ptr()
+            if gg is not None:
+                a.grad_gate = gg.data_ptr()
+            if gbw is not None:
+                a.grad_branch_weight = gbw.data_ptr()
+            if gw is not None:
+                a.grad_weight = gw.data_ptr()
+            if gw is not None or gbw is not None or (gg is not None and a.gate_kind == _native.EMRS_NORM_GATE_CHANNEL):
                 scratch = workspace(_native.norm_workspace(a), device)
                 a.workspace, a.workspace_bytes = scratch.data_ptr(), scratch.numel()
             run_on(device, _native.norm_backward, a)
@@ -185,12 +205,44 @@ class _ResidualNorm(torch.autograd.Function):
         return gr, gr if one else gb, gg, gbw, gw, None, None
 
 
+_DTYPES = {code: dtype for dtype, code in DTYPE_CODES.items()}
+
+
+def _again(ctx, stream, rms, others):
+    """The record anew, for tensors that hooks on saved tensors handed back; and those tensors."""
+    a, size, rest = ctx.record, ctx.size, iter(others)
+    on_device("the stream", stream, stream.device)
+    on_device("the statistics", rms, stream.device)
+    if rms.size() != (2, a.tokens) or rms.dtype != torch.float32 or stream.numel() != size.numel() or stream.dtype != _DTYPES[a.residual_dtype]:
+        raise ValueError("the saved tensors are not those of the forward pass")
+    branch, gate, branch_weight, weight = (next(rest) if has else None for has in ctx.has)
+    stream = stream.reshape(size)
+    branch = None if branch is None else branch.reshape(size)
+    if gate is not None:
+        gate = gate.reshape(size if a.gate_kind == _native.EMRS_NORM_GATE_TOKEN else size[-1:])
+    if branch is None and weight is None:  # a sum alone
+        b = _native.Norm.from_buffer_copy(a)
+    else:
+        b, *others = _record(stream, branch, gate, branch_weight, weight, a.residual_scale, a.eps)
+        if b.dtype != a.dtype:
+            raise ValueError("the saved tensors are not those of the forward pass")
+        others = [t for t in others if t is not None]
+    rms = rms.contiguous()
+    b.gate_kind, b.stream_rms = a.gate_kind, rms.data_ptr()
+    b.branch_rms = b.stream_rms + 4 * a.tokens
+    return (b, stream, rms, *others)
+
+
+def _wants_gradient(t) -> bool:
+    return isinstance(t, torch.Tensor) and t.requires_grad
+
+
 def _call(residual, branch, gate, branch_weight, weight, scale, eps):
-    tensors = (residual, branch, gate, branch_weight, weight)
-    refuse_tangents(*tensors)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        return _ResidualNorm.apply(*tensors, scale, eps)
-    stream, normed = _forward(*tensors, scale, eps, False)[:2]
+    refuse_tangents(residual, branch, gate, branch_weight, weight)
+    if torch.is_grad_enabled() and (_wants_gradient(residual) or _wants_gradient(branch) or _wants_gradient(weight) or _wants_gradient(gate) or
+                                    _wants_gradient(branch_weight)):
+        return _ResidualNorm.apply(residual, branch, gate, branch_weight, weight, scale, eps)
+    stream, normed = _forward(residual, branch, gate, branch_weight, weight, scale, eps, False)[:2]
     if stream is None:
         return normed
     return stream if normed is None else (stream, normed)

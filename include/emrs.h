@@ -568,7 +568,7 @@ typedef struct emrs_norm {
   uint64_t hidden;                /* 1 to 16384 */
   const void *residual;           /* [tokens][hidden], rows *_stride elements apart: forward */
   uint64_t residual_stride;
-  const void *branch;
+  const void *branch;             /* backward: read where it has a norm or a gate */
   uint64_t branch_stride;
   const void *gate;
   uint64_t gate_stride;           /* of a gate for each token */
