@@ -718,33 +718,32 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
 }
 
 // grad_k and grad_v of one head of keys: the sums over the queries of every head that shares it, or, with splits, of
-// a run of these heads.  Two waves share 32 keys, each with its own half of a tile's queries, and add their sums at the
-// end: that makes two waves for each SIMD, whose turns at the matrix units and at everything else fill each other's
-// waits.  What a wave holds of its keys and both sums leaves no registers for v, which stays in LDS.
-constexpr int kPairs = 2 * kWaves;
+// a run of these heads.  Tiles of 32 queries, and v in LDS: what a wave holds of its keys and both sums leaves no
+// registers for it.  So two workgroups fit a CU, and the two waves of a SIMD, which no barrier joins, fill each other's
+// waits.  (One workgroup of two waves for each 32 keys, which take the same turns at the matrix units: 4096 rows, 32
+// heads of 128 in 296 us; one wave for each SIMD, v in registers: 357.)
+constexpr int kQueries = 32;
 
 template <class T, int DIM>
-__global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Attention p) {
+__global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attention p) {
   using x8 = typename emrs_gemm::Vec<T>::x8;
-  constexpr int kBytes = kTile * DIM * 2;
-  __shared__ __attribute__((aligned(1024))) char q_even[kBytes];
-  __shared__ __attribute__((aligned(1024))) char q_odd[kBytes];
-  __shared__ __attribute__((aligned(1024))) char g_even[kBytes];
-  __shared__ __attribute__((aligned(1024))) char g_odd[kBytes];
+  constexpr int kBytes = kQueries * DIM * 2;
+  __shared__ __attribute__((aligned(1024))) char even[2 * kBytes];  // rows of q and of grad_out
+  __shared__ __attribute__((aligned(1024))) char odd[2 * kBytes];
   __shared__ __attribute__((aligned(1024))) char v_own[kOwn * DIM * 2];
-  __shared__ __attribute__((aligned(256))) float sums_even[2][kTile];  // exponent and delta of the tile's queries
-  __shared__ __attribute__((aligned(256))) float sums_odd[2][kTile];
+  __shared__ __attribute__((aligned(256))) float sums_even[2][64];  // exponent and delta of the tile's queries, and zeros
+  __shared__ __attribute__((aligned(256))) float sums_odd[2][64];
   const int kv_heads = p.heads / p.group;
   Place at;
   if (!find<false>(p.keys, p.queries, kv_heads, p.splits, at)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of(), half = wave / kWaves, block = wave % kWaves;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
   const int keys = at.own.end - at.own.first, queries = at.other.end - at.other.first;
-  const int mine = at.row + block * 32, key = mine + (lane & 31);
+  const int mine = at.row + wave * 32, key = mine + (lane & 31);
   const bool valid = key < keys;
   const int64_t row = at.own.first + key;
 
   {
-    TileLoader<T, DIM, kPairs, kOwn> loader;
+    TileLoader<T, DIM, kWaves, kOwn> loader;
     loader.init(p.v_at.row, p.dim, wave);
     loader.load(v_own, static_cast<const T *>(p.v) + (int64_t)(at.own.first + at.row) * p.v_at.row + at.head * p.v_at.head, keys - at.row, wave);
   }
@@ -757,32 +756,30 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
   auto first_for = [&](int j) { return p.causal ? min(max(j - shift, 0), queries) : 0; };
   const int first = first_for(at.row), first_wave = mine < keys ? first_for(mine) : queries, first_lane = first_for(key), all_from = first_for(mine + 31);
   const bool all_valid = mine + 32 <= keys;
-  const int from_tile = first / kTile, tiles = (queries + kTile - 1) / kTile - from_tile;  // of a head
+  const int from_tile = first / kQueries, tiles = (queries + kQueries - 1) / kQueries - from_tile;  // of a head
   const Span heads = share_of(p.group, at.split, p.splits);
   const int total = max(tiles, 0) * (heads.end - heads.first);
 
-  TileLoader<T, DIM, kPairs> q_loader, g_loader;
+  TileLoader<T, DIM, kWaves, kQueries> q_loader, g_loader;
   q_loader.init(p.q_at.row, p.dim, wave);
   g_loader.init(p.grad_out_at.row, p.dim, wave);
-  // Of the wave's half of a tile, and of its keys: the places are far above the bits that exclusive ors change.
+  // Of a tile, and of the wave's keys, whose place is far above the bits that exclusive ors change.
   TileReader<T, DIM> reader, own_reader;
   reader.init();
   own_reader = reader;
-  reader.by_rows += half * 32 * reader.kRow;
-  reader.by_columns += half * 32 * reader.kRow;
-  own_reader.by_rows += block * 32 * reader.kRow;
+  own_reader.by_rows += wave * 32 * reader.kRow;
   const T *const q = static_cast<const T *>(p.q) + at.other.first * p.q_at.row;
   const T *const g = static_cast<const T *>(p.grad_out) + at.other.first * p.grad_out_at.row;
   // The next tile to be loaded and the one that is worked on: tile of a head, head.
   int load_tile = 0, load_head = at.head * p.group + heads.first, work_tile = 0;
-  auto load = [&](char *to_q, char *to_g, float (*sums)[kTile], bool any) __attribute__((always_inline)) {
-    const int64_t from = any ? (from_tile + load_tile) * kTile : 0;
+  auto load = [&](char *to, float (*sums)[64], bool any) __attribute__((always_inline)) {
+    const int64_t from = any ? (from_tile + load_tile) * kQueries : 0;
     const int rows = any ? queries - (int)from : 0, head = any ? load_head : 0;
-    q_loader.load(to_q, q + from * p.q_at.row + head * p.q_at.head, rows, wave);
-    g_loader.load(to_g, g + from * p.grad_out_at.row + head * p.grad_out_at.head, rows, wave);
+    q_loader.load(to, q + from * p.q_at.row + head * p.q_at.head, rows, wave);
+    g_loader.load(to + kBytes, g + from * p.grad_out_at.row + head * p.grad_out_at.head, rows, wave);
     if (wave < 2) {  // zeros where there is no query: its operands are zeros
       const float *const of = (wave ? p.delta : p.exponent) + (int64_t)head * p.queries.rows + at.other.first + from;
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(of), 0, max(0, min(rows, kTile)) * 4, 0x00020000);
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(of), 0, max(0, min(rows, kQueries)) * 4, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)sums[wave], 4, lane * 4, 0, 0, 0);
     }
     if (++load_tile == tiles) load_tile = 0, ++load_head;
@@ -797,10 +794,11 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
 #pragma unroll
     for (int r = 0; r < 16; ++r) grad_k[d][r] = grad_v[d][r] = 0.f;
 
-  auto work = [&](const char *qt, const char *gt, const float (*sums)[kTile]) __attribute__((always_inline)) {
-    const int from = (from_tile + work_tile) * kTile + half * 32;
+  auto work = [&](const char *qt, const float (*sums)[64]) __attribute__((always_inline)) {
+    const char *const gt = qt + kBytes;
+    const int from = (from_tile + work_tile) * kQueries;
     if (++work_tile == tiles) work_tile = 0;
-    if (from + 32 <= first_wave || from >= queries) return;
+    if (from + kQueries <= first_wave) return;
     asm("" : "+v"(reader.by_rows), "+v"(reader.by_columns), "+v"(own_reader.by_rows));  // their exclusive ors are taken again: registers
     f32x16 s, dp;
 #pragma unroll
@@ -824,7 +822,7 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
     };
     Products<4, 2, Sums> values;
     auto sums_of = [&](int i) __attribute__((always_inline)) {
-      return Sums{*reinterpret_cast<const f32x4 *>(&sums[0][half * 32 + row_of(i * 4)]), *reinterpret_cast<const f32x4 *>(&sums[1][half * 32 + row_of(i * 4)])};
+      return Sums{*reinterpret_cast<const f32x4 *>(&sums[0][row_of(i * 4)]), *reinterpret_cast<const f32x4 *>(&sums[1][row_of(i * 4)])};
     };
     values.first(sums_of);
     Products<4 * kD, 3, x8> products;
@@ -857,44 +855,19 @@ __global__ __launch_bounds__(64 * kPairs, 2) void attention_grad_kv_kernel(Atten
     __builtin_amdgcn_s_setprio(0);
   };
 
-  load(q_even, g_even, sums_even, total > 0);
+  load(even, sums_even, total > 0);
   for (int n = 0; n < total; n += 2) {
     arrive();
-    load(q_odd, g_odd, sums_odd, n + 1 < total);
-    work(q_even, g_even, sums_even);
+    load(odd, sums_odd, n + 1 < total);
+    work(even, sums_even);
     if (n + 1 >= total) break;
     arrive();
-    load(q_even, g_even, sums_even, n + 2 < total);
-    work(q_odd, g_odd, sums_odd);
+    load(even, sums_even, n + 2 < total);
+    work(odd, sums_odd);
   }
   arrive();
 
-  // The second halves' sums pass through the tiles' LDS.
-  char *const room = block == 0 ? q_even : block == 1 ? q_odd : block == 2 ? g_even : g_odd;
-  auto join = [&](f32x16 (&acc)[DIM / 32]) __attribute__((always_inline)) {
-    f32x4 *const part = reinterpret_cast<f32x4 *>(room) + lane;
-    if (half) {
-#pragma unroll
-      for (int d = 0; d < DIM / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part[(d * 4 + i) * 64] = f32x4{acc[d][i * 4], acc[d][i * 4 + 1], acc[d][i * 4 + 2], acc[d][i * 4 + 3]};
-    }
-    arrive();
-    if (!half) {
-#pragma unroll
-      for (int d = 0; d < DIM / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 v = part[(d * 4 + i) * 64];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[d][i * 4 + e] += v[e];
-        }
-    }
-    arrive();
-  };
-  join(grad_k);
-  join(grad_v);
-  if (half) return;
+  char *const room = wave == 0 ? v_own : wave == 1 ? v_own + 2 * kBytes : wave == 2 ? even : odd;
   const int64_t stride = (int64_t)kv_heads * p.real_dim, corner = (int64_t)(at.own.first + mine) * stride + at.head * p.real_dim, part = at.split * (p.keys.rows * stride);
   const float back_k = p.scale / lift, back_v = kHalf ? 1.f / 32768.f : 1.f;
   auto value_k = [&](int d, int r) { return grad_k[d][r] * back_k; };
@@ -940,12 +913,13 @@ uint32_t key_splits(const emrs_attention *a) {
   if (units >= kWanted) return 1;
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kWanted / units, each / (4 * kTile), 32}));
 }
-// Of the heads that share a key's.
+// Of the heads that share a key's.  Where keys are seen by very different numbers of queries, one round of workgroups
+// would take as long as its longest (8192 rows, 8 heads of keys: 446 us against 330 with two parts).
 uint32_t head_splits(const emrs_attention *a) {
-  const uint32_t group = a->heads / a->kv_heads;
+  const uint32_t group = a->heads / a->kv_heads, wanted = a->causal && a->rows * 2 > a->key_rows ? 2 * kWanted : kWanted;
   const uint64_t units = std::max<uint64_t>(1, (a->key_rows + kOwn - 1) / kOwn) * a->kv_heads;
   uint32_t splits = 1;
-  while (splits < group && units * splits < kWanted) {
+  while (splits < group && units * splits < wanted) {
     do ++splits;
     while (group % splits);
   }
@@ -1087,7 +1061,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
       p.splits = (int32_t)head_splits(a);
       p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
       p.parts2 = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts2) : nullptr;
-      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), 64 * kPairs, 0, st>>>(p);
+      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
       if (p.splits > 1) {
         sum_parts<T>(p.parts, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_k, st);
         sum_parts<T>(p.parts2, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_v, st);
