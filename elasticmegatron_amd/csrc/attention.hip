@@ -130,7 +130,7 @@ __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, int
   // Causal work falls along the places: of those that fill a XCD's CUs twice, the second half goes backwards, so that
   // each CU begins with the same sum (4096 rows, 32 heads: 157 us against 161, grad_q 207 against 214).
   constexpr uint32_t kCus = 32;
-  uint32_t t = x * q + min(x, r) + (kLastFirst && q >= 2 * kCus && nth >= kCus && nth < 2 * kCus ? 3 * kCus - 1 - nth : nth);
+  uint32_t t = x * q + min(x, r) + (q >= 2 * kCus && nth >= kCus && nth < 2 * kCus ? 3 * kCus - 1 - nth : nth);
   const uint32_t chunk = (heads % kXcds ? 1 : heads / kXcds) * splits, each = chunk * tiles;
   const uint32_t first_head = t / each * chunk;
   t -= t / each * each;
