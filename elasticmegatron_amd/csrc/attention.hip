@@ -71,43 +71,34 @@ struct Span {
   int first, end;
 };
 
-// This lane's segment of a run of 64: ends that never go back, and tiles up to and with it.
+// This lane's segment, of at most 64: ends that never go back, and tiles up to and with it.
 struct Walk {
-  int first, end, tiles, end_before, tiles_before;
+  int first, end, tiles;
 
-  __device__ __forceinline__ void begin() { end_before = tiles_before = 0; }
-  __device__ __forceinline__ void step(const Bounds &b, int from) {
-    const int e = from + lane_of();
+  __device__ __forceinline__ explicit Walk(const Bounds &b) {
+    const int e = lane_of();
     end = e <= b.documents ? b.at(e) : b.rows;
-    end = max(end, end_before);
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int before = __shfl_up(end, o);
       if (lane_of() >= o) end = max(end, before);
     }
     const int below = __shfl_up(end, 1);
-    first = lane_of() ? below : end_before;
+    first = lane_of() ? below : 0;
     tiles = (end - first + kOwn - 1) / kOwn;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int before = __shfl_up(tiles, o);
       if (lane_of() >= o) tiles += before;
     }
-    tiles += tiles_before;
-    end_before = __builtin_amdgcn_readlane(end, 63);
-    tiles_before = __builtin_amdgcn_readlane(tiles, 63);
   }
+  __device__ __forceinline__ Span span(int lane) const { return {__builtin_amdgcn_readlane(first, lane), __builtin_amdgcn_readlane(end, lane)}; }
 };
-
-// Segment `segment` of a side, a document.
-__device__ __forceinline__ Span span_of(const Bounds &b, int segment) {
-  if (!b.offsets) return {b.at(segment - 1), b.at(segment)};
-  Walk walk;
-  walk.begin();
-  for (int from = 0; from <= segment; from += 64) walk.step(b, from);
-  const int lane = segment & 63;
-  return {__builtin_amdgcn_readlane(walk.first, lane), __builtin_amdgcn_readlane(walk.end, lane)};
-}
+// Documents that are walked; with the rows before and behind them they are a wave's lanes.  More of them have their
+// tiles listed by a launch of its own.  (Forward and backward of 32 heads of 128, listed and walked: 60 documents of 64
+// rows 183 us and 172; walked in steps of 64, 100 documents 229 and 266, 256 documents 519 and 826, 1024 of 8 rows 1180
+// and 4199.)
+constexpr uint64_t kWalked = 62;
 
 struct Place {
   Span own, other;  // the document's rows on both sides
@@ -115,17 +106,26 @@ struct Place {
   int head, split;
 };
 
-// The workgroup's rows, head and share of the other side; false: there are none for it.  Each XCD gets a run of
-// consecutive places, heads that share keys one after the other: whole heads where they divide by the XCDs.  Within
-// it the last rows come first, whose causal work is the longest (grad_k: the first).
+// Where a tile's rows lie, as attention_places_kernel leaves it for every tile of a side with many documents.
+struct Entry {
+  Span own, other;
+  int row;
+};
+struct Places {
+  int tiles;
+  Entry tile[1];
+};
+
+// The workgroup's place in a launch of any size: see lines_of().
+__device__ __forceinline__ uint32_t block_of() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
+// The workgroup's tile, of `tiles` for each head and split, its head and its split; false: there is none for it.  Each
+// XCD gets a run of consecutive places, heads that share keys one after the other: whole heads where they divide by the
+// XCDs.  Within it the last rows come first, whose causal work is the longest (grad_k: the first).
 template <bool kLastFirst>
-__device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, int heads, int splits, Place &at) {
-  const int segments = own.documents + 2;
-  Walk walk;
-  walk.begin();
-  for (int from = 0; from < segments; from += 64) walk.step(own, from);
-  const uint32_t tiles = (uint32_t)walk.tiles_before, total = tiles * heads * splits;
-  const uint32_t q = total / kXcds, r = total % kXcds, x = blockIdx.x % kXcds, nth = blockIdx.x / kXcds;
+__device__ __forceinline__ bool pick(uint32_t tiles, int heads, int splits, Place &at, int &own_tile) {
+  const uint32_t block = block_of(), total = tiles * heads * splits;
+  const uint32_t q = total / kXcds, r = total % kXcds, x = block % kXcds, nth = block / kXcds;
   if (nth >= q + (x < r ? 1 : 0)) return false;
   // Causal work falls along the places: of those that fill a XCD's CUs twice, the second half goes backwards, so that
   // each CU begins with the same sum (4096 rows, 32 heads: 157 us against 161, grad_q 207 against 214).
@@ -134,27 +134,93 @@ __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, int
   const uint32_t chunk = (heads % kXcds ? 1 : heads / kXcds) * splits, each = chunk * tiles;
   const uint32_t first_head = t / each * chunk;
   t -= t / each * each;
-  uint32_t tile = t / chunk;
-  const uint32_t unit = first_head + t % chunk;
+  const uint32_t tile = t / chunk, unit = first_head + t % chunk;
   at.head = unit / splits, at.split = unit % splits;
-  if (kLastFirst) tile = tiles - 1 - tile;
-  if (segments > 64) walk.begin();
-  for (int from = 0;; from += 64) {
-    if (segments > 64) walk.step(own, from);
-    const uint64_t past = __ballot(tile < (uint32_t)walk.tiles);
-    if (!past) continue;  // never of the last 64: tile < tiles
-    const int lane = __builtin_ctzll(past), segment = from + lane;
-    at.own.first = __builtin_amdgcn_readlane(walk.first, lane);
-    at.own.end = __builtin_amdgcn_readlane(walk.end, lane);
-    const int rows = at.own.end - at.own.first;
-    at.row = ((int)tile - __builtin_amdgcn_readlane(walk.tiles, lane) + (rows + kOwn - 1) / kOwn) * kOwn;
-    if (segment > 0 && segment <= own.documents) {
-      at.other = own.offsets == other.offsets && own.offsets && own.rows == other.rows ? at.own : span_of(other, segment);
-    } else {
-      at.other.first = at.other.end = 0;
-    }
+  own_tile = (int)(kLastFirst ? tiles - 1 - tile : tile);
+  return true;
+}
+
+// The workgroup's rows, head and share of the other side; false: there are none for it.  Documents of one length are
+// counted off, others are walked by every workgroup for itself, one a lane, or, more than there are lanes, looked up.
+template <bool kLastFirst>
+__device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, const Places *places, int heads, int splits, Place &at) {
+  int tile;
+  if (!own.offsets) {
+    const int each_has = (own.each + kOwn - 1) / kOwn;
+    if (!pick<kLastFirst>((uint32_t)each_has * own.documents, heads, splits, at, tile)) return false;
+    const int document = tile / each_has;
+    at.own = {own.at(document), own.at(document + 1)}, at.other = {other.at(document), other.at(document + 1)};
+    at.row = (tile - document * each_has) * kOwn;
     return true;
   }
+  if (places) {
+    if (!pick<kLastFirst>((uint32_t)places->tiles, heads, splits, at, tile)) return false;
+    const Entry &e = places->tile[tile];
+    at.own = e.own, at.other = e.other, at.row = e.row;
+    return true;
+  }
+  const Walk walk(own);
+  if (!pick<kLastFirst>((uint32_t)__builtin_amdgcn_readlane(walk.tiles, 63), heads, splits, at, tile)) return false;
+  const int segment = __builtin_ctzll(__ballot(tile < walk.tiles));  // tile is less than all tiles
+  at.own = walk.span(segment);
+  at.row = (tile - __builtin_amdgcn_readlane(walk.tiles, segment) + (at.own.end - at.own.first + kOwn - 1) / kOwn) * kOwn;
+  at.other = {0, 0};
+  if (segment > 0 && segment <= own.documents) at.other = own.offsets == other.offsets && own.rows == other.rows ? at.own : Walk(other).span(segment);
+  return true;
+}
+
+// Inclusive maximum or sum over a workgroup's threads, and over all of them.
+constexpr int kPlaceThreads = 1024;
+template <class Op>
+__device__ __forceinline__ int scan(int v, int *room, int &all, Op op) {
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int before = __shfl_up(v, o);
+    if (lane_of() >= o) v = op(v, before);
+  }
+  const int wave = threadIdx.x / 64;
+  __syncthreads();
+  if (lane_of() == 63) room[wave] = v;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) v = op(v, room[i]);
+  all = room[0];
+  for (int i = 1; i < kPlaceThreads / 64; ++i) all = op(all, room[i]);
+  return v;
+}
+
+// The tiles of the queries' side (workgroup 0) and of the keys' (1), each document's by a thread.
+__global__ __launch_bounds__(kPlaceThreads) void attention_places_kernel(Bounds queries, Bounds keys, Places *of_queries, Places *of_keys) {
+  __shared__ int room[kPlaceThreads / 64], last[2];  // last: ends of the thread before
+  __shared__ int ends[2][kPlaceThreads];
+  const Bounds &own = blockIdx.x ? keys : queries, &other = blockIdx.x ? queries : keys;
+  Places *const places = blockIdx.x ? of_keys : of_queries;
+  if (threadIdx.x < 2) last[threadIdx.x] = 0;
+  const int segments = own.documents + 2;
+  auto most = [](int a, int b) { return max(a, b); };
+  auto sum = [](int a, int b) { return a + b; };
+  int tiles_before = 0;
+  for (int from = 0; from < segments; from += kPlaceThreads) {
+    const int segment = from + (int)threadIdx.x;
+    __syncthreads();
+    const int own_before = last[0], other_before = last[1];
+    int all_own, all_other, all_tiles;
+    const int end = max(scan(segment <= own.documents ? own.at(segment) : own.rows, room, all_own, most), own_before);
+    const int other_end = max(scan(segment <= own.documents ? other.at(segment) : other.rows, room, all_other, most), other_before);
+    ends[0][threadIdx.x] = end, ends[1][threadIdx.x] = other_end;
+    __syncthreads();
+    Entry e;
+    e.own = {threadIdx.x ? ends[0][threadIdx.x - 1] : own_before, end};
+    const bool document = segment > 0 && segment <= own.documents;
+    e.other = {document ? (threadIdx.x ? ends[1][threadIdx.x - 1] : other_before) : 0, document ? other_end : 0};
+    const int tiles = (e.own.end - e.own.first + kOwn - 1) / kOwn, upto = scan(tiles, room, all_tiles, sum) + tiles_before;
+    for (int i = 0; i < tiles; ++i) {
+      e.row = i * kOwn;
+      places->tile[upto - tiles + i] = e;
+    }
+    tiles_before += all_tiles;
+    if (threadIdx.x == 0) last[0] = max(own_before, all_own), last[1] = max(other_before, all_other);
+  }
+  if (threadIdx.x == 0) places->tiles = tiles_before;
 }
 
 // ---- tiles ----
@@ -284,6 +350,7 @@ struct Strides {
 
 struct Attention {
   Bounds queries, keys;
+  const Places *query_places, *key_places;  // NULL: they are found without
   const void *q, *k, *v, *grad_out;
   Strides q_at, k_at, v_at, grad_out_at;
   int32_t heads, group, dim, real_dim, causal, splits, wide_out, wide_grads;  // dim: of the operands' rows, a multiple of 8; real_dim: of the outputs'
@@ -359,7 +426,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward
   __shared__ __attribute__((aligned(1024))) char v_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char v_odd[kBytes];
   Place at;
-  if (!find<true>(p.queries, p.keys, p.heads, p.splits, at)) return;
+  if (!find<true>(p.queries, p.keys, p.query_places, p.heads, p.splits, at)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
   const int queries = at.own.end - at.own.first, keys = at.other.end - at.other.first;
   const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = at.head / p.group;
@@ -590,7 +657,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
   __shared__ __attribute__((aligned(1024))) char v_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char v_odd[kBytes];
   Place at;
-  if (!find<true>(p.queries, p.keys, p.heads, p.splits, at)) return;
+  if (!find<true>(p.queries, p.keys, p.query_places, p.heads, p.splits, at)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
   const int queries = at.own.end - at.own.first, keys = at.other.end - at.other.first;
   const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = at.head / p.group;
@@ -735,7 +802,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attentio
   __shared__ __attribute__((aligned(256))) float sums_odd[2][64];
   const int kv_heads = p.heads / p.group;
   Place at;
-  if (!find<false>(p.keys, p.queries, kv_heads, p.splits, at)) return;
+  if (!find<false>(p.keys, p.queries, p.key_places, kv_heads, p.splits, at)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
   const int keys = at.own.end - at.own.first, queries = at.other.end - at.other.first;
   const int mine = at.row + wave * 32, key = mine + (lane & 31);
@@ -929,8 +996,11 @@ uint32_t head_splits(const emrs_attention *a) {
 // What lies in the workspace, and where.
 struct Room {
   bool pad_q, pad_k, pad_v, pad_g;
-  uint64_t q, k, v, g, parts, parts2, part_lse, exponent, delta, largest, bytes;
+  uint64_t q, k, v, g, parts, parts2, part_lse, exponent, delta, largest, query_places, key_places, bytes;
 };
+
+bool lists(const emrs_attention *a) { return a->offsets && a->documents > kWalked; }
+uint64_t most_tiles(uint64_t rows, uint64_t documents) { return std::min(rows, rows / kOwn + documents + 2); }
 
 // Rows that a tile's loads cannot take as they lie: off 16 bytes, too far apart, or (expanded tensors) one over the
 // other, so that what is past the last of them is not past the end of their buffer.
@@ -961,6 +1031,10 @@ Room room_of(const emrs_attention *a, bool backward) {
   const uint64_t keys = key_splits(a), heads = backward ? head_splits(a) : 1;
   // grad_q's parts are summed before grad_k's and grad_v's are written.
   const uint64_t parts = std::max(keys > 1 ? keys * own * a->dim * 4 : 0, heads > 1 ? heads * other * a->dim * 4 : 0);
+  if (lists(a)) {
+    r.query_places = take(sizeof(Places) + most_tiles(a->rows, a->documents) * sizeof(Entry));
+    if (backward) r.key_places = take(sizeof(Places) + most_tiles(a->key_rows, a->documents) * sizeof(Entry));
+  }
   r.parts = take(parts);
   if (heads > 1) r.parts2 = take(heads * other * a->dim * 4);
   if (!backward && keys > 1) r.part_lse = take(keys * own * 4);
@@ -982,8 +1056,12 @@ int check_sizes(const emrs_attention *a) {
   return EMRS_OK;
 }
 
-uint32_t grid_of(uint64_t rows, uint64_t documents, uint64_t heads, uint64_t splits) {
-  return (uint32_t)(std::min(rows, rows / kOwn + documents + 2) * heads * splits);
+// Lines of 2^20 workgroups: a launch has less than 2^32 threads along a line.
+dim3 lines_of(uint64_t rows, uint64_t documents, uint64_t heads, uint64_t splits) {
+  constexpr uint64_t line = 1u << 20;
+  static_assert(line % kXcds == 0, "every line begins at the same XCD");
+  const uint64_t all = most_tiles(rows, documents) * heads * splits;
+  return dim3((uint32_t)std::min(all, line), (uint32_t)((all + line - 1) / line));
 }
 
 template <class T>
@@ -1025,12 +1103,17 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   p.scale = a->scale, p.out = a->out, p.rest = a->out_rest, p.lse = a->lse;
   p.wide_out = a->dim % 8 == 0 && on(a->out, 16) && on(a->out_rest, 16);
   p.wide_grads = a->dim % 8 == 0 && on(a->grad_q, 16) && on(a->grad_k, 16) && on(a->grad_v, 16);
+  if (lists(a) && a->rows + a->key_rows) {
+    Places *const of_queries = reinterpret_cast<Places *>(w + room.query_places), *const of_keys = backward ? reinterpret_cast<Places *>(w + room.key_places) : nullptr;
+    attention_places_kernel<<<backward ? 2 : 1, kPlaceThreads, 0, st>>>(p.queries, p.keys, of_queries, of_keys);
+    p.query_places = of_queries, p.key_places = of_keys;
+  }
   p.splits = (int32_t)key_splits(a);
   p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
   if (!backward) {
     if (a->rows == 0) return EMRS_OK;
     p.part_lse = reinterpret_cast<float *>(w + room.part_lse);
-    attention_forward_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
+    attention_forward_kernel<T, DIM><<<lines_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
     if (p.splits > 1) {
       const uint32_t e = a->dim % 4 ? 1 : 4, blocks = (uint32_t)((a->rows * a->heads * (a->dim / e) + 255) / 256);
       (e == 4 ? attention_join_kernel<T, 4> : attention_join_kernel<T, 1>)<<<blocks, 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,
@@ -1053,7 +1136,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
     p.grad_q = a->grad_q;
     if (!a->grad_q && p.splits > 1) p.splits = 1, p.parts = nullptr;
     if (a->rows) {
-      attention_grad_q_kernel<T, DIM><<<grid_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
+      attention_grad_q_kernel<T, DIM><<<lines_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
       if (p.splits > 1) sum_parts<T>(p.parts, p.splits, a->rows * a->heads * a->dim, a->grad_q, st);
     }
     if (a->grad_k && a->key_rows) {
@@ -1061,7 +1144,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
       p.splits = (int32_t)head_splits(a);
       p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
       p.parts2 = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts2) : nullptr;
-      attention_grad_kv_kernel<T, DIM><<<grid_of(a->key_rows, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
+      attention_grad_kv_kernel<T, DIM><<<lines_of(a->key_rows, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
       if (p.splits > 1) {
         sum_parts<T>(p.parts, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_k, st);
         sum_parts<T>(p.parts2, p.splits, a->key_rows * a->kv_heads * a->dim, a->grad_v, st);
@@ -1076,6 +1159,7 @@ int run(const emrs_attention *a, bool backward, hipStream_t st) {
   int rc = check_sizes(a);
   if (rc) return rc;
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: the scale is positive and finite");
+  if (a->reserved) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: reserved is not 0");
   if (!a->offsets != !a->key_offsets) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: offsets of both sides, or of none");
   if (a->offsets) {
     if (a->offset_bytes != 4 && a->offset_bytes != 8) return fail(EMRS_ERR_INVALID_ARGUMENT, "attention: offsets are of 4 or 8 bytes");

@@ -598,7 +598,7 @@ int emrs_norm_backward(const emrs_norm *norm, void *stream);
 typedef struct emrs_experts {
   uint32_t dtype;                 /* EMRS_BF16 or EMRS_FP16 */
   uint32_t n_experts;             /* 1 to EMRS_EXPERTS_MAX */
-  uint64_t rows;                  /* may be 0 */
+  uint64_t rows;                  /* 0 to 2^30 - 1 */
   uint64_t n_in, n_out;           /* 1 to 2^20 */
   const void *counts;             /* [n_experts], on the device */
   uint32_t counts_bytes;          /* of a count: 4 or 8 */
@@ -636,8 +636,8 @@ typedef struct emrs_attention {
   uint32_t heads, kv_heads;       /* heads a multiple of kv_heads */
   uint32_t dim;                   /* of a head, 1 to EMRS_ATTENTION_MAX_DIM */
   uint32_t offset_bytes;          /* of an offset: 4 or 8 */
-  uint64_t rows, key_rows;        /* may be 0 */
-  uint64_t documents;             /* >= 1 */
+  uint64_t rows, key_rows;        /* 0 to 2^28 */
+  uint64_t documents;             /* 1 to 2^20 */
   const void *offsets, *key_offsets; /* [documents + 1]; both NULL: documents of equal length that fill the rows */
   const void *q, *k, *v;          /* [rows][heads][dim], [key_rows][kv_heads][dim], unit stride along dim */
   uint64_t q_strides[2], k_strides[2], v_strides[2]; /* elements between rows and between heads */

@@ -327,3 +327,50 @@ def test_captured_and_on_another_stream(gpu_device, queries, keys, heads, dim, d
         want = _run(q, k, v, g, **kw)
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("documents,heads,kv_heads,dim,dtype,causal,others", [
+    (62, 2, 1, 16, BF16, True, True),
+    (63, 2, 1, 16, BF16, False, True),
+    (256, 2, 1, 16, BF16, True, False),
+    (1022, 1, 1, 64, FP16, True, True),
+    (1023, 8, 8, 8, BF16, True, False),
+    (2500, 2, 2, 72, BF16, True, True),
+])
+def test_many_documents(gpu_device, documents, heads, kv_heads, dim, dtype, causal, others):
+    """Those that one step of the search takes, and more, listed in one step or several; empty ones, and one of more than a tile."""
+    gen = torch.Generator().manual_seed(documents)
+    lengths = lambda: [300 if i == documents // 2 else int(n) for i, n in enumerate(torch.randint(0, 4, (documents,), generator=gen))]  # noqa: E731
+    queries = lengths()
+    q, k, v, g, q_at, k_at = _inputs(queries, heads, kv_heads, dim, dtype, lengths() if others else None, spare=2)
+    at, scale = torch.int64 if others else torch.int32, 1 / math.sqrt(dim)
+    got = _run(q, k, v, g, offsets=_offsets(q_at, at), key_offsets=_offsets(k_at, at) if others else None, causal=causal)
+    for t, want, err, what in zip(got, *_formula(q, k, v, g, q_at, k_at, causal, scale), ("out", "grad_q", "grad_k", "grad_v")):
+        _close(t, want, err, what)
+
+
+def test_many_offsets_that_do_not_fit(gpu_device):
+    """Those that go back count as the one before, and all are held within the rows, where tiles are listed too."""
+    q, k, v, g, _, _ = _inputs([40], 2, 2, 32, BF16)
+    raw = [-3, 2, 1, 9, 4] + [9] * 300 + [30, 5, 99, 7]
+    held, top = [], 0
+    for n in raw:
+        top = max(top, min(max(n, 0), 40))
+        held.append(top)
+    got = _run(q, k, v, g, offsets=_offsets(raw))
+    for t, want, err, what in zip(got, *_formula(q, k, v, g, held, held, True, 1 / math.sqrt(32)), ("out", "grad_q", "grad_k", "grad_v")):
+        _close(t, want, err, what)
+
+
+def test_more_workgroups_than_a_line_of_a_launch(gpu_device):
+    """Documents of one row each: out is v, grad_v sums grad_out over the heads that share it, and the others are 0."""
+    n, heads = 40000, 64
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, g = (torch.randn(n, h, 8, generator=gen, device="cuda").to(BF16) for h in (heads, heads, heads, heads))
+    out, gq, gk, gv = _run(q, k, v, g, offsets=torch.arange(n + 1, device="cuda"))
+    assert torch.equal(out, v) and torch.equal(gv, g)
+    # d = p (grad_out . v - grad_out . out): two sums of eight products in 32 bits, and out is off by what p and its sum are,
+    # whose exponents are off by the roundings of a score of this size.
+    score = float((q.float() * k.float()).abs().sum(2).max()) / math.sqrt(8) * math.log2(math.e)
+    room = 2.0 ** -24 * (2 * 16 + 4 * (score + 8)) * 8 * float(g.abs().max()) * float(v.abs().max()) * 1.05
+    assert float(gq.abs().max()) <= room * float(k.abs().max()) and float(gk.abs().max()) <= room * float(q.abs().max())
