@@ -31,7 +31,7 @@ using emrs_gemm::Product;
 using emrs_gemm::Where;
 using emrs_internal::fail;
 
-constexpr uint64_t kMaxRows = 1u << 30;
+constexpr uint64_t kMaxRows = (1u << 30) - 1;  // the sum of two counts fits 32 bits
 constexpr uint64_t kCutFrom = 8192;  // k from which on the tiles of a last round are cut along it
 constexpr uint64_t kFew = 2;         // rows up to which weights are read by rows, in vector arithmetic
 
@@ -428,7 +428,7 @@ int check_sizes(const emrs_experts *a) {
   if (a->dtype != EMRS_BF16 && a->dtype != EMRS_FP16) return fail(EMRS_ERR_INVALID_ARGUMENT, "experts: operands are bf16 or fp16");
   if (a->n_experts < 1 || a->n_experts > EMRS_EXPERTS_MAX) return fail(EMRS_ERR_INVALID_ARGUMENT, "experts: 1 to 256 experts");
   if (a->n_in < 1 || a->n_out < 1 || a->n_in > (1u << 20) || a->n_out > (1u << 20)) return fail(EMRS_ERR_TOO_LARGE, "experts: sides are 1 to 2^20");
-  if (a->rows > kMaxRows) return fail(EMRS_ERR_TOO_LARGE, "experts: at most 2^30 rows");
+  if (a->rows > kMaxRows) return fail(EMRS_ERR_TOO_LARGE, "experts: at most 2^30 - 1 rows");
   return EMRS_OK;
 }
 
@@ -567,6 +567,7 @@ int run(const emrs_experts *a, bool backward, hipStream_t st) {
   int rc = check_sizes(a);
   if (rc) return rc;
   if (a->counts_bytes != 4 && a->counts_bytes != 8) return fail(EMRS_ERR_INVALID_ARGUMENT, "experts: counts are of 4 or 8 bytes");
+  if (a->reserved) return fail(EMRS_ERR_INVALID_ARGUMENT, "experts: reserved is not 0");
   if (!a->counts) return fail(EMRS_ERR_INVALID_ARGUMENT, "experts: NULL counts");
   if (!on(a->counts, a->counts_bytes)) return fail(EMRS_ERR_MISALIGNED, "experts: counts off their type's alignment");
   const bool want_x = !backward || a->grad_weights, want_w = !backward || a->grad_x;

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_forward_kernel(Norm 
   constexpr int lanes = 64 * WAVES;
   __shared__ float room[2][WAVES];
   const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
-  const uint64_t row = (uint64_t)blockIdx.x * rows_of_block<WAVES>() + (WAVES == 1 ? wave : 0);
+  const uint64_t row = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * rows_of_block<WAVES>() + (WAVES == 1 ? wave : 0);
   if (row >= p.tokens) return;  // whole waves, and with several waves a row whole workgroups
   int turn = 0;
   const int hidden = p.hidden;
@@ -427,9 +427,12 @@ __global__ __launch_bounds__(kSumColumns * kSumRows) void sum_parts_kernel(const
 
 // ---- launches ----
 
+// Lines of 2^20 workgroups: a launch has less than 2^32 threads along a line.
 template <int WAVES>
-uint32_t blocks_of(uint64_t tokens) {
-  return (uint32_t)((tokens + rows_of_block<WAVES>() - 1) / rows_of_block<WAVES>());
+dim3 lines_of(uint64_t tokens) {
+  constexpr uint64_t line = 1u << 20;
+  const uint64_t all = (tokens + rows_of_block<WAVES>() - 1) / rows_of_block<WAVES>();
+  return dim3((uint32_t)std::min(all, line), (uint32_t)((all + line - 1) / line));
 }
 
 // Waves of a row: forward with up to four units a lane, backward with two (its sums take registers), up to eight waves.
@@ -446,7 +449,7 @@ inline uint32_t parts_of(const emrs_norm *a, bool is_wide) {
 
 template <class T, class R, int WAVES, int UNITS, bool kWide>
 void launch_forward(const Norm &p, hipStream_t st) {
-  norm_forward_kernel<T, R, WAVES, UNITS, kWide><<<blocks_of<WAVES>(p.tokens), threads_of<WAVES>(), 0, st>>>(p);
+  norm_forward_kernel<T, R, WAVES, UNITS, kWide><<<lines_of<WAVES>(p.tokens), threads_of<WAVES>(), 0, st>>>(p);
 }
 template <class T, class R, int WAVES, int UNITS, bool kWide>
 void launch_backward(const Norm &p, bool full, uint32_t blocks, hipStream_t st) {

@@ -44,6 +44,7 @@ int run(const emrs_norm *a, bool backward, hipStream_t st) {
   int rc = check_sizes(a);
   if (rc) return rc;
   if (a->gate_kind > EMRS_NORM_GATE_TOKEN) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: unknown kind of gate");
+  if (a->reserved) return fail(EMRS_ERR_INVALID_ARGUMENT, "norm: reserved is not 0");
   const uint64_t h = a->hidden;
   const bool full = a->gate_kind || a->branch_weight;
   if (!a->branch && (full || a->grad_gate || a->grad_branch_weight))

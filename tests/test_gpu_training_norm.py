@@ -322,3 +322,14 @@ def test_captured_and_on_another_stream(gpu_device):
         _run(x, grads, 0.5)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(grad[k], want_grad[k]) for k in x)
+
+
+def test_more_rows_than_a_line_of_a_launch(gpu_device):
+    n = (1 << 26) + 77
+    x = torch.ones(n, 8, dtype=torch.bfloat16, device="cuda")
+    x[-1] = torch.arange(1, 9)
+    w = torch.full((8,), 2.0, dtype=torch.bfloat16, device="cuda")
+    y = training.rms_norm(x, w, eps=0.0)
+    assert y[:-1].eq(2.0).all()
+    want = 2 * x[-1].double() / x[-1].double().square().mean().sqrt()
+    assert (y[-1].double() - want).abs().le(2.0 ** -8 * want * (1 + 2.0 ** -10)).all()
