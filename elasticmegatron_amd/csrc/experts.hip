@@ -32,8 +32,12 @@ using emrs_gemm::Where;
 using emrs_internal::fail;
 
 constexpr uint64_t kMaxRows = (1u << 30) - 1;  // the sum of two counts fits 32 bits
-constexpr uint64_t kCutFrom = 8192;  // k from which on the tiles of a last round are cut along it
-constexpr uint64_t kFew = 2;         // rows up to which weights are read by rows, in vector arithmetic
+// k from which on the tiles of a last round are cut along it: it has to be long enough to pay for 64 MB of parts (4096
+// rows, m 4096, k 14336: 272 tiles in 443 us, uncut 705; k of 4096 loses what it gains).
+constexpr uint64_t kCutFrom = 8192;
+// Rows up to which weights are read by rows, in vector arithmetic (2 experts' 28672 x 4096 with a row each, 84 us against
+// 110 in tiles; one expert's with two rows, 59 against 58).
+constexpr uint64_t kFew = 2;
 
 uint64_t round_up(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
 
@@ -432,12 +436,18 @@ int check_sizes(const emrs_experts *a) {
   return EMRS_OK;
 }
 
-// What a launch over the tokens' tiles takes, as gemm.h estimates it, for tiles of BN rows: half a tile more for
-// every expert that can have rows.
+// What launches take is estimated, in microseconds, as rounds of workgroups of `fixed` + `stage` for each of a group's
+// stages; the constants are fitted to 18 sets of experts, 1 to 256 of them with 16 to 8192 rows in all, at all tiles.  On
+// these sets the choice was at most 4% from the best of y, 15% of grad_x, 1% of grad_W; what it decides, for instance:
+// 64 uneven experts' 8192 rows, k 1024, m 1376: y 57 us in tiles of 256, 61 of 192, 74 of 128, 132 of 64; 8 experts of
+// 30 rows, k and m 4096: 88, 73, 53 and 55; 2 of 128 rows: 73, 58, 37 and 25; 1500 rows, k 4096, m 128: 70, 46, 27, 17 and,
+// of 32, 12.
+
+// Tiles of the tokens' rows: of every expert that can have rows one at the least, and half a tile that is not full.
 template <class Cfg>
 double tiles_expected(const Product &p, uint64_t rows, uint64_t experts) {
-  const double full = (double)rows / Cfg::BN, most = (double)std::min<uint64_t>(rows, experts);
-  return std::max(1.0, std::min(full + 0.5 * most, (double)rows)) * (double)emrs_gemm::tiles_of(p.m, Cfg::BM);
+  const double most = (double)std::min<uint64_t>(rows, experts), each = (double)rows / Cfg::BN / most;
+  return std::min(most * std::max(1.0, each + 0.5), (double)rows) * (double)emrs_gemm::tiles_of(p.m, Cfg::BM);
 }
 
 template <class Cfg>
@@ -463,11 +473,11 @@ template <class T, bool kTransposed>
 int launch(const Product &p, const OfTokens<T, kTransposed> &e, uint64_t rows, uint64_t experts, hipStream_t st) {
   using namespace emrs_gemm;
   const double k = p.k;
-  const double cost[5] = {cost_of<Large>(tiles_expected<Large>(p, rows, experts), k, 1.6, 8, e.parts),
-                          cost_of<Broad>(tiles_expected<Broad>(p, rows, experts), k, 1.2, 6),
-                          cost_of<Medium>(tiles_expected<Medium>(p, rows, experts), k, kTransposed ? 1.5 : 1.35, 4),
-                          cost_of<Small>(tiles_expected<Small>(p, rows, experts), k, kTransposed ? 1.3 : 1.15, 3),
-                          cost_of<Tiny>(tiles_expected<Tiny>(p, rows, experts), k, 1.0, 3)};
+  const double cost[5] = {cost_of<Large>(tiles_expected<Large>(p, rows, experts), k, kTransposed ? 1.45 : 1.5, kTransposed ? 8 : 5.5, e.parts),
+                          cost_of<Broad>(tiles_expected<Broad>(p, rows, experts), k, 1.3, 6.5),
+                          cost_of<Medium>(tiles_expected<Medium>(p, rows, experts), k, kTransposed ? 1.4 : 1.5, kTransposed ? 4.5 : 5.5),
+                          cost_of<Small>(tiles_expected<Small>(p, rows, experts), k, kTransposed ? 1.2 : 1.25, 4),
+                          cost_of<Tiny>(tiles_expected<Tiny>(p, rows, experts), k, 0.95, 5)};
   int best = kLarge;
   for (int i = kBroad; i <= kTiny; ++i)
     if (cost[i] < cost[best] && !(kTransposed && (i == kBroad || i == kTiny))) best = i;
@@ -492,8 +502,8 @@ template <class T>
 int launch(const Product &p, const OfWeights<T> &e, uint64_t rows, hipStream_t st) {
   using namespace emrs_gemm;
   const double k = (double)rows / p.batch;
-  const double cost[3] = {cost_of<Large>((double)tile_count<Large>(p), k, 1.7, 8), cost_of<Medium>((double)tile_count<Medium>(p), k, 1.8, 4),
-                          cost_of<Small>((double)tile_count<Small>(p), k, 2.1, 3)};
+  const double cost[3] = {cost_of<Large>((double)tile_count<Large>(p), k, 1.7, 8.5), cost_of<Medium>((double)tile_count<Medium>(p), k, 1.8, 3),
+                          cost_of<Small>((double)tile_count<Small>(p), k, 2.15, 3.5)};
   const int best = (int)(std::min_element(cost, cost + 3) - cost);
   if (best == 0) return launch_weights<Large>(p, e, st);
   if (best == 1) return launch_weights<Medium>(p, e, st);
