@@ -22,7 +22,7 @@
 //
 // What bounds it: the matrix units, with the arithmetic of the softmax beside them.  4096 rows, 32 heads of 128, causal:
 // forward 152 to 156 us (0.90 PFLOP/s; matrix instructions in 51% of the cycles that a CU is busy), grad_q 204 to 214
-// (0.98 PFLOP/s, 60%), grad_k and grad_v 260 to 267 (1.03 PFLOP/s, 60%), at about 1.9 GHz of 2.4.
+// (0.98 PFLOP/s, 57%), grad_k and grad_v 260 to 267 (1.03 PFLOP/s, 60%), at about 1.9 GHz of 2.4.
 
 #include <hip/hip_runtime.h>
 

@@ -9,9 +9,15 @@
 //   grad_weight = sum_t grad_normed hat,  grad_branch_weight = sum_t dn bh.
 //
 // Everything is bound by memory: a row is read once into registers, where its sums are taken and its results
-// made, and written once.  A row belongs to one wave up to 2048 elements and to two, four or eight above, in
-// units of eight elements a lane.  Statistics, sums and products are in 32 bits; the norm is of the stream before
-// its rounding, and backward takes hat from the rounded stream, which saves reading residual and branch again.
+// made, and written once.  A row belongs to one wave as long as four units of eight elements a lane hold it forward
+// (2048 elements) and two backward (1024), and to two, four or eight above.  Statistics, sums and products are in 32 bits;
+// the norm is of the stream before its rounding, and backward takes hat from the rounded stream, which saves reading
+// residual and branch again (a quarter more bytes for a plain sum) and is one rounding more in grad_weight.
+//
+// Measured: 4096 x 4096 in bf16, a plain sum, forward 24 us (5.6 TB/s) and backward 29 us (4.7 TB/s; 5 us more to sum
+// the parts); 8192 x 8192, the stream in 32 bits, a norm and a gate for each channel on
+// the branch, forward 154 us (5.2 TB/s) and backward 249 us (4.9 TB/s); a contiguous copy reaches 6.65 TB/s.  500 x 512 takes
+// 3 to 4 us a kernel, and the call's host time is most of it.
 
 #ifndef EMRS_NORM_H
 #define EMRS_NORM_H
@@ -29,7 +35,8 @@ constexpr int kMaxHidden = 16384;
 constexpr uint32_t kWavesOfSums = 2048;  // waves of a backward launch: eight for each CU, each workgroup with its own sums
 
 // A lane's units of a row are E elements, 16 bytes of the widest type among its arrays, and a wave's lie side by side:
-// every access is to whole lines.  (With eight fp32 elements a lane, every other 16 bytes: see the times below.)
+// every access is to whole lines.  (With eight fp32 elements a lane, two accesses of every other 16 bytes, backward of
+// 8192 x 8192 takes 255 us against 249; forward, which holds the whole row, is not slower with eight.)
 template <class R>
 constexpr int unit_of() {
   return 16 / sizeof(R);
