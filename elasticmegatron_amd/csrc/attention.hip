@@ -21,8 +21,9 @@
 // choose that scale: the same call gives the same bits.
 //
 // What bounds it: the matrix units, with the arithmetic of the softmax beside them.  4096 rows, 32 heads of 128, causal:
-// forward 152 to 156 us (0.90 PFLOP/s; matrix instructions in 51% of the cycles that a CU is busy), grad_q 204 to 214
-// (0.98 PFLOP/s, 57%), grad_k and grad_v 260 to 267 (1.03 PFLOP/s, 60%), at about 1.9 GHz of 2.4.
+// forward 152 to 156 us (0.89 PFLOP/s; matrix instructions in 51% of the cycles that a CU is busy), grad_q 204 to 214
+// (0.99 PFLOP/s, 57%), grad_k and grad_v 260 to 267 (1.04 PFLOP/s, 60%), at about 1.9 GHz of 2.4.  With a query or a few
+// to many keys, reading these: 64 single tokens to 8192 keys each, 5.9 TB/s.
 
 #include <hip/hip_runtime.h>
 
@@ -64,11 +65,13 @@ __device__ __forceinline__ int row_of(int r) { return (r >> 2) * 8 + (lane_of() 
 struct Bounds {
   const void *offsets;  // [documents + 1]; NULL: documents of equal length
   int32_t bytes, documents, rows, each;
+  int32_t fold;  // of a row here, heads of a query that count as rows
 
+  __device__ __forceinline__ int all() const { return rows * fold; }
   __device__ __forceinline__ int at(int i) const {  // i <= documents
-    if (!offsets) return i * each;
-    if (bytes == 8) return (int)min(max(static_cast<const int64_t *>(offsets)[i], (int64_t)0), (int64_t)rows);
-    return min(max(static_cast<const int32_t *>(offsets)[i], 0), rows);
+    if (!offsets) return i * each * fold;
+    if (bytes == 8) return (int)min(max(static_cast<const int64_t *>(offsets)[i], (int64_t)0), (int64_t)rows) * fold;
+    return min(max(static_cast<const int32_t *>(offsets)[i], 0), rows) * fold;
   }
 };
 
@@ -82,7 +85,7 @@ struct Walk {
 
   __device__ __forceinline__ explicit Walk(const Bounds &b) {
     const int e = lane_of();
-    end = e <= b.documents ? b.at(e) : b.rows;
+    end = e <= b.documents ? b.at(e) : b.all();
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
       const int before = __shfl_up(end, o);
@@ -151,7 +154,7 @@ template <bool kLastFirst>
 __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, const Places *places, int heads, int splits, Place &at) {
   int tile;
   if (!own.offsets) {
-    const int each_has = (own.each + kOwn - 1) / kOwn;
+    const int each_has = (own.each * own.fold + kOwn - 1) / kOwn;
     if (!pick<kLastFirst>((uint32_t)each_has * own.documents, heads, splits, at, tile)) return false;
     const int document = tile / each_has;
     at.own = {own.at(document), own.at(document + 1)}, at.other = {other.at(document), other.at(document + 1)};
@@ -170,7 +173,7 @@ __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, con
   at.own = walk.span(segment);
   at.row = (tile - __builtin_amdgcn_readlane(walk.tiles, segment) + (at.own.end - at.own.first + kOwn - 1) / kOwn) * kOwn;
   at.other = {0, 0};
-  if (segment > 0 && segment <= own.documents) at.other = own.offsets == other.offsets && own.rows == other.rows ? at.own : Walk(other).span(segment);
+  if (segment > 0 && segment <= own.documents) at.other = own.offsets == other.offsets && own.all() == other.all() ? at.own : Walk(other).span(segment);
   return true;
 }
 
@@ -209,8 +212,8 @@ __global__ __launch_bounds__(kPlaceThreads) void attention_places_kernel(Bounds 
     __syncthreads();
     const int own_before = last[0], other_before = last[1];
     int all_own, all_other, all_tiles;
-    const int end = max(scan(segment <= own.documents ? own.at(segment) : own.rows, room, all_own, most), own_before);
-    const int other_end = max(scan(segment <= own.documents ? other.at(segment) : other.rows, room, all_other, most), other_before);
+    const int end = max(scan(segment <= own.documents ? own.at(segment) : own.all(), room, all_own, most), own_before);
+    const int other_end = max(scan(segment <= own.documents ? other.at(segment) : other.all(), room, all_other, most), other_before);
     ends[0][threadIdx.x] = end, ends[1][threadIdx.x] = other_end;
     __syncthreads();
     Entry e;
@@ -391,9 +394,9 @@ template <class V, int DIM>
 struct RowStore {
   static constexpr int kEach = 16 / sizeof(V), kUnits = DIM / kEach, kMask = kUnits < 16 ? kUnits - 1 : 15;
   static __device__ __forceinline__ int at(int row, int unit) { return (row * kUnits + (unit ^ (row & kMask))) * 16; }
-  // value(d, r): of the lane's row, in 32 bits.  rows: how many of the wave's rows there are.
-  template <class Value>
-  static __device__ __forceinline__ void store(char *room, Value value, V *to, int64_t stride, int rows, int dim, bool wide) {
+  // value(d, r): of the lane's row, in 32 bits.  rows: how many of the wave's rows there are; from(row): where one is.
+  template <class Value, class From>
+  static __device__ __forceinline__ void store(char *room, Value value, V *to, From from, int rows, int dim, bool wide) {
     typedef __attribute__((ext_vector_type(4))) V v4;
     typedef __attribute__((ext_vector_type(kEach))) V unit_t;
     const int lane = lane_of();
@@ -411,8 +414,8 @@ struct RowStore {
     for (int pass = 0; pass < kUnits / 2; ++pass) {
       const int row = pass * (64 / kUnits) + lane / kUnits, unit = lane % kUnits;
       const unit_t v = *reinterpret_cast<const unit_t *>(room + at(row, unit));
-      V *const out = to + row * stride + unit * kEach;
       if (row >= rows || unit * kEach >= dim) continue;
+      V *const out = to + from(row) + unit * kEach;
       if (wide) {
         *reinterpret_cast<unit_t *>(out) = v;
       } else {
@@ -431,7 +434,8 @@ __device__ __forceinline__ Span share_of(int tiles, int split, int splits) {
 
 // ---- forward ----
 
-template <class T, int DIM>
+// kFold: the heads that share a key are rows of one tile, whose queries' documents are short.
+template <class T, int DIM, bool kFold>
 __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward_kernel(Attention p) {
   using x8 = typename emrs_gemm::Vec<T>::x8;
   constexpr int kBytes = kTile * DIM * 2;
@@ -440,19 +444,21 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward
   __shared__ __attribute__((aligned(1024))) char v_even[kBytes];
   __shared__ __attribute__((aligned(1024))) char v_odd[kBytes];
   Place at;
-  if (!find<true>(p.queries, p.keys, p.query_places, p.heads, p.splits, at)) return;
+  const int fold = kFold ? p.group : 1;
+  if (!find<true>(p.queries, p.keys, p.query_places, kFold ? p.heads / p.group : p.heads, p.splits, at)) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_of();
   const int queries = at.own.end - at.own.first, keys = at.other.end - at.other.first;
-  const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = at.head / p.group;
+  const int mine = at.row + wave * 32, query = mine + (lane & 31), kv_head = kFold ? at.head : at.head / p.group;
   const bool valid = query < queries;
-  const int64_t row = at.own.first + query;
+  const int64_t row = (at.own.first + query) / fold;
+  const int head = at.head * fold + (at.own.first + query) % fold;
 
   OwnRows<T, DIM> q;
-  q.load(static_cast<const T *>(p.q) + row * p.q_at.row + at.head * p.q_at.head, valid, p.dim);
+  q.load(static_cast<const T *>(p.q) + row * p.q_at.row + head * p.q_at.head, valid, p.dim);
 
   // Keys that the workgroup's, the wave's and the lane's last query sees.
-  const int shift = keys - queries;
-  auto seen_by = [&](int i) { return p.causal ? min(max(min(i, queries - 1) + shift + 1, 0), keys) : keys; };
+  const int shift = keys - queries / fold;
+  auto seen_by = [&](int i) { return p.causal ? min(max(min(i, queries - 1) / fold + shift + 1, 0), keys) : keys; };
   const int seen = seen_by(at.row + kOwn - 1), seen_wave = mine < queries ? seen_by(mine + 31) : 0, seen_lane = seen_by(query), seen_by_all = seen_by(mine);
   const Span tiles = share_of((seen + kTile - 1) / kTile, at.split, p.splits);
 
@@ -559,20 +565,24 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 4 : 2) void attention_forward
   sum = sum_of_halves(sum);
   const float lse = sum == 0.f ? -INFINITY : (top - kLift) * kLn2 + logf(sum);
   const float norm = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t place = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
+  const int64_t stride = (int64_t)p.heads * p.real_dim;
+  auto place = [&](int i) __attribute__((always_inline)) {  // of the wave's row i
+    const int at_row = at.own.first + mine + i;
+    return ((int64_t)(at_row / fold) * p.heads + at.head * fold + at_row % fold) * p.real_dim;
+  };
   char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
   const int rows = queries - mine;
   auto value = [&](int d, int r) { return out[d][r] * norm; };
   if (p.splits > 1) {
-    if (valid && lane < 32) p.part_lse[((int64_t)at.split * p.heads + at.head) * p.queries.rows + row] = lse;
-    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride + place, stride, rows, p.real_dim, p.real_dim % 4 == 0);
+    if (valid && lane < 32) p.part_lse[((int64_t)at.split * p.heads + head) * p.queries.rows + row] = lse;
+    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride, place, rows, p.real_dim, p.real_dim % 4 == 0);
     return;
   }
-  if (valid && lane < 32 && p.lse) p.lse[(int64_t)at.head * p.queries.rows + row] = lse;
-  RowStore<T, DIM>::store(room, value, static_cast<T *>(p.out) + place, stride, rows, p.real_dim, p.wide_out);
+  if (valid && lane < 32 && p.lse) p.lse[(int64_t)head * p.queries.rows + row] = lse;
+  RowStore<T, DIM>::store(room, value, static_cast<T *>(p.out), place, rows, p.real_dim, p.wide_out);
   if (p.rest)
-    RowStore<T, DIM>::store(room, [&](int d, int r) { return (float)rest_of<T>(value(d, r), (T)value(d, r)); }, static_cast<T *>(p.rest) + place, stride, rows,
-                            p.real_dim, p.wide_out);
+    RowStore<T, DIM>::store(room, [&](int d, int r) { return (float)rest_of<T>(value(d, r), (T)value(d, r)); }, static_cast<T *>(p.rest), place, rows, p.real_dim,
+                            p.wide_out);
 }
 
 // Joins the splits' outputs: four elements a thread where heads are whole units of four, and one else.
@@ -796,10 +806,11 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
   char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
   const float back = p.scale / lift;
   auto value = [&](int d, int r) { return acc[d][r] * back; };
+  auto place_of = [&](int i) { return i * stride; };
   if (p.splits > 1)
-    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride + corner, stride, queries - mine, p.real_dim, p.real_dim % 4 == 0);
+    RowStore<float, DIM>::store(room, value, p.parts + (int64_t)at.split * p.queries.rows * stride + corner, place_of, queries - mine, p.real_dim, p.real_dim % 4 == 0);
   else
-    RowStore<T, DIM>::store(room, value, static_cast<T *>(p.grad_q) + corner, stride, queries - mine, p.real_dim, p.wide_grads);
+    RowStore<T, DIM>::store(room, value, static_cast<T *>(p.grad_q) + corner, place_of, queries - mine, p.real_dim, p.wide_grads);
 }
 
 // grad_k and grad_v of one head of keys: the sums over the queries of every head that shares it, or, with splits, of
@@ -961,12 +972,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attentio
   const float back_k = p.scale / lift, back_v = kHalf ? 1.f / 32768.f : 1.f;
   auto value_k = [&](int d, int r) { return grad_k[d][r] * back_k; };
   auto value_v = [&](int d, int r) { return grad_v[d][r] * back_v; };
+  auto place_of = [&](int i) { return i * stride; };
   if (p.splits > 1) {
-    RowStore<float, DIM>::store(room, value_k, p.parts + part + corner, stride, keys - mine, p.real_dim, p.real_dim % 4 == 0);
-    RowStore<float, DIM>::store(room, value_v, p.parts2 + part + corner, stride, keys - mine, p.real_dim, p.real_dim % 4 == 0);
+    RowStore<float, DIM>::store(room, value_k, p.parts + part + corner, place_of, keys - mine, p.real_dim, p.real_dim % 4 == 0);
+    RowStore<float, DIM>::store(room, value_v, p.parts2 + part + corner, place_of, keys - mine, p.real_dim, p.real_dim % 4 == 0);
   } else {
-    RowStore<T, DIM>::store(room, value_k, static_cast<T *>(p.grad_k) + corner, stride, keys - mine, p.real_dim, p.wide_grads);
-    RowStore<T, DIM>::store(room, value_v, static_cast<T *>(p.grad_v) + corner, stride, keys - mine, p.real_dim, p.wide_grads);
+    RowStore<T, DIM>::store(room, value_k, static_cast<T *>(p.grad_k) + corner, place_of, keys - mine, p.real_dim, p.wide_grads);
+    RowStore<T, DIM>::store(room, value_v, static_cast<T *>(p.grad_v) + corner, place_of, keys - mine, p.real_dim, p.wide_grads);
   }
 }
 
@@ -995,12 +1007,23 @@ bool on(const void *p, uint64_t bytes) { return reinterpret_cast<uintptr_t>(p) %
 // Workgroups that a launch ought to have: as many as the card holds at a time.  (Twice as many make twice the parts to
 // be joined: 2048 queries of 8 heads to 16384 keys, 760 us for all kernels against 700.)
 constexpr uint64_t kWanted = 512;
+constexpr uint64_t kMostSplits = 32;  // (a token of 32 heads to 131072 keys of 8 heads, 120 us; with 64, 128)
 
+// Whether forward takes the heads that share a key's as rows of one tile: where documents have few queries, tiles of
+// one head would be empty for the most part, and every head would read the keys again.  (32 heads of 128, 8 of keys: 64
+// single tokens to 8192 keys each, 366 us against 733; 16 documents of 64 queries to 2048 keys, 53 against 57, of 96, 68
+// against 63.)
+bool folds(const emrs_attention *a) {
+  const uint64_t group = a->heads / a->kv_heads;
+  return group > 1 && a->rows * 2 <= a->documents * kOwn && a->rows * group < (1u << 30);
+}
 // Splits of the keys that queries walk: as many as fill the card, with four tiles for each at the least.
-uint32_t key_splits(const emrs_attention *a) {
-  const uint64_t units = std::max<uint64_t>(1, (a->rows + kOwn - 1) / kOwn) * a->heads, each = a->key_rows / std::max<uint64_t>(1, a->documents);
-  if (units >= kWanted) return 1;
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kWanted / units, each / (4 * kTile), 32}));
+uint32_t key_splits(const emrs_attention *a, bool backward) {
+  const bool fold = !backward && folds(a);
+  const uint64_t rows = a->rows * (fold ? a->heads / a->kv_heads : 1), heads = fold ? a->kv_heads : a->heads;
+  const uint64_t tiles = std::max<uint64_t>({1, (rows + kOwn - 1) / kOwn, std::min(a->rows, a->documents)}), each = a->key_rows / std::max<uint64_t>(1, a->documents);
+  if (tiles * heads >= kWanted) return 1;
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({kWanted / (tiles * heads), each / (4 * kTile), kMostSplits}));
 }
 // Of the heads that share a key's.  Where keys are seen by very different numbers of queries, one round of workgroups
 // would take as long as its longest (8192 rows, 8 heads of keys: 446 us against 330 with two parts).
@@ -1050,11 +1073,11 @@ Room room_of(const emrs_attention *a, bool backward) {
     r.delta = take(own * 4);
     r.largest = take(8);
   }
-  const uint64_t keys = key_splits(a), heads = backward ? head_splits(a) : 1;
+  const uint64_t keys = key_splits(a, backward), heads = backward ? head_splits(a) : 1;
   // grad_q's parts are summed before grad_k's and grad_v's are written.
   const uint64_t parts = std::max(keys > 1 ? keys * own * a->dim * 4 : 0, heads > 1 ? heads * other * a->dim * 4 : 0);
   if (lists(a)) {
-    r.query_places = take(sizeof(Places) + most_tiles(a->rows, a->documents) * sizeof(Entry));
+    r.query_places = take(sizeof(Places) + most_tiles(a->rows * (!backward && folds(a) ? a->heads / a->kv_heads : 1), a->documents) * sizeof(Entry));
     if (backward) r.key_places = take(sizeof(Places) + most_tiles(a->key_rows, a->documents) * sizeof(Entry));
   }
   r.parts = take(parts);
@@ -1072,7 +1095,7 @@ int check_sizes(const emrs_attention *a) {
   if (a->dim < 1 || a->dim > EMRS_ATTENTION_MAX_DIM) return fail(EMRS_ERR_TOO_LARGE, "attention: heads of 1 to 128 elements");
   if (a->documents < 1 || a->documents > (1u << 20)) return fail(EMRS_ERR_TOO_LARGE, "attention: 1 to 2^20 documents");
   if (a->rows > (1u << 28) || a->key_rows > (1u << 28)) return fail(EMRS_ERR_TOO_LARGE, "attention: at most 2^28 rows");
-  const uint64_t heads = (uint64_t)a->heads * 32;
+  const uint64_t heads = (uint64_t)a->heads * kMostSplits;
   if ((a->rows / kOwn + a->documents + 2) * heads > 0x3fffffffull || (a->key_rows / kOwn + a->documents + 2) * heads > 0x3fffffffull)
     return fail(EMRS_ERR_TOO_LARGE, "attention: too many tiles for one launch");
   return EMRS_OK;
@@ -1112,8 +1135,9 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   const uint32_t dim8 = (uint32_t)round_up(a->dim, 8);
   Attention p{};
   const bool uniform = !a->offsets;
-  p.queries = {a->offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->rows, uniform ? (int32_t)(a->rows / a->documents) : 0};
-  p.keys = {a->key_offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->key_rows, uniform ? (int32_t)(a->key_rows / a->documents) : 0};
+  const int32_t fold = !backward && folds(a) ? (int32_t)(a->heads / a->kv_heads) : 1;
+  p.queries = {a->offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->rows, uniform ? (int32_t)(a->rows / a->documents) : 0, fold};
+  p.keys = {a->key_offsets, (int32_t)a->offset_bytes, (int32_t)a->documents, (int32_t)a->key_rows, uniform ? (int32_t)(a->key_rows / a->documents) : 0, 1};
   auto strides = [](const uint64_t *s) { return Strides{(int64_t)s[0], (int64_t)s[1]}; };
   p.q = a->q, p.k = a->k, p.v = a->v, p.grad_out = a->grad_out;
   p.q_at = strides(a->q_strides), p.k_at = strides(a->k_strides), p.v_at = strides(a->v_strides), p.grad_out_at = strides(a->grad_out_strides);
@@ -1130,12 +1154,15 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
     attention_places_kernel<<<backward ? 2 : 1, kPlaceThreads, 0, st>>>(p.queries, p.keys, of_queries, of_keys);
     p.query_places = of_queries, p.key_places = of_keys;
   }
-  p.splits = (int32_t)key_splits(a);
+  p.splits = (int32_t)key_splits(a, backward);
   p.parts = p.splits > 1 ? reinterpret_cast<float *>(w + room.parts) : nullptr;
   if (!backward) {
     if (a->rows == 0) return EMRS_OK;
     p.part_lse = reinterpret_cast<float *>(w + room.part_lse);
-    attention_forward_kernel<T, DIM><<<lines_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
+    if (fold > 1)
+      attention_forward_kernel<T, DIM, true><<<lines_of(a->rows * fold, a->documents, a->kv_heads, p.splits), kThreads, 0, st>>>(p);
+    else
+      attention_forward_kernel<T, DIM, false><<<lines_of(a->rows, a->documents, a->heads, p.splits), kThreads, 0, st>>>(p);
     if (p.splits > 1) {
       const uint32_t e = a->dim % 4 ? 1 : 4, blocks = (uint32_t)((a->rows * a->heads * (a->dim / e) + 255) / 256);
       (e == 4 ? attention_join_kernel<T, 4> : attention_join_kernel<T, 1>)<<<blocks, 256, 0, st>>>(p.parts, p.part_lse, p.splits, (int64_t)a->rows, (int)a->heads,

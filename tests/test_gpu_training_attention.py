@@ -374,3 +374,32 @@ def test_more_workgroups_than_a_line_of_a_launch(gpu_device):
     score = float((q.float() * k.float()).abs().sum(2).max()) / math.sqrt(8) * math.log2(math.e)
     room = 2.0 ** -24 * (2 * 16 + 4 * (score + 8)) * 8 * float(g.abs().max()) * float(v.abs().max()) * 1.05
     assert float(gq.abs().max()) <= room * float(k.abs().max()) and float(gk.abs().max()) <= room * float(q.abs().max())
+
+
+@pytest.mark.parametrize("queries,keys,heads,kv_heads,dim,dtype,causal,spare", [
+    ([1] * 3, [300, 1, 77], 8, 2, 128, BF16, True, 0),             # single tokens: the heads that share a key are rows of one tile
+    ([1] * 5, [64, 0, 65, 1, 500], 6, 2, 64, FP16, True, 2),
+    ([1], [4000], 16, 1, 128, BF16, True, 0),                       # split keys
+    ([1], [700], 200, 1, 40, BF16, False, 0),                       # more heads than a tile has rows
+    ([2, 3, 0, 1], [100, 2, 5, 1], 15, 5, 100, BF16, True, 0),
+    ([64], [64], 4, 1, 128, BF16, True, 0),                         # the longest
+    ([65], [65], 4, 1, 128, BF16, True, 0),                         # and one that is too long
+    ([17, 90, 33, 4], [30, 90, 200, 1], 12, 4, 72, FP16, True, 9),  # fewer keys than queries
+    ([1] * 100, [5, 9] * 50, 8, 2, 32, BF16, True, 1),              # listed documents
+])
+def test_few_queries_and_shared_keys(gpu_device, queries, keys, heads, kv_heads, dim, dtype, causal, spare):
+    q, k, v, g, q_at, k_at = _inputs(queries, heads, kv_heads, dim, dtype, keys, spare)
+    kw = dict(offsets=_offsets(q_at), key_offsets=_offsets(k_at), causal=causal)
+    got, scale = _run(q, k, v, g, **kw), 1 / math.sqrt(dim)
+    for t, want, err, what in zip(got, *_formula(q, k, v, g, q_at, k_at, causal, scale), ("out", "grad_q", "grad_k", "grad_v")):
+        _close(t, want, err, what)
+    assert torch.equal(training.attention(q, k, v, **kw), got[0])
+
+
+@pytest.mark.parametrize("batch,n,m,heads,kv_heads", [(5, 1, 333, 8, 2), (3, 4, 129, 12, 3), (2, 64, 64, 4, 2), (600, 1, 70, 4, 1)])
+def test_batches_of_few_queries(gpu_device, batch, n, m, heads, kv_heads):
+    q, k, v, g, q_at, k_at = _inputs([n] * batch, heads, kv_heads, 64, BF16, [m] * batch)
+    shaped = lambda t, rows: t.view(batch, rows, *t.shape[1:])  # noqa: E731
+    got = training.attention(shaped(q, n), shaped(k, m), shaped(v, m)).flatten(0, 1)
+    (want, *_), (err, *_) = _formula(q, k, v, g, q_at, k_at, True, 0.125)
+    _close(got, want, err, "out")
