@@ -10,7 +10,7 @@
 //
 // Everything is bound by memory: a row is read once into registers, where its sums are taken and its results
 // made, and written once.  A row belongs to one wave as long as four units of eight elements a lane hold it forward
-// (2048 elements) and two backward (1024), and to two, four or eight above.  Statistics, sums and products are in 32 bits;
+// (2048 elements) and two backward (1024), and to two, four or eight above; up to 256 elements, two or four rows share one.  Statistics, sums and products are in 32 bits;
 // the norm is of the stream before its rounding, and backward takes hat from the rounded stream, which saves reading
 // residual and branch again (a quarter more bytes for a plain sum) and is one rounding more in grad_weight.
 //
@@ -77,17 +77,24 @@ __device__ __forceinline__ void store_unit(T *row, int at, int hidden, const flo
     if (at + e < hidden) row[at + e] = (T)v[e];
 }
 
+// Over a row's lanes of one wave, all of which have it.
+template <int LANES>
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
-  for (int o = 32; o; o /= 2) v += __shfl_xor(v, o);
+  for (int o = LANES < 64 ? LANES / 2 : 32; o; o /= 2) v += __shfl_xor(v, o);
   return v;
 }
 
 // The sum over a row's waves, the same in every lane.  `room` alternates between two calls' places, so that one
 // barrier a call is enough.
-template <int WAVES>
-__device__ __forceinline__ float row_sum(float v, float (*room)[WAVES], int &turn, int wave) {
-  v = wave_sum(v);
+template <int LANES>
+constexpr int waves_of_row() {
+  return LANES <= 64 ? 1 : LANES / 64;
+}
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float (*room)[waves_of_row<LANES>()], int &turn, int wave) {
+  constexpr int WAVES = waves_of_row<LANES>();
+  v = wave_sum<LANES>(v);
   if (WAVES == 1) return v;
   turn ^= 1;
   if ((threadIdx.x & 63) == 0) room[turn][wave] = v;
@@ -98,13 +105,18 @@ __device__ __forceinline__ float row_sum(float v, float (*room)[WAVES], int &tur
   return sum;
 }
 
-template <int WAVES>
+// Rows of up to a wave's lanes share a workgroup of four waves.
+template <int LANES>
 constexpr int rows_of_block() {
-  return WAVES == 1 ? 4 : 1;
+  return LANES <= 64 ? 256 / LANES : 1;
 }
-template <int WAVES>
+template <int LANES>
+__device__ __forceinline__ int row_of_block() {
+  return LANES <= 64 ? threadIdx.x / LANES : 0;  // the 0 keeps what goes by the row scalar
+}
+template <int LANES>
 constexpr int threads_of() {
-  return 64 * WAVES * rows_of_block<WAVES>();
+  return LANES * rows_of_block<LANES>();
 }
 
 struct Norm {
@@ -121,15 +133,15 @@ struct Norm {
   float *parts;              // [workgroups][3][hidden]: weight, branch_weight, gate
 };
 
-template <class T, class R, int WAVES, int UNITS, bool kWide>
-__global__ __launch_bounds__(threads_of<WAVES>()) void norm_forward_kernel(Norm p) {
+template <class T, class R, int LANES, int UNITS, bool kWide>
+__global__ __launch_bounds__(threads_of<LANES>()) void norm_forward_kernel(Norm p) {
   constexpr int E = 8, N = UNITS;
   using V = typename Unit<T, E>::type;
-  constexpr int lanes = 64 * WAVES;
-  __shared__ float room[2][WAVES];
-  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
-  const uint64_t row = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * rows_of_block<WAVES>() + (WAVES == 1 ? wave : 0);
-  if (row >= p.tokens) return;  // whole waves, and with several waves a row whole workgroups
+  constexpr int lanes = LANES;
+  __shared__ float room[2][waves_of_row<LANES>()];
+  const int lane = LANES <= 64 ? threadIdx.x % LANES : threadIdx.x, wave = threadIdx.x >> 6;
+  const uint64_t row = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * rows_of_block<LANES>() + row_of_block<LANES>();
+  if (row >= p.tokens) return;  // whole rows, and with several waves a row whole workgroups
   int turn = 0;
   const int hidden = p.hidden;
   const R *const residual = static_cast<const R *>(p.residual) + row * p.residual_stride;
@@ -149,7 +161,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_forward_kernel(Norm 
       for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) sum = fmaf((float)b[u][e], (float)b[u][e], sum);
-      rms = 1.f / sqrtf(row_sum<WAVES>(sum, room, turn, wave) * p.share + p.eps);
+      rms = 1.f / sqrtf(row_sum<LANES>(sum, room, turn, wave) * p.share + p.eps);
       if (lane == 0 && p.branch_rms) p.branch_rms[row] = rms;
     }
 #pragma unroll
@@ -188,7 +200,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_forward_kernel(Norm 
   for (int u = 0; u < N; ++u)
 #pragma unroll
     for (int e = 0; e < E; ++e) sum = fmaf(s[u][e], s[u][e], sum);
-  const float rms = 1.f / sqrtf(row_sum<WAVES>(sum, room, turn, wave) * p.share + p.eps);
+  const float rms = 1.f / sqrtf(row_sum<LANES>(sum, room, turn, wave) * p.share + p.eps);
   if (lane == 0 && p.stream_rms) p.stream_rms[row] = rms;
   T *const to = static_cast<T *>(p.normed) + row * hidden;
 #pragma unroll
@@ -217,16 +229,16 @@ struct RowOf {
 // read while the one before it is worked on: with two sums over the row in a chain, a workgroup that reads and works in
 // turn leaves memory idle half of the time, and registers hold too few workgroups to fill that.  (Four units a lane
 // leave no registers for it.)
-template <class T, class R, int WAVES, int UNITS, bool kWide, Kind kKind>
-__global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm p) {
+template <class T, class R, int LANES, int UNITS, bool kWide, Kind kKind>
+__global__ __launch_bounds__(threads_of<LANES>()) void norm_backward_kernel(Norm p) {
   constexpr int E = unit_of<R>(), N = UNITS * 8 / E;
   using V = typename Unit<T, E>::type;
   using Row = RowOf<T, R, N, kKind>;
-  constexpr int lanes = 64 * WAVES, rows = rows_of_block<WAVES>();
+  constexpr int lanes = LANES, rows = rows_of_block<LANES>();
   constexpr int kSums = kKind == kPlain ? 1 : kKind == kToken ? 2 : 3;  // weight, branch_weight, gate
   constexpr bool kFull = kKind != kPlain, by_token = kKind == kToken, kAhead = UNITS <= 2;
-  __shared__ float room[2][WAVES];
-  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
+  __shared__ float room[2][waves_of_row<LANES>()];
+  const int lane = LANES <= 64 ? threadIdx.x % LANES : threadIdx.x, wave = threadIdx.x >> 6, mine = row_of_block<LANES>();
   int turn = 0;
   const int hidden = p.hidden;
   auto at = [&](int u) { return (u * lanes + lane) * E; };
@@ -293,7 +305,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm
           sum = fmaf(g * (float)w[e], hat, sum);
         }
       }
-      const float mean = row_sum<WAVES>(sum, room, turn, wave) * p.share;
+      const float mean = row_sum<LANES>(sum, room, turn, wave) * p.share;
 #pragma unroll
       for (int u = 0; u < N; ++u) {
         const V w = of_all(0, u);
@@ -349,7 +361,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm
             sum = fmaf(ds[u][e], hat, sum);
           }
         }
-        const float mean = row_sum<WAVES>(sum, room, turn, wave) * p.share;
+        const float mean = row_sum<LANES>(sum, room, turn, wave) * p.share;
 #pragma unroll
         for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -362,7 +374,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm
   };
 
   const uint64_t step = (uint64_t)gridDim.x * rows;
-  uint64_t row = (uint64_t)blockIdx.x * rows + (WAVES == 1 ? wave : 0);
+  uint64_t row = (uint64_t)blockIdx.x * rows + mine;
   Row even;
   if constexpr (kAhead) {
     Row odd;
@@ -384,7 +396,7 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm
 
   if (!p.parts) return;
   float *const parts = p.parts + (uint64_t)blockIdx.x * 3 * hidden;
-  // The rows of a workgroup of single waves meet in LDS first.
+  // A workgroup's rows meet in LDS first.
   constexpr int kUnit = rows == 1 ? 1 : lanes * E;
   __shared__ float meet[rows][kUnit];
 #pragma unroll
@@ -394,15 +406,15 @@ __global__ __launch_bounds__(threads_of<WAVES>()) void norm_backward_kernel(Norm
       if (rows > 1) {
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < E; ++e) meet[wave % rows][(rows == 1 ? 0 : e * lanes + lane)] = sums[k][u][e];
+        for (int e = 0; e < E; ++e) meet[mine % rows][(rows == 1 ? 0 : e * lanes + lane)] = sums[k][u][e];
         __syncthreads();
-        if (wave == 0)
+        if (mine == 0)
 #pragma unroll
           for (int e = 0; e < E; ++e)
 #pragma unroll
             for (int i = 1; i < rows; ++i) sums[k][u][e] += meet[i][(rows == 1 ? 0 : e * lanes + lane)];
       }
-      if (rows == 1 || wave == 0)
+      if (rows == 1 || mine == 0)
 #pragma unroll
         for (int e = 0; e < E; ++e)
           if (at(u) + e < hidden) parts[(uint64_t)k * hidden + at(u) + e] = sums[k][u][e];
@@ -435,61 +447,68 @@ __global__ __launch_bounds__(kSumColumns * kSumRows) void sum_parts_kernel(const
 // ---- launches ----
 
 // Lines of 2^20 workgroups: a launch has less than 2^32 threads along a line.
-template <int WAVES>
+template <int LANES>
 dim3 lines_of(uint64_t tokens) {
   constexpr uint64_t line = 1u << 20;
-  const uint64_t all = (tokens + rows_of_block<WAVES>() - 1) / rows_of_block<WAVES>();
+  const uint64_t all = (tokens + rows_of_block<LANES>() - 1) / rows_of_block<LANES>();
   return dim3((uint32_t)std::min(all, line), (uint32_t)((all + line - 1) / line));
 }
 
-// Waves of a row: forward with up to four units a lane, backward with two (its sums take registers), up to eight waves.
-inline int waves_of(uint64_t hidden, bool backward, bool is_wide) {
+// Lanes of a row: of a wave, forward with up to four units a lane, backward with two (its sums take registers), up to
+// eight waves; and 16 or 32 where one unit a lane of those is enough, as for the heads of queries and keys (100000 rows of
+// 128 forward 11 us against 24 with a wave for each, 500000 of 64 29 against 102).
+inline int lanes_of(uint64_t hidden, bool backward, bool is_wide) {
+  if (is_wide && hidden <= 256) return hidden <= 128 ? 16 : 32;
   int waves = 1;
   while (waves < 8 && hidden > (uint64_t)waves * 64 * 8 * (backward ? 2 : 4)) waves *= is_wide ? 2 : 8;
-  return waves;
+  return waves * 64;
 }
 // As many as each CU has room for eight waves.
 inline uint32_t parts_of(const emrs_norm *a, bool is_wide) {
-  const int waves = waves_of(a->hidden, true, is_wide);
-  return (uint32_t)std::min<uint64_t>(kWavesOfSums / (waves == 1 ? 4 : waves), waves == 1 ? (a->tokens + 3) / 4 : a->tokens);
+  const int lanes = lanes_of(a->hidden, true, is_wide), rows = lanes <= 64 ? 256 / lanes : 1;
+  return (uint32_t)std::min<uint64_t>(kWavesOfSums * 64 / (lanes * rows), (a->tokens + rows - 1) / rows);
 }
 
-template <class T, class R, int WAVES, int UNITS, bool kWide>
+template <class T, class R, int LANES, int UNITS, bool kWide>
 void launch_forward(const Norm &p, hipStream_t st) {
-  norm_forward_kernel<T, R, WAVES, UNITS, kWide><<<lines_of<WAVES>(p.tokens), threads_of<WAVES>(), 0, st>>>(p);
+  norm_forward_kernel<T, R, LANES, UNITS, kWide><<<lines_of<LANES>(p.tokens), threads_of<LANES>(), 0, st>>>(p);
 }
-template <class T, class R, int WAVES, int UNITS, bool kWide>
+template <class T, class R, int LANES, int UNITS, bool kWide>
 void launch_backward(const Norm &p, bool full, uint32_t blocks, hipStream_t st) {
   if (p.gate_kind == EMRS_NORM_GATE_TOKEN)
-    norm_backward_kernel<T, R, WAVES, UNITS, kWide, kToken><<<blocks, threads_of<WAVES>(), 0, st>>>(p);
+    norm_backward_kernel<T, R, LANES, UNITS, kWide, kToken><<<blocks, threads_of<LANES>(), 0, st>>>(p);
   else if (full)
-    norm_backward_kernel<T, R, WAVES, UNITS, kWide, kShared><<<blocks, threads_of<WAVES>(), 0, st>>>(p);
+    norm_backward_kernel<T, R, LANES, UNITS, kWide, kShared><<<blocks, threads_of<LANES>(), 0, st>>>(p);
   else
-    norm_backward_kernel<T, R, WAVES, UNITS, kWide, kPlain><<<blocks, threads_of<WAVES>(), 0, st>>>(p);
+    norm_backward_kernel<T, R, LANES, UNITS, kWide, kPlain><<<blocks, threads_of<LANES>(), 0, st>>>(p);
 }
 
 // Rows off their units have two shapes: their accesses by elements bound them anyway.
 template <class T, class R>
 void launch(const Norm &p, bool backward, bool full, bool is_wide, uint32_t blocks, hipStream_t st) {
-  const int waves = waves_of(p.hidden, backward, is_wide), units = (p.hidden + 511) / 512;
+  const int lanes = lanes_of(p.hidden, backward, is_wide), units = (p.hidden + 511) / 512;
   if (!is_wide) {
-    if (waves == 1) return backward ? launch_backward<T, R, 1, 2, false>(p, full, blocks, st) : launch_forward<T, R, 1, 4, false>(p, st);
-    return backward ? launch_backward<T, R, 8, 4, false>(p, full, blocks, st) : launch_forward<T, R, 8, 4, false>(p, st);
+    if (lanes == 64) return backward ? launch_backward<T, R, 64, 2, false>(p, full, blocks, st) : launch_forward<T, R, 64, 4, false>(p, st);
+    return backward ? launch_backward<T, R, 512, 4, false>(p, full, blocks, st) : launch_forward<T, R, 512, 4, false>(p, st);
   }
   if (backward) {
-    if (units <= 1) return launch_backward<T, R, 1, 1, true>(p, full, blocks, st);
-    if (waves == 1) return launch_backward<T, R, 1, 2, true>(p, full, blocks, st);
-    if (waves == 2) return launch_backward<T, R, 2, 2, true>(p, full, blocks, st);
-    if (waves == 4) return launch_backward<T, R, 4, 2, true>(p, full, blocks, st);
-    if (units <= 16) return launch_backward<T, R, 8, 2, true>(p, full, blocks, st);
-    return launch_backward<T, R, 8, 4, true>(p, full, blocks, st);
+    if (lanes == 16) return launch_backward<T, R, 16, 1, true>(p, full, blocks, st);
+    if (lanes == 32) return launch_backward<T, R, 32, 1, true>(p, full, blocks, st);
+    if (units <= 1) return launch_backward<T, R, 64, 1, true>(p, full, blocks, st);
+    if (lanes == 64) return launch_backward<T, R, 64, 2, true>(p, full, blocks, st);
+    if (lanes == 128) return launch_backward<T, R, 128, 2, true>(p, full, blocks, st);
+    if (lanes == 256) return launch_backward<T, R, 256, 2, true>(p, full, blocks, st);
+    if (units <= 16) return launch_backward<T, R, 512, 2, true>(p, full, blocks, st);
+    return launch_backward<T, R, 512, 4, true>(p, full, blocks, st);
   }
-  if (units <= 1) return launch_forward<T, R, 1, 1, true>(p, st);
-  if (units <= 2) return launch_forward<T, R, 1, 2, true>(p, st);
-  if (waves == 1) return launch_forward<T, R, 1, 4, true>(p, st);
-  if (waves == 2) return launch_forward<T, R, 2, 4, true>(p, st);
-  if (waves == 4) return launch_forward<T, R, 4, 4, true>(p, st);
-  return launch_forward<T, R, 8, 4, true>(p, st);
+  if (lanes == 16) return launch_forward<T, R, 16, 1, true>(p, st);
+  if (lanes == 32) return launch_forward<T, R, 32, 1, true>(p, st);
+  if (units <= 1) return launch_forward<T, R, 64, 1, true>(p, st);
+  if (units <= 2) return launch_forward<T, R, 64, 2, true>(p, st);
+  if (lanes == 64) return launch_forward<T, R, 64, 4, true>(p, st);
+  if (lanes == 128) return launch_forward<T, R, 128, 4, true>(p, st);
+  if (lanes == 256) return launch_forward<T, R, 256, 4, true>(p, st);
+  return launch_forward<T, R, 512, 4, true>(p, st);
 }
 
 // The sums over tokens that were wanted.

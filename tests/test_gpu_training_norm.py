@@ -333,3 +333,19 @@ def test_more_rows_than_a_line_of_a_launch(gpu_device):
     assert y[:-1].eq(2.0).all()
     want = 2 * x[-1].double() / x[-1].double().square().mean().sqrt()
     assert (y[-1].double() - want).abs().le(2.0 ** -8 * want * (1 + 2.0 ** -10)).all()
+
+
+@pytest.mark.parametrize("tokens,h,dtype,stream,branch_norm,gate", [
+    (1, 8, BF16, None, True, "token"), (15, 64, BF16, None, False, None), (16, 128, FP16, None, True, "channel"), (17, 128, BF16, FP32, True, "token"),
+    (333, 104, BF16, FP32, False, "channel"), (7, 136, BF16, None, True, "channel"), (8, 256, FP16, FP32, True, "token"), (9, 256, BF16, None, False, None),
+    (20000, 128, BF16, None, False, None), (10001, 200, FP16, None, True, "channel"), (50, 264, BF16, None, True, "channel"),
+])
+def test_short_rows(gpu_device, tokens, h, dtype, stream, branch_norm, gate):
+    """Several rows to a wave, whose last may have none; and more rows than all workgroups take at once."""
+    x, grads = _inputs(tokens, h, dtype, stream, branch_norm, gate)
+    want, err, grad, grad_err = _formula(x, grads, 0.75)
+    got, got_grad = _run(x, grads, 0.75)
+    for g, w, e, what in zip(got, want, err, ("stream", "normed")):
+        _close(g, w, e, what)
+    for k, v in x.items():
+        _close(got_grad[k], grad[k], grad_err[k], k)
