@@ -1171,14 +1171,17 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   } else {
     p.exponent = reinterpret_cast<float *>(w + room.exponent);
     p.delta = reinterpret_cast<float *>(w + room.delta);
-    if (std::is_same<T, _Float16>::value && a->rows && a->key_rows) {
+    if (std::is_same<T, _Float16>::value) {
+      // Both kernels read these, of which a side without rows leaves 0.
       uint32_t *const largest = reinterpret_cast<uint32_t *>(w + room.largest);
       attention_clear_kernel<<<1, 2, 0, st>>>(largest);
       auto grid = [&](uint64_t n) { return (uint32_t)std::min<uint64_t>((n * (dim8 / 8) + 255) / 256, 1024); };
-      attention_largest_kernel<T><<<grid(a->rows * a->heads), 256, 0, st>>>(static_cast<const T *>(p.grad_out), p.grad_out_at, (int64_t)a->rows, (int)a->heads,
-                                                                           (int)dim8, largest);
-      attention_largest_kernel<T><<<grid(a->key_rows * a->kv_heads), 256, 0, st>>>(static_cast<const T *>(p.v), p.v_at, (int64_t)a->key_rows, (int)a->kv_heads,
-                                                                                  (int)dim8, largest + 1);
+      if (a->rows)
+        attention_largest_kernel<T><<<grid(a->rows * a->heads), 256, 0, st>>>(static_cast<const T *>(p.grad_out), p.grad_out_at, (int64_t)a->rows,
+                                                                             (int)a->heads, (int)dim8, largest);
+      if (a->key_rows)
+        attention_largest_kernel<T><<<grid(a->key_rows * a->kv_heads), 256, 0, st>>>(static_cast<const T *>(p.v), p.v_at, (int64_t)a->key_rows,
+                                                                                    (int)a->kv_heads, (int)dim8, largest + 1);
       p.largest = largest;
     }
     // delta and exponent come out of grad_q's kernel, so that it runs in any case.
