@@ -144,7 +144,7 @@ class _Call:
         a.out, a.out_rest, a.lse, a.grad_out = out.data_ptr(), rest.data_ptr(), lse.data_ptr(), grad.data_ptr()
         a.grad_q = None if gq is None else gq.data_ptr()
         a.grad_k, a.grad_v = (gk.data_ptr(), gv.data_ptr()) if want_kv else (None, None)
-        if a.rows or (want_kv and a.key_rows):
+        if (want_q and a.rows) or (want_kv and a.key_rows):
             self._run(_native.attention_backward, True)
         return gq, gk, gv
 

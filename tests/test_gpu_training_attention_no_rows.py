@@ -28,3 +28,16 @@ def test_a_side_without_rows(gpu_device, rows, key_rows, wanted, dim, dtype):
         leaves = [t for t in leaves if t.requires_grad]
         for t, grad in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
             assert grad.shape == t.shape and grad.dtype == dtype and not grad.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,key_rows", [(0, 0), (0, 5), (5, 0), (300, 0)])
+@pytest.mark.parametrize("wanted", ["k", "v", "kv"])
+def test_keys_and_values_alone(gpu_device, wanted, rows, key_rows, dtype):
+    """Gradients of no rows are wanted, and none of the queries' rows."""
+    make = lambda n, heads: torch.ones(1, n, heads, 64, dtype=dtype, device="cuda")  # noqa: E731
+    leaves = [t.requires_grad_(name in wanted) for t, name in zip((make(rows, 4), make(key_rows, 2), make(key_rows, 2)), "qkv")]
+    out = training.attention(*leaves)
+    leaves = [t for t in leaves if t.requires_grad]
+    for t, grad in zip(leaves, torch.autograd.grad(out, leaves, torch.ones_like(out))):
+        assert grad.shape == t.shape and grad.dtype == dtype and not grad.any()
