@@ -173,7 +173,11 @@ __device__ __forceinline__ bool find(const Bounds &own, const Bounds &other, con
   at.own = walk.span(segment);
   at.row = (tile - __builtin_amdgcn_readlane(walk.tiles, segment) + (at.own.end - at.own.first + kOwn - 1) / kOwn) * kOwn;
   at.other = {0, 0};
-  if (segment > 0 && segment <= own.documents) at.other = own.offsets == other.offsets && own.all() == other.all() ? at.own : Walk(other).span(segment);
+  if (segment > 0 && segment <= own.documents) {
+    // One tensor of offsets, held within as many rows of as many heads each, gives one span.
+    const bool one = own.offsets == other.offsets && own.rows == other.rows && own.fold == other.fold;
+    at.other = one ? at.own : Walk(other).span(segment);
+  }
   return true;
 }
 
