@@ -16,9 +16,9 @@
 //
 // Statistics and sums are in 32 bits; p and d are rounded to the operands' type, as the matrix instructions take
 // them (two parts of every d would be a third more products in grad_q, and there are no registers for them in grad_k).
-// fp16 holds p and d scaled by powers of two (p by 2^7 or 2^15, d by what its largest possible value allows), so that
-// only what is 2^-29 of the largest or less loses bits.  No result passes through atomics but the largest entries that
-// choose that scale: the same call gives the same bits.
+// fp16 holds p and d scaled by powers of two.  Of p, forward keeps all bits down to 2^-21 of a row's largest (scaled by
+// 2^7, with room for a maximum that grows) and grad_v down to 2^-29 (by 2^15); of d, each row of grad_q and of grad_k down
+// to 2^-20 of the largest of its own sum (Lift).  No result passes through atomics: the same call gives the same bits.
 //
 // What bounds it: the matrix units, with the arithmetic of the softmax beside them.  4096 rows, 32 heads of 128, causal:
 // forward 152 to 156 us (0.89 PFLOP/s; matrix instructions in 51% of the cycles that a CU is busy), grad_q 204 to 214
@@ -381,7 +381,6 @@ struct Attention {
   float *exponent, *delta;  // the same, backward: lse in units of log 2 (infinity where a query sees nothing), and delta
   void *grad_q, *grad_k, *grad_v;
   float *parts, *parts2, *part_lse;  // of every split, where there are several
-  const uint32_t *largest;  // fp16: the largest |grad_out| and |v|, as bits
 };
 
 // What rounding x to `rounded` left over (nothing of infinities and NaN).
@@ -644,36 +643,41 @@ __global__ __launch_bounds__(256) void attention_sum_kernel(const float *parts, 
 
 // ---- backward ----
 
-// fp16: 2^e that brings the largest possible |d| (2 dim |grad_out| |v| of the largest entries) below 2^15.
-__device__ __forceinline__ float lift_of(const uint32_t *largest, int dim) {
-  const float a = __uint_as_float(largest[0]), b = __uint_as_float(largest[1]);
-  if (!(a > 0.f) || !(b > 0.f)) return 1.f;
-  const int e = 14 - __builtin_amdgcn_frexp_expf(a) - __builtin_amdgcn_frexp_expf(b) - __builtin_amdgcn_frexp_expf((float)dim);
-  return __builtin_amdgcn_ldexpf(1.f, min(max(e, -100), 100));
-}
-
-__global__ void attention_clear_kernel(uint32_t *largest) { largest[threadIdx.x] = 0; }
-
-// The largest finite |entry| of an operand's rows, joined over the workgroups by an unsigned maximum of the bits.
+// fp16: the power of two that a lane's d are multiplied by on their way into products.  It goes by the largest |d| of the
+// lane's own row (of its key in grad_k) so far, with room for a 2^8 times larger one: beyond that the row's sums are
+// brought to a new one, as those of forward to a new maximum.  Other rows, and what stands in rows of no document, do not
+// count.  (With one power of two for all rows, from the largest entries of grad_out and v, grad_q of rows whose grad_out
+// was 2^-16 of the largest was 9.7e-3 off, now 3.1e-4; 6e4 in rows of no document changed all gradients; and the search for
+// these entries cost more: 4096 rows, 32 heads of 128, forward and backward 781 us against 700.)
 template <class T>
-__global__ __launch_bounds__(256) void attention_largest_kernel(const T *x, Strides at, int64_t rows, int heads, int dim, uint32_t *largest) {
-  using x8 = typename emrs_gemm::Vec<T>::x8;
-  const int units = dim / 8;
-  float top = 0.f;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * heads * units; u += (int64_t)gridDim.x * 256) {
-    const int64_t row = u / (heads * units);
-    const int rest = (int)(u % (heads * units));
-    const x8 v = *reinterpret_cast<const x8 *>(x + row * at.row + rest / units * at.head + rest % units * 8);
+struct Lift {
+  static constexpr bool kAny = std::is_same<T, _Float16>::value;
+  static constexpr int kMost = 15, kRoom = 8, kLeast = -85;
+  float limit = 0x1p-85f;  // a power of two: |d| up to it become 2^15 at most
+  __device__ __forceinline__ float by() const { return kAny ? __uint_as_float(((254u + kMost) << 23) - __float_as_uint(limit)) : 1.f; }  // 2^15 / limit
+
+  template <int N>
+  __device__ __forceinline__ void apply(f32x16 &d, f32x16 (&sums)[N]) {
+    if constexpr (kAny) {
+      float most = fabsf(d[0]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf((float)v[e]);
-      top = a < INFINITY ? fmaxf(top, a) : top;
+      for (int r = 1; r < 16; ++r) most = fmaxf(most, fabsf(d[r]));  // NaN is passed over
+      most = most_of_halves(most);
+      if (__any(most > limit)) {
+        const float before = limit;  // (the exponent of an infinity is 0)
+        if (most > limit) limit = fmaxf(limit, __builtin_amdgcn_ldexpf(1.f, max(__builtin_amdgcn_frexp_expf(most) + kRoom, kLeast)));
+        const float less = before / limit;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sums[n][r] *= less;
+      }
+      const float x = by();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) d[r] *= x;
     }
   }
-#pragma unroll
-  for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-  if (lane_of() == 0 && top > 0.f) atomicMax(largest, __float_as_uint(top));
-}
+};
 
 // grad_q, and on the way delta and the exponent (split 0 leaves them for grad_k).
 template <class T, int DIM>
@@ -744,8 +748,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
     v_loader.load(to_v, v + from * p.v_at.row, rows, wave);
   };
   const float by = p.scale * kLog2e;
-  constexpr bool kHalf = std::is_same<T, _Float16>::value;
-  const float lift = kHalf ? lift_of(p.largest, p.real_dim) : 1.f;
+  Lift<T> lift;
 
   f32x16 acc[DIM / 32];
 #pragma unroll
@@ -775,15 +778,14 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
       auto columns = [&](int i) __attribute__((always_inline)) { return reader.columns(kt, i % kD, b * 2 + i / kD); };
       sums.first(columns);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float d = __builtin_amdgcn_exp2f(fmaf(s[r], by, -lse)) * (dp[r] - delta);
-        if (kHalf) d *= lift;
-        s[r] = d;
-      }
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], by, -lse)) * (dp[r] - delta);
       if (from + kTile > seen_by_all) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (from + b * 32 + row_of(r) >= seen_lane) s[r] = 0.f;
+      }
+      lift.apply(s, acc);
+      if (from + kTile > seen_by_all) {
         // Tiles that the mask cuts hold all that the first queries of a document see, whose gradients are the largest:
         // here d is taken in two parts (4096 rows, 32 heads of 128: error 2.43e-3 against 2.50e-3, 209 us against 204).
 #pragma unroll
@@ -808,7 +810,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
   if (!p.grad_q && !p.parts) return;
   const int64_t corner = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
   char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
-  const float back = p.scale / lift;
+  const float back = p.scale / lift.by();
   auto value = [&](int d, int r) { return acc[d][r] * back; };
   auto place_of = [&](int i) { return i * stride; };
   if (p.splits > 1)
@@ -886,7 +888,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attentio
   };
   const float by = p.scale * kLog2e;
   constexpr bool kHalf = std::is_same<T, _Float16>::value;
-  const float lift = kHalf ? lift_of(p.largest, p.real_dim) : 1.f;
+  Lift<T> lift;
 
   f32x16 grad_k[DIM / 32], grad_v[DIM / 32];
 #pragma unroll
@@ -932,20 +934,20 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attentio
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = __builtin_amdgcn_exp2f(fmaf(s[i * 4 + e], by, -f.exponent[e]));
-        float d = x * (dp[i * 4 + e] - f.delta[e]);
-        if (kHalf) d *= lift;
+        dp[i * 4 + e] = x * (dp[i * 4 + e] - f.delta[e]);
         s[i * 4 + e] = kHalf ? x * 32768.f : x;
-        dp[i * 4 + e] = d;
       }
     });
     if (from < all_from || !all_valid) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (from + row_of(r) < first_lane || !valid) s[r] = dp[r] = 0.f;
+    }
+    lift.apply(dp, grad_k);
+    if (DIM == 64 && (from < all_from || !all_valid)) {
       // As in grad_q, d in two parts where queries see few keys.  (At 128 registers run out: 300 us against 266.)
-      if (DIM == 64)
 #pragma unroll
-        for (int i = 0; i < 2 * kD; ++i) grad_k[i % kD] = mfma(reader.columns(qt, i % kD, i / kD), rest_of_eight<T>(dp, i / kD), grad_k[i % kD]);
+      for (int i = 0; i < 2 * kD; ++i) grad_k[i % kD] = mfma(reader.columns(qt, i % kD, i / kD), rest_of_eight<T>(dp, i / kD), grad_k[i % kD]);
     }
     const x8 prob[2] = {eight_of<T>(s, 0), eight_of<T>(s, 1)}, ds[2] = {eight_of<T>(dp, 0), eight_of<T>(dp, 1)};
     __builtin_amdgcn_s_setprio(1);
@@ -973,7 +975,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_grad_kv_kernel(Attentio
 
   char *const room = wave == 0 ? v_own : wave == 1 ? v_own + 2 * kBytes : wave == 2 ? even : odd;
   const int64_t stride = (int64_t)kv_heads * p.real_dim, corner = (int64_t)(at.own.first + mine) * stride + at.head * p.real_dim, part = at.split * (p.keys.rows * stride);
-  const float back_k = p.scale / lift, back_v = kHalf ? 1.f / 32768.f : 1.f;
+  const float back_k = p.scale / lift.by(), back_v = kHalf ? 1.f / 32768.f : 1.f;
   auto value_k = [&](int d, int r) { return grad_k[d][r] * back_k; };
   auto value_v = [&](int d, int r) { return grad_v[d][r] * back_v; };
   auto place_of = [&](int i) { return i * stride; };
@@ -1045,7 +1047,7 @@ uint32_t head_splits(const emrs_attention *a) {
 // What lies in the workspace, and where.
 struct Room {
   bool pad_q, pad_k, pad_v, pad_g;
-  uint64_t q, k, v, g, parts, parts2, part_lse, exponent, delta, largest, query_places, key_places, bytes;
+  uint64_t q, k, v, g, parts, parts2, part_lse, exponent, delta, query_places, key_places, bytes;
 };
 
 bool lists(const emrs_attention *a) { return a->offsets && a->documents > kWalked; }
@@ -1075,7 +1077,6 @@ Room room_of(const emrs_attention *a, bool backward) {
   if (backward) {
     r.exponent = take(own * 4);
     r.delta = take(own * 4);
-    r.largest = take(8);
   }
   const uint64_t keys = key_splits(a, backward), heads = backward ? head_splits(a) : 1;
   // grad_q's parts are summed before grad_k's and grad_v's are written.
@@ -1175,19 +1176,6 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   } else {
     p.exponent = reinterpret_cast<float *>(w + room.exponent);
     p.delta = reinterpret_cast<float *>(w + room.delta);
-    if (std::is_same<T, _Float16>::value) {
-      // Both kernels read these, of which a side without rows leaves 0.
-      uint32_t *const largest = reinterpret_cast<uint32_t *>(w + room.largest);
-      attention_clear_kernel<<<1, 2, 0, st>>>(largest);
-      auto grid = [&](uint64_t n) { return (uint32_t)std::min<uint64_t>((n * (dim8 / 8) + 255) / 256, 1024); };
-      if (a->rows)
-        attention_largest_kernel<T><<<grid(a->rows * a->heads), 256, 0, st>>>(static_cast<const T *>(p.grad_out), p.grad_out_at, (int64_t)a->rows,
-                                                                             (int)a->heads, (int)dim8, largest);
-      if (a->key_rows)
-        attention_largest_kernel<T><<<grid(a->key_rows * a->kv_heads), 256, 0, st>>>(static_cast<const T *>(p.v), p.v_at, (int64_t)a->key_rows,
-                                                                                    (int)a->kv_heads, (int)dim8, largest + 1);
-      p.largest = largest;
-    }
     // delta and exponent come out of grad_q's kernel, so that it runs in any case.
     p.grad_q = a->grad_q;
     if (!a->grad_q && p.splits > 1) p.splits = 1, p.parts = nullptr;
