@@ -135,11 +135,13 @@ def _forward(residual, branch, gate, branch_weight, weight, scale, eps, statisti
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, branch, gate, branch_weight, weight, scale, eps):
-        stream, normed, rms, a, read = _forward(residual, branch, gate, branch_weight, weight, scale, eps, True)
+        # Only a norm has statistics, and only the gradient of that before the next block reads the stream.
+        normalises = weight is not None or branch_weight is not None
+        stream, normed, rms, a, read = _forward(residual, branch, gate, branch_weight, weight, scale, eps, normalises)
         # What the kernels read: the inputs, or the copies that had to be made of them.
-        saved = [residual if stream is None else stream, rms, *[t for t in read if t is not None]]
+        saved = [t for t in ((residual if stream is None else stream) if weight is not None else None, rms, *read) if t is not None]
         ctx.save_for_backward(*saved)
-        ctx.record, ctx.lies, ctx.has, ctx.size = a, lies(*saved), [t is not None for t in read], residual.size()
+        ctx.record, ctx.lies, ctx.has, ctx.size, ctx.device = a, lies(*saved), [t is not None for t in read], residual.size(), residual.device
         ctx.set_materialize_grads(False)
         if stream is None:
             return normed
@@ -148,7 +150,7 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
-        stream, rms, *others = saved = ctx.saved_tensors  # raises where one was changed in place
+        saved = ctx.saved_tensors  # raises where one was changed in place
         need, size, has = ctx.needs_input_grad, ctx.size, ctx.has
         # Without a branch there is no stream to be differentiated to, without a weight no norm.
         grad_normed = grads[-1] if has[3] else None
@@ -158,13 +160,12 @@ class _ResidualNorm(torch.autograd.Function):
         if lies(*saved) == ctx.lies:
             a = _native.Norm.from_buffer_copy(ctx.record)
         else:
-            a, stream, rms, *others = _again(ctx, stream, rms, others)
-        device, tokens, h, dtype = stream.device, a.tokens, size[-1], others[0].dtype if others else None
-        dtype = dtype or _DTYPES[a.dtype]
+            a, saved = _again(ctx, saved)
+        device, tokens, h, dtype, stream_dtype = ctx.device, a.tokens, size[-1], _DTYPES[a.dtype], _DTYPES[a.residual_dtype]
         out = torch.empty
         # With nothing between them, residual and branch have one gradient, as those of a sum have.
-        one = need[0] and need[1] and not has[0] and a.residual_scale == 1.0 and stream.dtype is dtype
-        gr = out(size, dtype=stream.dtype, device=device) if need[0] else None
+        one = need[0] and need[1] and not has[0] and a.residual_scale == 1.0 and stream_dtype is dtype
+        gr = out(size, dtype=stream_dtype, device=device) if need[0] else None
         gb = out(size, dtype=dtype, device=device) if need[1] and not one else None
         gg = gbw = gw = None
         if need[2]:
@@ -176,13 +177,13 @@ class _ResidualNorm(torch.autograd.Function):
         if tokens:
             a.stream = a.normed = None
             if grad_normed is not None:
-                rows, a.stream_stride = _rows(stream, h)
+                rows, a.stream_stride = _rows(saved[0], h)
                 if not (grad_normed.dtype is dtype and grad_normed.is_contiguous()):
                     grad_normed = grad_normed.to(dtype).contiguous()
                 a.stream, a.grad_normed = rows.data_ptr(), grad_normed.data_ptr()
             if grad_stream is not None:
-                if not (grad_stream.dtype is stream.dtype and grad_stream.is_contiguous()):
-                    grad_stream = grad_stream.to(stream.dtype).contiguous()
+                if not (grad_stream.dtype is stream_dtype and grad_stream.is_contiguous()):
+                    grad_stream = grad_stream.to(stream_dtype).contiguous()
                 a.grad_stream = grad_stream.data_ptr()
             if gr is not None:
                 a.grad_residual = gr.data_ptr()
@@ -208,29 +209,32 @@ class _ResidualNorm(torch.autograd.Function):
 _DTYPES = {code: dtype for dtype, code in DTYPE_CODES.items()}
 
 
-def _again(ctx, stream, rms, others):
+def _again(ctx, saved):
     """The record anew, for tensors that hooks on saved tensors handed back; and those tensors."""
-    a, size, rest = ctx.record, ctx.size, iter(others)
-    on_device("the stream", stream, stream.device)
-    on_device("the statistics", rms, stream.device)
-    if rms.size() != (2, a.tokens) or rms.dtype != torch.float32 or stream.numel() != size.numel() or stream.dtype != _DTYPES[a.residual_dtype]:
+    a, size, rest = ctx.record, ctx.size, iter(saved)
+    kept = [next(rest) if has else None for has in (ctx.has[3], ctx.has[2] or ctx.has[3], *ctx.has)]
+    stream, rms, branch, gate, branch_weight, weight = kept
+    for what, t in zip(("the stream", "the statistics", "the branch", "the gate", "the branch's weight", "the weight"), kept):
+        if t is not None:
+            on_device(what, t, ctx.device)
+    if rms is not None and (rms.size() != (2, a.tokens) or rms.dtype != torch.float32):
         raise ValueError("the saved tensors are not those of the forward pass")
-    branch, gate, branch_weight, weight = (next(rest) if has else None for has in ctx.has)
-    stream = stream.reshape(size)
+    if stream is not None and (stream.numel() != size.numel() or stream.dtype != _DTYPES[a.residual_dtype]):
+        raise ValueError("the saved tensors are not those of the forward pass")
+    # Where the stream is not read, one element stands for its shape.
+    stream = torch.empty((), dtype=_DTYPES[a.residual_dtype], device=ctx.device).expand(size) if stream is None else stream.reshape(size)
     branch = None if branch is None else branch.reshape(size)
     if gate is not None:
         gate = gate.reshape(size if a.gate_kind == _native.EMRS_NORM_GATE_TOKEN else size[-1:])
-    if branch is None and weight is None:  # a sum alone
-        b = _native.Norm.from_buffer_copy(a)
-    else:
-        b, *others = _record(stream, branch, gate, branch_weight, weight, a.residual_scale, a.eps)
-        if b.dtype != a.dtype:
-            raise ValueError("the saved tensors are not those of the forward pass")
-        others = [t for t in others if t is not None]
-    rms = rms.contiguous()
-    b.gate_kind, b.stream_rms = a.gate_kind, rms.data_ptr()
-    b.branch_rms = b.stream_rms + 4 * a.tokens
-    return (b, stream, rms, *others)
+    b, *others = _record(stream, branch, gate, branch_weight, weight, a.residual_scale, a.eps)
+    if b.dtype != a.dtype:
+        raise ValueError("the saved tensors are not those of the forward pass")
+    b.gate_kind = a.gate_kind
+    if rms is not None:
+        rms = rms.contiguous()
+        b.stream_rms = rms.data_ptr()
+        b.branch_rms = b.stream_rms + 4 * a.tokens
+    return b, [t for t in (stream, rms, *others) if t is not None]
 
 
 def _wants_gradient(t) -> bool:
