@@ -728,6 +728,7 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
     p.exponent[(int64_t)at.head * p.queries.rows + row] = lse;
     p.delta[(int64_t)at.head * p.queries.rows + row] = delta;
   }
+  if (!p.grad_q) return;  // of gradients of keys and values alone, these are all that is wanted
 
   const int shift = keys - queries;
   auto seen_by = [&](int i) { return p.causal ? min(max(min(i, queries - 1) + shift + 1, 0), keys) : keys; };
@@ -807,7 +808,6 @@ __global__ __launch_bounds__(kThreads, DIM == 64 ? 3 : 2) void attention_grad_q_
     work(k_odd, v_odd, t + 1);
   }
   arrive();
-  if (!p.grad_q && !p.parts) return;
   const int64_t corner = ((int64_t)(at.own.first + mine) * p.heads + at.head) * p.real_dim, stride = (int64_t)p.heads * p.real_dim;
   char *const room = wave == 0 ? k_even : wave == 1 ? k_odd : wave == 2 ? v_even : v_odd;
   const float back = p.scale / lift.by();
@@ -1176,7 +1176,7 @@ int run_as(const emrs_attention *a, bool backward, hipStream_t st) {
   } else {
     p.exponent = reinterpret_cast<float *>(w + room.exponent);
     p.delta = reinterpret_cast<float *>(w + room.delta);
-    // delta and exponent come out of grad_q's kernel, so that it runs in any case.
+    // delta and exponent come out of grad_q's kernel, so that it runs in any case; without grad_q it ends there.
     p.grad_q = a->grad_q;
     if (!a->grad_q && p.splits > 1) p.splits = 1, p.parts = nullptr;
     if (a->rows) {
