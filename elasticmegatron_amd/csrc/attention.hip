@@ -20,10 +20,11 @@
 // 2^7, with room for a maximum that grows) and grad_v down to 2^-29 (by 2^15); of d, each row of grad_q and of grad_k down
 // to 2^-20 of the largest of its own sum (Lift).  No result passes through atomics: the same call gives the same bits.
 //
-// What bounds it: the matrix units, with the arithmetic of the softmax beside them.  4096 rows, 32 heads of 128, causal:
-// forward 152 to 156 us (0.89 PFLOP/s; matrix instructions in 51% of the cycles that a CU is busy), grad_q 204 to 214
-// (0.99 PFLOP/s, 57%), grad_k and grad_v 260 to 267 (1.04 PFLOP/s, 60%), at about 1.9 GHz of 2.4.  With a query or a few
-// to many keys, reading these: 64 single tokens to 8192 keys each, 5.9 TB/s.
+// What bounds it: the matrix units, with the arithmetic of the softmax beside them.  4096 rows, 32 heads of 128, causal, one
+// call behind the other: forward 145 to 147 us (0.94 PFLOP/s), the two backward kernels 472 to 487 (1.0 PFLOP/s of what they
+// execute); in fp16 152 and 531 to 540.  Under the profiler, mean and least: forward 172 and 158 us, with matrix instructions in
+// 51% of the cycles that a CU is busy, grad_q 236 and 218, 57%, grad_k and grad_v 297 and 273, 60%.  With a query or a few to
+// many keys, reading these: 64 single tokens to 8192 keys each, 5.9 TB/s.
 
 #include <hip/hip_runtime.h>
 

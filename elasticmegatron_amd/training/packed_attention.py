@@ -185,7 +185,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, offsets: Opt
 
     Differentiable once, to ``q``, ``k`` and ``v``.  Probabilities and their gradients are rounded to the operands' type on
     their way into the sums.  What is not finite in a key or value reaches queries of its own document that do not
-    see it."""
+    see it, and what is not finite in a query or its gradient the gradients of keys there that it does not see."""
     refuse_tangents(q, k, v)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         return _Attention.apply(q, k, v, offsets, key_offsets, causal, scale)

@@ -551,8 +551,8 @@ int emrs_adamw_step(const emrs_adamw *adamw, void *stream);
  *   stream = residual_scale residual + gate n(branch)       (branch == NULL: the residual's part alone)
  *   normed = stream / rms(stream) weight                    (of the stream before its rounding)
  * stream and normed are contiguous; NULL: not wanted.  stream_rms and branch_rms get 1 / rms of every token (NULL:
- * not wanted).  Backward reads them, the stream that forward wrote (without a branch: the residual, where
- * residual_scale is 1), and the gradients of stream and normed, either of which may be NULL.  The gradients that it
+ * not wanted).  Backward reads, for the gradient of normed, stream_rms and the stream that forward wrote (without a
+ * branch: the residual, where residual_scale is 1), for that of n, branch_rms; and the gradients of stream and normed, either of which may be NULL.  The gradients that it
  * writes are contiguous, of their input's type; NULL: not wanted.  A gate for each channel is [hidden], one for each
  * token [tokens][hidden].  Operands, normed and all but the stream's gradients are of `dtype`. */
 #define EMRS_NORM_GATE_NONE 0u
@@ -612,7 +612,8 @@ typedef struct emrs_experts {
   uint64_t grad_y_stride;
   void *grad_x;                   /* [rows][n_in], contiguous; NULL: not wanted */
   void *const *grad_weights;      /* per expert, contiguous; NULL: not wanted */
-  void *workspace;                /* 256-byte aligned: copies of operands whose rows lie off 16 bytes */
+  void *workspace;                /* 256-byte aligned: copies of operands whose rows lie off 16 bytes, and 64 MB for the
+                                   * parts of tiles, where these may be cut along a sum over 8192 or more */
   uint64_t workspace_bytes;
 } emrs_experts;
 
